@@ -16,6 +16,7 @@ library's other rotations, the float32 product position * theta_i of the
 float32 frequency theta_i; its cosine and sine are taken in 64 bits.
 """
 import math
+import sys
 
 import numpy as np
 import torch
@@ -188,14 +189,19 @@ def prepare(case, seed):
             length=torch.tensor([case["prefix"]], device="cuda", dtype=torch.int32),
             own_length=torch.tensor(tails, device="cuda", dtype=torch.int32))
     if own:
-        import sys
-        sys.path.insert(0, "kvmem-llama.cpp_b200")
-        import kvmret
+        kvmret = _library()
         state["pages"] = kvmret.Pages(state["kc"], state["vc"], page, hkv, d, case["kt"], case["vt"])
         if op == "attn":
             state["own_pages"] = kvmret.Pages(state["tk"], state["tv"], page, hkv, d, case["kt"],
                                               case["vt"])
     return state
+
+
+def _library():
+    if "kvmret" not in sys.modules:
+        sys.path.insert(0, "kvmem-llama.cpp_b200")  # the package's folder is no module name
+    import kvmret
+    return kvmret
 
 
 def _cos_sin(pos, d):
@@ -327,7 +333,7 @@ def run(state):
     op = state["op"]
     if not own:
         return {"qk": _plain_qk, "append": _plain_append, "attn": _plain_attn}[op](state)
-    import kvmret
+    kvmret = _library()
     if op == "qk":
         raw = state["raw"]
         got = kvmret.qk_norm_rope(state["q"], state["k"], state["pos"], state["wq"], state["wk"],
