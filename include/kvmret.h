@@ -39,6 +39,9 @@ extern "C" {
 #define KVMRET_TYPE_F16 1
 #define KVMRET_TYPE_Q4_0 2
 #define KVMRET_TYPE_Q8_0 8
+/* Activation formats of kvmret_qk_norm_rope (with F16): F32 = 0, BF16 = 30. */
+#define KVMRET_TYPE_F32 0
+#define KVMRET_TYPE_BF16 30
 
 typedef struct kvmret_ctx kvmret_ctx;
 typedef struct kvmret_table kvmret_table;
@@ -561,6 +564,66 @@ int kvmret_score_noalloc(const float *summ_dev, uint32_t summ_stride, const floa
                          const uint32_t *q_count_dev, const uint8_t *has_block_dev,
                          uint32_t n_blocks, uint32_t n_layer, uint32_t n_head,
                          uint32_t n_head_kv, uint32_t d_head, double *scores_dev, void *stream);
+
+/* ---- the attention step beside the window: norms of the query and key heads
+ *      with the position rotation, and the append of new keys and values to a
+ *      paged cache. No counterpart in the reference, whose model graph does
+ *      this work around the retrieval. Stateless, asynchronous on `stream` (a
+ *      cudaStream_t of the current device, NULL = legacy default stream); the
+ *      buffers belong to that device. Nothing is allocated, so the calls may
+ *      be captured into graphs. ---- */
+/* One pass over the query and key heads of n_tok tokens:
+ *   y = x / sqrt(mean(x^2) + eps) * weight   per head, in f32
+ *   z = RoPE(y) at pos_dev[t]                (NeoX pairs (i, i + d_head / 2);
+ *                                            the angle as in kvmret_rope_f16)
+ * with the orthonormal Hadamard transform of z when fwht_n = d_head (the
+ * queries of a window whose quantised K is Hadamard-rotated), and each wanted
+ * form rounded once to f16. Head h of token t of q lies at element
+ * t * q_stride + h * d_head of `type` (KVMRET_TYPE_F16, _BF16 or _F32), k
+ * likewise, so both may be views of one projection's rows. */
+typedef struct kvmret_qk {
+    const void *q_dev, *k_dev;           /* n_head / n_head_kv heads a token */
+    uint64_t q_stride, k_stride;         /* elements between tokens */
+    const float *q_weight_dev, *k_weight_dev;  /* [d_head], NULL: ones */
+    const int32_t *pos_dev;              /* [n_tok] */
+    /* f16 outputs [n_tok][heads][d_head], NULL: not wanted. *_rot = z;
+     * *_raw = y (kvmret_query_add_f16 rows, kvmret_append's k_cap rows). */
+    uint16_t *q_rot_dev, *k_rot_dev, *q_raw_dev, *k_raw_dev;
+    uint32_t n_tok, n_head, n_head_kv, d_head;
+    uint32_t n_rot;                      /* = d_head (full NeoX rotary) */
+    uint32_t fwht_n;                     /* 0 or d_head */
+    int32_t type;
+    float eps, freq_base, freq_scale;
+} kvmret_qk;
+/* q_dev or k_dev may be NULL with its outputs (its head count is then not
+ * used). Inputs and outputs 16-byte aligned, strides multiples of 16 bytes;
+ * outputs overlap neither the inputs nor one another. */
+int kvmret_qk_norm_rope(const kvmret_qk *a, void *stream);
+
+/* A paged cache of one layer: token `off` of page p has its K row (n_head_kv *
+ * d_head elements of k_type, kvmret_row_bytes) at k_dev + p * k_page_bytes +
+ * off * row, its V row likewise. A layer of a context's window is one (page =
+ * window slot, cell = kvmret_cells' number). Rows and page strides are
+ * multiples of 16 bytes, bases 16-byte aligned, n_pages * page_tokens <= 2^31 - 1. */
+typedef struct kvmret_pages {
+    void *k_dev, *v_dev;
+    uint64_t k_page_bytes, v_page_bytes; /* between pages; 0: page_tokens rows */
+    uint32_t n_pages, page_tokens, n_head_kv, d_head;
+    int32_t k_type, v_type;
+} kvmret_pages;
+/* File n_tok tokens' f16 K and V (row t at element t * stride; strides of 0:
+ * dense) into cells: page = cell / page_tokens, offset = cell % page_tokens.
+ * A token whose cell is negative or past the last page is skipped; cells that
+ * no token names keep their bytes. K is rotated at pos_dev[t] (NULL: stored
+ * as it is, no rotation), Hadamard-transformed when fwht_n = d_head, and
+ * written in k_type: the bits that kvmret_rope_f16 gives the same row, or the
+ * quantised form of the rotated f32 values; V is written in v_type. The
+ * non-negative cells must differ: what a cell named twice holds is one token's
+ * values or a mixture. */
+int kvmret_paged_append(const kvmret_pages *pages, const uint16_t *k_dev, uint64_t k_stride,
+                        const uint16_t *v_dev, uint64_t v_stride, const int32_t *cells_dev,
+                        const int32_t *pos_dev, uint32_t n_tok, float freq_base,
+                        float freq_scale, uint32_t fwht_n, void *stream);
 
 /* ---- host block table: the selection / plan logic alone, no GPU needed
  *      (KvMemStore, kvmem/include/kvmem/kvmem_store.hpp:329-491). ---- */

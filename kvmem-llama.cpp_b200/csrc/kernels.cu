@@ -13,6 +13,7 @@
 #include <cub/block/block_scan.cuh>
 
 #include "kvmret.h"
+#include "quant.cuh"
 
 namespace kvmret {
 namespace {
@@ -39,14 +40,6 @@ cudaError_t launch_dep(void (*kfn)(KArgs...), dim3 grid, dim3 block, size_t smem
 }
 
 __device__ __forceinline__ void dep_wait() { cudaGridDependencySynchronize(); }
-
-
-__device__ __forceinline__ float h2f(uint16_t h) {
-    return __half2float(__ushort_as_half(h));
-}
-__device__ __forceinline__ uint16_t f2h(float f) {
-    return __half_as_ushort(__float2half_rn(f));
-}
 
 // ---------------------------------------------------------------------------
 // S1: q_sum += rows, row order (llama-memory-kvmem.cpp:3417-3432); with
@@ -705,19 +698,6 @@ __global__ void __launch_bounds__(1024) select_radix_kernel(const double *__rest
 }
 
 // ---------------------------------------------------------------------------
-// RoPE table: cos / sin of the float angle pos * theta[i] (rope.cpp:27-33).
-// The angle is the reference's float product; cos and sin are evaluated in
-// double and rounded once to float, i.e. correctly rounded, so the table does
-// not add the few-ulp error of a float sincos. Window positions come from a
-// per-context table built once at creation; the stateless entry points build a
-// temporary table for their positions.
-__device__ __forceinline__ float2 rope_cs(int32_t pos, float theta) {
-    const float ang = __fmul_rn(static_cast<float>(pos), theta);
-    double s, c;
-    sincos(static_cast<double>(ang), &s, &c);
-    return make_float2(__double2float_rn(c), __double2float_rn(s));
-}
-
 // Position table: cs[p][j] = {c_2j, c_2j+1, s_2j, s_2j+1} of position
 // pos_base + p, for p in [0, n_pos).
 __global__ void rope_table_kernel(float4 *__restrict__ cs, uint32_t n_pos, uint32_t half,
@@ -1083,19 +1063,6 @@ __device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
     return r;
 }
 
-// round-half-away-from-zero (C roundf) for |y| < 2^23: truncate y + s, s =
-// copysign(0.5 - 2^-25, y) (the float just below one half). Exactness: for
-// |y| >= 1 the sum is exact or rounds only across the binade edge, where
-// truncation already gives the rounded value; for |y| < 1 the only
-// candidates for a wrong carry are the ties y = +-0.5 (sum 1 - 2^-25 rounds
-// to 1, as wanted) and y = +-(0.5 - 2^-25) (sum 1 - 2^-24, exact, truncates
-// to 0). Checked against the host roundf on every float of magnitude < 256.
-// The truncation is the conversion to an integer (toward zero), whose low
-// byte is then the int8.
-__device__ __forceinline__ int round_away_int(float y) {
-    return __float2int_rz(__fadd_rn(y, copysignf(0.49999997f, y)));
-}
-
 // Reads the quant block at byte offset o of a shared-memory segment: scale
 // bits and the payload as words (payload byte 4j+k = byte k of p[j]).
 template <int KT>
@@ -1166,22 +1133,6 @@ __device__ __forceinline__ void dequant_qblock(uint32_t d16, const uint32_t (&p)
             }
         }
     }
-}
-
-__device__ __forceinline__ uint32_t pack_low_bytes(uint32_t b0, uint32_t b1, uint32_t b2,
-                                                   uint32_t b3) {
-    return __byte_perm(__byte_perm(b0, b1, 0x0040u), __byte_perm(b2, b3, 0x0040u), 0x5410u);
-}
-
-// x / 127 correctly rounded, by division by a constant known in advance
-// (Brisebarre, Muller and Raina, IEEE Trans. Computers 53(8), 2004): with
-// zh = RN(1/127) and zl = RN(1/127 - zh), RN(x zh + RN(x zl)) is the
-// correctly rounded quotient. Checked against IEEE division on every
-// non-negative float: it holds for all x >= 2^-100 (below that x zl loses
-// bits to underflow), so smaller x take the division.
-__device__ __forceinline__ float div127_rn(float x) {
-    if (!(x >= 0x1p-100f)) return __fdiv_rn(x, 127.0f);
-    return __fmaf_rn(x, 0x1.020408p-7f, __fmul_rn(x, 0x1.020408p-35f));
 }
 
 template <int KT>

@@ -27,6 +27,8 @@ LIB_PATH = os.path.join(_HERE, "libkvmret.so")
 TYPE_F16 = 1
 TYPE_Q4_0 = 2
 TYPE_Q8_0 = 8
+TYPE_F32 = 0    # activations only (qk_norm_rope)
+TYPE_BF16 = 30  # activations only
 
 OK = 0
 
@@ -108,6 +110,31 @@ class Prof(ctypes.Structure):
 
     def as_dict(self):
         return {k: getattr(self, k) for k, _ in self._fields_}
+
+
+class QkArgs(ctypes.Structure):
+    _fields_ = [
+        ("q_dev", ctypes.c_void_p), ("k_dev", ctypes.c_void_p),
+        ("q_stride", ctypes.c_uint64), ("k_stride", ctypes.c_uint64),
+        ("q_weight_dev", ctypes.c_void_p), ("k_weight_dev", ctypes.c_void_p),
+        ("pos_dev", ctypes.c_void_p),
+        ("q_rot_dev", ctypes.c_void_p), ("k_rot_dev", ctypes.c_void_p),
+        ("q_raw_dev", ctypes.c_void_p), ("k_raw_dev", ctypes.c_void_p),
+        ("n_tok", ctypes.c_uint32), ("n_head", ctypes.c_uint32), ("n_head_kv", ctypes.c_uint32),
+        ("d_head", ctypes.c_uint32), ("n_rot", ctypes.c_uint32), ("fwht_n", ctypes.c_uint32),
+        ("type", ctypes.c_int32), ("eps", ctypes.c_float), ("freq_base", ctypes.c_float),
+        ("freq_scale", ctypes.c_float),
+    ]
+
+
+class PagesDesc(ctypes.Structure):
+    _fields_ = [
+        ("k_dev", ctypes.c_void_p), ("v_dev", ctypes.c_void_p),
+        ("k_page_bytes", ctypes.c_uint64), ("v_page_bytes", ctypes.c_uint64),
+        ("n_pages", ctypes.c_uint32), ("page_tokens", ctypes.c_uint32),
+        ("n_head_kv", ctypes.c_uint32), ("d_head", ctypes.c_uint32),
+        ("k_type", ctypes.c_int32), ("v_type", ctypes.c_int32),
+    ]
 
 
 _P = ctypes.c_void_p
@@ -225,6 +252,9 @@ SIGNATURES = {
                                           ctypes.POINTER(_U64), ctypes.c_int]),
     "kvmret_score_noalloc": (ctypes.c_int, [_P, _U32, _P, _P, _P, _U32, _U32, _U32, _U32, _U32,
                                             _P, _P]),
+    "kvmret_qk_norm_rope": (ctypes.c_int, [ctypes.POINTER(QkArgs), _P]),
+    "kvmret_paged_append": (ctypes.c_int, [ctypes.POINTER(PagesDesc), _P, _U64, _P, _U64, _P, _P,
+                                           _U32, ctypes.c_float, ctypes.c_float, _U32, _P]),
     "kvmret_table_create": (ctypes.c_int, [ctypes.POINTER(Config), ctypes.POINTER(_P)]),
     "kvmret_table_destroy": (None, [_P]),
     "kvmret_table_append": (ctypes.c_int, [_P, _U32]),
@@ -907,3 +937,114 @@ def rope_q4_0(k, out, n_tok, pos0, n_head_kv, d_head, freq_base=1e6, freq_scale=
     """k, out: q4_0 rows [n_tok][n_head_kv*d_head/32*18] uint8 CUDA tensors."""
     _check(lib.kvmret_rope_q4_0(k.data_ptr(), out.data_ptr(), n_tok, n_head_kv, d_head, d_head,
                                 pos0, freq_base, freq_scale, fwht_n, _torch_stream(stream)))
+
+
+def _want(ok, msg):
+    if not ok:
+        raise KvmretError(msg)
+
+
+def _launch(dev, stream, fn, *args):
+    """Call a stateless entry point with its buffers' device current, on the
+    given stream of that device or torch's current one."""
+    import torch
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            _check(fn(*args, _torch_stream(stream)))
+    else:
+        _check(fn(*args, _torch_stream(stream)))
+
+
+def _head_rows(x, name):
+    """A [n_tok][heads][d_head] view whose tokens may be strided: its strides
+    inside a token must be dense."""
+    _want(x.is_cuda and x.dim() == 3, f"{name}: a [n_tok][heads][d_head] CUDA tensor")
+    row = x.shape[1] * x.shape[2]
+    _want(x.numel() == 0 or (x.stride(2) == 1 and (x.shape[1] == 1 or x.stride(1) == x.shape[2])),
+          f"{name}: the heads of a token must be contiguous")
+    _want(x.shape[0] < 2 or x.stride(0) >= row, f"{name}: the tokens must not overlap")
+    return x.stride(0) if x.shape[0] > 1 else row
+
+
+def _index(x, n, dev, name):
+    """A contiguous int32 tensor of n elements (None: any) on dev."""
+    import torch
+    _want(x.dtype == torch.int32 and x.device == dev and x.is_contiguous() and
+          (n is None or x.numel() == n),
+          f"{name}: a contiguous int32 tensor{'' if n is None else f' of {n}'} on {dev}")
+    return x.data_ptr()
+
+
+def qk_norm_rope(q, k, pos, q_weight=None, k_weight=None, eps=1e-6, freq_base=1e6,
+                 freq_scale=1.0, fwht_n=0, q_rot=True, k_rot=True, q_raw=False, k_raw=False,
+                 stream=0):
+    """RMS norm of every query and key head and its position rotation, in one pass.
+
+    q: [n_tok][n_head][d_head], k: [n_tok][n_head_kv][d_head], f16 / bf16 / f32
+    CUDA tensors (views with a token stride are read in place); pos: [n_tok]
+    int32; weights: [d_head] f32 or None. fwht_n = d_head: the rotated rows are
+    Hadamard-transformed too (queries of a quantised window). Returns (q_rot,
+    k_rot, q_raw, k_raw): f16 tensors, None where not wanted; *_raw is the
+    normed row without the rotation (query_add rows, append's k_cap)."""
+    import torch
+    types = {torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16, torch.float32: TYPE_F32}
+    dev = q.device
+    _want(q.dtype in types and k.dtype == q.dtype and k.device == dev,
+          "q and k: f16, bf16 or f32, of one type and device")
+    qs, ks = _head_rows(q, "q"), _head_rows(k, "k")
+    n, hq, d = q.shape
+    hkv = k.shape[1]
+    _want(k.shape[0] == n and k.shape[2] == d, "k: [n_tok][n_head_kv][d_head] like q")
+    ptrs = []
+    for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+        _want(w is None or (w.dtype == torch.float32 and w.device == dev and w.is_contiguous() and
+                            w.numel() == d), f"{name}: {d} contiguous f32 values on {dev}")
+        ptrs.append(None if w is None else w.data_ptr())
+    outs = [torch.empty((n, h, d), dtype=torch.float16, device=dev) if on else None
+            for on, h in ((q_rot, hq), (k_rot, hkv), (q_raw, hq), (k_raw, hkv))]
+    a = QkArgs(q.data_ptr(), k.data_ptr(), qs, ks, ptrs[0], ptrs[1], _index(pos, n, dev, "pos"),
+               *[None if o is None else o.data_ptr() for o in outs], n, hq, hkv, d, d, fwht_n,
+               types[q.dtype], eps, freq_base, freq_scale)
+    _launch(dev, stream, lib.kvmret_qk_norm_rope, ctypes.byref(a))
+    return tuple(outs)
+
+
+class Pages:
+    """A paged cache of one layer: k and v are CUDA tensors whose first axis is
+    the page and whose other axes hold page_tokens rows of n_head_kv * d_head
+    elements of k_type / v_type (f16 values, or the bytes of q8_0 / q4_0
+    blocks); the page axis may be strided. Cell c is token c % page_tokens of
+    page c // page_tokens."""
+
+    def __init__(self, k, v, page_tokens, n_head_kv, d_head, k_type=TYPE_F16, v_type=TYPE_F16):
+        _want(k.is_cuda and v.device == k.device and k.shape[0] == v.shape[0],
+              "pages: k and v CUDA tensors of one device, with one first axis")
+        strides = []
+        for x, t in ((k, k_type), (v, v_type)):
+            _want(x.shape[0] > 0 and x[0].is_contiguous() and x[0].numel() * x.element_size() ==
+                  page_tokens * row_bytes(t, n_head_kv * d_head),
+                  "pages: a page must be page_tokens contiguous rows of its type")
+            strides.append(x.stride(0) * x.element_size() if x.shape[0] > 1 else 0)
+        self.k, self.v, self.device = k, v, k.device
+        self.desc = PagesDesc(k.data_ptr(), v.data_ptr(), strides[0], strides[1], k.shape[0],
+                              page_tokens, n_head_kv, d_head, k_type, v_type)
+
+
+def paged_append(pages, k, v, cells, pos=None, freq_base=1e6, freq_scale=1.0, fwht_n=0, stream=0):
+    """File the tokens' K and V ([n_tok][n_head_kv][d_head] f16 CUDA tensors,
+    tokens may be strided) into the cells of a paged cache, K rotated at
+    pos[t] (None: as it is) and both written in the pages' types. cells, pos:
+    [n_tok] int32; a token with a negative cell is skipped; the others' cells
+    must differ."""
+    import torch
+    p = pages.desc
+    for x, name in ((k, "k"), (v, "v")):
+        _want(x.dtype == torch.float16 and x.device == pages.device and
+              x.shape == (k.shape[0], p.n_head_kv, p.d_head),
+              f"{name}: [n_tok][{p.n_head_kv}][{p.d_head}] f16 on {pages.device}")
+    n = k.shape[0]
+    ks, vs = _head_rows(k, "k"), _head_rows(v, "v")
+    _launch(pages.device, stream, lib.kvmret_paged_append, ctypes.byref(p), k.data_ptr(), ks,
+            v.data_ptr(), vs, _index(cells, n, pages.device, "cells"),
+            None if pos is None else _index(pos, n, pages.device, "pos"), n, freq_base, freq_scale,
+            fwht_n)
