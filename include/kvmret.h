@@ -625,6 +625,56 @@ int kvmret_paged_append(const kvmret_pages *pages, const uint16_t *k_dev, uint64
                         const int32_t *pos_dev, uint32_t n_tok, float freq_base,
                         float freq_scale, uint32_t fwht_n, void *stream);
 
+/* Attention of n_q query rows over a prefix that all of them share and, for
+ * the rows of each sequence, that sequence's own tail:
+ *   out = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale * q . k_j)
+ * for query head h against KV head h / (n_head / n_head_kv). The prefix is read
+ * once for the whole batch. Rows q_start[s] .. q_start[s + 1] - 1 are the new
+ * tokens of sequence s and the last of its tail's tokens: the last row sees the
+ * whole tail, the row before it one token less, and so on (a row whose place
+ * would be before the tail's first token sees no tail). With n_seq = 0 every
+ * row sees the prefix alone. */
+typedef struct kvmret_attn {
+    const uint16_t *q_dev;           /* f16, row t at t * q_stride: n_head * d_head elements */
+    uint64_t q_stride;               /* elements between rows; 0: dense */
+    uint16_t *out_dev;               /* f16 [n_q][n_head][d_head] */
+    float *lse_dev;                  /* [n_q][n_head] log of the sum (natural), NULL: not wanted */
+    uint32_t n_q, n_head;
+    float scale;                     /* of the scores, e.g. 1 / sqrt(d_head) */
+    uint32_t max_prefix;             /* bound on the prefix's tokens; 0: no prefix */
+    const int32_t *prefix_len_dev;   /* its tokens (one word), NULL: max_prefix */
+    const int32_t *prefix_table_dev; /* its pages in order, NULL: pages 0, 1, 2, ... */
+    const uint32_t *prefix_ntok_dev; /* tokens held by each listed page (a window's slots may
+                                        be partly filled), NULL: full pages */
+    uint32_t n_seq, tail_pages;      /* tail_pages: row length of tail_table */
+    const int32_t *q_start_dev;      /* [n_seq + 1], ascending */
+    const int32_t *tail_table_dev;   /* [n_seq][tail_pages] */
+    const int32_t *tail_len_dev;     /* [n_seq] tokens, the new ones included */
+} kvmret_attn;
+/* Lengths and tables are read on the device, so a captured call follows them.
+ * Lengths are cut to [0, max_prefix] and [0, tail_pages * page_tokens]; a page id
+ * outside its pool counts as a page without tokens. A row that sees no token gets
+ * zeros and an lse of -inf; rows before q_start[0] or from q_start[n_seq] on are
+ * left as they were. Tokens past a length may hold anything; those within it
+ * must be finite. `prefix` (NULL with max_prefix = 0) and `tail` (NULL with
+ * n_seq = 0) have one n_head_kv and d_head; page_tokens is a multiple of 16; the
+ * types may differ. Scores, statistics and sums are f32; quantised values are
+ * rounded to f16 (d * q) before the products. ws_dev: 256-byte aligned workspace
+ * of kvmret_prefix_attn_ws_bytes, written and read by this call alone (calls that
+ * may overlap, graphs included, need one each). n_q <= 65535, n_head <= 65535. */
+size_t kvmret_prefix_attn_ws_bytes(uint32_t n_q, uint32_t n_head, uint32_t n_head_kv,
+                                   uint32_t d_head, uint32_t n_seq);
+int kvmret_prefix_attn(const kvmret_pages *prefix, const kvmret_pages *tail, const kvmret_attn *a,
+                       void *ws_dev, size_t ws_bytes, void *stream);
+/* The same over one layer of a context's window as the prefix (its n_head_kv,
+ * d_head and types, every occupied slot's tokens), on the context's stream after
+ * the steps and appends enqueued so far; a->max_prefix, prefix_len_dev,
+ * prefix_table_dev and prefix_ntok_dev are not read. block_tokens must be a
+ * multiple of 16. K of the window is rotated at window positions 0 .., so the
+ * next token's position is the window's token count. */
+int kvmret_window_attn(kvmret_ctx *ctx, uint32_t layer, const kvmret_pages *tail,
+                       const kvmret_attn *a, void *ws_dev, size_t ws_bytes);
+
 /* ---- host block table: the selection / plan logic alone, no GPU needed
  *      (KvMemStore, kvmem/include/kvmem/kvmem_store.hpp:329-491). ---- */
 int kvmret_table_create(const kvmret_config *cfg, kvmret_table **out);

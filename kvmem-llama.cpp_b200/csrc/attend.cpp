@@ -1,5 +1,6 @@
 // C ABI of the attention step beside the window: per-head norms with the
-// position rotation and the append to a paged cache. Every argument is checked
+// position rotation, the append to a paged cache and the attention over a
+// shared prefix. Every argument is checked
 // on the host before the launch; no C++ exception leaves this file.
 #include "attend.hpp"
 
@@ -87,6 +88,67 @@ int resolve_pages(const kvmret_pages *p, const char *what, PageView *out) {
                     static_cast<unsigned long long>(v.v_page));
     *out = v;
     return KVMRET_OK;
+}
+
+int prefix_attn_call(const KeyList &prefix, const kvmret_pages *tail, const kvmret_attn *a,
+                     void *ws, size_t ws_bytes, cudaStream_t st) {
+    if (!a) return fail(KVMRET_ERR_ARG, "null arguments");
+    PrefixAttn r{};
+    r.prefix = prefix;
+    if (a->n_seq) {
+        if (const int rc = resolve_pages(tail, "tail", &r.tail.pages); rc != KVMRET_OK) return rc;
+        if (r.prefix.max_len && (r.prefix.pages.n_head_kv != r.tail.pages.n_head_kv ||
+                                 r.prefix.pages.d_head != r.tail.pages.d_head))
+            return fail(KVMRET_ERR_ARG, "prefix of %u heads of %u, tail of %u heads of %u",
+                        r.prefix.pages.n_head_kv, r.prefix.pages.d_head, r.tail.pages.n_head_kv,
+                        r.tail.pages.d_head);
+    } else if (!r.prefix.max_len) {
+        return fail(KVMRET_ERR_ARG, "attention without a prefix or tails");
+    }
+    const PageView &pv = r.prefix.max_len ? r.prefix.pages : r.tail.pages;
+    if ((r.prefix.max_len && r.prefix.pages.page_tokens % 16) ||
+        (a->n_seq && r.tail.pages.page_tokens % 16))
+        return fail(KVMRET_ERR_ARG, "attention needs pages of a multiple of 16 tokens");
+    if (a->n_head == 0 || a->n_head % pv.n_head_kv || a->n_head > 65535)
+        return fail(KVMRET_ERR_ARG, "n_head %u over %u KV heads", a->n_head, pv.n_head_kv);
+    if (!std::isfinite(a->scale)) return fail(KVMRET_ERR_ARG, "scale must be finite");
+    if (a->n_q > 65535 || a->n_seq > 65535)
+        return fail(KVMRET_ERR_ARG, "n_q %u / n_seq %u above 65535", a->n_q, a->n_seq);
+    if (a->n_q == 0) return KVMRET_OK;
+    if (!a->q_dev || !a->out_dev) return fail(KVMRET_ERR_ARG, "null query or output");
+    const uint64_t row = static_cast<uint64_t>(a->n_head) * pv.d_head;
+    r.q_stride = a->q_stride ? a->q_stride : row;
+    if (!aligned16(a->q_dev) || !aligned16(a->out_dev) || r.q_stride % 8)
+        return fail(KVMRET_ERR_ARG, "query rows and output must be 16-byte aligned");
+    if (a->n_q > 1 && r.q_stride < row)
+        return fail(KVMRET_ERR_ARG, "query rows of %llu elements overlap",
+                    static_cast<unsigned long long>(row));
+    if (a->n_seq) {
+        if (!a->q_start_dev || !a->tail_len_dev || !a->tail_table_dev || a->tail_pages == 0)
+            return fail(KVMRET_ERR_ARG, "tails without their rows, lengths or pages");
+        const uint64_t most = static_cast<uint64_t>(a->tail_pages) * r.tail.pages.page_tokens;
+        if (most > 0x7fffffffull)
+            return fail(KVMRET_ERR_ARG, "tails of %u pages pass 2^31 tokens", a->tail_pages);
+        r.tail.table = a->tail_table_dev;
+        r.tail.len = a->tail_len_dev;
+        r.tail.n_list = a->tail_pages;
+        r.tail.max_len = static_cast<uint32_t>(most);
+    }
+    r.q = a->q_dev;
+    r.out = a->out_dev;
+    r.lse = a->lse_dev;
+    r.n_q = a->n_q;
+    r.n_head = a->n_head;
+    r.n_head_kv = pv.n_head_kv;
+    r.d_head = pv.d_head;
+    r.scale = a->scale;
+    r.n_seq = a->n_seq;
+    r.q_start = a->q_start_dev;
+    const size_t need = prefix_attn_ws_bytes(a->n_q, a->n_head, pv.n_head_kv, pv.d_head, a->n_seq);
+    if (need && (!ws || ws_bytes < need || (reinterpret_cast<uintptr_t>(ws) & 255)))
+        return fail(KVMRET_ERR_ARG, "workspace of %zu bytes at 256-byte alignment, %zu needed",
+                    ws_bytes, need);
+    return launched(launch_prefix_attn(r, ws, st));
 }
 
 }  // namespace kvmret
@@ -185,6 +247,34 @@ int kvmret_paged_append(const kvmret_pages *pages, const uint16_t *k, uint64_t k
     a.fwht_n = fwht_n;
     if (pos) a.theta = make_theta(a.pages.d_head, freq_base, freq_scale);
     return launched(kvmret::launch_paged_append(a, static_cast<cudaStream_t>(stream)));
+}
+
+size_t kvmret_prefix_attn_ws_bytes(uint32_t n_q, uint32_t n_head, uint32_t n_head_kv,
+                                   uint32_t d_head, uint32_t n_seq) {
+    if (n_head_kv == 0 || n_head % n_head_kv || !head_ok(d_head) || n_q > 65535 || n_seq > 65535)
+        return 0;
+    return kvmret::prefix_attn_ws_bytes(n_q, n_head, n_head_kv, d_head, n_seq);
+}
+
+int kvmret_prefix_attn(const kvmret_pages *prefix, const kvmret_pages *tail, const kvmret_attn *a,
+                       void *ws, size_t ws_bytes, void *stream) {
+    if (!a) return fail(KVMRET_ERR_ARG, "null arguments");
+    kvmret::KeyList p{};
+    if (a->max_prefix) {
+        if (a->max_prefix > 0x7fffffffu)
+            return fail(KVMRET_ERR_ARG, "max_prefix %u passes 2^31 - 1", a->max_prefix);
+        if (const int rc = kvmret::resolve_pages(prefix, "prefix", &p.pages); rc != KVMRET_OK)
+            return rc;
+        p.table = a->prefix_table_dev;
+        p.ntok = a->prefix_ntok_dev;
+        p.len = a->prefix_len_dev;
+        p.max_len = a->max_prefix;
+        p.n_list = (a->max_prefix - 1) / p.pages.page_tokens + 1;
+        if (!p.table && p.n_list > p.pages.n_pages)
+            return fail(KVMRET_ERR_ARG, "max_prefix %u passes the %u pages", a->max_prefix,
+                        p.pages.n_pages);
+    }
+    return kvmret::prefix_attn_call(p, tail, a, ws, ws_bytes, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -27,6 +27,7 @@
 #include <string>
 #include <vector>
 
+#include "attend.hpp"
 #include "kernels.cuh"
 #include "kvmret.h"
 #include "prefill.cuh"
@@ -1410,6 +1411,28 @@ void *kvmret_window_v(kvmret_ctx *c, uint32_t layer) {
     return (c && layer < c->cfg.n_layer) ? c->win_v + layer * c->win_v_layer : nullptr;
 }
 uint32_t kvmret_window_slots(kvmret_ctx *c) { return c ? c->win_slots : 0; }
+
+int kvmret_window_attn(kvmret_ctx *c, uint32_t layer, const kvmret_pages *tail,
+                       const kvmret_attn *a, void *ws, size_t ws_bytes) {
+    NEED_CTX(c);
+    if (layer >= c->cfg.n_layer)
+        return fail(KVMRET_ERR_ARG, "layer %u of %u", layer, c->cfg.n_layer);
+    kvmret_pages w{};
+    w.k_dev = c->win_k + layer * c->win_k_layer;
+    w.v_dev = c->win_v + layer * c->win_v_layer;
+    w.n_pages = c->win_slots;
+    w.page_tokens = c->cfg.block_tokens;
+    w.n_head_kv = c->cfg.n_head_kv;
+    w.d_head = c->cfg.d_head;
+    w.k_type = c->cfg.k_type;
+    w.v_type = c->cfg.v_type;
+    kvmret::KeyList p{};
+    TRY(kvmret::resolve_pages(&w, "window", &p.pages));
+    p.ntok = c->d_win_ntok;  // 0 for an empty slot
+    p.n_list = c->win_slots;
+    p.max_len = c->win_slots * c->cfg.block_tokens;
+    return kvmret::prefix_attn_call(p, tail, a, ws, ws_bytes, c->st);
+}
 
 int kvmret_window_layout(kvmret_ctx *c, uint32_t *ids, int32_t *bases, uint32_t *n_out) {
     NEED_CTX(c);

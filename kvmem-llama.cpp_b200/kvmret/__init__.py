@@ -137,6 +137,18 @@ class PagesDesc(ctypes.Structure):
     ]
 
 
+class AttnArgs(ctypes.Structure):
+    _fields_ = [
+        ("q_dev", ctypes.c_void_p), ("q_stride", ctypes.c_uint64), ("out_dev", ctypes.c_void_p),
+        ("lse_dev", ctypes.c_void_p), ("n_q", ctypes.c_uint32), ("n_head", ctypes.c_uint32),
+        ("scale", ctypes.c_float), ("max_prefix", ctypes.c_uint32),
+        ("prefix_len_dev", ctypes.c_void_p), ("prefix_table_dev", ctypes.c_void_p),
+        ("prefix_ntok_dev", ctypes.c_void_p), ("n_seq", ctypes.c_uint32),
+        ("tail_pages", ctypes.c_uint32), ("q_start_dev", ctypes.c_void_p),
+        ("tail_table_dev", ctypes.c_void_p), ("tail_len_dev", ctypes.c_void_p),
+    ]
+
+
 _P = ctypes.c_void_p
 _U32 = ctypes.c_uint32
 _I32 = ctypes.c_int32
@@ -255,6 +267,11 @@ SIGNATURES = {
     "kvmret_qk_norm_rope": (ctypes.c_int, [ctypes.POINTER(QkArgs), _P]),
     "kvmret_paged_append": (ctypes.c_int, [ctypes.POINTER(PagesDesc), _P, _U64, _P, _U64, _P, _P,
                                            _U32, ctypes.c_float, ctypes.c_float, _U32, _P]),
+    "kvmret_prefix_attn_ws_bytes": (ctypes.c_size_t, [_U32, _U32, _U32, _U32, _U32]),
+    "kvmret_prefix_attn": (ctypes.c_int, [ctypes.POINTER(PagesDesc), ctypes.POINTER(PagesDesc),
+                                          ctypes.POINTER(AttnArgs), _P, ctypes.c_size_t, _P]),
+    "kvmret_window_attn": (ctypes.c_int, [_P, _U32, ctypes.POINTER(PagesDesc),
+                                          ctypes.POINTER(AttnArgs), _P, ctypes.c_size_t]),
     "kvmret_table_create": (ctypes.c_int, [ctypes.POINTER(Config), ctypes.POINTER(_P)]),
     "kvmret_table_destroy": (None, [_P]),
     "kvmret_table_append": (ctypes.c_int, [_P, _U32]),
@@ -627,6 +644,21 @@ class Retriever:
         return Plan(rm[: nr.value].copy(), si[: ni.value].copy(), so[: no.value].copy())
 
     # --- window
+    def window_attn(self, layer, q, tail=None, tail_table=None, tail_len=None, q_start=None,
+                    scale=None, lse=False, out=None):
+        """prefix_attn with one layer of this context's window as the shared
+        prefix, after the steps enqueued so far. Arguments and result as there."""
+        import torch
+        c = self.cfg
+        _want(q.device.type == "cuda" and q.device.index == c.device,
+              f"q: a tensor on the context's device cuda:{c.device}")
+        a, got, keep = _attn_args(q, c.d_head, tail, tail_table, tail_len, q_start, scale, lse, out)
+        ws, nb = _attn_ws(q, c.n_head_kv, a.n_seq)
+        with torch.cuda.device(q.device), _Ordered(self.stream_ptr):
+            _check(lib.kvmret_window_attn(self.h, layer, None if tail is None else
+                                          ctypes.byref(tail.desc), ctypes.byref(a), ws.data_ptr(), nb))
+        return got
+
     def window_layout(self):
         cap = int(lib.kvmret_window_slots(self.h))
         ids = np.zeros(cap, np.uint32)
@@ -1048,3 +1080,73 @@ def paged_append(pages, k, v, cells, pos=None, freq_base=1e6, freq_scale=1.0, fw
             v.data_ptr(), vs, _index(cells, n, pages.device, "cells"),
             None if pos is None else _index(pos, n, pages.device, "pos"), n, freq_base, freq_scale,
             fwht_n)
+
+
+def _attn_args(q, d_head, tail, tail_table, tail_len, q_start, scale, lse, out):
+    """The arguments that prefix_attn and window_attn share, and their result."""
+    import torch
+    dev = q.device
+    _want(q.dtype == torch.float16, "q: f16")
+    stride = _head_rows(q, "q")
+    n, h, d = q.shape
+    _want(d == d_head, f"q: heads of {d_head}")
+    if out is None:
+        out = torch.empty((n, h, d), dtype=torch.float16, device=dev)
+    else:
+        _want(out.dtype == torch.float16 and out.device == dev and out.shape == q.shape and
+              out.is_contiguous(), "out: contiguous f16 like q")
+    sums = torch.empty((n, h), dtype=torch.float32, device=dev) if lse else None
+    a = AttnArgs(q.data_ptr(), stride, out.data_ptr(), None if sums is None else sums.data_ptr(), n,
+                 h, d ** -0.5 if scale is None else scale)
+    if tail is not None:
+        _want(tail.device == dev and tail_table is not None and tail_len is not None and
+              q_start is not None and tail_table.dim() == 2,
+              "tails need [n_seq][pages] table, lengths and q_start")
+        s = a.n_seq = tail_table.shape[0]
+        a.tail_pages = tail_table.shape[1]
+        a.q_start_dev = _index(q_start, s + 1, dev, "q_start")
+        a.tail_table_dev = _index(tail_table, None, dev, "tail_table")
+        a.tail_len_dev = _index(tail_len, s, dev, "tail_len")
+    return a, ((out, sums) if lse else out), stride
+
+
+def _attn_ws(q, n_head_kv, n_seq):
+    import torch
+    nb = int(lib.kvmret_prefix_attn_ws_bytes(q.shape[0], q.shape[1], n_head_kv, q.shape[2], n_seq))
+    return torch.empty(nb, dtype=torch.uint8, device=q.device), nb
+
+
+def prefix_attn(q, prefix, prefix_len, tail=None, tail_table=None, tail_len=None, q_start=None,
+                prefix_table=None, prefix_ntok=None, max_prefix=None, scale=None, lse=False,
+                out=None, stream=0):
+    """Attention of all rows of q ([n_q][n_head][d_head] f16, rows may be
+    strided) over the shared prefix (Pages, its first prefix_len tokens: a
+    one-element int32 CUDA tensor, or None for max_prefix) and over each
+    sequence's own tail (Pages with tail_table [n_seq][pages] and tail_len
+    [n_seq] int32; sequence s has rows q_start[s] .. q_start[s + 1] - 1, the
+    last tokens of its tail). prefix_table: the prefix's pages in order;
+    prefix_ntok: the tokens that each of them holds; max_prefix: a bound on
+    the prefix (default: what its pages hold). Either part may be None.
+    scale defaults to d_head ** -0.5. Returns out (rows of no sequence: as
+    they were), with lse=True also the f32 [n_q][n_head] log-sum-exp."""
+    dev = q.device
+    pages = prefix if prefix is not None else tail
+    _want(pages is not None and pages.device == dev, "a prefix or tails, on q's device")
+    a, got, _ = _attn_args(q, pages.desc.d_head, tail, tail_table, tail_len, q_start, scale, lse, out)
+    if prefix is not None:
+        held = prefix.desc.n_pages if prefix_table is None else prefix_table.numel()
+        if prefix_ntok is not None:
+            a.prefix_ntok_dev = _index(prefix_ntok, held if prefix_table is not None else None, dev,
+                                       "prefix_ntok")
+            held = min(held, prefix_ntok.numel())
+        held *= prefix.desc.page_tokens
+        a.max_prefix = held if max_prefix is None else max_prefix
+        _want(0 <= a.max_prefix <= held, f"max_prefix: at most the {held} tokens of the pages")
+        if prefix_table is not None:
+            a.prefix_table_dev = _index(prefix_table, None, dev, "prefix_table")
+        if prefix_len is not None:
+            a.prefix_len_dev = _index(prefix_len, 1, dev, "prefix_len")
+    ws, nb = _attn_ws(q, pages.desc.n_head_kv, a.n_seq)
+    _launch(dev, stream, lib.kvmret_prefix_attn, None if prefix is None else ctypes.byref(prefix.desc),
+            None if tail is None else ctypes.byref(tail.desc), ctypes.byref(a), ws.data_ptr(), nb)
+    return got

@@ -78,3 +78,53 @@ def test_paged_append_refuses(args, word):
 def test_paged_append_of_no_tokens():
     assert lib.kvmret_paged_append(ctypes.byref(pages_desc()), None, 0, None, 0, None, None, 0, 1e6,
                                    1.0, 0, None) == 0
+
+
+def attn_args(**kw):
+    a = dict(q_dev=A, q_stride=0, out_dev=A, lse_dev=None, n_q=3, n_head=4, scale=0.1, max_prefix=100,
+             prefix_len_dev=None, prefix_table_dev=None, prefix_ntok_dev=None, n_seq=2, tail_pages=3,
+             q_start_dev=A, tail_table_dev=A, tail_len_dev=A)
+    a.update(kw)
+    return kvmret.AttnArgs(**a)
+
+
+def attn(prefix=None, tail=None, ws=A, ws_bytes=1 << 40, **kw):
+    ref = lambda x: None if x is None else ctypes.byref(x)  # noqa: E731
+    return lib.kvmret_prefix_attn(ref(prefix), ref(tail), ctypes.byref(attn_args(**kw)), ws, ws_bytes, None)
+
+
+@pytest.mark.parametrize("kw,word", BAD_PAGES)
+def test_prefix_attn_refuses_pages(kw, word):
+    for pages in ((pages_desc(**kw), pages_desc()), (pages_desc(), pages_desc(**kw))):
+        assert attn(*pages) == -1 and word in lib.kvmret_last_error()
+
+
+@pytest.mark.parametrize("kw,word", [
+    (dict(n_head=5), b"n_head"), (dict(n_head=0), b"n_head"), (dict(scale=float("inf")), b"scale"),
+    (dict(n_q=65536), b"65535"), (dict(n_seq=70000), b"65535"), (dict(q_dev=None), b"null"),
+    (dict(out_dev=None), b"null"), (dict(q_dev=A + 4), b"aligned"), (dict(q_stride=516), b"aligned"),
+    (dict(q_stride=504), b"overlap"), (dict(q_start_dev=None), b"tails"),
+    (dict(tail_len_dev=None), b"tails"), (dict(tail_table_dev=None), b"tails"),
+    (dict(tail_pages=0), b"tails"), (dict(tail_pages=1 << 27), b"2^31"),
+    (dict(max_prefix=1 << 31), b"max_prefix"), (dict(max_prefix=129), b"max_prefix"),
+    (dict(max_prefix=0, n_seq=0), b"without"),
+])
+def test_prefix_attn_refuses(kw, word):
+    assert attn(pages_desc(), pages_desc(), **kw) == -1 and word in lib.kvmret_last_error()
+
+
+def test_prefix_attn_refuses_mixed_geometry_and_odd_pages():
+    assert attn(pages_desc(), pages_desc(n_head_kv=4)) == -1 and b"prefix of" in lib.kvmret_last_error()
+    assert attn(pages_desc(page_tokens=24), pages_desc(), max_prefix=90) == -1 and b"16 tokens" in lib.kvmret_last_error()
+    assert attn(pages_desc(), pages_desc(page_tokens=8)) == -1 and b"16 tokens" in lib.kvmret_last_error()
+    assert attn(None, pages_desc()) == -1 and attn(pages_desc(), None) == -1
+    assert attn(pages_desc(), pages_desc(), n_q=0, q_dev=None) == 0
+
+
+def test_window_attn_refuses_no_context():
+    assert lib.kvmret_window_attn(None, 0, None, ctypes.byref(attn_args()), None, 0) == -1
+
+
+def test_ws_bytes_of_bad_shapes():
+    for shape in ((1, 3, 2, 128, 1), (1, 4, 0, 128, 1), (1, 4, 2, 96, 1), (70000, 4, 2, 128, 1)):
+        assert lib.kvmret_prefix_attn_ws_bytes(*shape) == 0

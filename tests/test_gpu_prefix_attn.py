@@ -1,0 +1,437 @@
+"""Attention over a shared prefix and each sequence's own tail (prefix_attn,
+Retriever.window_attn) against a float64 softmax of the stored values.
+
+Tolerance, per output row, from the roundings the operator states (scores f32,
+probabilities and quantised values f16, sums f32):
+  dS   the error of a scaled score: 2e-6 of scale * sum |q_i k_i| for f32 sums
+       of f16 products (the bound the GEMM tests use), 2^-22 of the score for
+       forming the exponent; K in quant blocks is rounded to f16 (half a step,
+       2^-11 of scale * sum |q_i k_i|);
+  out  2 dS (numerator and denominator) + 2^-11 (the probability) + 1e-5 (f32
+       sums and joins), all of sum p |v| / sum p; 2^-11 of it more for V in
+       quant blocks; 2^-25 |v| a key for probabilities below f16's normal
+       range (the largest one is at least 1 before the division); the output's
+       own rounding 2^-11 |out| + 2^-25.
+  lse  dS + 2e-6 * (1 + |lse|).
+Unused cells hold NaN.
+"""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import kvmret
+from kvm_helpers import append_history, config_for
+from kvmret import synth
+
+pytestmark = pytest.mark.gpu
+
+F16, Q4, Q8 = kvmret.TYPE_F16, kvmret.TYPE_Q4_0, kvmret.TYPE_Q8_0
+SIZE = {Q8: 34, Q4: 18}
+
+
+def values(raw, kind):
+    """float64 values of a page buffer [pages][page][hkv * d]."""
+    if kind == F16:
+        return raw.astype(np.float64).reshape(*raw.shape[:2], -1)
+    scale = np.ascontiguousarray(raw[..., :2]).view(np.float16).astype(np.float64)
+    body = raw[..., 2:]
+    x = (body.view(np.int8).astype(np.float64) if kind == Q8 else
+         np.concatenate([body & 15, body >> 4], -1).astype(np.float64) - 8)
+    return (scale * x).reshape(*raw.shape[:2], -1)
+
+
+class Pool:
+    """Pages of one kind; every cell unused (NaN) until it is filled."""
+
+    def __init__(self, rng, n, page, hkv, d, kt, vt):
+        self.page, self.hkv, self.d, self.kinds = page, hkv, d, (kt, vt)
+        self.bufs = []
+        for kind in self.kinds:
+            if kind == F16:
+                b = np.full((n, page, hkv, d), np.nan, np.float16)
+            else:
+                b = rng.integers(0, 256, (n, page, hkv * d // 32, SIZE[kind])).astype(np.uint8)
+                b[..., :2] = np.full(1, np.nan, np.float16).view(np.uint8)
+            self.bufs.append(b)
+        self.rng = rng
+
+    def fill(self, pages, length, ntok=None):
+        """Random values for the tokens of a page list; (k, v) float64
+        [tokens][hkv][d]."""
+        got = []
+        for b, kind in zip(self.bufs, self.kinds):
+            rows = []
+            for i, p in enumerate(pages):
+                n = min(self.page, max(0, length - i * self.page))
+                n = n if ntok is None else min(n, ntok[i])
+                if n == 0:
+                    continue
+                if kind == F16:
+                    b[p, :n] = self.rng.standard_normal((n, self.hkv, self.d)).astype(np.float16)
+                else:
+                    top = 127 if kind == Q8 else 8
+                    s = ((self.rng.random(b[p, :n].shape[:-1]) + 0.5) * 2 / top).astype(np.float16)
+                    b[p, :n, :, :2] = s[..., None].view(np.uint8)
+                rows.append(values(b[p:p + 1, :n], kind)[0])
+            got.append(np.concatenate(rows).reshape(-1, self.hkv, self.d) if rows else
+                       np.zeros((0, self.hkv, self.d)))
+        return got
+
+    def device(self):
+        k, v = (torch.from_numpy(b).cuda() for b in self.bufs)
+        return kvmret.Pages(k, v, self.page, self.hkv, self.d, *self.kinds)
+
+
+def softmax64(q, k, v, scale, quant_k, quant_v):
+    """One row of one head: out, lse and their tolerances."""
+    d = q.shape[-1]
+    if k.shape[0] == 0:
+        return np.zeros(d), -np.inf, np.zeros(d), 0.0
+    s = k @ q * scale
+    mag = (np.abs(k) @ np.abs(q)) * abs(scale)
+    top = s.max()
+    p = np.exp(s - top)
+    l = p.sum()
+    ds = ((2e-6 + (2.0 ** -11 if quant_k else 0)) * mag + 2.0 ** -22 * np.abs(s)).max()
+    w = p @ np.abs(v) / l
+    out = p @ v / l
+    tol = (2 * ds + 2.0 ** -11 + 1e-5 + (2.0 ** -11 if quant_v else 0)) * w + \
+        2.0 ** -25 * np.abs(v).sum(0) / l + 2.0 ** -11 * np.abs(out) + 2.0 ** -25
+    return out, top + math.log(l), tol, ds + 2e-6 * (1 + abs(top + math.log(l)))
+
+
+def reference(q, hkv, scale, pre, tails, start, kinds):
+    """q: float64 [n][h][d]; pre, tails[s]: (k, v); the rows of every sequence."""
+    n, h, d = q.shape
+    g = h // hkv
+    out, lse = np.zeros((n, h, d)), np.full((n, h), -np.inf)
+    tol, ltol = np.zeros((n, h, d)), np.zeros((n, h))
+    real = np.zeros(n, bool)
+    spans = [(0, n, None)] if tails is None else \
+        [(start[s], start[s + 1], t) for s, t in enumerate(tails)]
+    for a, b, t in spans:
+        for r in range(a, b):
+            real[r] = True
+            for x in range(h):
+                k, v = (pre[i][:, x // g] for i in (0, 1))
+                if t is not None:
+                    m = max(0, t[0].shape[0] - (b - 1 - r))
+                    k = np.concatenate([k, t[0][:m, x // g]])
+                    v = np.concatenate([v, t[1][:m, x // g]])
+                out[r, x], lse[r, x], tol[r, x], ltol[r, x] = softmax64(
+                    q[r, x], k, v, scale, kinds[0] != F16, kinds[1] != F16)
+    return out, lse, tol, ltol, real
+
+
+def check(got, lse, want):
+    out, wl, tol, ltol, real = want
+    got, lse = got.double().cpu().numpy()[real], lse.double().cpu().numpy()[real]
+    err = np.abs(got - out[real])
+    assert np.all(err <= tol[real]), (err - tol[real]).max()
+    empty = np.isneginf(wl[real])
+    assert np.array_equal(np.isneginf(lse), empty)
+    assert np.all(np.abs(lse - wl[real])[~empty] <= ltol[real][~empty])
+
+
+CASES = [
+    # new tokens, tail lengths, prefix, hq, hkv, d, prefix page, tail page, kt, vt
+    ([1], [1], 1, 1, 1, 64, 16, 16, F16, F16),
+    ([1], [5], 0, 8, 2, 128, 128, 16, F16, F16),            # no prefix
+    ([1, 1, 1], [1, 40, 129], 130, 8, 2, 128, 128, 32, F16, F16),
+    ([1] * 5, [0, 3, 16, 17, 200], 255, 20, 4, 128, 64, 64, F16, F16),  # an empty tail
+    ([3, 0, 5, 1], [3, 9, 4, 30], 100, 16, 2, 128, 32, 16, F16, F16),   # a row before its tail
+    ([2, 1], [2, 0], 0, 4, 4, 64, 16, 16, F16, F16),        # a row that sees nothing
+    ([40], [70], 300, 8, 2, 128, 128, 128, F16, F16),       # rows past one tile
+    ([130], [130], 513, 8, 1, 128, 128, 64, F16, F16),
+    ([300], [411], 140, 2, 2, 64, 48, 48, F16, F16),        # pages of 48 end inside tiles
+    ([7, 6], [144, 20], 700, 16, 4, 256, 144, 16, F16, F16),
+    ([20, 3], [33, 66], 257, 16, 2, 256, 128, 128, F16, F16),
+    ([1] * 17, list(range(1, 18)), 1000, 8, 8, 64, 16, 32, F16, F16),
+    ([1, 4, 2], [1, 100, 64], 333, 8, 2, 128, 128, 32, Q8, Q4),
+    ([1, 1], [64, 31], 200, 16, 4, 64, 32, 32, Q8, Q8),
+    ([5], [90], 129, 5, 1, 256, 64, 64, Q4, Q4),
+    ([2, 2, 2], [2, 200, 70], 150, 8, 2, 128, 48, 16, Q4, F16),
+    ([33], [50], 260, 16, 2, 128, 128, 128, F16, Q8),
+    ([1] * 40, [9] * 40, 2000, 8, 2, 128, 128, 16, F16, F16),
+]
+
+
+def build(case, seed=0):
+    new, tl, prefix, hq, hkv, d, page, tpage, kt, vt = case
+    rng = np.random.default_rng(seed + prefix + d + len(new))
+    n_pre, width = -(-prefix // page) if prefix else 0, max(1, -(-max(tl) // tpage))
+    pool = Pool(rng, n_pre + 2, page, hkv, d, kt, vt)
+    tpool = Pool(rng, width * len(new) + 1, tpage, hkv, d, kt, vt)
+    table = rng.permutation(n_pre + 2)[:n_pre].astype(np.int32)
+    own = rng.permutation(width * len(new) + 1)[:width * len(new)].reshape(len(new), width).astype(
+        np.int32)
+    pre = pool.fill(table, prefix)
+    tails = [tpool.fill(own[s], t) for s, t in enumerate(tl)]
+    start = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+    q = (rng.standard_normal((int(start[-1]), hq, d)) * 1.5).astype(np.float16)
+    return pool, tpool, table, own, pre, tails, start, q, np.array(tl, np.int32)
+
+
+def dev(a):
+    return torch.from_numpy(np.ascontiguousarray(a)).cuda()
+
+
+@pytest.mark.parametrize("case", CASES)
+def test_matches_float64(case):
+    prefix, hkv, d, kinds = case[2], case[4], case[5], case[8:]
+    pool, tpool, table, own, pre, tails, start, q, tl = build(case)
+    # rows of no sequence in front of and behind the batch's, strided
+    n = q.shape[0]
+    rows = torch.full((n + 5, q.shape[1] + 1, d), float("nan"), dtype=torch.float16, device="cuda")
+    rows[2:n + 2, :-1] = dev(q)
+    out = torch.full((n + 5, q.shape[1], d), 7.0, dtype=torch.float16, device="cuda")
+    got, lse = kvmret.prefix_attn(
+        rows[:, :-1], pool.device() if prefix else None, dev(np.array([prefix], np.int32)), tpool.device(),
+        dev(own), dev(tl), dev(start + 2), prefix_table=dev(table) if prefix else None, lse=True, out=out)
+    assert got is out and torch.all(out[:2] == 7) and torch.all(out[n + 2:] == 7)
+    want = reference(q.astype(np.float64), hkv, d ** -0.5, pre, tails, start, kinds)
+    check(out[2:n + 2], lse[2:n + 2], want)
+
+
+@pytest.mark.parametrize("n,prefix,hq,hkv,d,page,kt,vt", [
+    (1, 1, 1, 1, 128, 16, F16, F16), (3, 127, 8, 2, 64, 128, F16, F16),
+    (200, 640, 4, 2, 128, 128, F16, F16), (9, 500, 10, 2, 128, 16, Q8, Q4),
+])
+def test_prefix_alone(n, prefix, hq, hkv, d, page, kt, vt):
+    """No sequences: every row sees the prefix; pages in their own order, the
+    length on the host. A length of zero gives zeros."""
+    rng = np.random.default_rng(n)
+    pool = Pool(rng, -(-prefix // page) + 1, page, hkv, d, kt, vt)
+    pre = pool.fill(np.arange(-(-prefix // page)), prefix)
+    q = rng.standard_normal((n, hq, d)).astype(np.float16)
+    pages = pool.device()
+    got, lse = kvmret.prefix_attn(dev(q), pages, None, max_prefix=prefix, lse=True, scale=0.3)
+    want = reference(q.astype(np.float64), hkv, 0.3, pre, None, None, (kt, vt))
+    check(got, lse, want)
+    none, lse = kvmret.prefix_attn(dev(q), pages, torch.zeros(1, dtype=torch.int32, device="cuda"),
+                                   max_prefix=prefix, lse=True)
+    assert torch.all(none == 0) and torch.all(torch.isneginf(lse))
+
+
+def test_partly_filled_and_absent_pages():
+    """prefix_ntok: pages that hold fewer tokens, in the middle too; page ids
+    outside the pool and tail pages of -1 count as pages without tokens;
+    lengths past the tables are cut, negative ones are none."""
+    rng = np.random.default_rng(5)
+    hq, hkv, d, page = 8, 2, 128, 32
+    pool, tpool = (Pool(rng, 9, page, hkv, d, F16, F16) for _ in range(2))
+    table = np.array([4, 1, 7, 0, 99, 3, -1, 8], np.int32)
+    ntok = np.array([32, 5, 0, 31, 32, 32, 32, 7], np.int32)
+    held = np.where((table >= 0) & (table < 9), ntok, 0)
+    pre = pool.fill(np.where(held > 0, table, 0), 8 * page, held)
+    own = np.array([[2, -1, 5], [6, 0, 1], [-1, -1, -1], [4, 7, 8]], np.int32)
+    lens = np.array([96, 1000, 3, -4], np.int32)
+    tails = []
+    for s, (keep, n) in enumerate((([32, 0, 32], 96), ([32] * 3, 96), ([0] * 3, 3), ([0] * 3, 0))):
+        k, v = tpool.fill(np.maximum(own[s], 0), n, keep)
+        tails.append((k, v))
+    start = np.array([0, 1, 2, 3, 4], np.int32)
+    q = rng.standard_normal((4, hq, d)).astype(np.float16)
+    got, lse = kvmret.prefix_attn(dev(q), pool.device(), None, tpool.device(), dev(own), dev(lens),
+                                  dev(start), prefix_table=dev(table), prefix_ntok=dev(ntok), lse=True)
+    check(got, lse, reference(q.astype(np.float64), hkv, d ** -0.5, pre, tails, start, (F16, F16)))
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.7, 40.0])
+def test_scores_of_any_size(scale):
+    """Equal scores, negative scales, scores in the thousands whose largest
+    comes late or early: no overflow, no loss of the sum."""
+    rng = np.random.default_rng(8)
+    hq, hkv, d, page, n = 4, 1, 128, 64, 900
+    pool = Pool(rng, 15, page, hkv, d, F16, F16)
+    pre = pool.fill(np.arange(15), n)
+    q = rng.standard_normal((6, hq, d)).astype(np.float16)
+    got, lse = kvmret.prefix_attn(dev(q), pool.device(), None, max_prefix=n, lse=True, scale=scale)
+    check(got, lse, reference(q.astype(np.float64), hkv, scale, pre, None, None, (F16, F16)))
+
+
+def test_rising_scores():
+    """Every tile's scores above the last one's: the running maximum moves all
+    the way, in small steps (under a factor of 2^8 a tile) and in large ones."""
+    hq, hkv, d, page, n = 8, 2, 128, 128, 2048
+    rng = np.random.default_rng(9)
+    for step in (0.002, 0.2):
+        pool = Pool(rng, 16, page, hkv, d, F16, F16)
+        pool.fill(np.arange(16), n)
+        ramp = np.arange(n).reshape(16, page)
+        pool.bufs[0][..., :] = (0.05 * pool.bufs[0].astype(np.float32)).astype(np.float16)
+        pool.bufs[0][..., 0] = (ramp * step)[..., None].astype(np.float16)
+        pre = [values(b, F16).reshape(n, hkv, d) for b in pool.bufs]
+        q = rng.standard_normal((3, hq, d)).astype(np.float16)
+        q[..., 0] = 3.0
+        got, lse = kvmret.prefix_attn(dev(q), pool.device(), None, scale=1.0, lse=True)
+        check(got, lse, reference(q.astype(np.float64), hkv, 1.0, pre, None, None, (F16, F16)))
+
+
+def test_far_pages():
+    """Pages whose byte offset passes 32 bits, by the list and in order."""
+    hq, hkv, d, page, n_pages = 8, 8, 128, 128, 17000  # 256 KiB a page
+    k = torch.zeros(n_pages, page, hkv, d, dtype=torch.float16, device="cuda")
+    v = torch.zeros(n_pages, page, hkv, d, dtype=torch.float16, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(1)
+    at = torch.tensor([16999, 3], device="cuda", dtype=torch.int32)
+    k[at.long()] = torch.randn(2, page, hkv, d, device="cuda", generator=g).half()
+    v[at.long()] = torch.randn(2, page, hkv, d, device="cuda", generator=g).half()
+    q = torch.randn(2, hq, d, device="cuda", generator=g).half()
+    big = kvmret.Pages(k, v, page, hkv, d)
+    small = kvmret.Pages(k[at.long()], v[at.long()], page, hkv, d)
+    args = (torch.tensor([[0], [1]], device="cuda", dtype=torch.int32),
+            torch.tensor([100, 128], device="cuda", dtype=torch.int32),
+            torch.tensor([0, 1, 2], device="cuda", dtype=torch.int32))
+    want = kvmret.prefix_attn(q, small, None, small, *args)
+    got = kvmret.prefix_attn(q, big, None, big, at[:, None].contiguous(), *args[1:], prefix_table=at)
+    assert torch.equal(got, want)
+
+
+def test_repeats_bit_for_bit_and_across_streams():
+    case = ([1] * 9 + [30], [50] * 9 + [300], 3000, 16, 4, 128, 128, 32, F16, F16)
+    pool, tpool, table, own, _, _, start, q, tl = build(case)
+    args = (dev(q), pool.device(), dev(np.array([3000], np.int32)), tpool.device(), dev(own), dev(tl),
+            dev(start))
+    first = kvmret.prefix_attn(*args, prefix_table=dev(table))
+    t = dev(table)
+    side = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    got = []
+    for s in side:  # calls under way at once, each with its workspace
+        with torch.cuda.stream(s):
+            got += [kvmret.prefix_attn(*args, prefix_table=t) for _ in range(3)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, first) for x in got)
+
+
+def test_captured_call_follows_lengths_and_tables():
+    case = ([1, 1, 2], [9, 40, 77], 600, 8, 2, 128, 64, 32, F16, F16)
+    pool, tpool, table, own, pre, tails, start, q, tl = build(case)
+    pages, tpages = pool.device(), tpool.device()
+    qd, length, own_d, tl_d, start_d, table_d = (dev(q), dev(np.array([600], np.int32)), dev(own),
+                                                 dev(tl), dev(start), dev(table))
+    call = lambda: kvmret.prefix_attn(qd, pages, length, tpages, own_d, tl_d, start_d,  # noqa: E731
+                                      prefix_table=table_d, lse=True)
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got, lse = call()
+    for cut, lens, at in ((600, [9, 40, 77], start), (33, [1, 40, 12], start), (0, [9, 5, 77], [0, 2, 3, 4])):
+        length.fill_(cut)
+        tl_d.copy_(torch.tensor(lens, dtype=torch.int32))
+        start_d.copy_(torch.tensor(list(at), dtype=torch.int32))
+        qd.copy_(torch.randn_like(qd))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = reference(qd.double().cpu().numpy(), 2, 128 ** -0.5, [x[:cut] for x in pre],
+                         [(k[:n], v[:n]) for (k, v), n in zip(tails, lens)], list(at), (F16, F16))
+        check(got, lse, want)
+
+
+@pytest.mark.parametrize("quant", [False, True])
+def test_step_around_a_window(quant):
+    """A step as a user runs it, on one layer's tensors: norms and rotations,
+    the retrieval's own append and query, the window, the new tokens of three
+    branches filed into their pages, attention over the window and the tails.
+    The window's and the pages' bytes give the float64 answer."""
+    w = synth.Workload("step", n_layer=2, n_head=8, n_head_kv=2, d_head=128, block_tokens=64,
+                       n_blocks=24, budget_blocks=6, sink_blocks=1, reserve_blocks=2, n_planted=3,
+                       seed=77)
+    kt, vt = (Q8, Q4) if quant else (F16, F16)
+    hist = synth.NumpyHistory(w)
+    r = kvmret.Retriever(config_for(w, k_type=kt, v_type=vt))
+    n0 = w.n_tokens - 41  # a partial newest block
+    fn = {}
+    if quant:
+        def rows(kind):
+            return lambda x: kvmret.quantize_f16(dev(x.reshape(-1, w.E)), kind).cpu().numpy().reshape(
+                x.shape[0], x.shape[1], -1)
+        fn = dict(k_rows_fn=rows(Q8), v_rows_fn=rows(Q4))
+    append_history(r, hist, cuts=[], stop=n0, **fn)
+    g = torch.Generator(device="cuda").manual_seed(11)
+    hq, hkv, d, T = 8, 2, 128, 64
+    proj = torch.randn(3, hq + 2 * hkv, d, device="cuda", generator=g).half()
+    wq = 1 + 0.1 * torch.randn(d, device="cuda", generator=g)
+    fw = d if quant else 0
+    # the unrotated queries steer the retrieval
+    zero = torch.zeros(3, dtype=torch.int32, device="cuda")
+    _, _, q_raw, k_raw = kvmret.qk_norm_rope(proj[:, :hq], proj[:, hq:hq + hkv], zero, wq, wq,
+                                             q_rot=False, k_rot=False, q_raw=True, k_raw=True)
+    r.query_reset()
+    r.query_add(q_raw.reshape(1, 3, -1).expand(w.n_layer, 3, hq * d).contiguous())
+    r.score()
+    r.select_apply_async()
+    # the newest block's tokens beyond what the window's plan saw: gen mode
+    # binds it (or a new slot) and writes them in
+    ids, st = r.step_collect()
+    base = st["total_window_tokens"]
+    tails = kvmret.Pages(*(torch.zeros(7, 16 * kvmret.row_bytes(t, hkv * d), dtype=torch.uint8,
+                                       device="cuda") for t in (kt, vt)), 16, hkv, d, kt, vt)
+    own = torch.tensor([[2, 5], [0, 3], [6, 1]], dtype=torch.int32, device="cuda")
+    start = torch.arange(4, dtype=torch.int32, device="cuda")
+    lens = torch.zeros(3, dtype=torch.int32, device="cuda")
+    for step in range(18):  # past the first page
+        pos = base + lens
+        cells = own.gather(1, (lens // 16).long()[:, None])[:, 0] * 16 + lens % 16
+        proj = torch.randn(3, hq + 2 * hkv, d, device="cuda", generator=g).half()
+        q_rot, _, _, k_raw = kvmret.qk_norm_rope(proj[:, :hq], proj[:, hq:hq + hkv], pos, wq, wq,
+                                                 fwht_n=fw, k_rot=False, k_raw=True)
+        kvmret.paged_append(tails, k_raw, proj[:, hq + hkv:], cells, pos, fwht_n=fw)
+        lens += 1
+        got, lse = r.window_attn(1, q_rot, tails, own, lens, start, lse=True)
+    lay, bases = r.window_layout()
+    n_tok = [min(T, n0 - int(b) * T) for b in lay]
+    assert sum(n_tok) == base
+
+    def stored(buf, kind):
+        return values(buf.view(np.float16) if kind == F16 else buf, kind)
+
+    pre = []
+    for is_v, kind in ((False, kt), (True, vt)):
+        b = r.window_read(1, is_v, 0, len(lay))
+        b = b.view(np.float16).reshape(len(lay), T, -1) if kind == F16 else b.reshape(
+            len(lay), T, -1, SIZE[kind])
+        x = values(b, kind)
+        pre.append(np.concatenate([x[i, :n] for i, n in enumerate(n_tok)]).reshape(-1, hkv, d))
+    own_h, tail_vals = own.cpu().numpy(), []
+    for s in range(3):
+        kv = []
+        for buf, kind in ((tails.k, kt), (tails.v, vt)):
+            b = buf.cpu().numpy()[own_h[s]]
+            b = b.view(np.float16).reshape(2, 16, -1) if kind == F16 else b.reshape(2, 16, -1, SIZE[kind])
+            kv.append(values(b, kind).reshape(-1, hkv, d)[:18])
+        tail_vals.append(kv)
+    want = reference(q_rot.double().cpu().numpy(), hkv, d ** -0.5, pre, tail_vals, [0, 1, 2, 3], (kt, vt))
+    check(got, lse, want)
+    # a cleared working set: the tails alone
+    r.clear_working_set()
+    got, lse = r.window_attn(0, q_rot, tails, own, lens, start, lse=True)
+    none = [np.zeros((0, hkv, d))] * 2
+    check(got, lse, reference(q_rot.double().cpu().numpy(), hkv, d ** -0.5, none, tail_vals, [0, 1, 2, 3],
+                              (kt, vt)))
+    r.close()
+
+
+def test_wrapper_refusals():
+    z = lambda *s, dt=torch.float16: torch.zeros(*s, dtype=dt, device="cuda")  # noqa: E731
+    i = lambda *s: z(*s, dt=torch.int32)  # noqa: E731
+    p = kvmret.Pages(z(4, 16, 2, 128), z(4, 16, 2, 128), 16, 2, 128)
+    odd = kvmret.Pages(z(4, 12, 2, 128), z(4, 12, 2, 128), 12, 2, 128)
+    other = kvmret.Pages(z(4, 16, 4, 64), z(4, 16, 4, 64), 16, 4, 64)
+    q = z(3, 4, 128)
+    for call in (
+            lambda: kvmret.prefix_attn(q.float(), p, None), lambda: kvmret.prefix_attn(z(3, 4, 64), p, None),
+            lambda: kvmret.prefix_attn(z(3, 3, 128), p, None), lambda: kvmret.prefix_attn(q, odd, None),
+            lambda: kvmret.prefix_attn(q, p, None, max_prefix=65), lambda: kvmret.prefix_attn(q, None, None),
+            lambda: kvmret.prefix_attn(q, p, None, p), lambda: kvmret.prefix_attn(q, p, i(2)),
+            lambda: kvmret.prefix_attn(q, p, None, p, i(2, 2), i(3), i(3)),
+            lambda: kvmret.prefix_attn(q, p, None, other, i(2, 2), i(2), i(3)),
+            lambda: kvmret.prefix_attn(q, p, None, out=z(3, 4, 64)),
+            lambda: kvmret.prefix_attn(q, p, None, scale=float("nan"))):
+        with pytest.raises(kvmret.KvmretError):
+            call()
+    assert kvmret.prefix_attn(z(0, 4, 128), p, None).shape == (0, 4, 128)
