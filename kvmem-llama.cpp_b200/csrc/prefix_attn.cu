@@ -129,9 +129,7 @@ __global__ void __launch_bounds__(32 * kWarps) attn_kernel(const __grid_constant
 
 }  // namespace
 
-size_t prefix_attn_ws_bytes(uint32_t, uint32_t, uint32_t, uint32_t, uint32_t) { return 0; }
-
-cudaError_t launch_prefix_attn(const PrefixAttn &a, void *, cudaStream_t st) {
+cudaError_t launch_prefix_attn_rows(const PrefixAttn &a, cudaStream_t st) {
     const dim3 grid(a.n_q, a.n_head);
     if (a.d_head == 64)
         attn_kernel<64><<<grid, 32 * kWarps, 0, st>>>(a);

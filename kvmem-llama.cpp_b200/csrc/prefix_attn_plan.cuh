@@ -1,0 +1,203 @@
+// Work split of the shared-prefix attention, computed on the device from the
+// lengths and read alike by the attention kernel and by the join.
+//
+// Rows: the G = n_head / n_head_kv query heads of a KV head stand as rows
+// r = token * G + head beside one another, so one tile of keys serves all of
+// them. A unit is (KV head, up to PR rows) against one key list; its keys go by
+// tiles of BN. The units' tiles, laid end to end, are cut into equal
+// contiguous ranges, one per CTA, so a long list is shared by many CTAs and a
+// short one by none; each (unit, CTA) piece leaves its unnormalised output,
+// maximum and sum in a workspace slot, and the join adds a row's pieces in a
+// fixed order, so results repeat run to run.
+//   Prefix: when a KV head has more than PR rows (n_pair > 1), `gs` CTAs walk
+//     the same keys side by side, one row pair each, so that all but one of
+//     them find the tile in L2; the ranges are then per group of gs CTAs.
+//   Tails: units (sequence, row pair, KV head) in that order.
+// With gs == 1 prefix and tails form one line; otherwise each has its own.
+#pragma once
+
+#include "prefix_attn.cuh"
+
+namespace kvmret {
+namespace {
+
+// Key tiles of a list with pages of T tokens: a page of at least BN tokens is
+// ceil(T / BN) tiles, else BN / T whole pages make one.
+template <int BN>
+struct TileGeom {
+    uint32_t T, tpp, ppt;  // page tokens, tiles per page (T >= BN), pages per tile (T < BN)
+    __device__ __forceinline__ explicit TileGeom(uint32_t t)
+        : T(t), tpp(t >= BN ? (t + BN - 1) / BN : 1), ppt(t >= BN ? 1 : BN / t) {}
+    __device__ __forceinline__ uint32_t tiles(uint32_t len) const {
+        if (T < BN) return (len + ppt * T - 1) / (ppt * T);
+        const uint32_t full = len / T, rem = len - full * T;
+        return full * tpp + (rem + BN - 1) / BN;
+    }
+    __device__ __forceinline__ void locate(uint32_t tile, uint32_t &page, uint32_t &off) const {
+        if (T < BN) {
+            page = tile * ppt;
+            off = 0;
+        } else {
+            page = tile / tpp;
+            off = (tile - page * tpp) * BN;
+        }
+    }
+};
+
+// The header of the workspace.
+struct Plan {
+    uint64_t p_total, t_total;  // tiles of the prefix line and of the tails
+    uint32_t np;                // tiles of the prefix
+    uint32_t p_len;             // its tokens
+    uint32_t q0, rows;          // first row token; rows of a KV head (all sequences)
+    uint32_t n_pair, n_pg, gs, groups;
+    uint32_t t_slot0;           // first workspace slot of the tails
+};
+
+__device__ __forceinline__ uint64_t cut(uint64_t total, uint32_t i, uint32_t n) {
+    return total * i / n;
+}
+// the range that holds x (x < total)
+__device__ __forceinline__ uint32_t owner(uint64_t x, uint64_t total, uint32_t n) {
+    const uint64_t g = x * n / total;
+    uint32_t i = g < n - 1 ? static_cast<uint32_t>(g) : n - 1;
+    while (i + 1 < n && cut(total, i + 1, n) <= x) ++i;
+    while (i > 0 && cut(total, i, n) > x) --i;
+    return i;
+}
+
+// Rows and keys of one sequence, all cut to what the host's bounds allow.
+struct SeqShape {
+    uint32_t q0, q_len, len;
+};
+__device__ __forceinline__ SeqShape seq_shape(const PrefixAttn &a, uint32_t s) {
+    SeqShape r;
+    const int32_t n = static_cast<int32_t>(a.n_q);
+    const int32_t q0 = min(max(__ldg(a.q_start + s), 0), n);
+    const int32_t q1 = min(max(__ldg(a.q_start + s + 1), q0), n);
+    r.q0 = static_cast<uint32_t>(q0);
+    r.q_len = static_cast<uint32_t>(q1 - q0);
+    r.len = min(static_cast<uint32_t>(max(__ldg(a.tail.len + s), 0)), a.tail.max_len);
+    return r;
+}
+// tail tokens that row token i of the sequence sees
+__device__ __forceinline__ uint32_t tail_seen(const SeqShape &s, uint32_t i) {
+    const uint32_t after = s.q_len - 1 - i;
+    return s.len > after ? s.len - after : 0;
+}
+// tiles of a tail that the rows of a pair reach
+template <int BN, int PR>
+__device__ __forceinline__ uint32_t pair_tiles(const SeqShape &s, const TileGeom<BN> &g,
+                                               uint32_t pair, uint32_t G) {
+    const uint32_t last = min(s.q_len - 1, (pair * PR + PR - 1) / G);
+    return g.tiles(tail_seen(s, last));
+}
+
+// One piece of work of a CTA.
+struct Seg {
+    bool tail;
+    uint32_t seq, h, q0, row0, rows;  // rows [row0, row0 + rows) of the unit's tokens from q0
+    uint32_t tile0, n;                // key tiles
+    uint32_t slot;
+};
+
+template <int BN, int PR>
+struct Walk {
+    const PrefixAttn &a;
+    const Plan &p;
+    uint32_t G, cta, n_cta;
+    uint64_t x, x1;       // prefix line: next tile, end
+    uint32_t part, lane;  // the range and the CTA's place in its group
+    uint64_t y, y1;       // tails' line
+    uint32_t seq;         // the sequence that holds y, its first tile and pair
+    uint64_t seq_tile;
+    uint32_t seq_pair;
+    SeqShape sh;
+    bool fresh;
+
+    __device__ __forceinline__ Walk(const PrefixAttn &a_, const Plan &p_, uint32_t s, uint64_t tile,
+                                    uint32_t pair)
+        : a(a_), p(p_), G(a_.n_head / a_.n_head_kv), cta(blockIdx.x), n_cta(gridDim.x), seq(s),
+          seq_tile(tile), seq_pair(pair), fresh(true) {
+        ranges(p, cta, n_cta, x, x1, y, y1);
+        part = cta / p.gs;
+        lane = cta - part * p.gs;
+    }
+    static __device__ __forceinline__ void ranges(const Plan &p, uint32_t cta, uint32_t n_cta,
+                                                  uint64_t &x, uint64_t &x1, uint64_t &y,
+                                                  uint64_t &y1) {
+        if (p.gs == 1) {
+            const uint64_t all = p.p_total + p.t_total;
+            const uint64_t b = cut(all, cta, n_cta), e = cut(all, cta + 1, n_cta);
+            x = min(b, p.p_total);
+            x1 = min(e, p.p_total);
+            y = max(b, p.p_total) - p.p_total;
+            y1 = max(e, p.p_total) - p.p_total;
+        } else {
+            const uint32_t part = cta / p.gs;
+            x = part < p.groups ? cut(p.p_total, part, p.groups) : 0;
+            x1 = part < p.groups ? cut(p.p_total, part + 1, p.groups) : 0;
+            y = cut(p.t_total, cta, n_cta);
+            y1 = cut(p.t_total, cta + 1, n_cta);
+        }
+    }
+
+    __device__ __forceinline__ bool next(Seg &g) {
+        while (x < x1) {
+            const uint64_t u = x / p.np;
+            const uint32_t t = static_cast<uint32_t>(x - u * p.np);
+            const uint32_t n = static_cast<uint32_t>(min(x1 - x, static_cast<uint64_t>(p.np - t)));
+            x += n;
+            const uint32_t pair = static_cast<uint32_t>(u / a.n_head_kv) * p.gs + lane;
+            if (pair >= p.n_pair) continue;
+            g.tail = false;
+            g.seq = 0;
+            g.h = static_cast<uint32_t>(u % a.n_head_kv);
+            g.q0 = p.q0;
+            g.row0 = pair * PR;
+            g.rows = min(static_cast<uint32_t>(PR), p.rows - g.row0);
+            g.tile0 = t;
+            g.n = n;
+            g.slot = (static_cast<uint32_t>(u) + part) * p.gs + lane;
+            return true;
+        }
+        const TileGeom<BN> geom(a.tail.pages.page_tokens);
+        while (y < y1 && seq < a.n_seq) {
+            if (fresh) sh = seq_shape(a, seq);
+            fresh = false;
+            const uint32_t tiles = sh.q_len ? geom.tiles(sh.len) : 0;
+            const uint32_t pairs = (sh.q_len * G + PR - 1) / PR;
+            const uint64_t mine = static_cast<uint64_t>(tiles) * pairs * a.n_head_kv;
+            if (y >= seq_tile + mine) {
+                seq_tile += mine;
+                seq_pair += pairs;
+                ++seq;
+                fresh = true;
+                continue;
+            }
+            const uint64_t at = y - seq_tile;
+            const uint32_t u = static_cast<uint32_t>(at / tiles);
+            const uint32_t t = static_cast<uint32_t>(at - static_cast<uint64_t>(u) * tiles);
+            uint32_t n = static_cast<uint32_t>(min(y1 - y, static_cast<uint64_t>(tiles - t)));
+            y += n;
+            const uint32_t pair = u / a.n_head_kv;
+            const uint32_t lim = pair_tiles<BN, PR>(sh, geom, pair, G);
+            if (t >= lim) continue;
+            n = min(n, lim - t);
+            g.tail = true;
+            g.seq = seq;
+            g.h = u - pair * a.n_head_kv;
+            g.q0 = sh.q0;
+            g.row0 = pair * PR;
+            g.rows = min(static_cast<uint32_t>(PR), sh.q_len * G - g.row0);
+            g.tile0 = t;
+            g.n = n;
+            g.slot = p.t_slot0 + seq_pair * a.n_head_kv + u + cta;
+            return true;
+        }
+        return false;
+    }
+};
+
+}  // namespace
+}  // namespace kvmret
