@@ -44,27 +44,37 @@ struct TileGeom {
     }
 };
 
+// Quotient of tile counts: 32-bit division where both fit.
+__device__ __forceinline__ uint64_t quot(uint64_t x, uint64_t d) {
+    return ((x | d) >> 32) ? x / d : static_cast<uint32_t>(x) / static_cast<uint32_t>(d);
+}
+
+// A line of tiles cut into `parts` ranges: the first r of them hold q + 1.
+struct Cuts {
+    uint64_t q;
+    uint32_t r;
+    __device__ __forceinline__ void set(uint64_t total, uint32_t parts) {
+        q = quot(total, parts);
+        r = static_cast<uint32_t>(total - q * parts);
+    }
+    __device__ __forceinline__ uint64_t at(uint32_t i) const { return q * i + min(i, r); }
+    // the range that holds tile x of the line
+    __device__ __forceinline__ uint32_t owner(uint64_t x) const {
+        const uint64_t head = (q + 1) * r;
+        return static_cast<uint32_t>(x < head ? quot(x, q + 1) : r + quot(x - head, q));
+    }
+};
+
 // The header of the workspace.
 struct Plan {
     uint64_t p_total, t_total;  // tiles of the prefix line and of the tails
+    Cuts pre, own;              // their ranges (gs == 1: of the joint line)
     uint32_t np;                // tiles of the prefix
     uint32_t p_len;             // its tokens
     uint32_t q0, rows;          // first row token; rows of a KV head (all sequences)
     uint32_t n_pair, n_pg, gs, groups;
     uint32_t t_slot0;           // first workspace slot of the tails
 };
-
-__device__ __forceinline__ uint64_t cut(uint64_t total, uint32_t i, uint32_t n) {
-    return total * i / n;
-}
-// the range that holds x (x < total)
-__device__ __forceinline__ uint32_t owner(uint64_t x, uint64_t total, uint32_t n) {
-    const uint64_t g = x * n / total;
-    uint32_t i = g < n - 1 ? static_cast<uint32_t>(g) : n - 1;
-    while (i + 1 < n && cut(total, i + 1, n) <= x) ++i;
-    while (i > 0 && cut(total, i, n) > x) --i;
-    return i;
-}
 
 // Rows and keys of one sequence, all cut to what the host's bounds allow.
 struct SeqShape {
@@ -81,31 +91,33 @@ __device__ __forceinline__ SeqShape seq_shape(const PrefixAttn &a, uint32_t s) {
     return r;
 }
 // tail tokens that row token i of the sequence sees
-__device__ __forceinline__ uint32_t tail_seen(const SeqShape &s, uint32_t i) {
-    const uint32_t after = s.q_len - 1 - i;
-    return s.len > after ? s.len - after : 0;
+__device__ __forceinline__ uint32_t tail_seen(uint32_t len, uint32_t q_len, uint32_t i) {
+    const uint32_t after = q_len - 1 - i;
+    return len > after ? len - after : 0;
 }
 // tiles of a tail that the rows of a pair reach
 template <int BN, int PR>
 __device__ __forceinline__ uint32_t pair_tiles(const SeqShape &s, const TileGeom<BN> &g,
                                                uint32_t pair, uint32_t G) {
     const uint32_t last = min(s.q_len - 1, (pair * PR + PR - 1) / G);
-    return g.tiles(tail_seen(s, last));
+    return g.tiles(tail_seen(s.len, s.q_len, last));
 }
 
 // One piece of work of a CTA.
 struct Seg {
-    bool tail;
-    uint32_t seq, h, q0, row0, rows;  // rows [row0, row0 + rows) of the unit's tokens from q0
-    uint32_t tile0, n;                // key tiles
+    uint32_t tail, seq, h;
+    uint32_t q0, row0, rows;  // rows [row0, row0 + rows) of the unit's tokens from q0
+    uint32_t len, q_len;      // the list's tokens; a tail's new ones
+    uint32_t tile0, n;        // key tiles (n == 0: no more pieces)
+    uint32_t j0;              // tiles of the CTA's pieces before this one
     uint32_t slot;
 };
 
 template <int BN, int PR>
 struct Walk {
     const PrefixAttn &a;
-    const Plan &p;
-    uint32_t G, cta, n_cta;
+    const Plan &p;  // in shared memory
+    uint32_t G, cta;
     uint64_t x, x1;       // prefix line: next tile, end
     uint32_t part, lane;  // the range and the CTA's place in its group
     uint64_t y, y1;       // tails' line
@@ -117,42 +129,42 @@ struct Walk {
 
     __device__ __forceinline__ Walk(const PrefixAttn &a_, const Plan &p_, uint32_t s, uint64_t tile,
                                     uint32_t pair)
-        : a(a_), p(p_), G(a_.n_head / a_.n_head_kv), cta(blockIdx.x), n_cta(gridDim.x), seq(s),
+        : a(a_), p(p_), G(a_.n_head / a_.n_head_kv), cta(blockIdx.x), seq(s),
           seq_tile(tile), seq_pair(pair), fresh(true) {
-        ranges(p, cta, n_cta, x, x1, y, y1);
+        ranges(p, cta, x, x1, y, y1);
         part = cta / p.gs;
         lane = cta - part * p.gs;
     }
-    static __device__ __forceinline__ void ranges(const Plan &p, uint32_t cta, uint32_t n_cta,
-                                                  uint64_t &x, uint64_t &x1, uint64_t &y,
-                                                  uint64_t &y1) {
+    static __device__ __forceinline__ void ranges(const Plan &p, uint32_t cta, uint64_t &x,
+                                                  uint64_t &x1, uint64_t &y, uint64_t &y1) {
         if (p.gs == 1) {
-            const uint64_t all = p.p_total + p.t_total;
-            const uint64_t b = cut(all, cta, n_cta), e = cut(all, cta + 1, n_cta);
+            const uint64_t b = p.pre.at(cta), e = p.pre.at(cta + 1);
             x = min(b, p.p_total);
             x1 = min(e, p.p_total);
             y = max(b, p.p_total) - p.p_total;
             y1 = max(e, p.p_total) - p.p_total;
         } else {
             const uint32_t part = cta / p.gs;
-            x = part < p.groups ? cut(p.p_total, part, p.groups) : 0;
-            x1 = part < p.groups ? cut(p.p_total, part + 1, p.groups) : 0;
-            y = cut(p.t_total, cta, n_cta);
-            y1 = cut(p.t_total, cta + 1, n_cta);
+            x = part < p.groups ? p.pre.at(part) : 0;
+            x1 = part < p.groups ? p.pre.at(part + 1) : 0;
+            y = p.own.at(cta);
+            y1 = p.own.at(cta + 1);
         }
     }
 
     __device__ __forceinline__ bool next(Seg &g) {
         while (x < x1) {
-            const uint64_t u = x / p.np;
+            const uint64_t u = quot(x, p.np);
             const uint32_t t = static_cast<uint32_t>(x - u * p.np);
             const uint32_t n = static_cast<uint32_t>(min(x1 - x, static_cast<uint64_t>(p.np - t)));
             x += n;
-            const uint32_t pair = static_cast<uint32_t>(u / a.n_head_kv) * p.gs + lane;
+            const uint32_t pair = static_cast<uint32_t>(quot(u, a.n_head_kv)) * p.gs + lane;
             if (pair >= p.n_pair) continue;
-            g.tail = false;
+            g.tail = 0;
             g.seq = 0;
-            g.h = static_cast<uint32_t>(u % a.n_head_kv);
+            g.len = p.p_len;
+            g.q_len = 0;
+            g.h = static_cast<uint32_t>(u - quot(u, a.n_head_kv) * a.n_head_kv);
             g.q0 = p.q0;
             g.row0 = pair * PR;
             g.rows = min(static_cast<uint32_t>(PR), p.rows - g.row0);
@@ -176,7 +188,7 @@ struct Walk {
                 continue;
             }
             const uint64_t at = y - seq_tile;
-            const uint32_t u = static_cast<uint32_t>(at / tiles);
+            const uint32_t u = static_cast<uint32_t>(quot(at, tiles));
             const uint32_t t = static_cast<uint32_t>(at - static_cast<uint64_t>(u) * tiles);
             uint32_t n = static_cast<uint32_t>(min(y1 - y, static_cast<uint64_t>(tiles - t)));
             y += n;
@@ -184,8 +196,10 @@ struct Walk {
             const uint32_t lim = pair_tiles<BN, PR>(sh, geom, pair, G);
             if (t >= lim) continue;
             n = min(n, lim - t);
-            g.tail = true;
+            g.tail = 1;
             g.seq = seq;
+            g.len = sh.len;
+            g.q_len = sh.q_len;
             g.h = u - pair * a.n_head_kv;
             g.q0 = sh.q0;
             g.row0 = pair * PR;
@@ -197,6 +211,23 @@ struct Walk {
         }
         return false;
     }
+};
+
+// The tiles of a piece that stream s takes: with more than 128 rows both streams
+// take every tile (a row tile each), otherwise stream s takes those whose number
+// in the CTA's order has parity s. Two tiles in a row of one stream are then at
+// most two apart in that order.
+template <int NS>
+struct Share {
+    uint32_t tile, step, end;  // in the CTA's order
+    bool both;
+    __device__ __forceinline__ void set(const Seg &g, uint32_t s) {
+        both = NS == 2 && g.rows > 128;
+        step = NS == 1 || both ? 1 : 2;
+        tile = step == 1 ? g.j0 : g.j0 + ((g.j0 ^ s) & 1u);
+        end = g.j0 + g.n;
+    }
+    __device__ __forceinline__ bool any() const { return tile < end; }
 };
 
 }  // namespace

@@ -13,6 +13,7 @@
 //   0      producer: page list, the tile's mask of valid keys, TMA loads of K
 //          and V tiles into a ring of shared-memory stages (128-byte swizzle,
 //          no multicast);
+//   2      walks the pieces and leaves each in a short ring for the others;
 //   1      one lane issues the products: S = Q K^T (both in shared memory)
 //          and O += P V (P in tensor memory over its S, V as it lies: keys
 //          along K, MN-major);
@@ -57,6 +58,7 @@ struct Cfg {
     static __host__ __device__ constexpr uint32_t o_col(int s) { return 256 + s * (D == 64 ? 64 : 128); }
 };
 constexpr uint32_t kAttnTmem = 512;
+constexpr int kSegs = 4;  // pieces ahead
 constexpr int kMeta = 8;  // tiles whose masks are held (more than the ring reaches back)
 
 struct AttnLaunch {
@@ -94,8 +96,55 @@ __device__ __forceinline__ void tmem_ld32_nowait(uint32_t taddr, uint32_t *r) {
           "=r"(r[31])
         : "r"(taddr));
 }
-__device__ __forceinline__ void tmem_ld_wait() {
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32"
+        " {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+          "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]),
+                   "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]),
+                   "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0],"
+        " {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+// Two products and two sums at a time (each rounded like the scalar operation).
+__device__ __forceinline__ void fma_pair(uint32_t &x, uint32_t &y, float a, float b) {
+    asm("{\n\t.reg .b64 p, q, r;\n\t"
+        "mov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %2};\n\tmov.b64 r, {%3, %3};\n\t"
+        "fma.rn.f32x2 p, p, q, r;\n\tmov.b64 {%0, %1}, p;\n\t}"
+        : "+r"(x), "+r"(y)
+        : "f"(a), "f"(b));
+}
+__device__ __forceinline__ void add_pair(float &x, float &y, float a, float b) {
+    asm("{\n\t.reg .b64 p, q;\n\t"
+        "mov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %3};\n\t"
+        "add.rn.f32x2 p, p, q;\n\tmov.b64 {%0, %1}, p;\n\t}"
+        : "+f"(x), "+f"(y)
+        : "f"(a), "f"(b));
+}
+// The wait for loads under way; it names the registers, so that nothing that
+// reads them can be moved before it.
+__device__ __forceinline__ void tmem_ld_wait(uint32_t *r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]),
+                   "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]),
+                   "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]),
+                   "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]),
+                   "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
 }
 
 // Instruction descriptor: D f32, A and B f16, M = 128, N; B K-major or MN-major.
@@ -107,8 +156,8 @@ __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint3
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(id), "r"(accumulate), "r"(0u)
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b),
+        "r"(id), "r"(accumulate)
         : "memory");
 }
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id,
@@ -116,44 +165,62 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(id), "r"(accumulate), "r"(0u)
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b),
+        "r"(id), "r"(accumulate)
         : "memory");
 }
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(p));
+    return p;
+}
 
-// Block-wide plan of the split, in every CTA alike; CTA 0 also leaves it and
-// the sequences' offsets in the workspace for the join. `start` receives the
-// sequence that holds the CTA's first tail tile.
+// The plan of the split, by one warp, in every CTA alike; CTA 0 also leaves it
+// and the sequences' offsets in the workspace for the join. `start` receives
+// the sequence that holds the CTA's first tail tile.
 struct Start {
     uint32_t seq, pair;
     uint64_t tile;
 };
 template <int D>
-__device__ void make_plan(const AttnLaunch &l, Plan &p, Start &start, uint32_t &fail,
-                          uint64_t (&red)[2][16]) {
+__device__ bool make_plan(const AttnLaunch &l, Plan &p, Start &start) {
     constexpr int BN = Cfg<D>::BN, PR = Cfg<D>::PR;
     const PrefixAttn &a = l.a;
-    const uint32_t tid = threadIdx.x, nthr = blockDim.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t lane = threadIdx.x & 31;
     const uint32_t G = a.n_head / a.n_head_kv, H = a.n_head_kv;
     const TileGeom<BN> tg(a.n_seq ? a.tail.pages.page_tokens : BN);
     auto shape = [&](uint32_t s, uint64_t &tiles, uint32_t &pairs) {
+        tiles = 0;
+        pairs = 0;
+        if (s >= a.n_seq) return;
         const SeqShape sh = seq_shape(a, s);
         pairs = (sh.q_len * G + PR - 1) / PR;
         tiles = static_cast<uint64_t>(sh.q_len ? tg.tiles(sh.len) : 0) * pairs * H;
     };
+    const bool pre = a.prefix.max_len != 0;
+    const int32_t len0 = pre && a.prefix.len ? __ldg(a.prefix.len) : 0x7fffffff;
+    const int32_t q_first = a.n_seq ? __ldg(a.q_start) : 0;
+    const int32_t q_last = a.n_seq ? __ldg(a.q_start + a.n_seq) : static_cast<int32_t>(a.n_q);
     // totals of the tails; the last listed page that holds tokens
-    uint64_t tiles = 0, pairs = 0;
-    for (uint32_t s = tid; s < a.n_seq; s += nthr) {
+    uint64_t tiles = 0, pairs = 0, t0;
+    uint32_t n0;
+    shape(lane, t0, n0);
+    tiles = t0;
+    pairs = n0;
+#pragma unroll 4
+    for (uint32_t s = 32 + lane; s < a.n_seq; s += 32) {
         uint64_t t;
         uint32_t n;
         shape(s, t, n);
         tiles += t;
         pairs += n;
     }
-    uint32_t held = a.prefix.max_len ? a.prefix.n_list : 0;
+    uint32_t held = pre ? a.prefix.n_list : 0;
     if (held && a.prefix.ntok) {
         held = 0;
-        for (uint32_t i = tid; i < a.prefix.n_list; i += nthr)
+#pragma unroll 8
+        for (uint32_t i = lane; i < a.prefix.n_list; i += 32)
             if (__ldg(a.prefix.ntok + i)) held = i + 1;
     }
     for (int o = 16; o; o >>= 1) {
@@ -161,101 +228,78 @@ __device__ void make_plan(const AttnLaunch &l, Plan &p, Start &start, uint32_t &
         pairs += __shfl_xor_sync(0xffffffffu, pairs, o);
         held = max(held, __shfl_xor_sync(0xffffffffu, held, o));
     }
-    if (lane == 0) {
-        red[0][warp] = tiles;
-        red[1][warp] = pairs << 32 | held;
+    p.p_len = 0;
+    p.np = 0;
+    if (pre) {
+        const uint64_t most = static_cast<uint64_t>(held) * a.prefix.pages.page_tokens;
+        const uint32_t len = min(a.prefix.max_len, static_cast<uint32_t>(max(len0, 0)));
+        p.p_len = most < len ? static_cast<uint32_t>(most) : len;
+        p.np = TileGeom<BN>(a.prefix.pages.page_tokens).tiles(p.p_len);
     }
-    __syncthreads();
-    if (tid == 0) {
-        tiles = pairs = 0;
-        held = 0;
-        for (uint32_t w = 0; w < nthr / 32; ++w) {
-            tiles += red[0][w];
-            pairs += red[1][w] >> 32;
-            held = max(held, static_cast<uint32_t>(red[1][w]));
-        }
-        p.p_len = 0;
-        p.np = 0;
-        if (a.prefix.max_len) {
-            const uint64_t most = static_cast<uint64_t>(held) * a.prefix.pages.page_tokens;
-            uint32_t len = a.prefix.max_len;
-            if (a.prefix.len)
-                len = min(len, static_cast<uint32_t>(max(__ldg(a.prefix.len), 0)));
-            p.p_len = most < len ? static_cast<uint32_t>(most) : len;
-            p.np = TileGeom<BN>(a.prefix.pages.page_tokens).tiles(p.p_len);
-        }
-        p.q0 = 0;
-        uint32_t q1 = a.n_q;
-        if (a.n_seq) {
-            const int32_t n = static_cast<int32_t>(a.n_q);
-            p.q0 = static_cast<uint32_t>(min(max(__ldg(a.q_start), 0), n));
-            q1 = static_cast<uint32_t>(min(max(__ldg(a.q_start + a.n_seq), static_cast<int32_t>(p.q0)), n));
-        }
-        p.rows = (q1 - p.q0) * G;
-        p.n_pair = (p.rows + PR - 1) / PR;
-        // 8 CTAs side by side leave at most 4 % of the 148 SMs without a group
-        p.n_pg = (p.n_pair + 7) / 8;
-        p.gs = p.n_pg ? (p.n_pair + p.n_pg - 1) / p.n_pg : 1;
-        if (p.gs > gridDim.x) {
-            p.gs = gridDim.x;
-            p.n_pg = (p.n_pair + p.gs - 1) / p.gs;
-        }
-        p.groups = gridDim.x / p.gs;
-        p.p_total = static_cast<uint64_t>(p.np) * p.n_pg * H;
-        p.t_total = tiles;
-        p.t_slot0 = (p.n_pg * H + p.groups) * p.gs;
-        const uint64_t slots = p.t_slot0 + pairs * H + gridDim.x;
-        if (slots > l.max_slots) {  // q_start was not ascending
-            fail = 1;
-            p.p_total = p.t_total = 0;
-        }
+    const int32_t nq = static_cast<int32_t>(a.n_q);
+    p.q0 = static_cast<uint32_t>(min(max(q_first, 0), nq));
+    p.rows = (min(max(q_last, static_cast<int32_t>(p.q0)), nq) - p.q0) * G;
+    p.n_pair = (p.rows + PR - 1) / PR;
+    // 8 CTAs side by side leave at most 5 % of the 148 SMs without a group
+    p.n_pg = (p.n_pair + 7) / 8;
+    p.gs = p.n_pg ? (p.n_pair + p.n_pg - 1) / p.n_pg : 1;
+    if (p.gs > gridDim.x) {
+        p.gs = gridDim.x;
+        p.n_pg = (p.n_pair + p.gs - 1) / p.gs;
     }
-    __syncthreads();
+    p.groups = p.gs == 1 ? gridDim.x : gridDim.x / p.gs;
+    p.p_total = static_cast<uint64_t>(p.np) * p.n_pg * H;
+    p.t_total = tiles;
+    p.t_slot0 = (p.n_pg * H + p.groups) * p.gs;
+    const bool ok = p.t_slot0 + pairs * H + gridDim.x <= l.max_slots;
+    if (!ok) p.p_total = p.t_total = 0;  // q_start was not ascending
+    if (p.gs == 1) {
+        p.pre.set(p.p_total + p.t_total, gridDim.x);
+        p.own = p.pre;
+    } else {
+        p.pre.set(p.p_total, p.groups);
+        p.own.set(p.t_total, gridDim.x);
+    }
+    start = {0, 0, 0};
     uint64_t x, x1, y, y1;
-    Walk<BN, PR>::ranges(p, blockIdx.x, gridDim.x, x, x1, y, y1);
-    if (y >= y1 && blockIdx.x != 0) return;  // no tails here
+    Walk<BN, PR>::ranges(p, blockIdx.x, x, x1, y, y1);
+    if (blockIdx.x == 0 && lane == 0) *l.plan = p;
+    if (y >= y1 && blockIdx.x != 0) return ok;  // no tails here
     uint64_t base_t = 0;
     uint32_t base_p = 0;
-    for (uint32_t s0 = 0; s0 < a.n_seq; s0 += nthr) {
-        const uint32_t s = s0 + tid;
-        uint64_t t = 0;
-        uint32_t n = 0;
-        if (s < a.n_seq) shape(s, t, n);
-        uint64_t ti = t, pi = n;
+    for (uint32_t s0 = 0; s0 < a.n_seq; s0 += 32) {
+        const uint32_t s = s0 + lane;
+        if (s0) shape(s, t0, n0);
+        uint64_t ti = t0;
+        uint32_t pi = n0;
         for (int o = 1; o < 32; o <<= 1) {
-            const uint64_t u = __shfl_up_sync(0xffffffffu, ti, o), v = __shfl_up_sync(0xffffffffu, pi, o);
+            const uint64_t u = __shfl_up_sync(0xffffffffu, ti, o);
+            const uint32_t v = __shfl_up_sync(0xffffffffu, pi, o);
             if (lane >= o) {
                 ti += u;
                 pi += v;
             }
         }
-        if (lane == 31) {
-            red[0][warp] = ti;
-            red[1][warp] = pi;
+        const uint64_t all_t = __shfl_sync(0xffffffffu, ti, 31);
+        const uint32_t all_p = __shfl_sync(0xffffffffu, pi, 31);
+        ti += base_t - t0;
+        pi += base_p - n0;
+        if (blockIdx.x == 0 && s < a.n_seq) {
+            l.seq_tile[s] = ti;
+            l.seq_pair[s] = pi;
         }
-        __syncthreads();
-        uint64_t before_t = base_t, before_p = base_p, all_t = 0, all_p = 0;
-        for (uint32_t w = 0; w < nthr / 32; ++w) {
-            if (w < warp) {
-                before_t += red[0][w];
-                before_p += red[1][w];
-            }
-            all_t += red[0][w];
-            all_p += red[1][w];
-        }
-        ti += before_t - t;
-        pi += before_p - n;
-        if (s < a.n_seq) {
-            if (y >= ti && y < ti + t) start = {s, static_cast<uint32_t>(pi), ti};
-            if (blockIdx.x == 0) {
-                l.seq_tile[s] = ti;
-                l.seq_pair[s] = static_cast<uint32_t>(pi);
-            }
+        const uint32_t hit = __ballot_sync(0xffffffffu, y < y1 && y >= ti && y < ti + t0);
+        if (hit) {
+            const int w = __ffs(hit) - 1;
+            start.seq = s0 + w;
+            start.pair = __shfl_sync(0xffffffffu, pi, w);
+            start.tile = __shfl_sync(0xffffffffu, ti, w);
+            if (blockIdx.x != 0) break;
         }
         base_t += all_t;
-        base_p += static_cast<uint32_t>(all_p);
-        __syncthreads();
+        base_p += all_p;
     }
+    return ok;
 }
 
 template <int D>
@@ -266,10 +310,9 @@ __global__ void __launch_bounds__(Cfg<D>::threads, 1)
     constexpr uint32_t KB = BN * 128, QB = 128 * 128;  // bytes of a 64-column block of K / V, of Q
     extern __shared__ uint8_t smem_raw[];
     __shared__ Plan plan;
-    __shared__ Start start;
-    __shared__ uint64_t red[2][16];
-    __shared__ uint64_t bars[2 * ST + kMeta + 4 * NS + 1];
-    __shared__ uint32_t s_mask[kMeta][4];
+    __shared__ Seg s_seg[kSegs];
+    __shared__ uint64_t bars[2 * ST + kMeta + 2 * kSegs + 4 * NS + 1];
+    __shared__ __align__(16) uint32_t s_mask[kMeta][4];
     __shared__ uint32_t s_tmem, s_fail;
 
     const PrefixAttn &a = l.a;
@@ -280,28 +323,34 @@ __global__ void __launch_bounds__(Cfg<D>::threads, 1)
     auto full = [&](uint32_t i) { return bar0 + 8u * i; };
     auto empty = [&](uint32_t i) { return bar0 + 8u * (ST + i); };
     auto meta = [&](uint32_t i) { return bar0 + 8u * (2 * ST + i); };
-    auto q_ready = [&](uint32_t s) { return bar0 + 8u * (2 * ST + kMeta + s); };
-    auto s_full = [&](uint32_t s) { return bar0 + 8u * (2 * ST + kMeta + NS + s); };
-    auto p_ready = [&](uint32_t s) { return bar0 + 8u * (2 * ST + kMeta + 2 * NS + s); };
-    auto pv_done = [&](uint32_t s) { return bar0 + 8u * (2 * ST + kMeta + 3 * NS + s); };
-    const uint32_t drain = bar0 + 8u * (2 * ST + kMeta + 4 * NS);
-    auto failed = [&] { return *static_cast<volatile uint32_t *>(&s_fail) != 0; };
+    auto seg_full = [&](uint32_t i) { return bar0 + 8u * (2 * ST + kMeta + i); };
+    auto seg_empty = [&](uint32_t i) { return bar0 + 8u * (2 * ST + kMeta + kSegs + i); };
+    constexpr uint32_t SB = 2 * ST + kMeta + 2 * kSegs;
+    auto q_ready = [&](uint32_t s) { return bar0 + 8u * (SB + s); };
+    auto s_full = [&](uint32_t s) { return bar0 + 8u * (SB + NS + s); };
+    auto p_ready = [&](uint32_t s) { return bar0 + 8u * (SB + 2 * NS + s); };
+    auto pv_done = [&](uint32_t s) { return bar0 + 8u * (SB + 3 * NS + s); };
+    const uint32_t drain = bar0 + 8u * (SB + 4 * NS);
 
     if (threadIdx.x == 0) {
         s_fail = 0;
-        start = {0, 0, 0};
-        for (int i = 0; i < 2 * ST + kMeta; ++i) mbar_init(bar0 + 8u * i, 1);
-        mbar_init(drain, 1);
+        for (int i = 0; i < ST; ++i) {
+            mbar_init(full(i), 1);
+            mbar_init(empty(i), NS);  // one arrival per stream
+        }
+        for (int i = 0; i < kMeta; ++i) mbar_init(meta(i), 1);
+        for (int i = 0; i < kSegs; ++i) {
+            mbar_init(seg_full(i), 1);
+            mbar_init(seg_empty(i), 1 + NS + 4 * NS);  // producer, products, softmax warps
+        }
         for (int s = 0; s < NS; ++s) {
             mbar_init(q_ready(s), 4);
             mbar_init(s_full(s), 1);
             mbar_init(p_ready(s), 4);
             mbar_init(pv_done(s), 1);
         }
+        mbar_init(drain, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        for (int i = a.prefix.max_len ? 0 : 2; i < (a.n_seq ? 4 : 2); ++i)
-            asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&l.map[i]))
-                         : "memory");
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
@@ -312,26 +361,55 @@ __global__ void __launch_bounds__(Cfg<D>::threads, 1)
     }
     tc_fence_before();
     __syncthreads();
-    make_plan<D>(l, plan, start, s_fail, red);
-    __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = s_tmem;
-    Walk<BN, PR> walk(a, plan, start.seq, start.tile, start.pair);
-    Seg g;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
+    bool stop = false;
+    // a whole warp's wait; false once it has given up (the warps that wait for
+    // this one then do too)
+    auto wait = [&](uint32_t bar, uint32_t parity) {
+        if (!__all_sync(0xffffffffu, mbar_wait(bar, parity))) stop = true;
+        return !stop;
+    };
 
-    if (warp == 0) {  // ---- producer ----
+    if (warp == 2) {  // ---- the pieces ----
+        Start start;
+        Plan p;
+        if (!make_plan<D>(l, p, start)) stop = true;
+        if (lane == 0) plan = p;
+        __syncwarp();
+        Walk<BN, PR> walk(a, plan, start.seq, start.tile, start.pair);
+        uint32_t j = 0;
+        for (uint32_t i = 0;; ++i) {
+            Seg g = {};
+            if (!stop && walk.next(g)) {
+                g.j0 = j;
+                j += g.n;
+            }
+            if (i >= kSegs && !wait(seg_empty(i % kSegs), (i / kSegs - 1) & 1u)) break;
+            if (lane == 0) {
+                s_seg[i % kSegs] = g;
+                mbar_arrive(seg_full(i % kSegs));
+            }
+            __syncwarp();
+            if (g.n == 0) break;
+        }
+    } else if (warp == 0) {  // ---- producer ----
+        if (lane < 4 && (lane < 2 ? a.prefix.max_len != 0 : a.n_seq != 0))
+            asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&l.map[lane]))
+                         : "memory");
         uint32_t q = 0, j = 0;  // stages and tiles so far
-        bool stop = false;
-        while (!stop && walk.next(g)) {
+        for (uint32_t sg = 0; !stop; ++sg) {
+            if (!wait(seg_full(sg % kSegs), (sg / kSegs) & 1u)) break;
+            const Seg g = s_seg[sg % kSegs];
+            if (g.n == 0) break;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(seg_empty(sg % kSegs));
             const KeyList &kl = g.tail ? a.tail : a.prefix;
             const CUtensorMap *mk = &l.map[g.tail ? 2 : 0], *mv = mk + 1;
             const TileGeom<BN> geom(kl.pages.page_tokens);
             const uint32_t T = geom.T, box = min(T, static_cast<uint32_t>(BN));
             const uint64_t list = g.tail ? static_cast<uint64_t>(g.seq) * kl.n_list : 0;
-            const uint32_t len = g.tail ? min(static_cast<uint32_t>(max(__ldg(a.tail.len + g.seq), 0)),
-                                              a.tail.max_len)
-                                        : plan.p_len;
-            for (uint32_t i = 0; i < g.n; ++i, ++j) {
+            for (uint32_t i = 0; i < g.n && !stop; ++i, ++j) {
                 // lane p < ppt: page p of the tile, and how many of its tokens count
                 uint32_t page, off;
                 geom.locate(g.tile0 + i, page, off);
@@ -342,7 +420,7 @@ __global__ void __launch_bounds__(Cfg<D>::threads, 1)
                     id = kl.table ? __ldg(kl.table + list + at) : static_cast<int32_t>(at);
                     if (id >= 0 && static_cast<uint32_t>(id) < kl.pages.n_pages) {
                         held = kl.ntok ? min(__ldg(kl.ntok + at), T) : T;
-                        held = min(held, at * T < len ? len - at * T : 0);
+                        held = min(held, at * T < g.len ? g.len - at * T : 0);
                     }
                 }
                 const bool use = held > off;
@@ -355,16 +433,11 @@ __global__ void __launch_bounds__(Cfg<D>::threads, 1)
                     const uint32_t b = __ballot_sync(0xffffffffu, pk < geom.ppt && o < h);
                     if (lane == w) mask = b;
                 }
-                const uint32_t n_use = __popc(__ballot_sync(0xffffffffu, use));
-                const uint32_t bytes = n_use * box * D * 2;
+                const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, use)) * box * D * 2;
 #pragma unroll
-                for (uint32_t v = 0; v < 2; ++v, ++q) {  // K, then V
+                for (uint32_t v = 0; v < 2; ++v) {  // K, then V
                     const uint32_t st = q % ST, round = q / ST;
-                    const bool ok = round == 0 || mbar_wait(empty(st), (round - 1) & 1u);
-                    if (!__all_sync(0xffffffffu, ok) || failed()) {
-                        stop = true;
-                        break;
-                    }
+                    if (round && !wait(empty(st), (round - 1) & 1u)) break;
                     if (v == 0) {
                         if (lane < BN / 32) s_mask[j % kMeta][lane] = mask;
                         __syncwarp();
@@ -372,6 +445,7 @@ __global__ void __launch_bounds__(Cfg<D>::threads, 1)
                     }
                     if (lane == 0) mbar_expect_tx(full(st), bytes);
                     __syncwarp();
+                    ++q;
                     if (use) {
                         const uint32_t dst = ring + st * C::stage + lane * T * 128;
 #pragma unroll
@@ -381,263 +455,320 @@ __global__ void __launch_bounds__(Cfg<D>::threads, 1)
                                         full(st));
                     }
                 }
-                if (stop) break;
             }
         }
         if (stop) {  // gave up: drain the loads already issued (bounded)
             if (lane == 0) atomicExch(&s_fail, 1u);
             for (uint32_t i = q > ST ? q - ST : 0; i < q; ++i) mbar_wait(full(i % ST), (i / ST) & 1u);
         }
-    } else if (warp == 1) {
-        if (lane == 0) {  // ---- products ----
-            constexpr uint32_t id_s = idesc(BN, false), id_o = idesc(D, true);
-            uint32_t j = 0;  // tiles before this piece
-            uint32_t nq[2] = {0, 0}, np[2] = {0, 0}, npv[2] = {0, 0};
-            bool stop = false;
-            auto wait = [&](uint32_t bar, uint32_t parity) {
-                if (!mbar_wait(bar, parity) || failed()) stop = true;
-                return !stop;
-            };
-            while (!stop && walk.next(g)) {
-                const bool both = g.rows > 128;  // two row tiles, the same keys
-                uint32_t n[2] = {g.n, both ? g.n : 0};
-                if (NS == 2 && !both) {
-                    n[0] = (g.n + 1) / 2;
-                    n[1] = g.n / 2;
+    } else if (warp == 1) {  // ---- products ----
+        // Tiles are taken in the CTA's order: the stream whose current tile is
+        // first gets its P V product and, once that has read P, its next scores.
+        // While it waits for its softmax the other stream's turn comes, so the two
+        // stay half a period apart. (Both products of a turn being issued as soon
+        // as they could be, in any order, lets the streams fall into step: 3.9 ms
+        // instead of 3.2 ms for 2048 rows over 32,768 tokens.)
+        constexpr uint32_t id_s = idesc(BN, false), id_o = idesc(D, true);
+        constexpr uint32_t kHi = 64u | (1u << 14) | (2u << 29);  // upper halves of the descriptors
+        const uint32_t ubase = __shfl_sync(0xffffffffu, base, 0);
+        auto desc = [](uint32_t lo) { return static_cast<uint64_t>(kHi) << 32 | lo; };
+        Share<NS> sh[2];
+        uint32_t sg[2] = {0, 0}, tiles[2] = {0, 0};  // pieces taken up, tiles finished
+        bool live[2] = {true, NS == 2}, fresh[2] = {true, true};
+        auto open = [&](uint32_t s) {  // the stream's next piece with a tile for it
+            for (;;) {
+                if (!wait(seg_full(sg[s] % kSegs), (sg[s] / kSegs) & 1u)) return;
+                const Seg &g = s_seg[sg[s] % kSegs];
+                const bool end = g.n == 0;
+                if (!end) sh[s].set(g, s);
+                __syncwarp();
+                if (end) {
+                    live[s] = false;
+                    return;
                 }
-                auto tile = [&](uint32_t s, uint32_t i) { return j + (NS == 2 && !both ? 2 * i + s : i); };
-                auto scores = [&](uint32_t s, uint32_t i) {
-                    const uint32_t k = 2 * tile(s, i), st = k % ST;
-                    if (!wait(full(st), (k / ST) & 1u)) return;
-                    tc_fence_after();
-                    const uint64_t da = sw128_desc(base + s * C::q_bytes);
-                    const uint64_t db = sw128_desc(ring + st * C::stage);
-#pragma unroll
-                    for (uint32_t c = 0; c < D / 16; ++c)  // 16 columns: 32 bytes of a block
-                        mma_ss(tmem + C::s_col(s), da + (c / 4) * (QB / 16) + 2 * (c % 4),
-                               db + (c / 4) * (KB / 16) + 2 * (c % 4), id_s, c != 0);
-                    if (!both || s == 1) mma_commit(empty(st));
-                    mma_commit(s_full(s));
-                };
-                for (uint32_t s = 0; s < NS && !stop; ++s)
-                    if (n[s]) {
-                        if (!wait(q_ready(s), nq[s]++ & 1u)) break;
-                        tc_fence_after();
-                        scores(s, 0);
-                    }
-                for (uint32_t i = 0; i < n[0] && !stop; ++i)
-                    for (uint32_t s = 0; s < NS && !stop; ++s) {
-                        if (i >= n[s]) continue;
-                        const uint32_t v = 2 * tile(s, i) + 1, st = v % ST;
-                        if (!wait(p_ready(s), np[s]++ & 1u) || !wait(full(st), (v / ST) & 1u)) break;
-                        tc_fence_after();
-                        const uint64_t db = sw128_desc_mn(ring + st * C::stage, KB);
-#pragma unroll
-                        for (uint32_t c = 0; c < BN / 16; ++c)  // 16 keys: 8 columns of P, 2 KiB of V
-                            mma_ts(tmem + C::o_col(s), tmem + C::s_col(s) + 8 * c, db + 128 * c, id_o,
-                                   i != 0 || c != 0);
-                        if (!both || s == 1) mma_commit(empty(st));
-                        mma_commit(pv_done(s));
-                        ++npv[s];
-                        if (i + 1 < n[s]) {  // S over P: after the product that reads it
-                            if (!wait(pv_done(s), (npv[s] - 1) & 1u)) break;
-                            tc_fence_after();
-                            scores(s, i + 1);
-                        }
-                    }
-                j += g.n;
+                if (lane == 0) mbar_arrive(seg_empty(sg[s] % kSegs));
+                ++sg[s];
+                if (sh[s].any()) break;
             }
-            // on the regular path the softmax waits for the last products; here the
-            // issuer does, before the memory they use is given back
-            if (stop) {
+            fresh[s] = true;
+        };
+        uint32_t nq[2] = {0, 0};
+        // a stage is free once each stream has passed it: a tile of one stream
+        // alone counts for both
+        auto release = [&](uint32_t s, uint32_t st) {
+            mma_commit(empty(st));
+            if (NS == 2 && !sh[s].both) mma_commit(empty(st));
+        };
+        auto scores = [&](uint32_t s) {
+            if (fresh[s] && !wait(q_ready(s), nq[s]++ & 1u)) return;
+            const uint32_t k = 2 * sh[s].tile, st = __shfl_sync(0xffffffffu, k % ST, 0);
+            if (!wait(full(st), (k / ST) & 1u)) return;
+            tc_fence_after();
+            if (elect_one()) {
+                const uint32_t la = ((ubase + s * C::q_bytes) >> 4) | (1u << 16);
+                const uint32_t lb = ((ubase + NS * C::q_bytes + st * C::stage) >> 4) | (1u << 16);
+#pragma unroll
+                for (uint32_t c = 0; c < D / 16; ++c)  // 16 columns: 32 bytes of a block
+                    mma_ss(tmem + C::s_col(s), desc(la + (c / 4) * (QB / 16) + 2 * (c % 4)),
+                           desc(lb + (c / 4) * (KB / 16) + 2 * (c % 4)), id_s, c != 0);
+                release(s, st);
+                mma_commit(s_full(s));
+            }
+            __syncwarp();
+        };
+#pragma unroll
+        for (uint32_t s = 0; s < NS; ++s) {
+            if (!stop) open(s);
+            if (!stop && live[s]) scores(s);
+        }
+        auto turn = [&](uint32_t s) {
+            const uint32_t v = 2 * sh[s].tile + 1, st = __shfl_sync(0xffffffffu, v % ST, 0);
+            if (!wait(p_ready(s), tiles[s] & 1u) || !wait(full(st), (v / ST) & 1u)) return;
+            tc_fence_after();
+            if (elect_one()) {
+                const uint32_t lb = ((ubase + NS * C::q_bytes + st * C::stage) >> 4) | (KB / 16) << 16;
+                const uint32_t add = !fresh[s];
+#pragma unroll
+                for (uint32_t c = 0; c < BN / 16; ++c)  // 16 keys: 8 columns of P, 2 KiB of V
+                    mma_ts(tmem + C::o_col(s), tmem + C::s_col(s) + 8 * c, desc(lb + 128 * c), id_o,
+                           c ? 1u : add);
+                release(s, st);
+                mma_commit(pv_done(s));
+            }
+            __syncwarp();
+            fresh[s] = false;
+            sh[s].tile += sh[s].step;
+            if (!sh[s].any()) open(s);
+            // S over P: after the product that reads it
+            if (!stop && live[s] && wait(pv_done(s), tiles[s] & 1u)) scores(s);
+            ++tiles[s];
+        };
+        uint32_t last = 1;
+        while (!stop && (live[0] || (NS == 2 && live[1]))) {
+            const bool one = NS == 2 && live[1] &&
+                             (!live[0] || sh[1].tile < sh[0].tile ||
+                              (sh[1].tile == sh[0].tile && last == 0));
+            last = one;
+            if (NS == 2 && one)
+                turn(1);
+            else
+                turn(0);
+        }
+        // on the regular path the softmax waits for the last products; here the
+        // issuer does, before the memory they use is given back
+        if (stop) {
+            if (lane == 0) {
                 atomicExch(&s_fail, 1u);
                 mma_commit(drain);
-                mbar_wait(drain, 0);
             }
+            __syncwarp();
+            mbar_wait(drain, 0);
         }
     } else if (warp >= 4) {  // ---- softmax, a thread a row ----
         const uint32_t s = (warp - 4) >> 2, qd = warp & 3, r = 32 * qd + lane;
         const uint32_t tid = threadIdx.x & 127;
         const uint32_t G = a.n_head / a.n_head_kv;
-        const float c = fabsf(a.scale) * 1.44269504f;
+        // (above zero, so that -inf stays -inf; a scale of zero gives equal scores all the same)
+        const float c = fmaxf(fabsf(a.scale) * 1.44269504f, 1e-37f);
         const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;  // a negative scale turns Q
         const uint32_t ts = tmem + ((32 * qd) << 16) + C::s_col(s);
         const uint32_t to = tmem + ((32 * qd) << 16) + C::o_col(s);
-        uint32_t j = 0, ns = 0, npv = 0;
-        bool stop = false;
-        auto wait = [&](uint32_t bar, uint32_t parity) {
-            const bool ok = mbar_wait(bar, parity) && !failed();
-            if (!__all_sync(0xffffffffu, ok)) stop = true;
-            return !stop;
-        };
-        while (!stop && walk.next(g)) {
-            const bool both = g.rows > 128;
-            const uint32_t first = NS == 2 && both ? 128 * s : 0;  // of the unit's rows
-            const uint32_t n = NS == 1 || both ? g.n : (g.n + 1 - s) / 2;
-            const uint32_t rows = g.rows - first < 128 ? g.rows - first : 128;
-            const uint32_t j0 = j;
-            j += g.n;
-            if (n == 0) {  // a piece of one tile: nothing from the second stream
-                if (r < rows)
+        uint32_t ns = 0, sg = 0;  // tiles and pieces so far
+        Seg g = {};
+        Share<NS> sh = {};
+        auto row_first = [&] { return sh.both ? 128 * s : 0u; };  // of the unit's rows
+        auto row_count = [&] { return min(128u, g.rows - row_first()); };
+        // the stream's next piece: Q in the swizzled layout, rows past the last zeros
+        auto open = [&] {
+            for (;;) {
+                if (!wait(seg_full(sg % kSegs), (sg / kSegs) & 1u)) return false;
+                g = s_seg[sg % kSegs];
+                if (g.n == 0) return false;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(seg_empty(sg % kSegs));
+                ++sg;
+                sh.set(g, s);
+                if (sh.any()) break;
+                if (r < row_count())  // the other stream has the piece's only tile
                     l.ml[(static_cast<uint64_t>(g.slot) * NS + s) * 128 + r] = make_float2(-INFINITY, 0.0f);
-                continue;
             }
-            // Q, in the swizzled layout; rows past the last are zeros
-            for (uint32_t i = tid; i < 128 * (D / 8); i += 128) {
-                const uint32_t qr = i / (D / 8), ch = i % (D / 8);
-                uint4 w = make_uint4(0, 0, 0, 0);
-                if (qr < rows) {
-                    const uint32_t rr = g.row0 + first + qr, t = rr / G;
-                    w = __ldg(reinterpret_cast<const uint4 *>(
-                        a.q + static_cast<uint64_t>(g.q0 + t) * a.q_stride +
-                        static_cast<uint64_t>(g.h * G + rr - t * G) * D + 8 * ch));
-                    w.x ^= sign;
-                    w.y ^= sign;
-                    w.z ^= sign;
-                    w.w ^= sign;
+            const uint32_t rows = row_count(), at0 = g.row0 + row_first();
+            constexpr uint32_t CH = D / 8, RS = 128 / CH;  // 16-byte chunks of a row; rows a pass
+            constexpr uint32_t QL = CH < 16 ? CH : 16;      // loads in flight
+            const uint32_t ch = tid % CH;
+#pragma unroll
+            for (uint32_t i0 = 0; i0 < CH; i0 += QL) {
+                uint4 w[QL];
+#pragma unroll
+                for (uint32_t i = 0; i < QL; ++i) {  // all loads first
+                    const uint32_t qr = tid / CH + (i0 + i) * RS, rr = at0 + qr, t = rr / G;
+                    w[i] = make_uint4(0, 0, 0, 0);
+                    if (qr < rows)
+                        w[i] = __ldg(reinterpret_cast<const uint4 *>(
+                            a.q + static_cast<uint64_t>(g.q0 + t) * a.q_stride +
+                            static_cast<uint64_t>(g.h * G + rr - t * G) * D + 8 * ch));
                 }
-                const uint32_t at = base + s * C::q_bytes + (ch / 8) * QB + qr * 128 +
-                                    (((ch % 8) ^ (qr % 8)) * 16);
-                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w.x), "r"(w.y),
-                             "r"(w.z), "r"(w.w)
-                             : "memory");
+#pragma unroll
+                for (uint32_t i = 0; i < QL; ++i) {
+                    const uint32_t qr = tid / CH + (i0 + i) * RS;
+                    const uint32_t at = base + s * C::q_bytes + (ch / 8) * QB + qr * 128 +
+                                        (((ch % 8) ^ (qr % 8)) * 16);
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at),
+                                 "r"(w[i].x ^ sign), "r"(w[i].y ^ sign), "r"(w[i].z ^ sign),
+                                 "r"(w[i].w ^ sign)
+                                 : "memory");
+                }
             }
             fence_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(q_ready(s));
-
+            return true;
+        };
+        bool more = open();
+        while (more) {
+            const uint32_t rows = row_count();
+            const uint64_t slot = static_cast<uint64_t>(g.slot) * NS + s;
+            const bool idle = 32 * qd >= rows;  // no row of this warp: P may be anything
             // how far the row sees into the list
             uint32_t seen = 0xffffffffu;
-            const TileGeom<BN> geom((g.tail ? a.tail : a.prefix).pages.page_tokens);
-            if (g.tail) {
-                const SeqShape sh = seq_shape(a, g.seq);
-                const uint32_t i = (g.row0 + first + min(r, rows - 1)) / G;
-                seen = tail_seen(sh, i);
-            }
+            if (g.tail) seen = tail_seen(g.len, g.q_len, (g.row0 + row_first() + min(r, rows - 1)) / G);
+            const uint32_t tile0 = g.tile0 - g.j0;
             float m = -INFINITY, sum = 0.0f;  // of c q . k
-            for (uint32_t i = 0; i < n; ++i) {
-                const uint32_t tj = NS == 2 && !both ? 2 * i + s : i;  // of the piece
-                const uint32_t jj = j0 + tj;
+            for (bool begin = true; sh.any(); sh.tile += sh.step, begin = false) {
+                const uint32_t jj = sh.tile;
                 if (!wait(s_full(s), ns++ & 1u) || !wait(meta(jj % kMeta), (jj / kMeta) & 1u)) break;
                 tc_fence_after();
-                uint32_t mask[BN / 32], all = 0xffffffffu;
-#pragma unroll
-                for (int w = 0; w < BN / 32; ++w) {
-                    mask[w] = s_mask[jj % kMeta][w];
-                    all &= mask[w];
-                }
-                uint32_t page, off;
-                geom.locate(g.tile0 + tj, page, off);
-                const uint32_t pos0 = page * geom.T + off;
-                const uint32_t lim = seen > pos0 ? min(seen - pos0, static_cast<uint32_t>(BN)) : 0;
-                const bool whole = all == 0xffffffffu;
-                if (!whole) {  // V rows of cells without a token become zeros
-                    const uint32_t k = 2 * jj + 1;
-                    if (!wait(full(k % ST), (k / ST) & 1u)) break;
-                    for (uint32_t x = tid; x < BN * (D / 64); x += 128) {
-                        const uint32_t key = x % BN;
-                        if (s_mask[jj % kMeta][key / 32] >> (key % 32) & 1u) continue;
-                        const uint32_t at = ring + (k % ST) * C::stage + (x / BN) * KB + key * 128;
-#pragma unroll
-                        for (uint32_t z = 0; z < 128; z += 16)
-                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at + z), "r"(0u)
-                                         : "memory");
-                    }
-                    fence_async_smem();
-                }
-                uint32_t v[BN];
-#pragma unroll
-                for (int w = 0; w < BN / 32; ++w) tmem_ld32_nowait(ts + 32 * w, v + 32 * w);
-                tmem_ld_wait();
-                const bool clear = __all_sync(0xffffffffu, whole && lim >= BN);
-                float top = -INFINITY;
+                const uint4 mw = *reinterpret_cast<const uint4 *>(s_mask[jj % kMeta]);
+                const bool whole = (mw.x & mw.y & (BN == 128 ? mw.z & mw.w : 0xffffffffu)) == 0xffffffffu;
+                // a tile's first token is at most tile * BN: all of it seen?
+                const bool clear = whole && __all_sync(0xffffffffu, (tile0 + jj + 1) * BN <= seen);
+                uint32_t x[32];
                 if (!clear) {
+                    // the S columns of keys that do not count become -inf, the V rows of
+                    // cells without a token zeros
+                    if (!whole) {
+                        const uint32_t k = 2 * jj + 1;
+                        if (!wait(full(k % ST), (k / ST) & 1u)) break;
+                        for (uint32_t i = tid; i < BN * (D / 64); i += 128) {
+                            const uint32_t key = i % BN;
+                            if (s_mask[jj % kMeta][key / 32] >> (key % 32) & 1u) continue;
+                            const uint32_t at = ring + (k % ST) * C::stage + (i / BN) * KB + key * 128;
 #pragma unroll
-                    for (int k = 0; k < BN; ++k)
-                        if (!(mask[k / 32] >> (k % 32) & 1u) || k >= lim) v[k] = 0xff800000u;
-                }
-#pragma unroll
-                for (int k = 0; k < BN; k += 4)
-                    top = fmaxf(top, fmaxf(fmaxf(__uint_as_float(v[k]), __uint_as_float(v[k + 1])),
-                                           fmaxf(__uint_as_float(v[k + 2]), __uint_as_float(v[k + 3]))));
-                // a score of c q . k; c = 0 makes 0 of every finite one, and a masked one stays -inf
-                top = top == -INFINITY ? top : top * c;
-                if (__any_sync(0xffffffffu, top > m + 8.0f)) {
-                    const float mn = fmaxf(m, top);
-                    const float f = m == -INFINITY ? 0.0f : ex2(m - mn);
-                    m = mn;
-                    sum *= f;
-                    if (i != 0) {  // the product before has completed: S came after it
+                            for (uint32_t z = 0; z < 128; z += 16)
+                                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at + z),
+                                             "r"(0u)
+                                             : "memory");
+                        }
+                        fence_async_smem();
+                    }
+                    const TileGeom<BN> geom((g.tail ? a.tail : a.prefix).pages.page_tokens);
+                    uint32_t page, off;
+                    geom.locate(tile0 + jj, page, off);
+                    const uint32_t pos0 = page * geom.T + off;
+                    const uint32_t lim = seen > pos0 ? min(seen - pos0, static_cast<uint32_t>(BN)) : 0;
 #pragma unroll 1
-                        for (uint32_t col = 0; col < D; col += 32) {
-                            uint32_t o[32];
-                            tmem_ld32_nowait(to + col, o);
-                            tmem_ld_wait();
+                    for (uint32_t w = 0; w < BN / 32 && !idle; ++w) {
+                        const uint32_t left = lim > 32 * w ? lim - 32 * w : 0;
+                        const uint32_t mask = s_mask[jj % kMeta][w] &
+                                              (left >= 32 ? 0xffffffffu : (1u << left) - 1);
+                        tmem_ld32_nowait(ts + 32 * w, x);
+                        tmem_ld_wait(x);
 #pragma unroll
-                            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-                            tmem_st32(to + col, o);
+                        for (int k = 0; k < 32; ++k)
+                            if (!(mask >> k & 1u)) x[k] = 0xff800000u;
+                        tmem_st32(ts + 32 * w, x);
+                    }
+                    tmem_st_wait();
+                }
+                if (!idle) {
+                    // the tile's maximum, 32 columns at a time: the next ones are on
+                    // their way meanwhile
+                    float top = -INFINITY;
+                    uint32_t y[32];
+                    tmem_ld32_nowait(ts, x);
+#pragma unroll
+                    for (int w = 0; w < BN / 32; ++w) {
+                        uint32_t *const v = w & 1 ? y : x;
+                        tmem_ld_wait(v);
+                        tmem_ld32_nowait(ts + (w + 1 < BN / 32 ? 32 * (w + 1) : 0), w & 1 ? x : y);
+#pragma unroll
+                        for (int k = 0; k < 32; k += 2)
+                            top = fmaxf(top, fmaxf(__uint_as_float(v[k]), __uint_as_float(v[k + 1])));
+                    }
+                    top *= c;
+                    if (__any_sync(0xffffffffu, top > m + 8.0f)) {
+                        const float mn = fmaxf(m, top);
+                        const float f = m == -INFINITY ? 0.0f : ex2(m - mn);
+                        m = mn;
+                        sum *= f;
+                        if (!begin) {  // the product before has completed: S came after it
+#pragma unroll 1
+                            for (uint32_t col = 0; col < D; col += 16) {
+                                uint32_t o[16];
+                                tmem_ld16(to + col, o);
+#pragma unroll
+                                for (int k = 0; k < 16; ++k)
+                                    o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                                tmem_st16(to + col, o);
+                            }
                         }
                     }
-                }
-                const float neg = m == -INFINITY ? 0.0f : -m;
-                float s0 = 0.0f, s1 = 0.0f;
-                if (c == 0.0f && !clear) {  // -inf * 0
+                    const float neg = m == -INFINITY ? 0.0f : -m;
+                    float s0 = 0.0f, s1 = 0.0f;
+                    // columns 0 .. 31 are in x already
 #pragma unroll
-                    for (int k = 0; k < BN; ++k)
-                        v[k] = __float_as_uint(v[k] == 0xff800000u ? -INFINITY : neg);
-                } else {
+                    for (int w = 0; w < BN / 32; ++w) {
+                        uint32_t *const v = w & 1 ? y : x;
+                        tmem_ld_wait(v);
+                        if (w + 1 < BN / 32) tmem_ld32_nowait(ts + 32 * (w + 1), w & 1 ? x : y);
+                        uint32_t pk[16];
 #pragma unroll
-                    for (int k = 0; k < BN; ++k)
-                        v[k] = __float_as_uint(__fmaf_rn(__uint_as_float(v[k]), c, neg));
-                }
-#pragma unroll
-                for (int w = 0; w < BN / 64; ++w) {
-                    uint32_t pk[32];
-#pragma unroll
-                    for (int k = 0; k < 32; ++k) {
-                        const float x = ex2(__uint_as_float(v[64 * w + 2 * k]));
-                        const float y = ex2(__uint_as_float(v[64 * w + 2 * k + 1]));
-                        s0 += x;
-                        s1 += y;
-                        pk[k] = pack_h2(x, y);
+                        for (int k = 0; k < 16; ++k) {
+                            uint32_t e0 = v[2 * k], e1 = v[2 * k + 1];
+                            fma_pair(e0, e1, c, neg);
+                            const float p0 = ex2(__uint_as_float(e0)), p1 = ex2(__uint_as_float(e1));
+                            add_pair(s0, s1, p0, p1);
+                            pk[k] = pack_h2(p0, p1);
+                        }
+                        // P's columns lie on those of S that have been read
+                        tmem_st16(ts + 16 * w, pk);
                     }
-                    tmem_st32(ts + 32 * w, pk);
+                    sum += s0 + s1;
+                    tmem_st_wait();
                 }
-                sum += s0 + s1;
-                tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(p_ready(s));
-                ++npv;
             }
-            if (stop || !wait(pv_done(s), (npv - 1) & 1u)) break;
+            if (stop) break;
+            // the last scores are in: Q may be replaced while the last product runs
+            more = open();
+            if (!wait(pv_done(s), (ns - 1) & 1u)) break;
             tc_fence_after();
-            const uint64_t slot = static_cast<uint64_t>(g.slot) * NS + s;
-            if (r < rows) l.ml[slot * 128 + r] = make_float2(m, sum);
+            if (!idle) {
+                if (r < rows) l.ml[slot * 128 + r] = make_float2(m, sum);
 #pragma unroll 1
-            for (uint32_t col = 0; col < D; col += 32) {
-                uint32_t o[32];
-                tmem_ld32_nowait(to + col, o);
-                tmem_ld_wait();
-                if (r < rows) {
+                for (uint32_t col = 0; col < D; col += 32) {
+                    uint32_t o[32];
+                    tmem_ld32_nowait(to + col, o);
+                    tmem_ld_wait(o);
+                    if (r < rows) {
 #pragma unroll
-                    for (uint32_t k = 0; k < 8; ++k)
-                        l.o[(slot * (D / 4) + col / 4 + k) * 128 + r] =
-                            make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]),
-                                        __uint_as_float(o[4 * k + 2]), __uint_as_float(o[4 * k + 3]));
+                        for (uint32_t k = 0; k < 8; ++k)
+                            l.o[(slot * (D / 4) + col / 4 + k) * 128 + r] =
+                                make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]),
+                                            __uint_as_float(o[4 * k + 2]), __uint_as_float(o[4 * k + 3]));
+                    }
                 }
             }
             tc_fence_before();
         }
-        if (stop && lane == 0) atomicExch(&s_fail, 1u);
     }
+    if (stop && lane == 0) atomicExch(&s_fail, 1u);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (threadIdx.x == 0) {
-        l.fail[blockIdx.x] = s_fail;
-        if (blockIdx.x == 0) *l.plan = plan;
-    }
+    if (threadIdx.x == 0) l.fail[blockIdx.x] = s_fail;
     if (warp == 1) {
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
                      "r"(kAttnTmem)
@@ -651,8 +782,8 @@ __global__ void __launch_bounds__(Cfg<D>::threads, 1)
 constexpr uint32_t kJoinRows = 8, kMaxCtas = 160;
 struct JoinRow {
     uint64_t x0[2], x1[2];    // the row's unit on its line: prefix, tail
-    uint64_t total[2];
-    uint32_t parts[2], first[2], n[2];  // ranges of the line; the first and how many meet the unit
+    Cuts cuts[2];             // the line's ranges
+    uint32_t first[2], n[2];  // the first range that meets the unit, and how many
     uint32_t slot0[2], step[2];         // workspace slot of range i: slot0 + i * step
     uint32_t row[2];                    // within the slot's stream
     uint32_t stream[2], both[2];        // the row tile; whether the streams are row tiles
@@ -701,8 +832,7 @@ __global__ void __launch_bounds__(kJoinRows *D / 4)
         if (d.write && p.np && t >= p.q0 && (t - p.q0) * G + gq < p.rows) {
             const uint32_t r = (t - p.q0) * G + gq, pair = r / PR, pg = pair / p.gs;
             const uint64_t u = static_cast<uint64_t>(pg) * H + h;
-            d.total[0] = p.gs == 1 ? p.p_total + p.t_total : p.p_total;
-            d.parts[0] = p.gs == 1 ? n_cta : p.groups;
+            d.cuts[0] = p.pre;
             d.x0[0] = u * p.np;
             d.x1[0] = d.x0[0] + p.np;
             d.slot0[0] = static_cast<uint32_t>(u) * p.gs + pair - pg * p.gs;
@@ -718,8 +848,7 @@ __global__ void __launch_bounds__(kJoinRows *D / 4)
             if (t >= sh.q0 && i < sh.q_len && tiles && p.t_total) {
                 const uint32_t r = i * G + gq, pair = r / PR, u = pair * H + h;
                 const uint64_t base = p.gs == 1 ? p.p_total : 0;
-                d.total[1] = base + p.t_total;
-                d.parts[1] = n_cta;
+                d.cuts[1] = p.own;
                 d.x0[1] = base + l.seq_tile[seq] + static_cast<uint64_t>(u) * tiles;
                 d.x1[1] = d.x0[1] + min(tiles, pair_tiles<C::BN, PR>(sh, tg, pair, G));
                 d.slot0[1] = p.t_slot0 + l.seq_pair[seq] * H + u;
@@ -731,8 +860,8 @@ __global__ void __launch_bounds__(kJoinRows *D / 4)
         }
         for (int k = 0; k < 2; ++k)
             if (d.x1[k] > d.x0[k]) {
-                d.first[k] = owner(d.x0[k], d.total[k], d.parts[k]);
-                d.n[k] = owner(d.x1[k] - 1, d.total[k], d.parts[k]) + 1 - d.first[k];
+                d.first[k] = d.cuts[k].owner(d.x0[k]);
+                d.n[k] = d.cuts[k].owner(d.x1[k] - 1) + 1 - d.first[k];
             }
         rows[threadIdx.x] = d;
     }
@@ -748,9 +877,6 @@ __global__ void __launch_bounds__(kJoinRows *D / 4)
             for (uint32_t i0 = 0; i0 < d.n[k] * per; i0 += 32) {
                 const uint32_t i = i0 + lane, part = d.first[k] + i / per;
                 bool ok = i < d.n[k] * per;
-                // a range may be empty when there are fewer tiles than CTAs
-                ok = ok && max(d.x0[k], cut(d.total[k], part, d.parts[k])) <
-                               min(d.x1[k], cut(d.total[k], part + 1, d.parts[k]));
                 uint32_t id = 0;
                 float m = -INFINITY;
                 if (ok) {
