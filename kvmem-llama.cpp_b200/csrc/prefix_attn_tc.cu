@@ -499,10 +499,14 @@ __global__ void __launch_bounds__(Cfg<D>::threads, 1)
             mma_commit(empty(st));
             if (NS == 2 && !sh[s].both) mma_commit(empty(st));
         };
-        auto scores = [&](uint32_t s) {
+        // scores of the stream's current tile; `after`: once the product before,
+        // which reads the P that S will overwrite, has completed (the last wait, so
+        // that the issue follows it at once)
+        auto scores = [&](uint32_t s, bool after) {
             if (fresh[s] && !wait(q_ready(s), nq[s]++ & 1u)) return;
             const uint32_t k = 2 * sh[s].tile, st = __shfl_sync(0xffffffffu, k % ST, 0);
             if (!wait(full(st), (k / ST) & 1u)) return;
+            if (after && !wait(pv_done(s), tiles[s] & 1u)) return;
             tc_fence_after();
             if (elect_one()) {
                 const uint32_t la = ((ubase + s * C::q_bytes) >> 4) | (1u << 16);
@@ -511,19 +515,19 @@ __global__ void __launch_bounds__(Cfg<D>::threads, 1)
                 for (uint32_t c = 0; c < D / 16; ++c)  // 16 columns: 32 bytes of a block
                     mma_ss(tmem + C::s_col(s), desc(la + (c / 4) * (QB / 16) + 2 * (c % 4)),
                            desc(lb + (c / 4) * (KB / 16) + 2 * (c % 4)), id_s, c != 0);
-                release(s, st);
                 mma_commit(s_full(s));
+                release(s, st);
             }
             __syncwarp();
         };
 #pragma unroll
         for (uint32_t s = 0; s < NS; ++s) {
             if (!stop) open(s);
-            if (!stop && live[s]) scores(s);
+            if (!stop && live[s]) scores(s, false);
         }
         auto turn = [&](uint32_t s) {
             const uint32_t v = 2 * sh[s].tile + 1, st = __shfl_sync(0xffffffffu, v % ST, 0);
-            if (!wait(p_ready(s), tiles[s] & 1u) || !wait(full(st), (v / ST) & 1u)) return;
+            if (!wait(full(st), (v / ST) & 1u) || !wait(p_ready(s), tiles[s] & 1u)) return;
             tc_fence_after();
             if (elect_one()) {
                 const uint32_t lb = ((ubase + NS * C::q_bytes + st * C::stage) >> 4) | (KB / 16) << 16;
@@ -539,8 +543,7 @@ __global__ void __launch_bounds__(Cfg<D>::threads, 1)
             fresh[s] = false;
             sh[s].tile += sh[s].step;
             if (!sh[s].any()) open(s);
-            // S over P: after the product that reads it
-            if (!stop && live[s] && wait(pv_done(s), tiles[s] & 1u)) scores(s);
+            if (!stop && live[s]) scores(s, true);
             ++tiles[s];
         };
         uint32_t last = 1;
@@ -681,59 +684,72 @@ __global__ void __launch_bounds__(Cfg<D>::threads, 1)
                     tmem_st_wait();
                 }
                 if (!idle) {
-                    // the tile's maximum, 32 columns at a time: the next ones are on
-                    // their way meanwhile
-                    float top = -INFINITY;
-                    uint32_t y[32];
-                    tmem_ld32_nowait(ts, x);
-#pragma unroll
-                    for (int w = 0; w < BN / 32; ++w) {
-                        uint32_t *const v = w & 1 ? y : x;
-                        tmem_ld_wait(v);
-                        tmem_ld32_nowait(ts + (w + 1 < BN / 32 ? 32 * (w + 1) : 0), w & 1 ? x : y);
+                    // One pass with the maximum as it stands: p and the tile's own
+                    // maximum together, 32 columns at a time with the next ones on their
+                    // way. Only when a row's maximum has moved by more than 8 (and for
+                    // the first tile, whose maximum is taken beforehand) the pass is
+                    // repeated with the new one; S still stands, P is in registers.
+                    uint32_t y[32], pk[BN / 2];
+                    float top = -INFINITY, s0, s1;
+                    auto column_max = [&](const uint32_t *v) {
 #pragma unroll
                         for (int k = 0; k < 32; k += 2)
                             top = fmaxf(top, fmaxf(__uint_as_float(v[k]), __uint_as_float(v[k + 1])));
+                    };
+                    auto pass = [&] {
+                        const float neg = m == -INFINITY ? 0.0f : -m;
+                        s0 = s1 = 0.0f;
+                        top = -INFINITY;
+                        tmem_ld32_nowait(ts, x);
+#pragma unroll
+                        for (int w = 0; w < BN / 32; ++w) {
+                            uint32_t *const v = w & 1 ? y : x;
+                            tmem_ld_wait(v);
+                            if (w + 1 < BN / 32) tmem_ld32_nowait(ts + 32 * (w + 1), w & 1 ? x : y);
+                            column_max(v);
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) {
+                                uint32_t e0 = v[2 * k], e1 = v[2 * k + 1];
+                                fma_pair(e0, e1, c, neg);
+                                const float p0 = ex2(__uint_as_float(e0)), p1 = ex2(__uint_as_float(e1));
+                                add_pair(s0, s1, p0, p1);
+                                pk[16 * w + k] = pack_h2(p0, p1);
+                            }
+                        }
+                    };
+                    if (begin) {
+#pragma unroll 1
+                        for (uint32_t w = 0; w < BN / 32; ++w) {
+                            tmem_ld32_nowait(ts + 32 * w, x);
+                            tmem_ld_wait(x);
+                            column_max(x);
+                        }
+                        m = top * c;
                     }
-                    top *= c;
-                    if (__any_sync(0xffffffffu, top > m + 8.0f)) {
-                        const float mn = fmaxf(m, top);
+#pragma unroll 1
+                    for (;;) {
+                        pass();
+                        if (!__any_sync(0xffffffffu, top * c > m + 8.0f)) break;
+                        const float mn = fmaxf(m, top * c);
                         const float f = m == -INFINITY ? 0.0f : ex2(m - mn);
                         m = mn;
                         sum *= f;
-                        if (!begin) {  // the product before has completed: S came after it
+                        if (begin) continue;
+                        // O stands still: its last product came before these scores
 #pragma unroll 1
-                            for (uint32_t col = 0; col < D; col += 16) {
-                                uint32_t o[16];
-                                tmem_ld16(to + col, o);
+                        for (uint32_t col = 0; col < D; col += 16) {
+                            uint32_t o[16];
+                            tmem_ld16(to + col, o);
 #pragma unroll
-                                for (int k = 0; k < 16; ++k)
-                                    o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-                                tmem_st16(to + col, o);
-                            }
+                            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                            tmem_st16(to + col, o);
                         }
-                    }
-                    const float neg = m == -INFINITY ? 0.0f : -m;
-                    float s0 = 0.0f, s1 = 0.0f;
-                    // columns 0 .. 31 are in x already
-#pragma unroll
-                    for (int w = 0; w < BN / 32; ++w) {
-                        uint32_t *const v = w & 1 ? y : x;
-                        tmem_ld_wait(v);
-                        if (w + 1 < BN / 32) tmem_ld32_nowait(ts + 32 * (w + 1), w & 1 ? x : y);
-                        uint32_t pk[16];
-#pragma unroll
-                        for (int k = 0; k < 16; ++k) {
-                            uint32_t e0 = v[2 * k], e1 = v[2 * k + 1];
-                            fma_pair(e0, e1, c, neg);
-                            const float p0 = ex2(__uint_as_float(e0)), p1 = ex2(__uint_as_float(e1));
-                            add_pair(s0, s1, p0, p1);
-                            pk[k] = pack_h2(p0, p1);
-                        }
-                        // P's columns lie on those of S that have been read
-                        tmem_st16(ts + 16 * w, pk);
                     }
                     sum += s0 + s1;
+                    // P over the first columns of S
+#pragma unroll
+                    for (int w = 0; w < BN / 64; ++w)
+                        tmem_st32(ts + 32 * w, *reinterpret_cast<const uint32_t(*)[32]>(pk + 32 * w));
                     tmem_st_wait();
                 }
                 tc_fence_before();
@@ -777,16 +793,18 @@ __global__ void __launch_bounds__(Cfg<D>::threads, 1)
 }
 
 // The join: a row's pieces of the prefix and of its tail, weighted by
-// 2^(m_piece - m), in a fixed order. 8 rows a CTA, a thread per row and four
-// dimensions: reads of 128 bytes (8 rows of one float4 column).
+// 2^(m_piece - m), in a fixed order. 8 rows a CTA (neighbouring heads of a
+// token), a thread per row and four dimensions: reads of 128 bytes (8 rows of
+// one float4 column). What bounds it is the chain of dependent reads (lengths,
+// offsets, statistics, then the pieces, 16 at a time), so each step's reads are
+// issued together.
 constexpr uint32_t kJoinRows = 8, kMaxCtas = 160;
 struct JoinRow {
-    uint64_t x0[2], x1[2];    // the row's unit on its line: prefix, tail
-    Cuts cuts[2];             // the line's ranges
-    uint32_t first[2], n[2];  // the first range that meets the unit, and how many
-    uint32_t slot0[2], step[2];         // workspace slot of range i: slot0 + i * step
-    uint32_t row[2];                    // within the slot's stream
-    uint32_t stream[2], both[2];        // the row tile; whether the streams are row tiles
+    Cuts cuts[2];                // prefix, tail: the line's ranges
+    uint32_t first[2], n[2];     // the first range that meets the row's unit, and how many
+    uint32_t slot0[2], step[2];  // workspace slot of range i: slot0 + i * step
+    uint32_t row[2];             // within the slot's stream
+    uint32_t stream[2], per[2];  // the row tile; streams that hold part of the row
     bool write;
 };
 
@@ -796,112 +814,116 @@ __global__ void __launch_bounds__(kJoinRows *D / 4)
     using C = Cfg<D>;
     constexpr int PR = C::PR, NS = C::NS;
     constexpr uint32_t kList = 4 * kMaxCtas;  // two lines, two streams
+    constexpr uint32_t NT = kJoinRows * D / 4;
     __shared__ JoinRow rows[kJoinRows];
     __shared__ uint32_t s_id[kJoinRows][kList];
     __shared__ float s_w[kJoinRows][kList];
     __shared__ uint32_t s_n[kJoinRows];
     __shared__ float s_inv[kJoinRows];
     const PrefixAttn &a = l.a;
+    const uint32_t tid = threadIdx.x;
     const uint32_t G = a.n_head / a.n_head_kv, H = a.n_head_kv;
     const uint64_t row0 = static_cast<uint64_t>(blockIdx.x) * kJoinRows;
+    const uint32_t t_first = static_cast<uint32_t>(row0 / a.n_head);
+    const uint64_t last = min(row0 + kJoinRows, static_cast<uint64_t>(a.n_q) * a.n_head) - 1;
+    const uint32_t t_last = static_cast<uint32_t>(last / a.n_head);
+    const bool one_token = t_first == t_last;
+    // sequences that start at or before the first row's token: its own is the last of them
+    uint32_t before = 0;
+    for (uint32_t s0 = 0; s0 <= a.n_seq && a.n_seq; s0 += NT) {
+        const uint32_t s = s0 + tid;
+        before += __syncthreads_count(s <= a.n_seq && __ldg(a.q_start + s) <= static_cast<int32_t>(t_first));
+    }
     cudaGridDependencySynchronize();
     uint32_t bad = 0;
-    for (uint32_t i = threadIdx.x; i < n_cta; i += blockDim.x) bad |= l.fail[i];
-    if (threadIdx.x < kJoinRows) {
-        const Plan &p = *l.plan;
+    for (uint32_t i = tid; i < n_cta; i += NT) bad |= l.fail[i];
+    if (tid < kJoinRows) {
+        const Plan p = *l.plan;
         JoinRow d{};
-        const uint64_t x = row0 + threadIdx.x;
-        const uint32_t t = static_cast<uint32_t>(x / a.n_head);
+        const uint64_t x = row0 + tid;
+        const uint32_t t = one_token ? t_first : static_cast<uint32_t>(x / a.n_head);
         const uint32_t head = static_cast<uint32_t>(x - static_cast<uint64_t>(t) * a.n_head);
         const uint32_t h = head / G, gq = head - h * G;
-        uint32_t seq = 0;
-        d.write = t < a.n_q;
+        uint32_t from = before;
+        d.write = x <= last;
         if (d.write && a.n_seq) {
-            // the last sequence that starts at or before t
-            uint32_t lo = 0, hi = a.n_seq + 1;
-            while (lo < hi) {
-                const uint32_t mid = (lo + hi) / 2;
-                if (a.q_start[mid] <= static_cast<int32_t>(t))
-                    lo = mid + 1;
-                else
-                    hi = mid;
-            }
-            d.write = lo >= 1 && lo <= a.n_seq;
-            seq = lo - 1;
+            while (t != t_first && from <= a.n_seq && __ldg(a.q_start + from) <= static_cast<int32_t>(t))
+                ++from;
+            d.write = from >= 1 && from <= a.n_seq;
         }
         if (d.write && p.np && t >= p.q0 && (t - p.q0) * G + gq < p.rows) {
             const uint32_t r = (t - p.q0) * G + gq, pair = r / PR, pg = pair / p.gs;
-            const uint64_t u = static_cast<uint64_t>(pg) * H + h;
+            const uint32_t u = pg * H + h;
+            const uint64_t x0 = static_cast<uint64_t>(u) * p.np;
             d.cuts[0] = p.pre;
-            d.x0[0] = u * p.np;
-            d.x1[0] = d.x0[0] + p.np;
-            d.slot0[0] = static_cast<uint32_t>(u) * p.gs + pair - pg * p.gs;
+            d.first[0] = p.pre.owner(x0);
+            d.n[0] = p.pre.owner(x0 + p.np - 1) + 1 - d.first[0];
+            d.slot0[0] = u * p.gs + pair - pg * p.gs;
             d.step[0] = p.gs;
-            d.both[0] = p.rows - pair * PR > 128 && NS == 2;
+            d.per[0] = NS == 2 && p.rows - pair * PR <= 128 ? 2 : 1;
             d.row[0] = r % 128;
             d.stream[0] = r % PR / 128;
         }
         if (d.write && a.n_seq) {
+            const uint32_t seq = from - 1;
+            const uint64_t seq_tile = l.seq_tile[seq];
+            const uint32_t seq_pair = l.seq_pair[seq];
             const SeqShape sh = seq_shape(a, seq);
             const TileGeom<C::BN> tg(a.tail.pages.page_tokens);
             const uint32_t tiles = tg.tiles(sh.len), i = t - sh.q0;
             if (t >= sh.q0 && i < sh.q_len && tiles && p.t_total) {
                 const uint32_t r = i * G + gq, pair = r / PR, u = pair * H + h;
-                const uint64_t base = p.gs == 1 ? p.p_total : 0;
+                const uint32_t n = min(tiles, pair_tiles<C::BN, PR>(sh, tg, pair, G));
+                const uint64_t x0 = (p.gs == 1 ? p.p_total : 0) + seq_tile + static_cast<uint64_t>(u) * tiles;
                 d.cuts[1] = p.own;
-                d.x0[1] = base + l.seq_tile[seq] + static_cast<uint64_t>(u) * tiles;
-                d.x1[1] = d.x0[1] + min(tiles, pair_tiles<C::BN, PR>(sh, tg, pair, G));
-                d.slot0[1] = p.t_slot0 + l.seq_pair[seq] * H + u;
+                if (n) {
+                    d.first[1] = p.own.owner(x0);
+                    d.n[1] = p.own.owner(x0 + n - 1) + 1 - d.first[1];
+                }
+                d.slot0[1] = p.t_slot0 + seq_pair * H + u;
                 d.step[1] = 1;
-                d.both[1] = sh.q_len * G - pair * PR > 128 && NS == 2;
+                d.per[1] = NS == 2 && sh.q_len * G - pair * PR <= 128 ? 2 : 1;
                 d.row[1] = r % 128;
                 d.stream[1] = r % PR / 128;
             }
         }
-        for (int k = 0; k < 2; ++k)
-            if (d.x1[k] > d.x0[k]) {
-                d.first[k] = d.cuts[k].owner(d.x0[k]);
-                d.n[k] = d.cuts[k].owner(d.x1[k] - 1) + 1 - d.first[k];
-            }
-        rows[threadIdx.x] = d;
+        rows[tid] = d;
     }
     bad = __syncthreads_or(bad);
     // a warp lists a row's pieces and weighs them
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (uint32_t w = warp; w < kJoinRows; w += blockDim.x / 32) {
+    const uint32_t warp = tid >> 5, lane = tid & 31;
+    for (uint32_t w = warp; w < kJoinRows; w += NT / 32) {
         const JoinRow &d = rows[w];
         uint32_t n = 0;
-        float top = -INFINITY;
-        for (int k = 0; k < 2; ++k) {
-            const uint32_t per = NS == 2 && !d.both[k] ? 2 : 1;
-            for (uint32_t i0 = 0; i0 < d.n[k] * per; i0 += 32) {
-                const uint32_t i = i0 + lane, part = d.first[k] + i / per;
-                bool ok = i < d.n[k] * per;
-                uint32_t id = 0;
-                float m = -INFINITY;
-                if (ok) {
-                    id = ((d.slot0[k] + part * d.step[k]) * NS + (per == 2 ? i % 2 : d.stream[k])) * 128 +
-                         d.row[k];
-                    m = l.ml[id].x;
-                    ok = m != -INFINITY;
-                }
-                const uint32_t have = __ballot_sync(0xffffffffu, ok);
-                if (ok) {
-                    const uint32_t at = n + __popc(have & ((1u << lane) - 1));
-                    s_id[w][at] = id;
-                    s_w[w][at] = m;
-                    top = fmaxf(top, m);
-                }
-                n += __popc(have);
+        float top = -INFINITY, sum = 0.0f;
+        const uint32_t n_pre = d.n[0] * d.per[0], n_all = n_pre + d.n[1] * d.per[1];
+        for (uint32_t i0 = 0; i0 < n_all; i0 += 32) {
+            const uint32_t k = i0 + lane >= n_pre ? 1 : 0, i = i0 + lane - (k ? n_pre : 0);
+            uint32_t id = 0;
+            float2 ml = make_float2(-INFINITY, 0.0f);
+            if (i0 + lane < n_all) {
+                const uint32_t two = d.per[k] == 2, part = d.first[k] + (two ? i / 2 : i);
+                id = ((d.slot0[k] + part * d.step[k]) * NS + (two ? i % 2 : d.stream[k])) * 128 + d.row[k];
+                ml = l.ml[id];
             }
-        }
-        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        __syncwarp();
-        float sum = 0.0f;
-        for (uint32_t i = lane; i < n; i += 32) {
-            const float f = ex2(s_w[w][i] - top);
-            sum += f * l.ml[s_id[w][i]].y;
-            s_w[w][i] = f;
+            const uint32_t have = __ballot_sync(0xffffffffu, ml.x != -INFINITY);
+            float mt = ml.x;
+            for (int o = 16; o; o >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, o));
+            mt = fmaxf(mt, top);
+            // the weights so far, and this lane's, against the new maximum
+            const float f = top == -INFINITY ? 0.0f : ex2(top - mt);
+            for (uint32_t j = lane; j < n; j += 32) s_w[w][j] *= f;
+            sum *= f;
+            top = mt;
+            if (ml.x != -INFINITY) {
+                const uint32_t at = n + __popc(have & ((1u << lane) - 1));
+                const float e = ex2(ml.x - top);
+                s_id[w][at] = id;
+                s_w[w][at] = e;
+                sum += e * ml.y;
+            }
+            n += __popc(have);
+            __syncwarp();
         }
         for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == 0) {
@@ -912,19 +934,28 @@ __global__ void __launch_bounds__(kJoinRows *D / 4)
         }
     }
     __syncthreads();
-    const uint32_t r = threadIdx.x % kJoinRows, col = threadIdx.x / kJoinRows;
+    const uint32_t r = tid % kJoinRows, col = tid / kJoinRows;
     if (!rows[r].write) return;
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     const uint32_t n = s_n[r];
-#pragma unroll 4
-    for (uint32_t i = 0; i < n; ++i) {
-        const uint32_t id = s_id[r][i];
-        const float f = s_w[r][i];
-        const float4 o = l.o[(static_cast<uint64_t>(id / 128) * (D / 4) + col) * 128 + id % 128];
-        acc.x = __fmaf_rn(f, o.x, acc.x);
-        acc.y = __fmaf_rn(f, o.y, acc.y);
-        acc.z = __fmaf_rn(f, o.z, acc.z);
-        acc.w = __fmaf_rn(f, o.w, acc.w);
+    for (uint32_t i0 = 0; i0 < n; i0 += 16) {
+        float4 o[16];
+#pragma unroll
+        for (uint32_t i = 0; i < 16; ++i) {
+            o[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (i0 + i < n) {
+                const uint32_t id = s_id[r][i0 + i];
+                o[i] = l.o[(static_cast<uint64_t>(id / 128) * (D / 4) + col) * 128 + id % 128];
+            }
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < 16; ++i) {
+            const float f = i0 + i < n ? s_w[r][i0 + i] : 0.0f;
+            acc.x = __fmaf_rn(f, o[i].x, acc.x);
+            acc.y = __fmaf_rn(f, o[i].y, acc.y);
+            acc.z = __fmaf_rn(f, o[i].z, acc.z);
+            acc.w = __fmaf_rn(f, o[i].w, acc.w);
+        }
     }
     const float inv = s_inv[r];
     *reinterpret_cast<uint2 *>(a.out + (row0 + r) * D + 4 * col) =
