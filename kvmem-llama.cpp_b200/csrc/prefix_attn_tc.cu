@@ -35,6 +35,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "kvmret.h"
 #include "prefix_attn_plan.cuh"
@@ -196,7 +197,8 @@ __device__ bool make_plan(const AttnLaunch &l, Plan &p, Start &start) {
         if (s >= a.n_seq) return;
         const SeqShape sh = seq_shape(a, s);
         pairs = (sh.q_len * G + PR - 1) / PR;
-        tiles = static_cast<uint64_t>(sh.q_len ? tg.tiles(sh.len) : 0) * pairs * H;
+        const uint32_t n = sh.q_len ? tg.tiles(sh.len) : 0;
+        tiles = static_cast<uint64_t>(n ? n + kUnit : 0) * pairs * H;
     };
     const bool pre = a.prefix.max_len != 0;
     const int32_t len0 = pre && a.prefix.len ? __ldg(a.prefix.len) : 0x7fffffff;
@@ -576,6 +578,8 @@ __global__ void __launch_bounds__(Cfg<D>::threads, 1)
         const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;  // a negative scale turns Q
         const uint32_t ts = tmem + ((32 * qd) << 16) + C::s_col(s);
         const uint32_t to = tmem + ((32 * qd) << 16) + C::o_col(s);
+        constexpr uint32_t kRows = 128 / (D / 8);  // rows that one pass of the Q load covers
+        const uint32_t step_t = kRows / G, step_h = kRows - step_t * G;
         uint32_t ns = 0, sg = 0;  // tiles and pieces so far
         Seg g = {};
         Share<NS> sh = {};
@@ -597,23 +601,31 @@ __global__ void __launch_bounds__(Cfg<D>::threads, 1)
             }
             const uint32_t rows = row_count(), at0 = g.row0 + row_first();
             constexpr uint32_t CH = D / 8, RS = 128 / CH;  // 16-byte chunks of a row; rows a pass
-            constexpr uint32_t QL = CH < 16 ? CH : 16;      // loads in flight
-            const uint32_t ch = tid % CH;
+            const uint32_t ch = tid % CH, q1 = tid / CH;
+            const uint16_t *const q = a.q + static_cast<uint64_t>(g.q0) * a.q_stride +
+                                      static_cast<uint64_t>(g.h) * G * D + 8 * ch;
+            uint32_t t = (at0 + q1) / G, hg = at0 + q1 - t * G;
+            // n passes: all loads first. Only warps that hold a row look at their
+            // scores, so rows past the last one of 32 stay as they are.
+            auto load = [&](uint32_t i0, auto n) {
+                constexpr uint32_t N = decltype(n)::value;
+                uint4 w[N];
 #pragma unroll
-            for (uint32_t i0 = 0; i0 < CH; i0 += QL) {
-                uint4 w[QL];
-#pragma unroll
-                for (uint32_t i = 0; i < QL; ++i) {  // all loads first
-                    const uint32_t qr = tid / CH + (i0 + i) * RS, rr = at0 + qr, t = rr / G;
+                for (uint32_t i = 0; i < N; ++i) {
                     w[i] = make_uint4(0, 0, 0, 0);
-                    if (qr < rows)
+                    if (q1 + (i0 + i) * RS < rows)
                         w[i] = __ldg(reinterpret_cast<const uint4 *>(
-                            a.q + static_cast<uint64_t>(g.q0 + t) * a.q_stride +
-                            static_cast<uint64_t>(g.h * G + rr - t * G) * D + 8 * ch));
+                            q + static_cast<uint64_t>(t) * a.q_stride + hg * D));
+                    t += step_t;
+                    hg += step_h;
+                    if (hg >= G) {
+                        hg -= G;
+                        ++t;
+                    }
                 }
 #pragma unroll
-                for (uint32_t i = 0; i < QL; ++i) {
-                    const uint32_t qr = tid / CH + (i0 + i) * RS;
+                for (uint32_t i = 0; i < N; ++i) {
+                    const uint32_t qr = q1 + (i0 + i) * RS;
                     const uint32_t at = base + s * C::q_bytes + (ch / 8) * QB + qr * 128 +
                                         (((ch % 8) ^ (qr % 8)) * 16);
                     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at),
@@ -621,6 +633,13 @@ __global__ void __launch_bounds__(Cfg<D>::threads, 1)
                                  "r"(w[i].w ^ sign)
                                  : "memory");
                 }
+            };
+            if (rows <= 32) {
+                load(0, std::integral_constant<uint32_t, 32 / RS>());
+            } else {
+                constexpr uint32_t QL = CH < 16 ? CH : 16;  // loads in flight
+#pragma unroll
+                for (uint32_t i0 = 0; i0 < CH; i0 += QL) load(i0, std::integral_constant<uint32_t, QL>());
             }
             fence_async_smem();
             __syncwarp();
@@ -652,13 +671,13 @@ __global__ void __launch_bounds__(Cfg<D>::threads, 1)
                     if (!whole) {
                         const uint32_t k = 2 * jj + 1;
                         if (!wait(full(k % ST), (k / ST) & 1u)) break;
-                        for (uint32_t i = tid; i < BN * (D / 64); i += 128) {
-                            const uint32_t key = i % BN;
+                        for (uint32_t i = tid; i < BN * 8; i += 128) {  // a lane 16 bytes
+                            const uint32_t key = i / 8;
                             if (s_mask[jj % kMeta][key / 32] >> (key % 32) & 1u) continue;
-                            const uint32_t at = ring + (k % ST) * C::stage + (i / BN) * KB + key * 128;
+                            const uint32_t at = ring + (k % ST) * C::stage + i * 16;
 #pragma unroll
-                            for (uint32_t z = 0; z < 128; z += 16)
-                                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at + z),
+                            for (uint32_t z = 0; z < D / 64; ++z)
+                                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at + z * KB),
                                              "r"(0u)
                                              : "memory");
                         }
@@ -686,8 +705,8 @@ __global__ void __launch_bounds__(Cfg<D>::threads, 1)
                 if (!idle) {
                     // One pass with the maximum as it stands: p and the tile's own
                     // maximum together, 32 columns at a time with the next ones on their
-                    // way. Only when a row's maximum has moved by more than 8 (and for
-                    // the first tile, whose maximum is taken beforehand) the pass is
+                    // way (a piece's first tile starts with that of its first columns).
+                    // Only when a row's maximum has moved by more than 8 the pass is
                     // repeated with the new one; S still stands, P is in registers.
                     uint32_t y[32], pk[BN / 2];
                     float top = -INFINITY, s0, s1;
@@ -696,8 +715,8 @@ __global__ void __launch_bounds__(Cfg<D>::threads, 1)
                         for (int k = 0; k < 32; k += 2)
                             top = fmaxf(top, fmaxf(__uint_as_float(v[k]), __uint_as_float(v[k + 1])));
                     };
-                    auto pass = [&] {
-                        const float neg = m == -INFINITY ? 0.0f : -m;
+                    auto pass = [&](bool first) {
+                        float neg = m == -INFINITY ? 0.0f : -m;
                         s0 = s1 = 0.0f;
                         top = -INFINITY;
                         tmem_ld32_nowait(ts, x);
@@ -707,6 +726,10 @@ __global__ void __launch_bounds__(Cfg<D>::threads, 1)
                             tmem_ld_wait(v);
                             if (w + 1 < BN / 32) tmem_ld32_nowait(ts + 32 * (w + 1), w & 1 ? x : y);
                             column_max(v);
+                            if (w == 0 && first) {
+                                m = top * c;
+                                neg = m == -INFINITY ? 0.0f : -m;
+                            }
 #pragma unroll
                             for (int k = 0; k < 16; ++k) {
                                 uint32_t e0 = v[2 * k], e1 = v[2 * k + 1];
@@ -717,18 +740,11 @@ __global__ void __launch_bounds__(Cfg<D>::threads, 1)
                             }
                         }
                     };
-                    if (begin) {
-#pragma unroll 1
-                        for (uint32_t w = 0; w < BN / 32; ++w) {
-                            tmem_ld32_nowait(ts + 32 * w, x);
-                            tmem_ld_wait(x);
-                            column_max(x);
-                        }
-                        m = top * c;
-                    }
+                    bool first = begin;
 #pragma unroll 1
                     for (;;) {
-                        pass();
+                        pass(first);
+                        first = false;
                         if (!__any_sync(0xffffffffu, top * c > m + 8.0f)) break;
                         const float mn = fmaxf(m, top * c);
                         const float f = m == -INFINITY ? 0.0f : ex2(m - mn);
@@ -874,7 +890,8 @@ __global__ void __launch_bounds__(kJoinRows *D / 4)
             if (t >= sh.q0 && i < sh.q_len && tiles && p.t_total) {
                 const uint32_t r = i * G + gq, pair = r / PR, u = pair * H + h;
                 const uint32_t n = min(tiles, pair_tiles<C::BN, PR>(sh, tg, pair, G));
-                const uint64_t x0 = (p.gs == 1 ? p.p_total : 0) + seq_tile + static_cast<uint64_t>(u) * tiles;
+                const uint64_t x0 = (p.gs == 1 ? p.p_total : 0) + seq_tile +
+                                    static_cast<uint64_t>(u) * (tiles + kUnit) + kUnit;
                 d.cuts[1] = p.own;
                 if (n) {
                     d.first[1] = p.own.owner(x0);
