@@ -134,6 +134,13 @@ int prefix_attn_call(const KeyList &prefix, const kvmret_pages *tail, const kvmr
         r.tail.n_list = a->tail_pages;
         r.tail.max_len = static_cast<uint32_t>(most);
     }
+    // 32-bit rows and tile counts (at least 16 tokens a tile)
+    const uint64_t units = static_cast<uint64_t>(a->n_q) * (a->n_head / pv.n_head_kv) / 128 + a->n_seq + 1;
+    const uint64_t reach = r.prefix.max_len / 16ull + r.tail.max_len / 16ull + 4;
+    if (static_cast<uint64_t>(a->n_q) * a->n_head > 0x7fffffffull ||
+        reach > 0xffffffffull / pv.n_head_kv / units)
+        return fail(KVMRET_ERR_ARG, "%u rows of %u heads over %u + %u tokens are too many for one call",
+                    a->n_q, a->n_head, r.prefix.max_len, r.tail.max_len);
     r.q = a->q_dev;
     r.out = a->out_dev;
     r.lse = a->lse_dev;

@@ -1,5 +1,5 @@
 // Work split of the shared-prefix attention, computed on the device from the
-// lengths and read alike by the attention kernel and by the join.
+// lengths.
 //
 // Rows: the G = n_head / n_head_kv query heads of a KV head stand as rows
 // r = token * G + head beside one another, so one tile of keys serves all of
@@ -7,8 +7,9 @@
 // tiles of BN. The units' tiles, laid end to end, are cut into equal
 // contiguous ranges, one per CTA, so a long list is shared by many CTAs and a
 // short one by none; each (unit, CTA) piece leaves its unnormalised output,
-// maximum and sum in a workspace slot, and the join adds a row's pieces in a
-// fixed order, so results repeat run to run.
+// maximum and sum in a workspace slot (one part for each row tile), and the join
+// adds a row's pieces in a fixed order, so results repeat run to run. Where a
+// row's pieces lie is written down by a spare warp of the attention kernel.
 //   Prefix: when a KV head has more than PR rows (n_pair > 1), `gs` CTAs walk
 //     the same keys side by side, one row pair each, so that all but one of
 //     them find the tile in L2; the ranges are then per group of gs CTAs.
@@ -50,36 +51,32 @@ struct TileGeom {
     }
 };
 
-// Quotient of tile counts: 32-bit division where both fit.
-__device__ __forceinline__ uint64_t quot(uint64_t x, uint64_t d) {
-    return ((x | d) >> 32) ? x / d : static_cast<uint32_t>(x) / static_cast<uint32_t>(d);
-}
-
 // A line of tiles cut into `parts` ranges: the first r of them hold q + 1.
 struct Cuts {
-    uint64_t q;
-    uint32_t r;
-    __device__ __forceinline__ void set(uint64_t total, uint32_t parts) {
-        q = quot(total, parts);
-        r = static_cast<uint32_t>(total - q * parts);
+    uint32_t q, r;
+    __device__ __forceinline__ void set(uint32_t total, uint32_t parts) {
+        q = total / parts;
+        r = total - q * parts;
     }
-    __device__ __forceinline__ uint64_t at(uint32_t i) const { return q * i + min(i, r); }
+    __device__ __forceinline__ uint32_t at(uint32_t i) const { return q * i + min(i, r); }
     // the range that holds tile x of the line
-    __device__ __forceinline__ uint32_t owner(uint64_t x) const {
-        const uint64_t head = (q + 1) * r;
-        return static_cast<uint32_t>(x < head ? quot(x, q + 1) : r + quot(x - head, q));
+    __device__ __forceinline__ uint32_t owner(uint32_t x) const {
+        const uint32_t head = (q + 1) * r;
+        return x < head ? x / (q + 1) : r + (x - head) / q;
     }
 };
 
-// The header of the workspace.
+// The split, alike in every CTA. (Tile counts fit 32 bits: the host checks their
+// bound.)
 struct Plan {
-    uint64_t p_total, t_total;  // tiles of the prefix line and of the tails
+    uint32_t p_total, t_total;  // tiles of the prefix line and of the tails
     Cuts pre, own;              // their ranges (gs == 1: of the joint line)
     uint32_t np;                // tiles of the prefix
     uint32_t p_len;             // its tokens
     uint32_t q0, rows;          // first row token; rows of a KV head (all sequences)
     uint32_t n_pair, n_pg, gs, groups;
     uint32_t t_slot0;           // first workspace slot of the tails
+    uint32_t ok;                // 0: q_start descends somewhere, nothing is done
 };
 
 // Rows and keys of one sequence, all cut to what the host's bounds allow.
@@ -124,16 +121,15 @@ struct Walk {
     const PrefixAttn &a;
     const Plan &p;  // in shared memory
     uint32_t G, cta;
-    uint64_t x, x1;       // prefix line: next tile, end
+    uint32_t x, x1;       // prefix line: next tile, end
     uint32_t part, lane;  // the range and the CTA's place in its group
-    uint64_t y, y1;       // tails' line
+    uint32_t y, y1;       // tails' line
     uint32_t seq;         // the sequence that holds y, its first tile and pair
-    uint64_t seq_tile;
-    uint32_t seq_pair;
+    uint32_t seq_tile, seq_pair;
     SeqShape sh;
     bool fresh;
 
-    __device__ __forceinline__ Walk(const PrefixAttn &a_, const Plan &p_, uint32_t s, uint64_t tile,
+    __device__ __forceinline__ Walk(const PrefixAttn &a_, const Plan &p_, uint32_t s, uint32_t tile,
                                     uint32_t pair)
         : a(a_), p(p_), G(a_.n_head / a_.n_head_kv), cta(blockIdx.x), seq(s),
           seq_tile(tile), seq_pair(pair), fresh(true) {
@@ -141,10 +137,10 @@ struct Walk {
         part = cta / p.gs;
         lane = cta - part * p.gs;
     }
-    static __device__ __forceinline__ void ranges(const Plan &p, uint32_t cta, uint64_t &x,
-                                                  uint64_t &x1, uint64_t &y, uint64_t &y1) {
+    static __device__ __forceinline__ void ranges(const Plan &p, uint32_t cta, uint32_t &x,
+                                                  uint32_t &x1, uint32_t &y, uint32_t &y1) {
         if (p.gs == 1) {
-            const uint64_t b = p.pre.at(cta), e = p.pre.at(cta + 1);
+            const uint32_t b = p.pre.at(cta), e = p.pre.at(cta + 1);
             x = min(b, p.p_total);
             x1 = min(e, p.p_total);
             y = max(b, p.p_total) - p.p_total;
@@ -160,23 +156,21 @@ struct Walk {
 
     __device__ __forceinline__ bool next(Seg &g) {
         while (x < x1) {
-            const uint64_t u = quot(x, p.np);
-            const uint32_t t = static_cast<uint32_t>(x - u * p.np);
-            const uint32_t n = static_cast<uint32_t>(min(x1 - x, static_cast<uint64_t>(p.np - t)));
+            const uint32_t u = x / p.np, t = x - u * p.np, n = min(x1 - x, p.np - t);
             x += n;
-            const uint32_t pair = static_cast<uint32_t>(quot(u, a.n_head_kv)) * p.gs + lane;
+            const uint32_t pg = u / a.n_head_kv, pair = pg * p.gs + lane;
             if (pair >= p.n_pair) continue;
             g.tail = 0;
             g.seq = 0;
             g.len = p.p_len;
             g.q_len = 0;
-            g.h = static_cast<uint32_t>(u - quot(u, a.n_head_kv) * a.n_head_kv);
+            g.h = u - pg * a.n_head_kv;
             g.q0 = p.q0;
             g.row0 = pair * PR;
             g.rows = min(static_cast<uint32_t>(PR), p.rows - g.row0);
             g.tile0 = t;
             g.n = n;
-            g.slot = (static_cast<uint32_t>(u) + part) * p.gs + lane;
+            g.slot = (u + part) * p.gs + lane;
             return true;
         }
         const TileGeom<BN> geom(a.tail.pages.page_tokens);
@@ -185,7 +179,7 @@ struct Walk {
             fresh = false;
             const uint32_t tiles = sh.q_len ? geom.tiles(sh.len) : 0;
             const uint32_t pairs = (sh.q_len * G + PR - 1) / PR;
-            const uint64_t mine = static_cast<uint64_t>(tiles ? tiles + kUnit : 0) * pairs * a.n_head_kv;
+            const uint32_t mine = (tiles ? tiles + kUnit : 0) * pairs * a.n_head_kv;
             if (y >= seq_tile + mine) {
                 seq_tile += mine;
                 seq_pair += pairs;
@@ -193,11 +187,8 @@ struct Walk {
                 fresh = true;
                 continue;
             }
-            const uint64_t at = y - seq_tile;
-            const uint32_t all = tiles + kUnit;
-            const uint32_t u = static_cast<uint32_t>(quot(at, all));
-            uint32_t t = static_cast<uint32_t>(at - static_cast<uint64_t>(u) * all);
-            uint32_t n = static_cast<uint32_t>(min(y1 - y, static_cast<uint64_t>(all - t)));
+            const uint32_t at = y - seq_tile, all = tiles + kUnit, u = at / all;
+            uint32_t t = at - u * all, n = min(y1 - y, all - t);
             y += n;
             if (t + n <= kUnit) continue;
             n -= t < kUnit ? kUnit - t : 0;

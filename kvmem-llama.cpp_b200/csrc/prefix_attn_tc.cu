@@ -14,6 +14,7 @@
 //          and V tiles into a ring of shared-memory stages (128-byte swizzle,
 //          no multicast);
 //   2      walks the pieces and leaves each in a short ring for the others;
+//   3      notes for the join where each row's pieces lie;
 //   1      one lane issues the products: S = Q K^T (both in shared memory)
 //          and O += P V (P in tensor memory over its S, V as it lies: keys
 //          along K, MN-major);
@@ -54,7 +55,7 @@ struct Cfg {
     static constexpr uint32_t stage = BN * D * 2;   // one K or V tile
     static constexpr int stages = D == 64 ? 8 : 5;
     static constexpr uint32_t q_bytes = 128 * D * 2;
-    static constexpr uint32_t smem = NS * q_bytes + stages * stage + 1024;
+    static constexpr uint32_t tiles = NS * q_bytes + stages * stage;
     static __host__ __device__ constexpr uint32_t s_col(int s) { return s * 128; }
     static __host__ __device__ constexpr uint32_t o_col(int s) { return 256 + s * (D == 64 ? 64 : 128); }
 };
@@ -62,15 +63,19 @@ constexpr uint32_t kAttnTmem = 512;
 constexpr int kSegs = 4;  // pieces ahead
 constexpr int kMeta = 8;  // tiles whose masks are held (more than the ring reaches back)
 
+// Where one row's pieces lie: entry i of n has its statistics at ml[id + i *
+// step], its output in the same slot and row.
+struct RowPieces {
+    uint32_t id, step, n, pad;
+};
+
 struct AttnLaunch {
     PrefixAttn a;
     CUtensorMap map[4];  // prefix K, V, tail K, V
-    Plan *plan;
-    uint32_t *fail;      // [CTA] 1: a wait gave up, or more pieces than slots
-    uint64_t *seq_tile;  // [n_seq] first tile of each sequence on the tails' line
-    uint32_t *seq_pair;  // [n_seq] its first row pair
-    float2 *ml;          // [slot][stream][128]
-    float4 *o;           // [slot][stream][D / 4][128]
+    uint32_t *fail;  // [CTA] 1: a wait gave up, or q_start was not ascending
+    RowPieces *at;   // [n_q * n_head][2] pieces of the prefix, of the tail
+    float2 *ml;      // [slot][row tile][128] maximum and sum
+    float4 *o;       // [slot][row tile][D / 4][128]
     uint32_t max_slots;
 };
 
@@ -177,13 +182,23 @@ __device__ __forceinline__ bool elect_one() {
     return p;
 }
 
-// The plan of the split, by one warp, in every CTA alike; CTA 0 also leaves it
-// and the sequences' offsets in the workspace for the join. `start` receives
-// the sequence that holds the CTA's first tail tile.
+// The plan of the split, by one warp, in every CTA alike. `start` receives the
+// sequence that holds the CTA's first tail tile. False when q_start descends.
 struct Start {
-    uint32_t seq, pair;
-    uint64_t tile;
+    uint32_t seq, pair, tile;
 };
+// inclusive sums over the warp's lanes
+__device__ __forceinline__ void scan(uint32_t &x, uint32_t &y) {
+    const uint32_t lane = threadIdx.x & 31;
+    for (uint32_t o = 1; o < 32; o <<= 1) {
+        const uint32_t u = __shfl_up_sync(0xffffffffu, x, o), v = __shfl_up_sync(0xffffffffu, y, o);
+        if (lane >= o) {
+            x += u;
+            y += v;
+        }
+    }
+}
+
 template <int D>
 __device__ bool make_plan(const AttnLaunch &l, Plan &p, Start &start) {
     constexpr int BN = Cfg<D>::BN, PR = Cfg<D>::PR;
@@ -191,33 +206,32 @@ __device__ bool make_plan(const AttnLaunch &l, Plan &p, Start &start) {
     const uint32_t lane = threadIdx.x & 31;
     const uint32_t G = a.n_head / a.n_head_kv, H = a.n_head_kv;
     const TileGeom<BN> tg(a.n_seq ? a.tail.pages.page_tokens : BN);
-    auto shape = [&](uint32_t s, uint64_t &tiles, uint32_t &pairs) {
-        tiles = 0;
-        pairs = 0;
+    bool ok = true;
+    auto shape = [&](uint32_t s, uint32_t &tiles, uint32_t &pairs) {
+        tiles = pairs = 0;
         if (s >= a.n_seq) return;
+        ok = ok && __ldg(a.q_start + s) <= __ldg(a.q_start + s + 1);
         const SeqShape sh = seq_shape(a, s);
         pairs = (sh.q_len * G + PR - 1) / PR;
         const uint32_t n = sh.q_len ? tg.tiles(sh.len) : 0;
-        tiles = static_cast<uint64_t>(n ? n + kUnit : 0) * pairs * H;
+        tiles = (n ? n + kUnit : 0) * pairs * H;
     };
     const bool pre = a.prefix.max_len != 0;
     const int32_t len0 = pre && a.prefix.len ? __ldg(a.prefix.len) : 0x7fffffff;
     const int32_t q_first = a.n_seq ? __ldg(a.q_start) : 0;
     const int32_t q_last = a.n_seq ? __ldg(a.q_start + a.n_seq) : static_cast<int32_t>(a.n_q);
     // totals of the tails; the last listed page that holds tokens
-    uint64_t tiles = 0, pairs = 0, t0;
-    uint32_t n0;
+    uint32_t t0, n0;
     shape(lane, t0, n0);
-    tiles = t0;
-    pairs = n0;
+    uint32_t tiles = t0, pairs = n0;
 #pragma unroll 4
     for (uint32_t s = 32 + lane; s < a.n_seq; s += 32) {
-        uint64_t t;
-        uint32_t n;
+        uint32_t t, n;
         shape(s, t, n);
         tiles += t;
         pairs += n;
     }
+    ok = __all_sync(0xffffffffu, ok);
     uint32_t held = pre ? a.prefix.n_list : 0;
     if (held && a.prefix.ntok) {
         held = 0;
@@ -250,11 +264,12 @@ __device__ bool make_plan(const AttnLaunch &l, Plan &p, Start &start) {
         p.n_pg = (p.n_pair + p.gs - 1) / p.gs;
     }
     p.groups = p.gs == 1 ? gridDim.x : gridDim.x / p.gs;
-    p.p_total = static_cast<uint64_t>(p.np) * p.n_pg * H;
+    p.p_total = p.np * p.n_pg * H;
     p.t_total = tiles;
     p.t_slot0 = (p.n_pg * H + p.groups) * p.gs;
-    const bool ok = p.t_slot0 + pairs * H + gridDim.x <= l.max_slots;
-    if (!ok) p.p_total = p.t_total = 0;  // q_start was not ascending
+    ok = ok && p.t_slot0 + pairs * H + gridDim.x <= l.max_slots;  // (so it is when it ascends)
+    p.ok = ok;
+    if (!ok) p.p_total = p.t_total = 0;
     if (p.gs == 1) {
         p.pre.set(p.p_total + p.t_total, gridDim.x);
         p.own = p.pre;
@@ -263,40 +278,24 @@ __device__ bool make_plan(const AttnLaunch &l, Plan &p, Start &start) {
         p.own.set(p.t_total, gridDim.x);
     }
     start = {0, 0, 0};
-    uint64_t x, x1, y, y1;
+    uint32_t x, x1, y, y1;
     Walk<BN, PR>::ranges(p, blockIdx.x, x, x1, y, y1);
-    if (blockIdx.x == 0 && lane == 0) *l.plan = p;
-    if (y >= y1 && blockIdx.x != 0) return ok;  // no tails here
-    uint64_t base_t = 0;
-    uint32_t base_p = 0;
+    if (y >= y1) return ok;  // no tails here
+    uint32_t base_t = 0, base_p = 0;
     for (uint32_t s0 = 0; s0 < a.n_seq; s0 += 32) {
-        const uint32_t s = s0 + lane;
-        if (s0) shape(s, t0, n0);
-        uint64_t ti = t0;
-        uint32_t pi = n0;
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint64_t u = __shfl_up_sync(0xffffffffu, ti, o);
-            const uint32_t v = __shfl_up_sync(0xffffffffu, pi, o);
-            if (lane >= o) {
-                ti += u;
-                pi += v;
-            }
-        }
-        const uint64_t all_t = __shfl_sync(0xffffffffu, ti, 31);
-        const uint32_t all_p = __shfl_sync(0xffffffffu, pi, 31);
+        if (s0) shape(s0 + lane, t0, n0);
+        uint32_t ti = t0, pi = n0;
+        scan(ti, pi);
+        const uint32_t all_t = __shfl_sync(0xffffffffu, ti, 31), all_p = __shfl_sync(0xffffffffu, pi, 31);
         ti += base_t - t0;
         pi += base_p - n0;
-        if (blockIdx.x == 0 && s < a.n_seq) {
-            l.seq_tile[s] = ti;
-            l.seq_pair[s] = pi;
-        }
-        const uint32_t hit = __ballot_sync(0xffffffffu, y < y1 && y >= ti && y < ti + t0);
+        const uint32_t hit = __ballot_sync(0xffffffffu, y >= ti && y < ti + t0);
         if (hit) {
             const int w = __ffs(hit) - 1;
             start.seq = s0 + w;
             start.pair = __shfl_sync(0xffffffffu, pi, w);
             start.tile = __shfl_sync(0xffffffffu, ti, w);
-            if (blockIdx.x != 0) break;
+            break;
         }
         base_t += all_t;
         base_p += all_p;
@@ -304,24 +303,107 @@ __device__ bool make_plan(const AttnLaunch &l, Plan &p, Start &start) {
     return ok;
 }
 
+// Where the pieces of every row lie, for the join: by one warp of each CTA, a
+// lane a row, the CTAs taking blocks of 32 rows in turn.
+template <int D>
+__device__ void note_rows(const AttnLaunch &l, const Plan &p) {
+    constexpr int BN = Cfg<D>::BN, PR = Cfg<D>::PR, NS = Cfg<D>::NS;
+    const PrefixAttn &a = l.a;
+    const uint32_t lane = threadIdx.x & 31, n_cta = gridDim.x;
+    const uint32_t G = a.n_head / a.n_head_kv, H = a.n_head_kv;
+    // rows of the tokens [q0, q0 + q_len); tails from tile `tile` and pair `pair` on
+    auto note = [&](uint32_t q0, uint32_t q_len, const SeqShape *sh, uint32_t tile, uint32_t pair0) {
+        const TileGeom<BN> tg(sh ? a.tail.pages.page_tokens : BN);
+        const uint32_t tiles = sh ? tg.tiles(sh->len) : 0;
+        const uint32_t begin = q0 * a.n_head, end = begin + q_len * a.n_head;
+        uint32_t b = begin / 32;
+        b += (blockIdx.x + n_cta - b % n_cta) % n_cta;  // the first block of this CTA
+        for (; b * 32 < end; b += n_cta) {
+            const uint32_t x = 32 * b + lane;
+            if (x < begin || x >= end) continue;
+            const uint32_t t = x / a.n_head, head = x - t * a.n_head, h = head / G, gq = head - h * G;
+            RowPieces r[2] = {};
+            auto put = [&](RowPieces &e, const Cuts &cuts, uint32_t x0, uint32_t n, uint32_t slot0,
+                           uint32_t step, uint32_t row) {
+                const uint32_t first = cuts.owner(x0);
+                e.n = cuts.owner(x0 + n - 1) + 1 - first;
+                e.id = ((slot0 + first * step) * NS + row % PR / 128) * 128 + row % 128;
+                e.step = step * NS * 128;
+            };
+            if (p.np) {
+                const uint32_t row = (t - p.q0) * G + gq, pair = row / PR, pg = pair / p.gs, u = pg * H + h;
+                put(r[0], p.pre, u * p.np, p.np, u * p.gs + pair - pg * p.gs, p.gs, row);
+            }
+            if (tiles) {
+                const uint32_t row = (t - q0) * G + gq, pair = row / PR, u = pair * H + h;
+                const uint32_t n = min(tiles, pair_tiles<BN, PR>(*sh, tg, pair, G));
+                if (n)
+                    put(r[1], p.own, (p.gs == 1 ? p.p_total : 0) + tile + u * (tiles + kUnit) + kUnit, n,
+                        p.t_slot0 + pair0 * H + u, 1, row);
+            }
+            l.at[2 * x] = r[0];
+            l.at[2 * x + 1] = r[1];
+        }
+    };
+    if (!a.n_seq) {
+        note(0, a.n_q, nullptr, 0, 0);
+        return;
+    }
+    const TileGeom<BN> tg(a.tail.pages.page_tokens);
+    uint32_t base_t = 0, base_p = 0;
+    for (uint32_t s0 = 0; s0 < a.n_seq; s0 += 32) {
+        SeqShape sh = {};
+        if (s0 + lane < a.n_seq) sh = seq_shape(a, s0 + lane);
+        const uint32_t pairs = (sh.q_len * G + PR - 1) / PR, n = sh.q_len ? tg.tiles(sh.len) : 0;
+        const uint32_t tiles = (n ? n + kUnit : 0) * pairs * H;
+        uint32_t ti = tiles, pi = pairs;
+        scan(ti, pi);
+        for (uint32_t w = 0; w < min(32u, a.n_seq - s0); ++w) {
+            SeqShape one;
+            one.q0 = __shfl_sync(0xffffffffu, sh.q0, w);
+            one.q_len = __shfl_sync(0xffffffffu, sh.q_len, w);
+            one.len = __shfl_sync(0xffffffffu, sh.len, w);
+            note(one.q0, one.q_len, &one, base_t + __shfl_sync(0xffffffffu, ti - tiles, w),
+                 base_p + __shfl_sync(0xffffffffu, pi - pairs, w));
+            __syncwarp();
+        }
+        base_t += __shfl_sync(0xffffffffu, ti, 31);
+        base_p += __shfl_sync(0xffffffffu, pi, 31);
+    }
+}
+
+// What a CTA keeps in shared memory behind the tiles.
+template <int D>
+struct Small {
+    static constexpr int NS = Cfg<D>::NS;
+    alignas(16) uint32_t mask[kMeta][4];  // valid keys of a tile
+    float2 ml[NS][128];                   // statistics on their way to the other stream
+    uint64_t bars[2 * Cfg<D>::stages + kMeta + 2 * kSegs + 6 * NS + 2];
+    Plan plan;
+    Seg seg[kSegs];
+    uint32_t tmem, fail;
+};
+static_assert(Cfg<128>::tiles + sizeof(Small<128>) <= 227 * 1024, "shared memory");
+
 template <int D>
 __global__ void __launch_bounds__(Cfg<D>::threads, 1)
     attn_tc_kernel(const __grid_constant__ AttnLaunch l) {
     using C = Cfg<D>;
     constexpr int BN = C::BN, PR = C::PR, NS = C::NS, ST = C::stages;
     constexpr uint32_t KB = BN * 128, QB = 128 * 128;  // bytes of a 64-column block of K / V, of Q
-    extern __shared__ uint8_t smem_raw[];
-    __shared__ Plan plan;
-    __shared__ Seg s_seg[kSegs];
-    __shared__ uint64_t bars[2 * ST + kMeta + 2 * kSegs + 4 * NS + 1];
-    __shared__ __align__(16) uint32_t s_mask[kMeta][4];
-    __shared__ uint32_t s_tmem, s_fail;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    Small<D> &sm = *reinterpret_cast<Small<D> *>(smem_raw + C::tiles);
+    Plan &plan = sm.plan;
 
     const PrefixAttn &a = l.a;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;  // the swizzle atom
+    const uint32_t base = smem_u32(smem_raw);
+    if (base & 1023u) {  // the tiles must lie on the swizzle's atoms
+        if (threadIdx.x == 0) l.fail[blockIdx.x] = 1;
+        return;
+    }
     const uint32_t ring = base + NS * C::q_bytes;
-    const uint32_t bar0 = smem_u32(bars);
+    const uint32_t bar0 = smem_u32(sm.bars);
     auto full = [&](uint32_t i) { return bar0 + 8u * i; };
     auto empty = [&](uint32_t i) { return bar0 + 8u * (ST + i); };
     auto meta = [&](uint32_t i) { return bar0 + 8u * (2 * ST + i); };
@@ -332,10 +414,12 @@ __global__ void __launch_bounds__(Cfg<D>::threads, 1)
     auto s_full = [&](uint32_t s) { return bar0 + 8u * (SB + NS + s); };
     auto p_ready = [&](uint32_t s) { return bar0 + 8u * (SB + 2 * NS + s); };
     auto pv_done = [&](uint32_t s) { return bar0 + 8u * (SB + 3 * NS + s); };
-    const uint32_t drain = bar0 + 8u * (SB + 4 * NS);
+    auto o_done = [&](uint32_t s) { return bar0 + 8u * (SB + 4 * NS + s); };
+    auto o_read = [&](uint32_t s) { return bar0 + 8u * (SB + 5 * NS + s); };
+    const uint32_t drain = bar0 + 8u * (SB + 6 * NS), planned = drain + 8;
 
     if (threadIdx.x == 0) {
-        s_fail = 0;
+        sm.fail = 0;
         for (int i = 0; i < ST; ++i) {
             mbar_init(full(i), 1);
             mbar_init(empty(i), NS);  // one arrival per stream
@@ -350,13 +434,16 @@ __global__ void __launch_bounds__(Cfg<D>::threads, 1)
             mbar_init(s_full(s), 1);
             mbar_init(p_ready(s), 4);
             mbar_init(pv_done(s), 1);
+            mbar_init(o_done(s), 4);
+            mbar_init(o_read(s), 4);
         }
         mbar_init(drain, 1);
+        mbar_init(planned, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                         smem_u32(&s_tmem)),
+                         smem_u32(&sm.tmem)),
                      "r"(kAttnTmem)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -364,7 +451,7 @@ __global__ void __launch_bounds__(Cfg<D>::threads, 1)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
+    const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0);
     bool stop = false;
     // a whole warp's wait; false once it has given up (the warps that wait for
     // this one then do too)
@@ -377,7 +464,10 @@ __global__ void __launch_bounds__(Cfg<D>::threads, 1)
         Start start;
         Plan p;
         if (!make_plan<D>(l, p, start)) stop = true;
-        if (lane == 0) plan = p;
+        if (lane == 0) {
+            plan = p;
+            mbar_arrive(planned);
+        }
         __syncwarp();
         Walk<BN, PR> walk(a, plan, start.seq, start.tile, start.pair);
         uint32_t j = 0;
@@ -389,12 +479,14 @@ __global__ void __launch_bounds__(Cfg<D>::threads, 1)
             }
             if (i >= kSegs && !wait(seg_empty(i % kSegs), (i / kSegs - 1) & 1u)) break;
             if (lane == 0) {
-                s_seg[i % kSegs] = g;
+                sm.seg[i % kSegs] = g;
                 mbar_arrive(seg_full(i % kSegs));
             }
             __syncwarp();
             if (g.n == 0) break;
         }
+    } else if (warp == 3) {  // ---- the join's notes ----
+        if (wait(planned, 0) && plan.ok) note_rows<D>(l, plan);
     } else if (warp == 0) {  // ---- producer ----
         if (lane < 4 && (lane < 2 ? a.prefix.max_len != 0 : a.n_seq != 0))
             asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&l.map[lane]))
@@ -402,7 +494,7 @@ __global__ void __launch_bounds__(Cfg<D>::threads, 1)
         uint32_t q = 0, j = 0;  // stages and tiles so far
         for (uint32_t sg = 0; !stop; ++sg) {
             if (!wait(seg_full(sg % kSegs), (sg / kSegs) & 1u)) break;
-            const Seg g = s_seg[sg % kSegs];
+            const Seg g = sm.seg[sg % kSegs];
             if (g.n == 0) break;
             __syncwarp();
             if (lane == 0) mbar_arrive(seg_empty(sg % kSegs));
@@ -441,7 +533,7 @@ __global__ void __launch_bounds__(Cfg<D>::threads, 1)
                     const uint32_t st = q % ST, round = q / ST;
                     if (round && !wait(empty(st), (round - 1) & 1u)) break;
                     if (v == 0) {
-                        if (lane < BN / 32) s_mask[j % kMeta][lane] = mask;
+                        if (lane < BN / 32) sm.mask[j % kMeta][lane] = mask;
                         __syncwarp();
                         if (lane == 0) mbar_arrive(meta(j % kMeta));
                     }
@@ -460,7 +552,7 @@ __global__ void __launch_bounds__(Cfg<D>::threads, 1)
             }
         }
         if (stop) {  // gave up: drain the loads already issued (bounded)
-            if (lane == 0) atomicExch(&s_fail, 1u);
+            if (lane == 0) atomicExch(&sm.fail, 1u);
             for (uint32_t i = q > ST ? q - ST : 0; i < q; ++i) mbar_wait(full(i % ST), (i / ST) & 1u);
         }
     } else if (warp == 1) {  // ---- products ----
@@ -480,7 +572,7 @@ __global__ void __launch_bounds__(Cfg<D>::threads, 1)
         auto open = [&](uint32_t s) {  // the stream's next piece with a tile for it
             for (;;) {
                 if (!wait(seg_full(sg[s] % kSegs), (sg[s] / kSegs) & 1u)) return;
-                const Seg &g = s_seg[sg[s] % kSegs];
+                const Seg &g = sm.seg[sg[s] % kSegs];
                 const bool end = g.n == 0;
                 if (!end) sh[s].set(g, s);
                 __syncwarp();
@@ -563,7 +655,7 @@ __global__ void __launch_bounds__(Cfg<D>::threads, 1)
         // issuer does, before the memory they use is given back
         if (stop) {
             if (lane == 0) {
-                atomicExch(&s_fail, 1u);
+                atomicExch(&sm.fail, 1u);
                 mma_commit(drain);
             }
             __syncwarp();
@@ -581,6 +673,8 @@ __global__ void __launch_bounds__(Cfg<D>::threads, 1)
         constexpr uint32_t kRows = 128 / (D / 8);  // rows that one pass of the Q load covers
         const uint32_t step_t = kRows / G, step_h = kRows - step_t * G;
         uint32_t ns = 0, sg = 0;  // tiles and pieces so far
+        uint32_t joins = 0;       // outputs joined with the other stream's
+        bool owed = false;        // it may still be reading this one's
         Seg g = {};
         Share<NS> sh = {};
         auto row_first = [&] { return sh.both ? 128 * s : 0u; };  // of the unit's rows
@@ -589,15 +683,13 @@ __global__ void __launch_bounds__(Cfg<D>::threads, 1)
         auto open = [&] {
             for (;;) {
                 if (!wait(seg_full(sg % kSegs), (sg / kSegs) & 1u)) return false;
-                g = s_seg[sg % kSegs];
+                g = sm.seg[sg % kSegs];
                 if (g.n == 0) return false;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(seg_empty(sg % kSegs));
                 ++sg;
                 sh.set(g, s);
-                if (sh.any()) break;
-                if (r < row_count())  // the other stream has the piece's only tile
-                    l.ml[(static_cast<uint64_t>(g.slot) * NS + s) * 128 + r] = make_float2(-INFINITY, 0.0f);
+                if (sh.any()) break;  // else the other stream has the piece's only tile
             }
             const uint32_t rows = row_count(), at0 = g.row0 + row_first();
             constexpr uint32_t CH = D / 8, RS = 128 / CH;  // 16-byte chunks of a row; rows a pass
@@ -649,7 +741,10 @@ __global__ void __launch_bounds__(Cfg<D>::threads, 1)
         bool more = open();
         while (more) {
             const uint32_t rows = row_count();
-            const uint64_t slot = static_cast<uint64_t>(g.slot) * NS + s;
+            // two streams over the same rows: their outputs are joined here, half of
+            // the columns by each
+            const bool two = NS == 2 && !sh.both && g.n > 1;
+            const uint64_t slot = static_cast<uint64_t>(g.slot) * NS + (sh.both ? s : 0);
             const bool idle = 32 * qd >= rows;  // no row of this warp: P may be anything
             // how far the row sees into the list
             uint32_t seen = 0xffffffffu;
@@ -660,7 +755,7 @@ __global__ void __launch_bounds__(Cfg<D>::threads, 1)
                 const uint32_t jj = sh.tile;
                 if (!wait(s_full(s), ns++ & 1u) || !wait(meta(jj % kMeta), (jj / kMeta) & 1u)) break;
                 tc_fence_after();
-                const uint4 mw = *reinterpret_cast<const uint4 *>(s_mask[jj % kMeta]);
+                const uint4 mw = *reinterpret_cast<const uint4 *>(sm.mask[jj % kMeta]);
                 const bool whole = (mw.x & mw.y & (BN == 128 ? mw.z & mw.w : 0xffffffffu)) == 0xffffffffu;
                 // a tile's first token is at most tile * BN: all of it seen?
                 const bool clear = whole && __all_sync(0xffffffffu, (tile0 + jj + 1) * BN <= seen);
@@ -673,7 +768,7 @@ __global__ void __launch_bounds__(Cfg<D>::threads, 1)
                         if (!wait(full(k % ST), (k / ST) & 1u)) break;
                         for (uint32_t i = tid; i < BN * 8; i += 128) {  // a lane 16 bytes
                             const uint32_t key = i / 8;
-                            if (s_mask[jj % kMeta][key / 32] >> (key % 32) & 1u) continue;
+                            if (sm.mask[jj % kMeta][key / 32] >> (key % 32) & 1u) continue;
                             const uint32_t at = ring + (k % ST) * C::stage + i * 16;
 #pragma unroll
                             for (uint32_t z = 0; z < D / 64; ++z)
@@ -691,7 +786,7 @@ __global__ void __launch_bounds__(Cfg<D>::threads, 1)
 #pragma unroll 1
                     for (uint32_t w = 0; w < BN / 32 && !idle; ++w) {
                         const uint32_t left = lim > 32 * w ? lim - 32 * w : 0;
-                        const uint32_t mask = s_mask[jj % kMeta][w] &
+                        const uint32_t mask = sm.mask[jj % kMeta][w] &
                                               (left >= 32 ? 0xffffffffu : (1u << left) - 1);
                         tmem_ld32_nowait(ts + 32 * w, x);
                         tmem_ld_wait(x);
@@ -768,6 +863,12 @@ __global__ void __launch_bounds__(Cfg<D>::threads, 1)
                         tmem_st32(ts + 32 * w, *reinterpret_cast<const uint32_t(*)[32]>(pk + 32 * w));
                     tmem_st_wait();
                 }
+                // a new piece's output begins with this tile's product: the other
+                // stream must have read the last one
+                if (begin && owed) {
+                    if (!wait(o_read(1 - s), (joins - 1) & 1u)) break;
+                    owed = false;
+                }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(p_ready(s));
@@ -777,13 +878,38 @@ __global__ void __launch_bounds__(Cfg<D>::threads, 1)
             more = open();
             if (!wait(pv_done(s), (ns - 1) & 1u)) break;
             tc_fence_after();
+            float f0 = 1.0f, f1 = 0.0f;  // weights of this stream's and the other's output
+            if (two) {
+                sm.ml[s][r] = make_float2(m, sum);
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(o_done(s));
+                if (!wait(o_done(1 - s), joins & 1u)) break;
+                tc_fence_after();
+                const float2 other = sm.ml[1 - s][r];
+                const float top = fmaxf(m, other.x);
+                f0 = m == -INFINITY ? 0.0f : ex2(m - top);
+                f1 = other.x == -INFINITY ? 0.0f : ex2(other.x - top);
+                m = top;
+                sum = f0 * sum + f1 * other.y;
+            }
             if (!idle) {
-                if (r < rows) l.ml[slot * 128 + r] = make_float2(m, sum);
+                if (r < rows && (s == 0 || !two)) l.ml[slot * 128 + r] = make_float2(m, sum);
+                const uint32_t tx = tmem + ((32 * qd) << 16) + C::o_col(NS - 1 - s);
+                const uint32_t c0 = two ? s * (D / 2) : 0, c1 = two ? c0 + D / 2 : D;
 #pragma unroll 1
-                for (uint32_t col = 0; col < D; col += 32) {
+                for (uint32_t col = c0; col < c1; col += 32) {
                     uint32_t o[32];
                     tmem_ld32_nowait(to + col, o);
                     tmem_ld_wait(o);
+                    if (two) {
+                        uint32_t e[32];
+                        tmem_ld32_nowait(tx + col, e);
+                        tmem_ld_wait(e);
+#pragma unroll
+                        for (int k = 0; k < 32; ++k)
+                            o[k] = __float_as_uint(f0 * __uint_as_float(o[k]) + f1 * __uint_as_float(e[k]));
+                    }
                     if (r < rows) {
 #pragma unroll
                         for (uint32_t k = 0; k < 8; ++k)
@@ -793,14 +919,21 @@ __global__ void __launch_bounds__(Cfg<D>::threads, 1)
                     }
                 }
             }
+            if (two) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(o_read(s));
+                ++joins;
+                owed = true;
+            }
             tc_fence_before();
         }
     }
-    if (stop && lane == 0) atomicExch(&s_fail, 1u);
+    if (stop && lane == 0) atomicExch(&sm.fail, 1u);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (threadIdx.x == 0) l.fail[blockIdx.x] = s_fail;
+    if (threadIdx.x == 0) l.fail[blockIdx.x] = sm.fail;
     if (warp == 1) {
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
                      "r"(kAttnTmem)
@@ -811,118 +944,50 @@ __global__ void __launch_bounds__(Cfg<D>::threads, 1)
 // The join: a row's pieces of the prefix and of its tail, weighted by
 // 2^(m_piece - m), in a fixed order. 8 rows a CTA (neighbouring heads of a
 // token), a thread per row and four dimensions: reads of 128 bytes (8 rows of
-// one float4 column). What bounds it is the chain of dependent reads (lengths,
-// offsets, statistics, then the pieces, 16 at a time), so each step's reads are
-// issued together.
+// one float4 column), 16 pieces at a time. What bounds it is three dependent
+// reads (where the pieces lie, their statistics, the pieces).
 constexpr uint32_t kJoinRows = 8, kMaxCtas = 160;
-struct JoinRow {
-    Cuts cuts[2];                // prefix, tail: the line's ranges
-    uint32_t first[2], n[2];     // the first range that meets the row's unit, and how many
-    uint32_t slot0[2], step[2];  // workspace slot of range i: slot0 + i * step
-    uint32_t row[2];             // within the slot's stream
-    uint32_t stream[2], per[2];  // the row tile; streams that hold part of the row
-    bool write;
-};
 
 template <int D>
 __global__ void __launch_bounds__(kJoinRows *D / 4)
     attn_join_kernel(const __grid_constant__ AttnLaunch l, uint32_t n_cta) {
-    using C = Cfg<D>;
-    constexpr int PR = C::PR, NS = C::NS;
-    constexpr uint32_t kList = 4 * kMaxCtas;  // two lines, two streams
-    constexpr uint32_t NT = kJoinRows * D / 4;
-    __shared__ JoinRow rows[kJoinRows];
+    constexpr uint32_t NT = kJoinRows * D / 4, kList = 2 * kMaxCtas;  // a piece per CTA and line at most
     __shared__ uint32_t s_id[kJoinRows][kList];
     __shared__ float s_w[kJoinRows][kList];
     __shared__ uint32_t s_n[kJoinRows];
     __shared__ float s_inv[kJoinRows];
     const PrefixAttn &a = l.a;
-    const uint32_t tid = threadIdx.x;
-    const uint32_t G = a.n_head / a.n_head_kv, H = a.n_head_kv;
-    const uint64_t row0 = static_cast<uint64_t>(blockIdx.x) * kJoinRows;
-    const uint32_t t_first = static_cast<uint32_t>(row0 / a.n_head);
-    const uint64_t last = min(row0 + kJoinRows, static_cast<uint64_t>(a.n_q) * a.n_head) - 1;
-    const uint32_t t_last = static_cast<uint32_t>(last / a.n_head);
-    const bool one_token = t_first == t_last;
-    // sequences that start at or before the first row's token: its own is the last of them
-    uint32_t before = 0;
-    for (uint32_t s0 = 0; s0 <= a.n_seq && a.n_seq; s0 += NT) {
-        const uint32_t s = s0 + tid;
-        before += __syncthreads_count(s <= a.n_seq && __ldg(a.q_start + s) <= static_cast<int32_t>(t_first));
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t row0 = blockIdx.x * kJoinRows, n_rows = a.n_q * a.n_head;
+    // the rows of a sequence
+    uint32_t begin = 0, end = n_rows;
+    if (a.n_seq) {
+        const int32_t n = static_cast<int32_t>(a.n_q);
+        begin = static_cast<uint32_t>(min(max(__ldg(a.q_start), 0), n)) * a.n_head;
+        end = static_cast<uint32_t>(min(max(__ldg(a.q_start + a.n_seq), 0), n)) * a.n_head;
     }
     cudaGridDependencySynchronize();
     uint32_t bad = 0;
     for (uint32_t i = tid; i < n_cta; i += NT) bad |= l.fail[i];
-    if (tid < kJoinRows) {
-        const Plan p = *l.plan;
-        JoinRow d{};
-        const uint64_t x = row0 + tid;
-        const uint32_t t = one_token ? t_first : static_cast<uint32_t>(x / a.n_head);
-        const uint32_t head = static_cast<uint32_t>(x - static_cast<uint64_t>(t) * a.n_head);
-        const uint32_t h = head / G, gq = head - h * G;
-        uint32_t from = before;
-        d.write = x <= last;
-        if (d.write && a.n_seq) {
-            while (t != t_first && from <= a.n_seq && __ldg(a.q_start + from) <= static_cast<int32_t>(t))
-                ++from;
-            d.write = from >= 1 && from <= a.n_seq;
-        }
-        if (d.write && p.np && t >= p.q0 && (t - p.q0) * G + gq < p.rows) {
-            const uint32_t r = (t - p.q0) * G + gq, pair = r / PR, pg = pair / p.gs;
-            const uint32_t u = pg * H + h;
-            const uint64_t x0 = static_cast<uint64_t>(u) * p.np;
-            d.cuts[0] = p.pre;
-            d.first[0] = p.pre.owner(x0);
-            d.n[0] = p.pre.owner(x0 + p.np - 1) + 1 - d.first[0];
-            d.slot0[0] = u * p.gs + pair - pg * p.gs;
-            d.step[0] = p.gs;
-            d.per[0] = NS == 2 && p.rows - pair * PR <= 128 ? 2 : 1;
-            d.row[0] = r % 128;
-            d.stream[0] = r % PR / 128;
-        }
-        if (d.write && a.n_seq) {
-            const uint32_t seq = from - 1;
-            const uint64_t seq_tile = l.seq_tile[seq];
-            const uint32_t seq_pair = l.seq_pair[seq];
-            const SeqShape sh = seq_shape(a, seq);
-            const TileGeom<C::BN> tg(a.tail.pages.page_tokens);
-            const uint32_t tiles = tg.tiles(sh.len), i = t - sh.q0;
-            if (t >= sh.q0 && i < sh.q_len && tiles && p.t_total) {
-                const uint32_t r = i * G + gq, pair = r / PR, u = pair * H + h;
-                const uint32_t n = min(tiles, pair_tiles<C::BN, PR>(sh, tg, pair, G));
-                const uint64_t x0 = (p.gs == 1 ? p.p_total : 0) + seq_tile +
-                                    static_cast<uint64_t>(u) * (tiles + kUnit) + kUnit;
-                d.cuts[1] = p.own;
-                if (n) {
-                    d.first[1] = p.own.owner(x0);
-                    d.n[1] = p.own.owner(x0 + n - 1) + 1 - d.first[1];
-                }
-                d.slot0[1] = p.t_slot0 + seq_pair * H + u;
-                d.step[1] = 1;
-                d.per[1] = NS == 2 && sh.q_len * G - pair * PR <= 128 ? 2 : 1;
-                d.row[1] = r % 128;
-                d.stream[1] = r % PR / 128;
-            }
-        }
-        rows[tid] = d;
-    }
     bad = __syncthreads_or(bad);
+    if (bad) {  // every row NaN
+        for (uint32_t i = tid; i < kJoinRows * D; i += NT)
+            if (row0 + i / D < n_rows) a.out[static_cast<uint64_t>(row0) * D + i] = 0x7fff;
+        if (a.lse && tid < kJoinRows && row0 + tid < n_rows) a.lse[row0 + tid] = NAN;
+        return;
+    }
     // a warp lists a row's pieces and weighs them
-    const uint32_t warp = tid >> 5, lane = tid & 31;
     for (uint32_t w = warp; w < kJoinRows; w += NT / 32) {
-        const JoinRow &d = rows[w];
+        const uint32_t row = row0 + w;
+        if (row < begin || row >= end) continue;
+        const RowPieces e0 = l.at[2 * static_cast<uint64_t>(row)], e1 = l.at[2 * static_cast<uint64_t>(row) + 1];
+        const uint32_t n_all = e0.n + e1.n;
         uint32_t n = 0;
         float top = -INFINITY, sum = 0.0f;
-        const uint32_t n_pre = d.n[0] * d.per[0], n_all = n_pre + d.n[1] * d.per[1];
         for (uint32_t i0 = 0; i0 < n_all; i0 += 32) {
-            const uint32_t k = i0 + lane >= n_pre ? 1 : 0, i = i0 + lane - (k ? n_pre : 0);
-            uint32_t id = 0;
-            float2 ml = make_float2(-INFINITY, 0.0f);
-            if (i0 + lane < n_all) {
-                const uint32_t two = d.per[k] == 2, part = d.first[k] + (two ? i / 2 : i);
-                id = ((d.slot0[k] + part * d.step[k]) * NS + (two ? i % 2 : d.stream[k])) * 128 + d.row[k];
-                ml = l.ml[id];
-            }
+            const uint32_t i = i0 + lane;
+            const uint32_t id = i < e0.n ? e0.id + i * e0.step : e1.id + (i - e0.n) * e1.step;
+            const float2 ml = i < n_all ? l.ml[id] : make_float2(-INFINITY, 0.0f);
             const uint32_t have = __ballot_sync(0xffffffffu, ml.x != -INFINITY);
             float mt = ml.x;
             for (int o = 16; o; o >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, o));
@@ -945,14 +1010,13 @@ __global__ void __launch_bounds__(kJoinRows *D / 4)
         for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == 0) {
             s_n[w] = n;
-            s_inv[w] = bad ? NAN : n ? 1.0f / sum : 0.0f;
-            if (a.lse && d.write)
-                a.lse[row0 + w] = bad ? NAN : n ? (top + log2f(sum)) * 0.693147181f : -INFINITY;
+            s_inv[w] = n ? 1.0f / sum : 0.0f;
+            if (a.lse) a.lse[row] = n ? (top + log2f(sum)) * 0.693147181f : -INFINITY;
         }
     }
     __syncthreads();
     const uint32_t r = tid % kJoinRows, col = tid / kJoinRows;
-    if (!rows[r].write) return;
+    if (row0 + r < begin || row0 + r >= end) return;
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     const uint32_t n = s_n[r];
     for (uint32_t i0 = 0; i0 < n; i0 += 16) {
@@ -975,7 +1039,7 @@ __global__ void __launch_bounds__(kJoinRows *D / 4)
         }
     }
     const float inv = s_inv[r];
-    *reinterpret_cast<uint2 *>(a.out + (row0 + r) * D + 4 * col) =
+    *reinterpret_cast<uint2 *>(a.out + static_cast<uint64_t>(row0 + r) * D + 4 * col) =
         make_uint2(pack_h2(acc.x * inv, acc.y * inv), pack_h2(acc.z * inv, acc.w * inv));
 }
 
@@ -1005,9 +1069,9 @@ uint32_t attn_ctas() {
 
 uint64_t up256(uint64_t v) { return (v + 255) / 256 * 256; }
 
-// The workspace: plan, one word per CTA, the sequences' offsets, the pieces.
+// The workspace: one word per CTA, the rows' notes, the pieces.
 struct WsLayout {
-    uint64_t fail, seq_tile, seq_pair, ml, o, bytes, slots;
+    uint64_t at, ml, o, bytes, slots;
     WsLayout(uint32_t n_q, uint32_t n_head, uint32_t n_head_kv, uint32_t d, uint32_t n_seq) {
         const uint64_t pr = d == 256 ? 128 : 256, ns = pr / 128;
         const uint64_t rows = static_cast<uint64_t>(n_q) * (n_head / n_head_kv);
@@ -1016,10 +1080,8 @@ struct WsLayout {
         // tails: a pair per sequence more than whole pairs of the rows
         slots = (pairs + pg) * n_head_kv + 2 * kMaxCtas +
                 (n_seq ? (n_seq + rows / pr) * n_head_kv : 0);
-        fail = up256(sizeof(Plan));
-        seq_tile = fail + up256(kMaxCtas * 4);
-        seq_pair = seq_tile + up256(8ull * n_seq);
-        ml = seq_pair + up256(4ull * n_seq);
+        at = up256(kMaxCtas * 4);
+        ml = at + up256(2ull * n_q * n_head * sizeof(RowPieces));
         o = ml + up256(slots * ns * 128 * 8);
         bytes = o + slots * ns * 128 * d * 4;
     }
@@ -1028,10 +1090,11 @@ struct WsLayout {
 template <int D>
 cudaError_t launch_t(const AttnLaunch &l, cudaStream_t st) {
     const uint32_t n_cta = attn_ctas();
+    const size_t smem = Cfg<D>::tiles + sizeof(Small<D>);
     cudaError_t e = cudaFuncSetAttribute(
-        attn_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Cfg<D>::smem));
+        attn_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return e;
-    attn_tc_kernel<D><<<n_cta, Cfg<D>::threads, Cfg<D>::smem, st>>>(l);
+    attn_tc_kernel<D><<<n_cta, Cfg<D>::threads, smem, st>>>(l);
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     const uint64_t rows = static_cast<uint64_t>(l.a.n_q) * l.a.n_head;
@@ -1064,10 +1127,8 @@ cudaError_t launch_prefix_attn(const PrefixAttn &a, void *ws, cudaStream_t st) {
     uint8_t *b = static_cast<uint8_t *>(ws);
     AttnLaunch l{};
     l.a = a;
-    l.plan = reinterpret_cast<Plan *>(b);
-    l.fail = reinterpret_cast<uint32_t *>(b + w.fail);
-    l.seq_tile = reinterpret_cast<uint64_t *>(b + w.seq_tile);
-    l.seq_pair = reinterpret_cast<uint32_t *>(b + w.seq_pair);
+    l.fail = reinterpret_cast<uint32_t *>(b);
+    l.at = reinterpret_cast<RowPieces *>(b + w.at);
     l.ml = reinterpret_cast<float2 *>(b + w.ml);
     l.o = reinterpret_cast<float4 *>(b + w.o);
     l.max_slots = static_cast<uint32_t>(w.slots);
