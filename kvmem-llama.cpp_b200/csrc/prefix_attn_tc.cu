@@ -456,7 +456,7 @@ __global__ void __launch_bounds__(Cfg<D>::threads, 1)
     // a whole warp's wait; false once it has given up (the warps that wait for
     // this one then do too)
     auto wait = [&](uint32_t bar, uint32_t parity) {
-        if (!__all_sync(0xffffffffu, mbar_wait(bar, parity))) stop = true;
+        if (!__all_sync(0xffffffffu, mbar_wait_clk(bar, parity))) stop = true;
         return !stop;
     };
 
@@ -553,7 +553,7 @@ __global__ void __launch_bounds__(Cfg<D>::threads, 1)
         }
         if (stop) {  // gave up: drain the loads already issued (bounded)
             if (lane == 0) atomicExch(&sm.fail, 1u);
-            for (uint32_t i = q > ST ? q - ST : 0; i < q; ++i) mbar_wait(full(i % ST), (i / ST) & 1u);
+            for (uint32_t i = q > ST ? q - ST : 0; i < q; ++i) mbar_wait_clk(full(i % ST), (i / ST) & 1u);
         }
     } else if (warp == 1) {  // ---- products ----
         // Tiles are taken in the CTA's order: the stream whose current tile is
