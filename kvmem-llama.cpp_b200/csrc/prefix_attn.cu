@@ -1,143 +1,1386 @@
-// Attention of a batch over a shared prefix and each sequence's own tail.
+// Attention of a batch over a shared prefix and each sequence's own tail, on
+// the tcgen05 tensor cores.
 //
 // For query row t (head h, KV head g = h / (n_head / n_head_kv)) of sequence s:
-//   out = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale * q . k_j - max)
-// over the prefix tokens and the tail tokens up to the row's own (the last
-// new token of a sequence sees its whole tail, the one before it one token
-// less). Rows that see nothing give zeros and an lse of -inf; rows of no
-// sequence are left as they were.
+//   out = sum_j p_j v_j / sum_j p_j,  p_j = 2^(c q . k_j - m),  c = scale log2 e
+// over the prefix tokens and the tail tokens up to the row's own. One pass
+// over the keys with a running maximum m and sum (f32); the output is kept
+// unnormalised in tensor memory and rescaled only when the maximum has grown
+// by more than 8 (a factor of 2^8), so p stays below 2^8 and exact in its
+// ratio; p is rounded to f16 for the second product, the sum is not.
 //
-// One CTA per (row, head): each warp takes 32 keys at a time (a lane a key
-// for the scores, a lane D / 32 dimensions for the values) with a running
-// maximum and sum, the warps are joined at the end.
+// A CTA (one per SM) walks its pieces (prefix_attn_plan.cuh). Warps:
+//   0      producer: page list, the tile's mask of valid keys, TMA loads of K
+//          and V tiles into a ring of shared-memory stages (128-byte swizzle,
+//          no multicast);
+//   2      walks the pieces and leaves each in a short ring for the others;
+//   3      notes for the join where each row's pieces lie;
+//   1      one lane issues the products: S = Q K^T (both in shared memory)
+//          and O += P V (P in tensor memory over its S, V as it lies: keys
+//          along K, MN-major);
+//   4-7    softmax of stream 0, a thread a row; also loads Q, rescales and
+//          hands on O;
+//   8-11   the same for stream 1 (head size 256 has one stream: its output
+//          takes half of the tensor memory).
+// With more than 128 rows the two streams are two tiles of rows over the same
+// key tiles; otherwise they are the same rows over every other key tile, each
+// with its own output. While one stream is in its softmax the other one's
+// products run. P and S of a stream share columns, so its next S waits until
+// the product that reads P has completed.
+// Cells without a token may hold anything, NaN too: their scores are replaced
+// after the product, their V rows zeroed in shared memory before it.
+// Every wait is bounded; on a timeout the outputs become NaN (the join).
 #include "prefix_attn.cuh"
 
+#include <cuda_fp16.h>
+
+#include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "kvmret.h"
+#include "prefix_attn_plan.cuh"
 #include "quant.cuh"
+#include "tc.cuh"
 
 namespace kvmret {
 namespace {
 
-constexpr int kWarps = 4;
+// QUANT: some K or V rows are q8_0 or q4_0 blocks.
+template <int D, bool QUANT>
+struct Cfg {
+    static constexpr int NS = D == 256 ? 1 : 2;     // streams
+    static constexpr int BN = D == 256 ? 64 : 128;  // keys of a tile
+    static constexpr int PR = 128 * NS;             // rows of a unit
+    static constexpr int threads = 128 + 128 * NS + (QUANT ? 128 : 0);
+    static constexpr uint32_t stage = BN * D * 2;   // one K or V tile
+    static constexpr int stages = QUANT ? (D == 64 ? 6 : 3) : D == 64 ? 8 : 5;
+    static constexpr uint32_t q_bytes = 128 * D * 2;
+    // tiles of quant blocks as they lie in memory, on their way
+    static constexpr int raws = QUANT ? (D == 64 ? 6 : 3) : 0;
+    static constexpr uint32_t raw = BN * (D == 64 ? 80 : D == 128 ? 144 : 272);
+    static constexpr uint32_t raw0 = NS * q_bytes + stages * stage;
+    static constexpr uint32_t tiles = raw0 + raws * raw;
+    static __host__ __device__ constexpr uint32_t s_col(int s) { return s * 128; }
+    static __host__ __device__ constexpr uint32_t o_col(int s) { return 256 + s * (D == 64 ? 64 : 128); }
+    // Ring positions of the K and V tiles of tile t. With conversions K goes a
+    // tile ahead (K0 K1 V0 K2 V1 ..), so that three stages are enough for scores
+    // not to wait for a stage that a V still holds.
+    static __device__ __forceinline__ uint32_t k_pos(uint32_t t) { return QUANT ? (t ? 2 * t - 1 : 0) : 2 * t; }
+    static __device__ __forceinline__ uint32_t v_pos(uint32_t t) { return QUANT ? 2 * t + 2 : 2 * t + 1; }
+};
+// Bytes of the box that holds a head's row of quant blocks: it starts on a
+// 16-byte boundary at or up to 12 bytes before the row.
+template <int D>
+__host__ __device__ constexpr uint32_t raw_box(int32_t type) {
+    return D == 64 ? (type == KVMRET_TYPE_Q8_0 ? 80 : 48) : D == 128 ? (type == KVMRET_TYPE_Q8_0 ? 144 : 80)
+                                                        : (type == KVMRET_TYPE_Q8_0 ? 272 : 144);
+}
+constexpr uint32_t kAttnTmem = 512;
+constexpr int kSegs = 4;  // pieces ahead
+constexpr int kMeta = 16;  // tiles whose masks are held (more than the ring reaches back)
 
-// element e of a row of the given format
-__device__ __forceinline__ float element(const uint8_t *row, int32_t type, uint32_t e) {
-    if (type == KVMRET_TYPE_F16) return h2f(reinterpret_cast<const uint16_t *>(row)[e]);
-    if (type == KVMRET_TYPE_Q8_0) {
-        const uint8_t *b = row + (e / 32) * 34;
-        return static_cast<float>(static_cast<int8_t>(b[2 + e % 32])) *
-               h2f(*reinterpret_cast<const uint16_t *>(b));
-    }
-    const uint8_t *b = row + (e / 32) * 18;
-    const uint32_t i = e % 32, x = b[2 + (i & 15)];
-    return static_cast<float>(static_cast<int>(i < 16 ? x & 15 : x >> 4) - 8) *
-           h2f(*reinterpret_cast<const uint16_t *>(b));
+// Where one row's pieces lie: entry i of n has its statistics at ml[id + i *
+// step], its output in the same slot and row.
+struct RowPieces {
+    uint32_t id, step, n, pad;
+};
+
+struct AttnLaunch {
+    PrefixAttn a;
+    CUtensorMap map[4];  // prefix K, V, tail K, V
+    uint32_t *fail;  // [CTA] 1: a wait gave up, or q_start was not ascending
+    RowPieces *at;   // [n_q * n_head][2] pieces of the prefix, of the tail
+    float2 *ml;      // [slot][row tile][128] maximum and sum
+    float4 *o;       // [slot][row tile][D / 4][128]
+    uint32_t max_slots;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_h2(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ void tmem_ld32_nowait(uint32_t taddr, uint32_t *r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32"
+        " {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15,"
+        " %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31},"
+        " [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
+          "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+          "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
+          "=r"(r[31])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32"
+        " {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+          "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]),
+                   "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]),
+                   "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0],"
+        " {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+// Two products and two sums at a time (each rounded like the scalar operation).
+__device__ __forceinline__ void fma_pair(uint32_t &x, uint32_t &y, float a, float b) {
+    asm("{\n\t.reg .b64 p, q, r;\n\t"
+        "mov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %2};\n\tmov.b64 r, {%3, %3};\n\t"
+        "fma.rn.f32x2 p, p, q, r;\n\tmov.b64 {%0, %1}, p;\n\t}"
+        : "+r"(x), "+r"(y)
+        : "f"(a), "f"(b));
+}
+__device__ __forceinline__ void add_pair(float &x, float &y, float a, float b) {
+    asm("{\n\t.reg .b64 p, q;\n\t"
+        "mov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %3};\n\t"
+        "add.rn.f32x2 p, p, q;\n\tmov.b64 {%0, %1}, p;\n\t}"
+        : "+f"(x), "+f"(y)
+        : "f"(a), "f"(b));
+}
+// The wait for loads under way; it names the registers, so that nothing that
+// reads them can be moved before it.
+__device__ __forceinline__ void tmem_ld_wait(uint32_t *r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]),
+                   "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]),
+                   "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]),
+                   "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]),
+                   "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
 }
 
-// K or V row of token i of a list, null when the list has no such token.
-__device__ __forceinline__ bool locate(const KeyList &l, uint32_t list, uint32_t i, uint32_t &page,
-                                       uint32_t &off) {
-    const uint32_t T = l.pages.page_tokens, at = i / T;
-    off = i - at * T;
-    if (at >= l.n_list) return false;
-    const uint64_t slot = static_cast<uint64_t>(list) * l.n_list + at;
-    const int32_t p = l.table ? l.table[slot] : static_cast<int32_t>(at);
-    if (p < 0 || static_cast<uint32_t>(p) >= l.pages.n_pages) return false;
-    page = static_cast<uint32_t>(p);
-    return !l.ntok || off < l.ntok[slot];
+// Instruction descriptor: D f32, A and B f16, M = 128, N; B K-major or MN-major.
+__host__ __device__ constexpr uint32_t idesc(uint32_t n, bool b_mn) {
+    return (1u << 4) | (b_mn ? 1u << 16 : 0u) | ((n >> 3) << 17) | ((128u >> 4) << 24);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id,
+                                       uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b),
+        "r"(id), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id,
+                                       uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b),
+        "r"(id), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(p));
+    return p;
+}
+
+// One key's COLS columns of quant blocks at shared address `src` (4-byte
+// aligned; 8-byte with 128 columns), eight columns at a time to put(chunk, x).
+// A block's payload starts two bytes after its start: with even blocks (which
+// start on a word) its words straddle two, with odd ones they are whole.
+template <int COLS, int TYPE, typename Put>
+__device__ __forceinline__ void convert_row(uint32_t src, Put put) {
+    constexpr uint32_t BLOCK = TYPE == KVMRET_TYPE_Q8_0 ? 34 : 18, NB = COLS / 32, W = NB * BLOCK / 4;
+    uint32_t w[W];
+    if constexpr (COLS == 128) {
+#pragma unroll
+        for (uint32_t i = 0; i < W; i += 2)
+            asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[i]), "=r"(w[i + 1]) : "r"(src + 4 * i));
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < W; ++i)
+            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[i]) : "r"(src + 4 * i));
+    }
+#pragma unroll
+    for (uint32_t b = 0; b < NB; ++b) {
+        constexpr uint32_t NW = (BLOCK - 2) / 4;
+        const uint32_t at = b * BLOCK / 4;  // the word of the block's start
+        const bool odd = b & 1;
+        const uint32_t dd = odd ? __byte_perm(w[at], 0, 0x3232) : __byte_perm(w[at], 0, 0x1010);
+        const __half2 d = *reinterpret_cast<const __half2 *>(&dd);
+        uint32_t p[NW];
+#pragma unroll
+        for (uint32_t i = 0; i < NW; ++i)
+            p[i] = odd ? w[at + 1 + i] : __byte_perm(w[at + i], w[at + i + 1 < W ? at + i + 1 : at + i], 0x5432);
+        // halves of bytes 2k, 2k + 1 of u, less `bias`, times d
+        auto pair = [&](uint32_t u, uint32_t k, uint32_t bias) {
+            const uint32_t h = __byte_perm(u, 0x64646464u, k ? 0x4342 : 0x4140);
+            const __half2 x = __hmul2(__hsub2(*reinterpret_cast<const __half2 *>(&h),
+                                              *reinterpret_cast<const __half2 *>(&bias)), d);
+            return *reinterpret_cast<const uint32_t *>(&x);
+        };
+        if constexpr (TYPE == KVMRET_TYPE_Q8_0) {
+#pragma unroll
+            for (uint32_t c = 0; c < 4; ++c) {
+                const uint32_t u0 = p[2 * c] ^ 0x80808080u, u1 = p[2 * c + 1] ^ 0x80808080u;
+                const uint32_t x[4] = {pair(u0, 0, 0x64806480u), pair(u0, 1, 0x64806480u),
+                                       pair(u1, 0, 0x64806480u), pair(u1, 1, 0x64806480u)};
+                put(4 * b + c, x);
+            }
+        } else {
+#pragma unroll
+            for (uint32_t c = 0; c < 4; ++c) {  // lower halves: columns 0 .. 15, upper: 16 .. 31
+                const uint32_t s = c < 2 ? 0 : 4;
+                const uint32_t u0 = (p[2 * (c % 2)] >> s) & 0x0f0f0f0fu, u1 = (p[2 * (c % 2) + 1] >> s) & 0x0f0f0f0fu;
+                const uint32_t x[4] = {pair(u0, 0, 0x64086408u), pair(u0, 1, 0x64086408u),
+                                       pair(u1, 0, 0x64086408u), pair(u1, 1, 0x64086408u)};
+                put(4 * b + c, x);
+            }
+        }
+    }
+}
+
+// The plan of the split, by one warp, in every CTA alike. `start` receives the
+// sequence that holds the CTA's first tail tile. False when q_start descends.
+struct Start {
+    uint32_t seq, pair, tile;
+};
+// inclusive sums over the warp's lanes
+__device__ __forceinline__ void scan(uint32_t &x, uint32_t &y) {
+    const uint32_t lane = threadIdx.x & 31;
+    for (uint32_t o = 1; o < 32; o <<= 1) {
+        const uint32_t u = __shfl_up_sync(0xffffffffu, x, o), v = __shfl_up_sync(0xffffffffu, y, o);
+        if (lane >= o) {
+            x += u;
+            y += v;
+        }
+    }
 }
 
 template <int D>
-__global__ void __launch_bounds__(32 * kWarps) attn_kernel(const __grid_constant__ PrefixAttn a) {
-    constexpr int E = D / 32;
-    __shared__ float q[D];
-    __shared__ float pm[kWarps], pl[kWarps], po[kWarps][D];
-    const uint32_t t = blockIdx.x, h = blockIdx.y, g = h / (a.n_head / a.n_head_kv);
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    uint32_t seq = 0, seen = 0;
-    if (a.n_seq) {
-        bool found = false;
-        for (uint32_t s = 0; s < a.n_seq && !found; ++s)
-            if (static_cast<int32_t>(t) >= a.q_start[s] && static_cast<int32_t>(t) < a.q_start[s + 1]) {
-                seq = s;
-                found = true;
+__device__ bool make_plan(const AttnLaunch &l, Plan &p, Start &start) {
+    constexpr int BN = Cfg<D, false>::BN, PR = Cfg<D, false>::PR;
+    const PrefixAttn &a = l.a;
+    const uint32_t lane = threadIdx.x & 31;
+    const uint32_t G = a.n_head / a.n_head_kv, H = a.n_head_kv;
+    const TileGeom<BN> tg(a.n_seq ? a.tail.pages.page_tokens : BN);
+    bool ok = true;
+    auto shape = [&](uint32_t s, uint32_t &tiles, uint32_t &pairs) {
+        tiles = pairs = 0;
+        if (s >= a.n_seq) return;
+        ok = ok && __ldg(a.q_start + s) <= __ldg(a.q_start + s + 1);
+        const SeqShape sh = seq_shape(a, s);
+        pairs = (sh.q_len * G + PR - 1) / PR;
+        const uint32_t n = sh.q_len ? tg.tiles(sh.len) : 0;
+        tiles = (n ? n + kUnit : 0) * pairs * H;
+    };
+    const bool pre = a.prefix.max_len != 0;
+    const int32_t len0 = pre && a.prefix.len ? __ldg(a.prefix.len) : 0x7fffffff;
+    const int32_t q_first = a.n_seq ? __ldg(a.q_start) : 0;
+    const int32_t q_last = a.n_seq ? __ldg(a.q_start + a.n_seq) : static_cast<int32_t>(a.n_q);
+    // totals of the tails; the last listed page that holds tokens
+    uint32_t t0, n0;
+    shape(lane, t0, n0);
+    uint32_t tiles = t0, pairs = n0;
+#pragma unroll 4
+    for (uint32_t s = 32 + lane; s < a.n_seq; s += 32) {
+        uint32_t t, n;
+        shape(s, t, n);
+        tiles += t;
+        pairs += n;
+    }
+    ok = __all_sync(0xffffffffu, ok);
+    uint32_t held = pre ? a.prefix.n_list : 0;
+    if (held && a.prefix.ntok) {
+        held = 0;
+#pragma unroll 8
+        for (uint32_t i = lane; i < a.prefix.n_list; i += 32)
+            if (__ldg(a.prefix.ntok + i)) held = i + 1;
+    }
+    for (int o = 16; o; o >>= 1) {
+        tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
+        pairs += __shfl_xor_sync(0xffffffffu, pairs, o);
+        held = max(held, __shfl_xor_sync(0xffffffffu, held, o));
+    }
+    p.p_len = 0;
+    p.np = 0;
+    if (pre) {
+        const uint64_t most = static_cast<uint64_t>(held) * a.prefix.pages.page_tokens;
+        const uint32_t len = min(a.prefix.max_len, static_cast<uint32_t>(max(len0, 0)));
+        p.p_len = most < len ? static_cast<uint32_t>(most) : len;
+        p.np = TileGeom<BN>(a.prefix.pages.page_tokens).tiles(p.p_len);
+    }
+    const int32_t nq = static_cast<int32_t>(a.n_q);
+    p.q0 = static_cast<uint32_t>(min(max(q_first, 0), nq));
+    p.rows = (min(max(q_last, static_cast<int32_t>(p.q0)), nq) - p.q0) * G;
+    p.n_pair = (p.rows + PR - 1) / PR;
+    // 8 CTAs side by side leave at most 5 % of the 148 SMs without a group
+    p.n_pg = (p.n_pair + 7) / 8;
+    p.gs = p.n_pg ? (p.n_pair + p.n_pg - 1) / p.n_pg : 1;
+    if (p.gs > gridDim.x) {
+        p.gs = gridDim.x;
+        p.n_pg = (p.n_pair + p.gs - 1) / p.gs;
+    }
+    p.groups = p.gs == 1 ? gridDim.x : gridDim.x / p.gs;
+    p.p_total = p.np * p.n_pg * H;
+    p.t_total = tiles;
+    p.t_slot0 = (p.n_pg * H + p.groups) * p.gs;
+    ok = ok && p.t_slot0 + pairs * H + gridDim.x <= l.max_slots;  // (so it is when it ascends)
+    p.ok = ok;
+    if (!ok) p.p_total = p.t_total = 0;
+    if (p.gs == 1) {
+        p.pre.set(p.p_total + p.t_total, gridDim.x);
+        p.own = p.pre;
+    } else {
+        p.pre.set(p.p_total, p.groups);
+        p.own.set(p.t_total, gridDim.x);
+    }
+    start = {0, 0, 0};
+    uint32_t x, x1, y, y1;
+    Walk<BN, PR>::ranges(p, blockIdx.x, x, x1, y, y1);
+    if (y >= y1) return ok;  // no tails here
+    uint32_t base_t = 0, base_p = 0;
+    for (uint32_t s0 = 0; s0 < a.n_seq; s0 += 32) {
+        if (s0) shape(s0 + lane, t0, n0);
+        uint32_t ti = t0, pi = n0;
+        scan(ti, pi);
+        const uint32_t all_t = __shfl_sync(0xffffffffu, ti, 31), all_p = __shfl_sync(0xffffffffu, pi, 31);
+        ti += base_t - t0;
+        pi += base_p - n0;
+        const uint32_t hit = __ballot_sync(0xffffffffu, y >= ti && y < ti + t0);
+        if (hit) {
+            const int w = __ffs(hit) - 1;
+            start.seq = s0 + w;
+            start.pair = __shfl_sync(0xffffffffu, pi, w);
+            start.tile = __shfl_sync(0xffffffffu, ti, w);
+            break;
+        }
+        base_t += all_t;
+        base_p += all_p;
+    }
+    return ok;
+}
+
+// Where the pieces of every row lie, for the join: by one warp of each CTA, a
+// lane a row, the CTAs taking blocks of 32 rows in turn.
+template <int D>
+__device__ void note_rows(const AttnLaunch &l, const Plan &p) {
+    constexpr int BN = Cfg<D, false>::BN, PR = Cfg<D, false>::PR, NS = Cfg<D, false>::NS;
+    const PrefixAttn &a = l.a;
+    const uint32_t lane = threadIdx.x & 31, n_cta = gridDim.x;
+    const uint32_t G = a.n_head / a.n_head_kv, H = a.n_head_kv;
+    // rows of the tokens [q0, q0 + q_len); tails from tile `tile` and pair `pair` on
+    auto note = [&](uint32_t q0, uint32_t q_len, const SeqShape *sh, uint32_t tile, uint32_t pair0) {
+        const TileGeom<BN> tg(sh ? a.tail.pages.page_tokens : BN);
+        const uint32_t tiles = sh ? tg.tiles(sh->len) : 0;
+        const uint32_t begin = q0 * a.n_head, end = begin + q_len * a.n_head;
+        uint32_t b = begin / 32;
+        b += (blockIdx.x + n_cta - b % n_cta) % n_cta;  // the first block of this CTA
+        for (; b * 32 < end; b += n_cta) {
+            const uint32_t x = 32 * b + lane;
+            if (x < begin || x >= end) continue;
+            const uint32_t t = x / a.n_head, head = x - t * a.n_head, h = head / G, gq = head - h * G;
+            RowPieces r[2] = {};
+            auto put = [&](RowPieces &e, const Cuts &cuts, uint32_t x0, uint32_t n, uint32_t slot0,
+                           uint32_t step, uint32_t row) {
+                const uint32_t first = cuts.owner(x0);
+                e.n = cuts.owner(x0 + n - 1) + 1 - first;
+                e.id = ((slot0 + first * step) * NS + row % PR / 128) * 128 + row % 128;
+                e.step = step * NS * 128;
+            };
+            if (p.np) {
+                const uint32_t row = (t - p.q0) * G + gq, pair = row / PR, pg = pair / p.gs, u = pg * H + h;
+                put(r[0], p.pre, u * p.np, p.np, u * p.gs + pair - pg * p.gs, p.gs, row);
             }
-        if (!found) return;
-        const int32_t len = min(a.tail.len[seq], static_cast<int32_t>(a.tail.max_len));
-        seen = static_cast<uint32_t>(max(0, len - (a.q_start[seq + 1] - static_cast<int32_t>(t)) + 1));
-    }
-    uint32_t np = a.prefix.max_len;
-    if (np && a.prefix.len) np = static_cast<uint32_t>(min(max(*a.prefix.len, 0), static_cast<int32_t>(np)));
-    for (uint32_t e = threadIdx.x; e < D; e += blockDim.x)
-        q[e] = h2f(a.q[t * a.q_stride + h * D + e]) * a.scale;
-    __syncthreads();
-    float m = -INFINITY, l = 0.0f, o[E] = {};
-    for (uint32_t i0 = warp * 32; i0 < np + seen; i0 += 32 * kWarps) {
-        const uint32_t i = i0 + lane;
-        const bool pre = i < np;
-        const KeyList &kl = pre ? a.prefix : a.tail;
-        uint32_t page = 0, off = 0;
-        const bool ok = i < np + seen && locate(kl, pre ? 0 : seq, pre ? i : i - np, page, off);
-        float s = -INFINITY;
-        if (ok) {
-            const uint8_t *row = kl.pages.k + page * kl.pages.k_page + off * kl.pages.k_row;
-            s = 0.0f;
-            for (uint32_t e = 0; e < D; ++e) s += q[e] * element(row, kl.pages.k_type, g * D + e);
+            if (tiles) {
+                const uint32_t row = (t - q0) * G + gq, pair = row / PR, u = pair * H + h;
+                const uint32_t n = min(tiles, pair_tiles<BN, PR>(*sh, tg, pair, G));
+                if (n)
+                    put(r[1], p.own, (p.gs == 1 ? p.p_total : 0) + tile + u * (tiles + kUnit) + kUnit, n,
+                        p.t_slot0 + pair0 * H + u, 1, row);
+            }
+            l.at[2 * x] = r[0];
+            l.at[2 * x + 1] = r[1];
         }
-        float top = s;
-        for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-        if (top == -INFINITY) continue;
-        const float mn = fmaxf(m, top), c = expf(m - mn), p = expf(s - mn);
-        float sum = p;
-        for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-        l = l * c + sum;
-        m = mn;
-        for (int e = 0; e < E; ++e) o[e] *= c;
-        for (int j = 0; j < 32; ++j) {
-            if (!__shfl_sync(0xffffffffu, static_cast<int>(ok), j)) continue;
-            const float pj = __shfl_sync(0xffffffffu, p, j);
-            const uint32_t pg = __shfl_sync(0xffffffffu, page, j), of = __shfl_sync(0xffffffffu, off, j);
-            const KeyList &vl = i0 + j < np ? a.prefix : a.tail;
-            const uint8_t *row = vl.pages.v + pg * vl.pages.v_page + of * vl.pages.v_row;
-            for (int e = 0; e < E; ++e)
-                o[e] += pj * element(row, vl.pages.v_type, g * D + lane * E + e);
+    };
+    if (!a.n_seq) {
+        note(0, a.n_q, nullptr, 0, 0);
+        return;
+    }
+    const TileGeom<BN> tg(a.tail.pages.page_tokens);
+    uint32_t base_t = 0, base_p = 0;
+    for (uint32_t s0 = 0; s0 < a.n_seq; s0 += 32) {
+        SeqShape sh = {};
+        if (s0 + lane < a.n_seq) sh = seq_shape(a, s0 + lane);
+        const uint32_t pairs = (sh.q_len * G + PR - 1) / PR, n = sh.q_len ? tg.tiles(sh.len) : 0;
+        const uint32_t tiles = (n ? n + kUnit : 0) * pairs * H;
+        uint32_t ti = tiles, pi = pairs;
+        scan(ti, pi);
+        for (uint32_t w = 0; w < min(32u, a.n_seq - s0); ++w) {
+            SeqShape one;
+            one.q0 = __shfl_sync(0xffffffffu, sh.q0, w);
+            one.q_len = __shfl_sync(0xffffffffu, sh.q_len, w);
+            one.len = __shfl_sync(0xffffffffu, sh.len, w);
+            note(one.q0, one.q_len, &one, base_t + __shfl_sync(0xffffffffu, ti - tiles, w),
+                 base_p + __shfl_sync(0xffffffffu, pi - pairs, w));
+            __syncwarp();
+        }
+        base_t += __shfl_sync(0xffffffffu, ti, 31);
+        base_p += __shfl_sync(0xffffffffu, pi, 31);
+    }
+}
+
+// A tile as the converting warps need it.
+struct TileInfo {
+    int32_t page[8];  // -1: nothing of it counts
+    uint32_t off, h;  // first token within the page, KV head
+    uint32_t kind;    // 0 prefix, 1 tail, 2 no more tiles
+    uint32_t pad;
+};
+
+// What a CTA keeps in shared memory behind the tiles.
+template <int D, bool QUANT>
+struct Small {
+    using C = Cfg<D, QUANT>;
+    static constexpr int NS = C::NS;
+    alignas(16) uint32_t mask[kMeta][4];  // valid keys of a tile
+    float2 ml[NS][128];                   // statistics on their way to the other stream
+    uint64_t bars[2 * C::stages + kMeta + 2 * kSegs + 6 * NS + 2 + 2 * C::raws + (QUANT ? kMeta : 0)];
+    TileInfo tile[QUANT ? kMeta : 1];
+    Plan plan;
+    Seg seg[kSegs];
+    uint32_t tmem, fail;
+};
+static_assert(Cfg<128, false>::tiles + sizeof(Small<128, false>) <= 227 * 1024, "shared memory");
+static_assert(Cfg<128, true>::tiles + sizeof(Small<128, true>) <= 227 * 1024, "shared memory");
+static_assert(Cfg<256, true>::tiles + sizeof(Small<256, true>) <= 227 * 1024, "shared memory");
+
+template <int D, bool QUANT>
+__global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
+    attn_tc_kernel(const __grid_constant__ AttnLaunch l) {
+    using C = Cfg<D, QUANT>;
+    constexpr int BN = C::BN, PR = C::PR, NS = C::NS, ST = C::stages, RS = C::raws;
+    constexpr uint32_t KB = BN * 128, QB = 128 * 128;  // bytes of a 64-column block of K / V, of Q
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    Small<D, QUANT> &sm = *reinterpret_cast<Small<D, QUANT> *>(smem_raw + C::tiles);
+    Plan &plan = sm.plan;
+
+    const PrefixAttn &a = l.a;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t base = smem_u32(smem_raw);
+    if (base & 1023u) {  // the tiles must lie on the swizzle's atoms
+        if (threadIdx.x == 0) l.fail[blockIdx.x] = 1;
+        return;
+    }
+    const uint32_t ring = base + NS * C::q_bytes;
+    const uint32_t bar0 = smem_u32(sm.bars);
+    auto full = [&](uint32_t i) { return bar0 + 8u * i; };
+    auto empty = [&](uint32_t i) { return bar0 + 8u * (ST + i); };
+    auto meta = [&](uint32_t i) { return bar0 + 8u * (2 * ST + i); };
+    auto seg_full = [&](uint32_t i) { return bar0 + 8u * (2 * ST + kMeta + i); };
+    auto seg_empty = [&](uint32_t i) { return bar0 + 8u * (2 * ST + kMeta + kSegs + i); };
+    constexpr uint32_t SB = 2 * ST + kMeta + 2 * kSegs;
+    auto q_ready = [&](uint32_t s) { return bar0 + 8u * (SB + s); };
+    auto s_full = [&](uint32_t s) { return bar0 + 8u * (SB + NS + s); };
+    auto p_ready = [&](uint32_t s) { return bar0 + 8u * (SB + 2 * NS + s); };
+    auto pv_done = [&](uint32_t s) { return bar0 + 8u * (SB + 3 * NS + s); };
+    auto o_done = [&](uint32_t s) { return bar0 + 8u * (SB + 4 * NS + s); };
+    auto o_read = [&](uint32_t s) { return bar0 + 8u * (SB + 5 * NS + s); };
+    const uint32_t drain = bar0 + 8u * (SB + 6 * NS), planned = drain + 8;
+    auto raw_full = [&](uint32_t i) { return drain + 16 + 8u * i; };
+    auto raw_empty = [&](uint32_t i) { return drain + 16 + 8u * (RS + i); };
+    auto meta_empty = [&](uint32_t i) { return drain + 16 + 8u * (2 * RS + i); };
+
+    if (threadIdx.x == 0) {
+        sm.fail = 0;
+        for (int i = 0; i < ST; ++i) {
+            mbar_init(full(i), QUANT ? 4 : 1);
+            mbar_init(empty(i), NS);  // one arrival per stream
+        }
+        for (int i = 0; i < kMeta; ++i) mbar_init(meta(i), 1);
+        for (int i = 0; i < kSegs; ++i) {
+            mbar_init(seg_full(i), 1);
+            mbar_init(seg_empty(i), 1 + NS + 4 * NS);  // producer, products, softmax warps
+        }
+        for (int s = 0; s < NS; ++s) {
+            mbar_init(q_ready(s), 4);
+            mbar_init(s_full(s), 1);
+            mbar_init(p_ready(s), 4);
+            mbar_init(pv_done(s), 1);
+            mbar_init(o_done(s), 4);
+            mbar_init(o_read(s), 4);
+        }
+        mbar_init(drain, 1);
+        mbar_init(planned, 1);
+        for (int i = 0; i < RS; ++i) {
+            mbar_init(raw_full(i), 1);
+            mbar_init(raw_empty(i), 4);
+        }
+        if constexpr (QUANT)
+            for (int i = 0; i < kMeta; ++i) mbar_init(meta_empty(i), 4);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                         smem_u32(&sm.tmem)),
+                     "r"(kAttnTmem)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0);
+    bool stop = false;
+    // a whole warp's wait; false once it has given up (the warps that wait for
+    // this one then do too)
+    auto wait = [&](uint32_t bar, uint32_t parity) {
+        if (!__all_sync(0xffffffffu, mbar_wait_clk(bar, parity))) stop = true;
+        return !stop;
+    };
+
+    if (warp == 2) {  // ---- the pieces ----
+        Start start;
+        Plan p;
+        if (!make_plan<D>(l, p, start)) stop = true;
+        if (lane == 0) {
+            plan = p;
+            mbar_arrive(planned);
+        }
+        __syncwarp();
+        Walk<BN, PR> walk(a, plan, start.seq, start.tile, start.pair);
+        uint32_t j = 0;
+        for (uint32_t i = 0;; ++i) {
+            Seg g = {};
+            if (!stop && walk.next(g)) {
+                g.j0 = j;
+                j += g.n;
+            }
+            if (i >= kSegs && !wait(seg_empty(i % kSegs), (i / kSegs - 1) & 1u)) break;
+            if (lane == 0) {
+                sm.seg[i % kSegs] = g;
+                mbar_arrive(seg_full(i % kSegs));
+            }
+            __syncwarp();
+            if (g.n == 0) break;
+        }
+    } else if (warp == 3) {  // ---- the join's notes ----
+        if (wait(planned, 0) && plan.ok) note_rows<D>(l, plan);
+    } else if (warp == 0) {  // ---- producer ----
+        if (lane < 4 && (lane < 2 ? a.prefix.max_len != 0 : a.n_seq != 0))
+            asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&l.map[lane]))
+                         : "memory");
+        uint32_t q = 0, j = 0;  // stages (quant: raw tiles) and tiles so far
+        // The raw tile of a K (v = 0) or V operand that is in quant blocks.
+        auto load_raw = [&](uint32_t kind, uint32_t v, uint32_t h, uint32_t off, int32_t id, bool use) {
+            const PageView &pv = (kind ? a.tail : a.prefix).pages;
+            const int32_t type = v ? pv.v_type : pv.k_type;
+            if (type == KVMRET_TYPE_F16) return;  // the converting warps fetch it
+            const uint32_t slot = q % (RS ? RS : 1), round = q / (RS ? RS : 1);
+            if (round && !wait(raw_empty(slot), (round - 1) & 1u)) return;
+            ++q;
+            const uint32_t T = pv.page_tokens, bx = raw_box<D>(type);
+            const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, use)) * min(T, static_cast<uint32_t>(BN)) * bx;
+            if (lane == 0) mbar_expect_tx(raw_full(slot), bytes);
+            __syncwarp();
+            const uint32_t row = D / 32 * (type == KVMRET_TYPE_Q8_0 ? 34 : 18);
+            if (use)
+                tma_load_3d(base + C::raw0 + slot * C::raw + lane * T * bx, &l.map[2 * kind + v],
+                            static_cast<int32_t>(h * row / 16 * 8), static_cast<int32_t>(off), id,
+                            raw_full(slot));
+        };
+        uint32_t k_kind = 2, k_h = 0, k_off = 0;  // the tile before
+        int32_t k_id = -1;
+        bool k_use = false;
+        for (uint32_t sg = 0; !stop; ++sg) {
+            if (!wait(seg_full(sg % kSegs), (sg / kSegs) & 1u)) break;
+            const Seg g = sm.seg[sg % kSegs];
+            if (g.n == 0) break;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(seg_empty(sg % kSegs));
+            const KeyList &kl = g.tail ? a.tail : a.prefix;
+            const CUtensorMap *mk = &l.map[g.tail ? 2 : 0], *mv = mk + 1;
+            const TileGeom<BN> geom(kl.pages.page_tokens);
+            const uint32_t T = geom.T, box = min(T, static_cast<uint32_t>(BN));
+            const uint64_t list = g.tail ? static_cast<uint64_t>(g.seq) * kl.n_list : 0;
+            for (uint32_t i = 0; i < g.n && !stop; ++i, ++j) {
+                // lane p < ppt: page p of the tile, and how many of its tokens count
+                uint32_t page, off;
+                geom.locate(g.tile0 + i, page, off);
+                int32_t id = -1;
+                uint32_t held = 0;
+                if (lane < geom.ppt && page + lane < kl.n_list) {
+                    const uint32_t at = page + lane;
+                    id = kl.table ? __ldg(kl.table + list + at) : static_cast<int32_t>(at);
+                    if (id >= 0 && static_cast<uint32_t>(id) < kl.pages.n_pages) {
+                        held = kl.ntok ? min(__ldg(kl.ntok + at), T) : T;
+                        held = min(held, at * T < g.len ? g.len - at * T : 0);
+                    }
+                }
+                const bool use = held > off;
+                uint32_t mask = 0;  // lane w keeps word w
+#pragma unroll
+                for (uint32_t w = 0; w < BN / 32; ++w) {
+                    const uint32_t key = 32 * w + lane, pk = T < BN ? key / T : 0;
+                    const uint32_t h = __shfl_sync(0xffffffffu, held, pk);
+                    const uint32_t o = T < BN ? key - pk * T : off + key;
+                    const uint32_t b = __ballot_sync(0xffffffffu, pk < geom.ppt && o < h);
+                    if (lane == w) mask = b;
+                }
+                if constexpr (QUANT) {
+                    const uint32_t slot = j % kMeta;
+                    if (j >= kMeta && !wait(meta_empty(slot), (j / kMeta - 1) & 1u)) break;
+                    if (lane < BN / 32) sm.mask[slot][lane] = mask;
+                    if (lane < 8) sm.tile[slot].page[lane] = use ? id : -1;
+                    if (lane == 0) {
+                        sm.tile[slot].off = off;
+                        sm.tile[slot].h = g.h;
+                        sm.tile[slot].kind = g.tail;
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(meta(slot));
+                    load_raw(g.tail, 0, g.h, off, id, use);
+                    if (!stop && k_kind < 2) load_raw(k_kind, 1, k_h, k_off, k_id, k_use);
+                    k_kind = g.tail;
+                    k_h = g.h;
+                    k_off = off;
+                    k_id = id;
+                    k_use = use;
+                    continue;
+                }
+                const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, use)) * box * D * 2;
+#pragma unroll
+                for (uint32_t v = 0; v < 2; ++v) {  // K, then V
+                    const uint32_t st = q % ST, round = q / ST;
+                    if (round && !wait(empty(st), (round - 1) & 1u)) break;
+                    if (v == 0) {
+                        if (lane < BN / 32) sm.mask[j % kMeta][lane] = mask;
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(meta(j % kMeta));
+                    }
+                    if (lane == 0) mbar_expect_tx(full(st), bytes);
+                    __syncwarp();
+                    ++q;
+                    if (use) {
+                        const uint32_t dst = ring + st * C::stage + lane * T * 128;
+#pragma unroll
+                        for (uint32_t b = 0; b < D / 64; ++b)
+                            tma_load_4d(dst + b * KB, v ? mv : mk, static_cast<int32_t>(64 * b),
+                                        static_cast<int32_t>(g.h), static_cast<int32_t>(off), id,
+                                        full(st));
+                    }
+                }
+            }
+        }
+        if constexpr (QUANT) {
+            if (!stop && k_kind < 2) load_raw(k_kind, 1, k_h, k_off, k_id, k_use);
+            if (!stop && (j < kMeta || wait(meta_empty(j % kMeta), (j / kMeta - 1) & 1u))) {
+                if (lane == 0) {
+                    sm.tile[j % kMeta].kind = 2;
+                    mbar_arrive(meta(j % kMeta));
+                }
+            }
+        }
+        if (stop) {  // gave up: drain the loads already issued (bounded)
+            if (lane == 0) atomicExch(&sm.fail, 1u);
+            constexpr uint32_t N = QUANT ? (RS ? RS : 1) : ST;
+            for (uint32_t i = q > N ? q - N : 0; i < q; ++i)
+                mbar_wait_clk(QUANT ? raw_full(i % N) : full(i % N), (i / N) & 1u);
+        }
+    } else if (warp == 1) {  // ---- products ----
+        // Tiles are taken in the CTA's order: the stream whose current tile is
+        // first gets its P V product and, once that has read P, its next scores.
+        // While it waits for its softmax the other stream's turn comes, so the two
+        // stay half a period apart. (Both products of a turn being issued as soon
+        // as they could be, in any order, lets the streams fall into step: 3.9 ms
+        // instead of 3.2 ms for 2048 rows over 32,768 tokens.)
+        constexpr uint32_t id_s = idesc(BN, false), id_o = idesc(D, true);
+        constexpr uint32_t kHi = 64u | (1u << 14) | (2u << 29);  // upper halves of the descriptors
+        const uint32_t ubase = __shfl_sync(0xffffffffu, base, 0);
+        auto desc = [](uint32_t lo) { return static_cast<uint64_t>(kHi) << 32 | lo; };
+        Share<NS> sh[2];
+        uint32_t sg[2] = {0, 0}, tiles[2] = {0, 0};  // pieces taken up, tiles finished
+        bool live[2] = {true, NS == 2}, fresh[2] = {true, true};
+        auto open = [&](uint32_t s) {  // the stream's next piece with a tile for it
+            for (;;) {
+                if (!wait(seg_full(sg[s] % kSegs), (sg[s] / kSegs) & 1u)) return;
+                const Seg &g = sm.seg[sg[s] % kSegs];
+                const bool end = g.n == 0;
+                if (!end) sh[s].set(g, s);
+                __syncwarp();
+                if (end) {
+                    live[s] = false;
+                    return;
+                }
+                if (lane == 0) mbar_arrive(seg_empty(sg[s] % kSegs));
+                ++sg[s];
+                if (sh[s].any()) break;
+            }
+            fresh[s] = true;
+        };
+        uint32_t nq[2] = {0, 0};
+        // a stage is free once each stream has passed it: a tile of one stream
+        // alone counts for both
+        auto release = [&](uint32_t s, uint32_t st) {
+            mma_commit(empty(st));
+            if (NS == 2 && !sh[s].both) mma_commit(empty(st));
+        };
+        // scores of the stream's current tile; `after`: once the product before,
+        // which reads the P that S will overwrite, has completed (the last wait, so
+        // that the issue follows it at once)
+        auto scores = [&](uint32_t s, bool after) {
+            if (fresh[s] && !wait(q_ready(s), nq[s]++ & 1u)) return;
+            const uint32_t k = C::k_pos(sh[s].tile), st = __shfl_sync(0xffffffffu, k % ST, 0);
+            if (!wait(full(st), (k / ST) & 1u)) return;
+            if (after && !wait(pv_done(s), tiles[s] & 1u)) return;
+            tc_fence_after();
+            if (elect_one()) {
+                const uint32_t la = ((ubase + s * C::q_bytes) >> 4) | (1u << 16);
+                const uint32_t lb = ((ubase + NS * C::q_bytes + st * C::stage) >> 4) | (1u << 16);
+#pragma unroll
+                for (uint32_t c = 0; c < D / 16; ++c)  // 16 columns: 32 bytes of a block
+                    mma_ss(tmem + C::s_col(s), desc(la + (c / 4) * (QB / 16) + 2 * (c % 4)),
+                           desc(lb + (c / 4) * (KB / 16) + 2 * (c % 4)), id_s, c != 0);
+                mma_commit(s_full(s));
+                release(s, st);
+            }
+            __syncwarp();
+        };
+#pragma unroll
+        for (uint32_t s = 0; s < NS; ++s) {
+            if (!stop) open(s);
+            if (!stop && live[s]) scores(s, false);
+        }
+        auto turn = [&](uint32_t s) {
+            const uint32_t v = C::v_pos(sh[s].tile), st = __shfl_sync(0xffffffffu, v % ST, 0);
+            if (!wait(full(st), (v / ST) & 1u) || !wait(p_ready(s), tiles[s] & 1u)) return;
+            tc_fence_after();
+            if (elect_one()) {
+                const uint32_t lb = ((ubase + NS * C::q_bytes + st * C::stage) >> 4) | (KB / 16) << 16;
+                const uint32_t add = !fresh[s];
+#pragma unroll
+                for (uint32_t c = 0; c < BN / 16; ++c)  // 16 keys: 8 columns of P, 2 KiB of V
+                    mma_ts(tmem + C::o_col(s), tmem + C::s_col(s) + 8 * c, desc(lb + 128 * c), id_o,
+                           c ? 1u : add);
+                release(s, st);
+                mma_commit(pv_done(s));
+            }
+            __syncwarp();
+            fresh[s] = false;
+            sh[s].tile += sh[s].step;
+            if (!sh[s].any()) open(s);
+            if (!stop && live[s]) scores(s, true);
+            ++tiles[s];
+        };
+        uint32_t last = 1;
+        while (!stop && (live[0] || (NS == 2 && live[1]))) {
+            const bool one = NS == 2 && live[1] &&
+                             (!live[0] || sh[1].tile < sh[0].tile ||
+                              (sh[1].tile == sh[0].tile && last == 0));
+            last = one;
+            if (NS == 2 && one)
+                turn(1);
+            else
+                turn(0);
+        }
+        // on the regular path the softmax waits for the last products; here the
+        // issuer does, before the memory they use is given back
+        if (stop) {
+            if (lane == 0) {
+                atomicExch(&sm.fail, 1u);
+                mma_commit(drain);
+            }
+            __syncwarp();
+            mbar_wait(drain, 0);
+        }
+    } else if (QUANT && warp >= 4 + 4 * NS) {  // ---- conversion of quant blocks ----
+        // A thread a key's row (head size 256: half of it): blocks from the raw
+        // tile to f16(d * q) in the stage's swizzled layout. Whole numbers become
+        // halves by their bits (0x6400 + u is 1024 + u), one subtraction and one
+        // product by d, rounded once. Operands in f16 go to their stage by TMA,
+        // issued by the first of these warps with all four arrivals.
+        const uint32_t tid = threadIdx.x & 127, wq = warp - 4 - 4 * NS;
+        const uint32_t key = tid % BN, half = tid / BN;  // half: 0 unless the head size is 256
+        uint32_t nr = 0;                                 // raw tiles so far
+        uint32_t flight = 0;                             // stages with an f16 load under way
+        auto unit = [&](uint32_t j, uint32_t v) {
+            const TileInfo &ti = sm.tile[j % kMeta];
+            const PageView &pv = (ti.kind ? a.tail : a.prefix).pages;
+            const int32_t type = v ? pv.v_type : pv.k_type;
+            const uint32_t pos = v ? C::v_pos(j) : C::k_pos(j), st = pos % ST;
+            if (pos >= ST && !wait(empty(st), (pos / ST - 1) & 1u)) return;
+            const uint32_t stage = ring + st * C::stage;
+            if (type == KVMRET_TYPE_F16) {
+                if (wq != 0) return;
+                const uint32_t T = pv.page_tokens, box = min(T, static_cast<uint32_t>(BN));
+                const int32_t id = lane < 8 ? ti.page[lane] : -1;
+                const uint32_t n = __popc(__ballot_sync(0xffffffffu, id >= 0));
+                if (lane == 0) {
+                    for (int i = 0; i < 3; ++i) mbar_arrive(full(st));
+                    mbar_expect_tx(full(st), n * box * D * 2);
+                }
+                __syncwarp();
+                if (id >= 0)
+#pragma unroll
+                    for (uint32_t b = 0; b < D / 64; ++b)
+                        tma_load_4d(stage + b * KB + lane * T * 128, &l.map[2 * ti.kind + v],
+                                    static_cast<int32_t>(64 * b), static_cast<int32_t>(ti.h),
+                                    static_cast<int32_t>(ti.off), id, full(st));
+                flight = pos + 1;
+                return;
+            }
+            const uint32_t slot = nr % (RS ? RS : 1);
+            if (!wait(raw_full(slot), (nr / (RS ? RS : 1)) & 1u)) return;
+            ++nr;
+            const bool q8 = type == KVMRET_TYPE_Q8_0;
+            const uint32_t block = q8 ? 34 : 18, row = D / 32 * block;
+            const uint32_t src = base + C::raw0 + slot * C::raw + key * raw_box<D>(type) +
+                                 (ti.h * row) % 16 + half * 4 * block;
+            constexpr uint32_t COLS = D < 128 ? D : 128;
+            const uint32_t dst = stage + key * 128;
+            auto put = [&](uint32_t chunk, const uint32_t(&x)[4]) {  // 8 columns
+                const uint32_t ch = half * 16 + chunk;
+                const uint32_t at = dst + (ch / 8) * KB + (((ch % 8) ^ (key % 8)) * 16);
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x[0]), "r"(x[1]),
+                             "r"(x[2]), "r"(x[3])
+                             : "memory");
+            };
+            if (q8)
+                convert_row<COLS, KVMRET_TYPE_Q8_0>(src, put);
+            else
+                convert_row<COLS, KVMRET_TYPE_Q4_0>(src, put);
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(full(st));
+                mbar_arrive(raw_empty(slot));
+            }
+        };
+        for (uint32_t j = 0;; ++j) {
+            if (!wait(meta(j % kMeta), (j / kMeta) & 1u)) break;
+            const bool end = sm.tile[j % kMeta].kind == 2;
+            if (!end) unit(j, 0);
+            if (!stop && j) unit(j - 1, 1);
+            if (stop || end) break;
+            // K of tile j in its stage: P V of tile j - 8 is past, its mask read
+            if (j >= 8 && lane == 0) mbar_arrive(meta_empty((j - 8) % kMeta));
+            __syncwarp();
+        }
+        if (stop) {
+            if (lane == 0) atomicExch(&sm.fail, 1u);
+            if (wq == 0 && flight)  // the f16 loads under way
+                for (uint32_t i = flight > ST ? flight - ST : 0; i < flight; ++i)
+                    mbar_wait_clk(full(i % ST), (i / ST) & 1u);
+        }
+    } else if (warp >= 4) {  // ---- softmax, a thread a row ----
+        const uint32_t s = (warp - 4) >> 2, qd = warp & 3, r = 32 * qd + lane;
+        const uint32_t tid = threadIdx.x & 127;
+        const uint32_t G = a.n_head / a.n_head_kv;
+        // (above zero, so that -inf stays -inf; a scale of zero gives equal scores all the same)
+        const float c = fmaxf(fabsf(a.scale) * 1.44269504f, 1e-37f);
+        const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;  // a negative scale turns Q
+        const uint32_t ts = tmem + ((32 * qd) << 16) + C::s_col(s);
+        const uint32_t to = tmem + ((32 * qd) << 16) + C::o_col(s);
+        constexpr uint32_t kRows = 128 / (D / 8);  // rows that one pass of the Q load covers
+        const uint32_t step_t = kRows / G, step_h = kRows - step_t * G;
+        uint32_t ns = 0, sg = 0;  // tiles and pieces so far
+        uint32_t joins = 0;       // outputs joined with the other stream's
+        bool owed = false;        // it may still be reading this one's
+        Seg g = {};
+        Share<NS> sh = {};
+        auto row_first = [&] { return sh.both ? 128 * s : 0u; };  // of the unit's rows
+        auto row_count = [&] { return min(128u, g.rows - row_first()); };
+        // the stream's next piece: Q in the swizzled layout, rows past the last zeros
+        auto open = [&] {
+            for (;;) {
+                if (!wait(seg_full(sg % kSegs), (sg / kSegs) & 1u)) return false;
+                g = sm.seg[sg % kSegs];
+                if (g.n == 0) return false;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(seg_empty(sg % kSegs));
+                ++sg;
+                sh.set(g, s);
+                if (sh.any()) break;  // else the other stream has the piece's only tile
+            }
+            const uint32_t rows = row_count(), at0 = g.row0 + row_first();
+            constexpr uint32_t CH = D / 8, RS = 128 / CH;  // 16-byte chunks of a row; rows a pass
+            const uint32_t ch = tid % CH, q1 = tid / CH;
+            const uint16_t *const q = a.q + static_cast<uint64_t>(g.q0) * a.q_stride +
+                                      static_cast<uint64_t>(g.h) * G * D + 8 * ch;
+            uint32_t t = (at0 + q1) / G, hg = at0 + q1 - t * G;
+            // n passes: all loads first. Only warps that hold a row look at their
+            // scores, so rows past the last one of 32 stay as they are.
+            auto load = [&](uint32_t i0, auto n) {
+                constexpr uint32_t N = decltype(n)::value;
+                uint4 w[N];
+#pragma unroll
+                for (uint32_t i = 0; i < N; ++i) {
+                    w[i] = make_uint4(0, 0, 0, 0);
+                    if (q1 + (i0 + i) * RS < rows)
+                        w[i] = __ldg(reinterpret_cast<const uint4 *>(
+                            q + static_cast<uint64_t>(t) * a.q_stride + hg * D));
+                    t += step_t;
+                    hg += step_h;
+                    if (hg >= G) {
+                        hg -= G;
+                        ++t;
+                    }
+                }
+#pragma unroll
+                for (uint32_t i = 0; i < N; ++i) {
+                    const uint32_t qr = q1 + (i0 + i) * RS;
+                    const uint32_t at = base + s * C::q_bytes + (ch / 8) * QB + qr * 128 +
+                                        (((ch % 8) ^ (qr % 8)) * 16);
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at),
+                                 "r"(w[i].x ^ sign), "r"(w[i].y ^ sign), "r"(w[i].z ^ sign),
+                                 "r"(w[i].w ^ sign)
+                                 : "memory");
+                }
+            };
+            if (rows <= 32) {
+                load(0, std::integral_constant<uint32_t, 32 / RS>());
+            } else {
+                constexpr uint32_t QL = CH < 16 ? CH : 16;  // loads in flight
+#pragma unroll
+                for (uint32_t i0 = 0; i0 < CH; i0 += QL) load(i0, std::integral_constant<uint32_t, QL>());
+            }
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_ready(s));
+            return true;
+        };
+        bool more = open();
+        while (more) {
+            const uint32_t rows = row_count();
+            // two streams over the same rows: their outputs are joined here, half of
+            // the columns by each
+            const bool two = NS == 2 && !sh.both && g.n > 1;
+            const uint64_t slot = static_cast<uint64_t>(g.slot) * NS + (sh.both ? s : 0);
+            const bool idle = 32 * qd >= rows;  // no row of this warp: P may be anything
+            // how far the row sees into the list
+            uint32_t seen = 0xffffffffu;
+            if (g.tail) seen = tail_seen(g.len, g.q_len, (g.row0 + row_first() + min(r, rows - 1)) / G);
+            const uint32_t tile0 = g.tile0 - g.j0;
+            float m = -INFINITY, sum = 0.0f;  // of c q . k
+            for (bool begin = true; sh.any(); sh.tile += sh.step, begin = false) {
+                const uint32_t jj = sh.tile;
+                if (!wait(s_full(s), ns++ & 1u) || !wait(meta(jj % kMeta), (jj / kMeta) & 1u)) break;
+                tc_fence_after();
+                const uint4 mw = *reinterpret_cast<const uint4 *>(sm.mask[jj % kMeta]);
+                const bool whole = (mw.x & mw.y & (BN == 128 ? mw.z & mw.w : 0xffffffffu)) == 0xffffffffu;
+                // a tile's first token is at most tile * BN: all of it seen?
+                const bool clear = whole && __all_sync(0xffffffffu, (tile0 + jj + 1) * BN <= seen);
+                uint32_t x[32];
+                if (!clear) {
+                    // the S columns of keys that do not count become -inf, the V rows of
+                    // cells without a token zeros
+                    if (!whole) {
+                        const uint32_t k = C::v_pos(jj);
+                        if (!wait(full(k % ST), (k / ST) & 1u)) break;
+                        for (uint32_t i = tid; i < BN * 8; i += 128) {  // a lane 16 bytes
+                            const uint32_t key = i / 8;
+                            if (sm.mask[jj % kMeta][key / 32] >> (key % 32) & 1u) continue;
+                            const uint32_t at = ring + (k % ST) * C::stage + i * 16;
+#pragma unroll
+                            for (uint32_t z = 0; z < D / 64; ++z)
+                                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at + z * KB),
+                                             "r"(0u)
+                                             : "memory");
+                        }
+                        fence_async_smem();
+                    }
+                    const TileGeom<BN> geom((g.tail ? a.tail : a.prefix).pages.page_tokens);
+                    uint32_t page, off;
+                    geom.locate(tile0 + jj, page, off);
+                    const uint32_t pos0 = page * geom.T + off;
+                    const uint32_t lim = seen > pos0 ? min(seen - pos0, static_cast<uint32_t>(BN)) : 0;
+#pragma unroll 1
+                    for (uint32_t w = 0; w < BN / 32 && !idle; ++w) {
+                        const uint32_t left = lim > 32 * w ? lim - 32 * w : 0;
+                        const uint32_t mask = sm.mask[jj % kMeta][w] &
+                                              (left >= 32 ? 0xffffffffu : (1u << left) - 1);
+                        tmem_ld32_nowait(ts + 32 * w, x);
+                        tmem_ld_wait(x);
+#pragma unroll
+                        for (int k = 0; k < 32; ++k)
+                            if (!(mask >> k & 1u)) x[k] = 0xff800000u;
+                        tmem_st32(ts + 32 * w, x);
+                    }
+                    tmem_st_wait();
+                }
+                if (!idle) {
+                    // One pass with the maximum as it stands: p and the tile's own
+                    // maximum together, 32 columns at a time with the next ones on their
+                    // way (a piece's first tile starts with that of its first columns).
+                    // Only when a row's maximum has moved by more than 8 the pass is
+                    // repeated with the new one; S still stands, P is in registers.
+                    uint32_t y[32], pk[BN / 2];
+                    float top = -INFINITY, s0, s1;
+                    auto column_max = [&](const uint32_t *v) {
+#pragma unroll
+                        for (int k = 0; k < 32; k += 2)
+                            top = fmaxf(top, fmaxf(__uint_as_float(v[k]), __uint_as_float(v[k + 1])));
+                    };
+                    auto pass = [&](bool first) {
+                        float neg = m == -INFINITY ? 0.0f : -m;
+                        s0 = s1 = 0.0f;
+                        top = -INFINITY;
+                        tmem_ld32_nowait(ts, x);
+#pragma unroll
+                        for (int w = 0; w < BN / 32; ++w) {
+                            uint32_t *const v = w & 1 ? y : x;
+                            tmem_ld_wait(v);
+                            if (w + 1 < BN / 32) tmem_ld32_nowait(ts + 32 * (w + 1), w & 1 ? x : y);
+                            column_max(v);
+                            if (w == 0 && first) {
+                                m = top * c;
+                                neg = m == -INFINITY ? 0.0f : -m;
+                            }
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) {
+                                uint32_t e0 = v[2 * k], e1 = v[2 * k + 1];
+                                fma_pair(e0, e1, c, neg);
+                                const float p0 = ex2(__uint_as_float(e0)), p1 = ex2(__uint_as_float(e1));
+                                add_pair(s0, s1, p0, p1);
+                                pk[16 * w + k] = pack_h2(p0, p1);
+                            }
+                        }
+                    };
+                    bool first = begin;
+#pragma unroll 1
+                    for (;;) {
+                        pass(first);
+                        first = false;
+                        if (!__any_sync(0xffffffffu, top * c > m + 8.0f)) break;
+                        const float mn = fmaxf(m, top * c);
+                        const float f = m == -INFINITY ? 0.0f : ex2(m - mn);
+                        m = mn;
+                        sum *= f;
+                        if (begin) continue;
+                        // O stands still: its last product came before these scores
+#pragma unroll 1
+                        for (uint32_t col = 0; col < D; col += 16) {
+                            uint32_t o[16];
+                            tmem_ld16(to + col, o);
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                            tmem_st16(to + col, o);
+                        }
+                    }
+                    sum += s0 + s1;
+                    // P over the first columns of S
+#pragma unroll
+                    for (int w = 0; w < BN / 64; ++w)
+                        tmem_st32(ts + 32 * w, *reinterpret_cast<const uint32_t(*)[32]>(pk + 32 * w));
+                    tmem_st_wait();
+                }
+                // a new piece's output begins with this tile's product: the other
+                // stream must have read the last one
+                if (begin && owed) {
+                    if (!wait(o_read(1 - s), (joins - 1) & 1u)) break;
+                    owed = false;
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_ready(s));
+            }
+            if (stop) break;
+            // the last scores are in: Q may be replaced while the last product runs
+            more = open();
+            if (!wait(pv_done(s), (ns - 1) & 1u)) break;
+            tc_fence_after();
+            float f0 = 1.0f, f1 = 0.0f;  // weights of this stream's and the other's output
+            if (two) {
+                sm.ml[s][r] = make_float2(m, sum);
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(o_done(s));
+                if (!wait(o_done(1 - s), joins & 1u)) break;
+                tc_fence_after();
+                const float2 other = sm.ml[1 - s][r];
+                const float top = fmaxf(m, other.x);
+                f0 = m == -INFINITY ? 0.0f : ex2(m - top);
+                f1 = other.x == -INFINITY ? 0.0f : ex2(other.x - top);
+                m = top;
+                sum = f0 * sum + f1 * other.y;
+            }
+            if (!idle) {
+                if (r < rows && (s == 0 || !two)) l.ml[slot * 128 + r] = make_float2(m, sum);
+                const uint32_t tx = tmem + ((32 * qd) << 16) + C::o_col(NS - 1 - s);
+                const uint32_t c0 = two ? s * (D / 2) : 0, c1 = two ? c0 + D / 2 : D;
+#pragma unroll 1
+                for (uint32_t col = c0; col < c1; col += 32) {
+                    uint32_t o[32];
+                    tmem_ld32_nowait(to + col, o);
+                    tmem_ld_wait(o);
+                    if (two) {
+                        uint32_t e[32];
+                        tmem_ld32_nowait(tx + col, e);
+                        tmem_ld_wait(e);
+#pragma unroll
+                        for (int k = 0; k < 32; ++k)
+                            o[k] = __float_as_uint(f0 * __uint_as_float(o[k]) + f1 * __uint_as_float(e[k]));
+                    }
+                    if (r < rows) {
+#pragma unroll
+                        for (uint32_t k = 0; k < 8; ++k)
+                            l.o[(slot * (D / 4) + col / 4 + k) * 128 + r] =
+                                make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]),
+                                            __uint_as_float(o[4 * k + 2]), __uint_as_float(o[4 * k + 3]));
+                    }
+                }
+            }
+            if (two) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(o_read(s));
+                ++joins;
+                owed = true;
+            }
+            tc_fence_before();
         }
     }
-    if (lane == 0) {
-        pm[warp] = m;
-        pl[warp] = l;
-    }
-    for (int e = 0; e < E; ++e) po[warp][lane * E + e] = o[e];
+    if (stop && lane == 0) atomicExch(&sm.fail, 1u);
+    tc_fence_before();
     __syncthreads();
-    float top = -INFINITY, sum = 0.0f;
-    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, pm[w]);
-    float c[kWarps];
-    for (int w = 0; w < kWarps; ++w) {
-        c[w] = top == -INFINITY ? 0.0f : expf(pm[w] - top);
-        sum += c[w] * pl[w];
+    tc_fence_after();
+    if (threadIdx.x == 0) l.fail[blockIdx.x] = sm.fail;
+    if (warp == 1) {
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                     "r"(kAttnTmem)
+                     : "memory");
     }
-    const uint64_t r = static_cast<uint64_t>(t) * a.n_head + h;
-    for (uint32_t e = threadIdx.x; e < D; e += blockDim.x) {
-        float x = 0.0f;
-        for (int w = 0; w < kWarps; ++w) x += c[w] * po[w][e];
-        a.out[r * D + e] = f2h(sum > 0.0f ? x / sum : 0.0f);
+}
+
+// The join: a row's pieces of the prefix and of its tail, weighted by
+// 2^(m_piece - m), in a fixed order. 8 rows a CTA (neighbouring heads of a
+// token), a thread per row and four dimensions: reads of 128 bytes (8 rows of
+// one float4 column), 16 pieces at a time. What bounds it is three dependent
+// reads (where the pieces lie, their statistics, the pieces).
+constexpr uint32_t kJoinRows = 8, kMaxCtas = 160;
+
+template <int D>
+__global__ void __launch_bounds__(kJoinRows *D / 4)
+    attn_join_kernel(const __grid_constant__ AttnLaunch l, uint32_t n_cta) {
+    constexpr uint32_t NT = kJoinRows * D / 4, kList = 2 * kMaxCtas;  // a piece per CTA and line at most
+    __shared__ uint32_t s_id[kJoinRows][kList];
+    __shared__ float s_w[kJoinRows][kList];
+    __shared__ uint32_t s_n[kJoinRows];
+    __shared__ float s_inv[kJoinRows];
+    const PrefixAttn &a = l.a;
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t row0 = blockIdx.x * kJoinRows, n_rows = a.n_q * a.n_head;
+    // the rows of a sequence
+    uint32_t begin = 0, end = n_rows;
+    if (a.n_seq) {
+        const int32_t n = static_cast<int32_t>(a.n_q);
+        begin = static_cast<uint32_t>(min(max(__ldg(a.q_start), 0), n)) * a.n_head;
+        end = static_cast<uint32_t>(min(max(__ldg(a.q_start + a.n_seq), 0), n)) * a.n_head;
     }
-    if (a.lse && threadIdx.x == 0) a.lse[r] = sum > 0.0f ? top + logf(sum) : -INFINITY;
+    cudaGridDependencySynchronize();
+    uint32_t bad = 0;
+    for (uint32_t i = tid; i < n_cta; i += NT) bad |= l.fail[i];
+    bad = __syncthreads_or(bad);
+    if (bad) {  // every row NaN
+        for (uint32_t i = tid; i < kJoinRows * D; i += NT)
+            if (row0 + i / D < n_rows) a.out[static_cast<uint64_t>(row0) * D + i] = 0x7fff;
+        if (a.lse && tid < kJoinRows && row0 + tid < n_rows) a.lse[row0 + tid] = NAN;
+        return;
+    }
+    // a warp lists a row's pieces and weighs them
+    for (uint32_t w = warp; w < kJoinRows; w += NT / 32) {
+        const uint32_t row = row0 + w;
+        if (row < begin || row >= end) continue;
+        const RowPieces e0 = l.at[2 * static_cast<uint64_t>(row)], e1 = l.at[2 * static_cast<uint64_t>(row) + 1];
+        const uint32_t n_all = e0.n + e1.n;
+        uint32_t n = 0;
+        float top = -INFINITY, sum = 0.0f;
+        for (uint32_t i0 = 0; i0 < n_all; i0 += 32) {
+            const uint32_t i = i0 + lane;
+            const uint32_t id = i < e0.n ? e0.id + i * e0.step : e1.id + (i - e0.n) * e1.step;
+            const float2 ml = i < n_all ? l.ml[id] : make_float2(-INFINITY, 0.0f);
+            const uint32_t have = __ballot_sync(0xffffffffu, ml.x != -INFINITY);
+            float mt = ml.x;
+            for (int o = 16; o; o >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, o));
+            mt = fmaxf(mt, top);
+            // the weights so far, and this lane's, against the new maximum
+            const float f = top == -INFINITY ? 0.0f : ex2(top - mt);
+            for (uint32_t j = lane; j < n; j += 32) s_w[w][j] *= f;
+            sum *= f;
+            top = mt;
+            if (ml.x != -INFINITY) {
+                const uint32_t at = n + __popc(have & ((1u << lane) - 1));
+                const float e = ex2(ml.x - top);
+                s_id[w][at] = id;
+                s_w[w][at] = e;
+                sum += e * ml.y;
+            }
+            n += __popc(have);
+            __syncwarp();
+        }
+        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0) {
+            s_n[w] = n;
+            s_inv[w] = n ? 1.0f / sum : 0.0f;
+            if (a.lse) a.lse[row] = n ? (top + log2f(sum)) * 0.693147181f : -INFINITY;
+        }
+    }
+    __syncthreads();
+    const uint32_t r = tid % kJoinRows, col = tid / kJoinRows;
+    if (row0 + r < begin || row0 + r >= end) return;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const uint32_t n = s_n[r];
+    for (uint32_t i0 = 0; i0 < n; i0 += 16) {
+        float4 o[16];
+#pragma unroll
+        for (uint32_t i = 0; i < 16; ++i) {
+            o[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (i0 + i < n) {
+                const uint32_t id = s_id[r][i0 + i];
+                o[i] = l.o[(static_cast<uint64_t>(id / 128) * (D / 4) + col) * 128 + id % 128];
+            }
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < 16; ++i) {
+            const float f = i0 + i < n ? s_w[r][i0 + i] : 0.0f;
+            acc.x = __fmaf_rn(f, o[i].x, acc.x);
+            acc.y = __fmaf_rn(f, o[i].y, acc.y);
+            acc.z = __fmaf_rn(f, o[i].z, acc.z);
+            acc.w = __fmaf_rn(f, o[i].w, acc.w);
+        }
+    }
+    const float inv = s_inv[r];
+    *reinterpret_cast<uint2 *>(a.out + static_cast<uint64_t>(row0 + r) * D + 4 * col) =
+        make_uint2(pack_h2(acc.x * inv, acc.y * inv), pack_h2(acc.z * inv, acc.w * inv));
+}
+
+// Tensor map of a page list's K or V rows. f16: 4-D {D, heads, tokens, pages},
+// box {64, 1, tokens of a tile, 1}, 128-byte swizzle. Quant blocks: 3-D
+// {row bytes / 2, tokens, pages}, box {raw_box / 2, tokens of a tile, 1}.
+template <int D>
+cudaError_t encode_pages(CUtensorMap *map, const uint8_t *at, uint64_t row, uint64_t page, int32_t type,
+                         const PageView &v) {
+    const EncodeTiledFn fn = encode_fn();
+    if (!fn) return cudaErrorNotSupported;
+    const bool f16 = type == KVMRET_TYPE_F16;
+    const cuuint32_t tok = std::min<uint32_t>(v.page_tokens, Cfg<D, false>::BN);
+    const cuuint64_t dims[4] = {f16 ? D : row / 2, f16 ? v.n_head_kv : v.page_tokens,
+                                f16 ? v.page_tokens : v.n_pages, v.n_pages};
+    const cuuint64_t strides[3] = {f16 ? D * 2ull : row, f16 ? row : page, page};
+    const cuuint32_t box[4] = {f16 ? 64 : raw_box<D>(type) / 2, f16 ? 1 : tok, f16 ? tok : 1, 1};
+    const cuuint32_t estr[4] = {1, 1, 1, 1};
+    const CUresult r = fn(map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT16,
+                          f16 ? 4 : 3, const_cast<uint8_t *>(at), dims, strides, box, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          f16 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+uint32_t attn_ctas() {
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess ||
+        cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0)
+        n = 148;
+    return std::min<uint32_t>(static_cast<uint32_t>(n), kMaxCtas);
+}
+
+uint64_t up256(uint64_t v) { return (v + 255) / 256 * 256; }
+
+// The workspace: one word per CTA, the rows' notes, the pieces.
+struct WsLayout {
+    uint64_t at, ml, o, bytes, slots;
+    WsLayout(uint32_t n_q, uint32_t n_head, uint32_t n_head_kv, uint32_t d, uint32_t n_seq) {
+        const uint64_t pr = d == 256 ? 128 : 256, ns = pr / 128;
+        const uint64_t rows = static_cast<uint64_t>(n_q) * (n_head / n_head_kv);
+        const uint64_t pairs = (rows + pr - 1) / pr, pg = (pairs + 7) / 8;
+        // prefix: n_pg * gs <= pairs + n_pg units a KV head, and a range each;
+        // tails: a pair per sequence more than whole pairs of the rows
+        slots = (pairs + pg) * n_head_kv + 2 * kMaxCtas +
+                (n_seq ? (n_seq + rows / pr) * n_head_kv : 0);
+        at = up256(kMaxCtas * 4);
+        ml = at + up256(2ull * n_q * n_head * sizeof(RowPieces));
+        o = ml + up256(slots * ns * 128 * 8);
+        bytes = o + slots * ns * 128 * d * 4;
+    }
+};
+
+template <int D, bool QUANT>
+cudaError_t launch_main(const AttnLaunch &l, uint32_t n_cta, cudaStream_t st) {
+    const size_t smem = Cfg<D, QUANT>::tiles + sizeof(Small<D, QUANT>);
+    const cudaError_t e =
+        cudaFuncSetAttribute(attn_tc_kernel<D, QUANT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(smem));
+    if (e != cudaSuccess) return e;
+    attn_tc_kernel<D, QUANT><<<n_cta, Cfg<D, QUANT>::threads, smem, st>>>(l);
+    return cudaGetLastError();
+}
+
+template <int D>
+cudaError_t launch_t(AttnLaunch &l, cudaStream_t st) {
+    const uint32_t n_cta = attn_ctas();
+    const KeyList *lists[2] = {&l.a.prefix, &l.a.tail};
+    bool quant = false;
+    cudaError_t e = cudaSuccess;
+    for (int i = 0; i < 2; ++i) {
+        const PageView &v = lists[i]->pages;
+        if (!lists[i]->max_len) continue;
+        quant = quant || v.k_type != KVMRET_TYPE_F16 || v.v_type != KVMRET_TYPE_F16;
+        e = encode_pages<D>(&l.map[2 * i], v.k, v.k_row, v.k_page, v.k_type, v);
+        if (e == cudaSuccess)
+            e = encode_pages<D>(&l.map[2 * i + 1], v.v, v.v_row, v.v_page, v.v_type, v);
+        if (e != cudaSuccess) return e;
+    }
+    e = quant ? launch_main<D, true>(l, n_cta, st) : launch_main<D, false>(l, n_cta, st);
+    if (e != cudaSuccess) return e;
+    const uint64_t rows = static_cast<uint64_t>(l.a.n_q) * l.a.n_head;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<uint32_t>((rows + kJoinRows - 1) / kJoinRows));
+    cfg.blockDim = dim3(kJoinRows * D / 4);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, attn_join_kernel<D>, l, n_cta);
 }
 
 }  // namespace
 
-cudaError_t launch_prefix_attn_rows(const PrefixAttn &a, cudaStream_t st) {
-    const dim3 grid(a.n_q, a.n_head);
-    if (a.d_head == 64)
-        attn_kernel<64><<<grid, 32 * kWarps, 0, st>>>(a);
-    else if (a.d_head == 128)
-        attn_kernel<128><<<grid, 32 * kWarps, 0, st>>>(a);
-    else
-        attn_kernel<256><<<grid, 32 * kWarps, 0, st>>>(a);
-    return cudaGetLastError();
+size_t prefix_attn_ws_bytes(uint32_t n_q, uint32_t n_head, uint32_t n_head_kv, uint32_t d_head,
+                            uint32_t n_seq) {
+    return WsLayout(n_q, n_head, n_head_kv, d_head, n_seq).bytes;
+}
+
+cudaError_t launch_prefix_attn(const PrefixAttn &a, void *ws, cudaStream_t st) {
+    const WsLayout w(a.n_q, a.n_head, a.n_head_kv, a.d_head, a.n_seq);
+    uint8_t *b = static_cast<uint8_t *>(ws);
+    AttnLaunch l{};
+    l.a = a;
+    l.fail = reinterpret_cast<uint32_t *>(b);
+    l.at = reinterpret_cast<RowPieces *>(b + w.at);
+    l.ml = reinterpret_cast<float2 *>(b + w.ml);
+    l.o = reinterpret_cast<float4 *>(b + w.o);
+    l.max_slots = static_cast<uint32_t>(w.slots);
+    if (a.d_head == 64) return launch_t<64>(l, st);
+    if (a.d_head == 128) return launch_t<128>(l, st);
+    return launch_t<256>(l, st);
 }
 
 }  // namespace kvmret
