@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from dataclasses import dataclass
 
 import numpy as np
@@ -650,13 +651,13 @@ class Retriever:
         prefix, after the steps enqueued so far. Arguments and result as there."""
         import torch
         c = self.cfg
-        _want(q.device.type == "cuda" and q.device.index == c.device,
-              f"q: a tensor on the context's device cuda:{c.device}")
-        a, got, keep = _attn_args(q, c.d_head, tail, tail_table, tail_len, q_start, scale, lse, out)
-        ws, nb = _attn_ws(q, c.n_head_kv, a.n_seq)
-        with torch.cuda.device(q.device), _Ordered(self.stream_ptr):
-            _check(lib.kvmret_window_attn(self.h, layer, None if tail is None else
-                                          ctypes.byref(tail.desc), ctypes.byref(a), ws.data_ptr(), nb))
+        front, tails, got, shape = _attn_args(q, c.device, c.d_head, tail, tail_table, tail_len,
+                                              q_start, scale, lse, out)
+        with torch.cuda.device(c.device):
+            ws, nb = _attn_ws(shape, c.n_head_kv, tails[0], q.device)
+            with _Ordered(self.stream_ptr):
+                _check(_window_attn_call(self.h, layer, None if tail is None else tail.ref,
+                                         _ATTN.pack(*front, 0, 0, 0, 0, *tails), ws.data_ptr(), nb))
         return got
 
     def window_layout(self):
@@ -976,34 +977,67 @@ def _want(ok, msg):
         raise KvmretError(msg)
 
 
-def _launch(dev, stream, fn, *args):
-    """Call a stateless entry point with its buffers' device current, on the
-    given stream of that device or torch's current one."""
+# The attention step's calls run once per layer and token, so their arguments
+# are packed in one go (struct) instead of field by field; the layouts are
+# those of QkArgs and AttnArgs.
+_QK = struct.Struct("=11Q6Iifff")
+_ATTN = struct.Struct("=QQQQIIfIQQQIIQQQ")
+assert _QK.size == ctypes.sizeof(QkArgs) and _ATTN.size == ctypes.sizeof(AttnArgs)
+_packed = ctypes.c_char_p
+_qk_call = ctypes.CFUNCTYPE(ctypes.c_int, _packed, _P)(("kvmret_qk_norm_rope", lib))
+_attn_call = ctypes.CFUNCTYPE(ctypes.c_int, _P, _P, _packed, _P, ctypes.c_size_t,
+                              _P)(("kvmret_prefix_attn", lib))
+_append_call = ctypes.CFUNCTYPE(ctypes.c_int, _P, _P, _U64, _P, _U64, _P, _P, _U32, ctypes.c_float,
+                                ctypes.c_float, _U32, _P)(("kvmret_paged_append", lib))
+_window_attn_call = ctypes.CFUNCTYPE(ctypes.c_int, _P, _U32, _P, _packed, _P,
+                                     ctypes.c_size_t)(("kvmret_window_attn", lib))
+
+
+def _launch(index, stream, fn, *args):
+    """Call a stateless entry point with device `index` (its buffers') current,
+    on the given stream of that device or torch's current one."""
     import torch
-    if dev.index != torch.cuda.current_device():
-        with torch.cuda.device(dev):
-            _check(fn(*args, _torch_stream(stream)))
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            rc = fn(*args, _torch_stream(stream))
     else:
-        _check(fn(*args, _torch_stream(stream)))
+        rc = fn(*args, stream or torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _check(rc)
+
+
+def _used_on(stream, index, *tensors):
+    """Tensors made here are used on the caller's stream: torch must not hand
+    their memory on before that stream has passed."""
+    import torch
+    ext = torch.cuda.ExternalStream(stream, device=index)
+    for x in tensors:
+        if x is not None:
+            x.record_stream(ext)
 
 
 def _head_rows(x, name):
     """A [n_tok][heads][d_head] view whose tokens may be strided: its strides
     inside a token must be dense."""
-    _want(x.is_cuda and x.dim() == 3, f"{name}: a [n_tok][heads][d_head] CUDA tensor")
-    row = x.shape[1] * x.shape[2]
-    _want(x.numel() == 0 or (x.stride(2) == 1 and (x.shape[1] == 1 or x.stride(1) == x.shape[2])),
-          f"{name}: the heads of a token must be contiguous")
-    _want(x.shape[0] < 2 or x.stride(0) >= row, f"{name}: the tokens must not overlap")
-    return x.stride(0) if x.shape[0] > 1 else row
+    shape = x.shape
+    _want(x.is_cuda and len(shape) == 3, f"{name}: a [n_tok][heads][d_head] CUDA tensor")
+    n, h, d = shape
+    row = h * d
+    s0, s1, s2 = x.stride()
+    if not (s2 == 1 and s1 == d and (n < 2 or s0 >= row)) and n * row:
+        _want((s2 == 1 or d == 1) and (s1 == d or h == 1),
+              f"{name}: the heads of a token must be contiguous")
+        _want(n < 2 or s0 >= row, f"{name}: the tokens must not overlap")
+    return shape, s0 if n > 1 else row
 
 
-def _index(x, n, dev, name):
-    """A contiguous int32 tensor of n elements (None: any) on dev."""
+def _index(x, n, index, name):
+    """A contiguous int32 tensor of n elements (None: any) on device `index`."""
     import torch
-    _want(x.dtype == torch.int32 and x.device == dev and x.is_contiguous() and
-          (n is None or x.numel() == n),
-          f"{name}: a contiguous int32 tensor{'' if n is None else f' of {n}'} on {dev}")
+    if not (x.dtype is torch.int32 and x.get_device() == index and x.is_contiguous() and
+            (n is None or x.numel() == n)):
+        raise KvmretError(f"{name}: a contiguous int32 tensor"
+                          f"{'' if n is None else f' of {n}'} on cuda:{index}")
     return x.data_ptr()
 
 
@@ -1019,26 +1053,33 @@ def qk_norm_rope(q, k, pos, q_weight=None, k_weight=None, eps=1e-6, freq_base=1e
     k_rot, q_raw, k_raw): f16 tensors, None where not wanted; *_raw is the
     normed row without the rotation (query_add rows, append's k_cap)."""
     import torch
-    types = {torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16, torch.float32: TYPE_F32}
-    dev = q.device
-    _want(q.dtype in types and k.dtype == q.dtype and k.device == dev,
+    empty, f16, index = torch.empty, torch.float16, q.get_device()
+    kind = q.dtype
+    t = (TYPE_F16 if kind is f16 else TYPE_BF16 if kind is torch.bfloat16 else
+         TYPE_F32 if kind is torch.float32 else None)
+    _want(t is not None and k.dtype is kind and k.get_device() == index,
           "q and k: f16, bf16 or f32, of one type and device")
-    qs, ks = _head_rows(q, "q"), _head_rows(k, "k")
-    n, hq, d = q.shape
-    hkv = k.shape[1]
-    _want(k.shape[0] == n and k.shape[2] == d, "k: [n_tok][n_head_kv][d_head] like q")
-    ptrs = []
+    (n, hq, d), qs = _head_rows(q, "q")
+    (nk, hkv, dk), ks = _head_rows(k, "k")
+    _want(nk == n and dk == d, "k: [n_tok][n_head_kv][d_head] like q")
     for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
-        _want(w is None or (w.dtype == torch.float32 and w.device == dev and w.is_contiguous() and
-                            w.numel() == d), f"{name}: {d} contiguous f32 values on {dev}")
-        ptrs.append(None if w is None else w.data_ptr())
-    outs = [torch.empty((n, h, d), dtype=torch.float16, device=dev) if on else None
-            for on, h in ((q_rot, hq), (k_rot, hkv), (q_raw, hq), (k_raw, hkv))]
-    a = QkArgs(q.data_ptr(), k.data_ptr(), qs, ks, ptrs[0], ptrs[1], _index(pos, n, dev, "pos"),
-               *[None if o is None else o.data_ptr() for o in outs], n, hq, hkv, d, d, fwht_n,
-               types[q.dtype], eps, freq_base, freq_scale)
-    _launch(dev, stream, lib.kvmret_qk_norm_rope, ctypes.byref(a))
-    return tuple(outs)
+        if w is not None and not (w.dtype is torch.float32 and w.get_device() == index and
+                                  w.is_contiguous() and w.numel() == d):
+            raise KvmretError(f"{name}: {d} contiguous f32 values on cuda:{index}")
+    dev = q.device
+    o0 = empty((n, hq, d), dtype=f16, device=dev) if q_rot else None
+    o1 = empty((n, hkv, d), dtype=f16, device=dev) if k_rot else None
+    o2 = empty((n, hq, d), dtype=f16, device=dev) if q_raw else None
+    o3 = empty((n, hkv, d), dtype=f16, device=dev) if k_raw else None
+    a = _QK.pack(q.data_ptr(), k.data_ptr(), qs, ks, 0 if q_weight is None else q_weight.data_ptr(),
+                 0 if k_weight is None else k_weight.data_ptr(), _index(pos, n, index, "pos"),
+                 o0.data_ptr() if q_rot else 0, o1.data_ptr() if k_rot else 0,
+                 o2.data_ptr() if q_raw else 0, o3.data_ptr() if k_raw else 0,
+                 n, hq, hkv, d, d, fwht_n, t, eps, freq_base, freq_scale)
+    _launch(index, stream, _qk_call, a)
+    if stream:
+        _used_on(stream, index, o0, o1, o2, o3)
+    return o0, o1, o2, o3
 
 
 class Pages:
@@ -1057,9 +1098,12 @@ class Pages:
                   page_tokens * row_bytes(t, n_head_kv * d_head),
                   "pages: a page must be page_tokens contiguous rows of its type")
             strides.append(x.stride(0) * x.element_size() if x.shape[0] > 1 else 0)
-        self.k, self.v, self.device = k, v, k.device
+        self.k, self.v, self.index = k, v, k.get_device()
+        self.n_pages, self.page_tokens = k.shape[0], page_tokens
+        self.n_head_kv, self.d_head = n_head_kv, d_head
         self.desc = PagesDesc(k.data_ptr(), v.data_ptr(), strides[0], strides[1], k.shape[0],
                               page_tokens, n_head_kv, d_head, k_type, v_type)
+        self.ref = ctypes.addressof(self.desc)
 
 
 def paged_append(pages, k, v, cells, pos=None, freq_base=1e6, freq_scale=1.0, fwht_n=0, stream=0):
@@ -1069,51 +1113,59 @@ def paged_append(pages, k, v, cells, pos=None, freq_base=1e6, freq_scale=1.0, fw
     [n_tok] int32; a token with a negative cell is skipped; the others' cells
     must differ."""
     import torch
-    p = pages.desc
-    for x, name in ((k, "k"), (v, "v")):
-        _want(x.dtype == torch.float16 and x.device == pages.device and
-              x.shape == (k.shape[0], p.n_head_kv, p.d_head),
-              f"{name}: [n_tok][{p.n_head_kv}][{p.d_head}] f16 on {pages.device}")
-    n = k.shape[0]
-    ks, vs = _head_rows(k, "k"), _head_rows(v, "v")
-    _launch(pages.device, stream, lib.kvmret_paged_append, ctypes.byref(p), k.data_ptr(), ks,
-            v.data_ptr(), vs, _index(cells, n, pages.device, "cells"),
-            None if pos is None else _index(pos, n, pages.device, "pos"), n, freq_base, freq_scale,
-            fwht_n)
+    index, f16 = pages.index, torch.float16
+    (n, h, d), ks = _head_rows(k, "k")
+    vshape, vs = _head_rows(v, "v")
+    if not (k.dtype is f16 and v.dtype is f16 and k.get_device() == index and v.get_device() == index and
+            h == pages.n_head_kv and d == pages.d_head and vshape == (n, h, d)):
+        raise KvmretError(f"k and v: [n_tok][{pages.n_head_kv}][{pages.d_head}] f16 on cuda:{index}")
+    _launch(index, stream, _append_call, pages.ref, k.data_ptr(), ks, v.data_ptr(), vs,
+            _index(cells, n, index, "cells"), 0 if pos is None else _index(pos, n, index, "pos"), n,
+            freq_base, freq_scale, fwht_n)
 
 
-def _attn_args(q, d_head, tail, tail_table, tail_len, q_start, scale, lse, out):
-    """The arguments that prefix_attn and window_attn share, and their result."""
+def _attn_args(q, index, d_head, tail, tail_table, tail_len, q_start, scale, lse, out):
+    """What prefix_attn and window_attn share: the fields of AttnArgs around the
+    prefix's, the result, the shape."""
     import torch
-    dev = q.device
-    _want(q.dtype == torch.float16, "q: f16")
-    stride = _head_rows(q, "q")
-    n, h, d = q.shape
+    f16 = torch.float16
+    _want(q.dtype is f16 and q.get_device() == index, f"q: f16 on cuda:{index}")
+    (n, h, d), stride = _head_rows(q, "q")
     _want(d == d_head, f"q: heads of {d_head}")
     if out is None:
-        out = torch.empty((n, h, d), dtype=torch.float16, device=dev)
+        out = torch.empty((n, h, d), dtype=f16, device=q.device)
     else:
-        _want(out.dtype == torch.float16 and out.device == dev and out.shape == q.shape and
+        _want(out.dtype is f16 and out.get_device() == index and out.shape == q.shape and
               out.is_contiguous(), "out: contiguous f16 like q")
-    sums = torch.empty((n, h), dtype=torch.float32, device=dev) if lse else None
-    a = AttnArgs(q.data_ptr(), stride, out.data_ptr(), None if sums is None else sums.data_ptr(), n,
-                 h, d ** -0.5 if scale is None else scale)
+    sums = torch.empty((n, h), dtype=torch.float32, device=q.device) if lse else None
+    tails = (0, 0, 0, 0, 0)
     if tail is not None:
-        _want(tail.device == dev and tail_table is not None and tail_len is not None and
+        _want(tail.index == index and tail_table is not None and tail_len is not None and
               q_start is not None and tail_table.dim() == 2,
               "tails need [n_seq][pages] table, lengths and q_start")
-        s = a.n_seq = tail_table.shape[0]
-        a.tail_pages = tail_table.shape[1]
-        a.q_start_dev = _index(q_start, s + 1, dev, "q_start")
-        a.tail_table_dev = _index(tail_table, None, dev, "tail_table")
-        a.tail_len_dev = _index(tail_len, s, dev, "tail_len")
-    return a, ((out, sums) if lse else out), stride
+        s, width = tail_table.shape
+        tails = (s, width, _index(q_start, s + 1, index, "q_start"),
+                 _index(tail_table, None, index, "tail_table"), _index(tail_len, s, index, "tail_len"))
+    front = (q.data_ptr(), stride, out.data_ptr(), sums.data_ptr() if lse else 0, n, h,
+             d ** -0.5 if scale is None else scale)
+    return front, tails, ((out, sums) if lse else out), (n, h, d)
 
 
-def _attn_ws(q, n_head_kv, n_seq):
+_ws_bytes = {}
+
+
+def _attn_ws(shape, n_head_kv, n_seq, dev):
+    """A workspace of the call's own: torch's allocator keeps it from other
+    work until this call's place on the stream has passed."""
     import torch
-    nb = int(lib.kvmret_prefix_attn_ws_bytes(q.shape[0], q.shape[1], n_head_kv, q.shape[2], n_seq))
-    return torch.empty(nb, dtype=torch.uint8, device=q.device), nb
+    key = (shape, n_head_kv, n_seq)
+    nb = _ws_bytes.get(key)
+    if nb is None:
+        if len(_ws_bytes) > 4096:
+            _ws_bytes.clear()
+        nb = _ws_bytes[key] = int(lib.kvmret_prefix_attn_ws_bytes(shape[0], shape[1], n_head_kv,
+                                                                  shape[2], n_seq))
+    return torch.empty(nb, dtype=torch.uint8, device=dev), nb
 
 
 def prefix_attn(q, prefix, prefix_len, tail=None, tail_table=None, tail_len=None, q_start=None,
@@ -1129,24 +1181,29 @@ def prefix_attn(q, prefix, prefix_len, tail=None, tail_table=None, tail_len=None
     the prefix (default: what its pages hold). Either part may be None.
     scale defaults to d_head ** -0.5. Returns out (rows of no sequence: as
     they were), with lse=True also the f32 [n_q][n_head] log-sum-exp."""
-    dev = q.device
     pages = prefix if prefix is not None else tail
-    _want(pages is not None and pages.device == dev, "a prefix or tails, on q's device")
-    a, got, _ = _attn_args(q, pages.desc.d_head, tail, tail_table, tail_len, q_start, scale, lse, out)
+    _want(pages is not None, "a prefix or tails")
+    index = pages.index
+    front, tails, got, shape = _attn_args(q, index, pages.d_head, tail, tail_table, tail_len, q_start,
+                                          scale, lse, out)
+    most = length = table = ntok = 0
     if prefix is not None:
-        held = prefix.desc.n_pages if prefix_table is None else prefix_table.numel()
-        if prefix_ntok is not None:
-            a.prefix_ntok_dev = _index(prefix_ntok, held if prefix_table is not None else None, dev,
-                                       "prefix_ntok")
-            held = min(held, prefix_ntok.numel())
-        held *= prefix.desc.page_tokens
-        a.max_prefix = held if max_prefix is None else max_prefix
-        _want(0 <= a.max_prefix <= held, f"max_prefix: at most the {held} tokens of the pages")
+        held = prefix.n_pages
         if prefix_table is not None:
-            a.prefix_table_dev = _index(prefix_table, None, dev, "prefix_table")
+            held = prefix_table.numel()
+            table = _index(prefix_table, None, index, "prefix_table")
+        if prefix_ntok is not None:
+            ntok = _index(prefix_ntok, held if table else None, index, "prefix_ntok")
+            held = min(held, prefix_ntok.numel())
+        held *= prefix.page_tokens
+        most = held if max_prefix is None else max_prefix
+        _want(0 <= most <= held, f"max_prefix: at most the {held} tokens of the pages")
         if prefix_len is not None:
-            a.prefix_len_dev = _index(prefix_len, 1, dev, "prefix_len")
-    ws, nb = _attn_ws(q, pages.desc.n_head_kv, a.n_seq)
-    _launch(dev, stream, lib.kvmret_prefix_attn, None if prefix is None else ctypes.byref(prefix.desc),
-            None if tail is None else ctypes.byref(tail.desc), ctypes.byref(a), ws.data_ptr(), nb)
+            length = _index(prefix_len, 1, index, "prefix_len")
+    ws, nb = _attn_ws(shape, pages.n_head_kv, tails[0], q.device)
+    _launch(index, stream, _attn_call, None if prefix is None else prefix.ref,
+            None if tail is None else tail.ref,
+            _ATTN.pack(*front, most, length, table, ntok, *tails), ws.data_ptr(), nb)
+    if stream:
+        _used_on(stream, index, ws, *(got if lse else (got,)))
     return got

@@ -435,3 +435,27 @@ def test_wrapper_refusals():
         with pytest.raises(kvmret.KvmretError):
             call()
     assert kvmret.prefix_attn(z(0, 4, 128), p, None).shape == (0, 4, 128)
+
+
+def test_on_a_stream_given_by_its_handle():
+    """The stream argument: results as on the current stream, the workspace
+    and the outputs kept from other work until that stream has passed."""
+    case = ([1] * 6, [30] * 6, 900, 8, 2, 128, 64, 32, F16, F16)
+    pool, tpool, table, own, _, _, start, q, tl = build(case)
+    args = (dev(q), pool.device(), dev(np.array([900], np.int32)), tpool.device(), dev(own), dev(tl),
+            dev(start))
+    t = dev(table)
+    want = kvmret.prefix_attn(*args, prefix_table=t)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(8):
+        got.append(kvmret.prefix_attn(*args, prefix_table=t, stream=side.cuda_stream))
+        torch.full((1 << 22,), float("nan"), device="cuda")  # would take over a freed workspace
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want) for x in got)
+    pos = torch.arange(6, device="cuda", dtype=torch.int32)
+    a = kvmret.qk_norm_rope(args[0], args[0][:, :2], pos, stream=side.cuda_stream)
+    torch.cuda.synchronize()
+    b = kvmret.qk_norm_rope(args[0], args[0][:, :2], pos)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
