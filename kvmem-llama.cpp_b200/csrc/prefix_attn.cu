@@ -35,6 +35,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <type_traits>
 
@@ -1292,12 +1293,26 @@ cudaError_t encode_pages(CUtensorMap *map, const uint8_t *at, uint64_t row, uint
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
-uint32_t attn_ctas() {
-    int dev = 0, n = 0;
+// What a launch asks of the device, kept per device: its SM count, and which
+// kernels have been allowed their shared memory (bit 2 * log2(D / 64) + QUANT).
+struct DeviceFacts {
+    std::atomic<uint32_t> ctas{0}, allowed{0};
+};
+DeviceFacts *device_facts() {
+    static DeviceFacts facts[64];
+    int dev = 0;
+    return cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64 ? &facts[dev] : nullptr;
+}
+uint32_t attn_ctas(DeviceFacts *f) {
+    uint32_t n = f ? f->ctas.load(std::memory_order_relaxed) : 0;
+    if (n) return n;
+    int dev = 0, sm = 0;
     if (cudaGetDevice(&dev) != cudaSuccess ||
-        cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0)
-        n = 148;
-    return std::min<uint32_t>(static_cast<uint32_t>(n), kMaxCtas);
+        cudaDeviceGetAttribute(&sm, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sm <= 0)
+        sm = 148;
+    n = std::min<uint32_t>(static_cast<uint32_t>(sm), kMaxCtas);
+    if (f) f->ctas.store(n, std::memory_order_relaxed);
+    return n;
 }
 
 uint64_t up256(uint64_t v) { return (v + 255) / 256 * 256; }
@@ -1321,19 +1336,24 @@ struct WsLayout {
 };
 
 template <int D, bool QUANT>
-cudaError_t launch_main(const AttnLaunch &l, uint32_t n_cta, cudaStream_t st) {
+cudaError_t launch_main(const AttnLaunch &l, uint32_t n_cta, DeviceFacts *f, cudaStream_t st) {
     const size_t smem = Cfg<D, QUANT>::tiles + sizeof(Small<D, QUANT>);
-    const cudaError_t e =
-        cudaFuncSetAttribute(attn_tc_kernel<D, QUANT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(smem));
-    if (e != cudaSuccess) return e;
+    constexpr uint32_t bit = 1u << ((D == 64 ? 0 : D == 128 ? 2 : 4) + QUANT);
+    if (!f || !(f->allowed.load(std::memory_order_relaxed) & bit)) {
+        const cudaError_t e =
+            cudaFuncSetAttribute(attn_tc_kernel<D, QUANT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 static_cast<int>(smem));
+        if (e != cudaSuccess) return e;
+        if (f) f->allowed.fetch_or(bit, std::memory_order_relaxed);
+    }
     attn_tc_kernel<D, QUANT><<<n_cta, Cfg<D, QUANT>::threads, smem, st>>>(l);
     return cudaGetLastError();
 }
 
 template <int D>
 cudaError_t launch_t(AttnLaunch &l, cudaStream_t st) {
-    const uint32_t n_cta = attn_ctas();
+    DeviceFacts *f = device_facts();
+    const uint32_t n_cta = attn_ctas(f);
     const KeyList *lists[2] = {&l.a.prefix, &l.a.tail};
     bool quant = false;
     cudaError_t e = cudaSuccess;
@@ -1346,7 +1366,7 @@ cudaError_t launch_t(AttnLaunch &l, cudaStream_t st) {
             e = encode_pages<D>(&l.map[2 * i + 1], v.v, v.v_row, v.v_page, v.v_type, v);
         if (e != cudaSuccess) return e;
     }
-    e = quant ? launch_main<D, true>(l, n_cta, st) : launch_main<D, false>(l, n_cta, st);
+    e = quant ? launch_main<D, true>(l, n_cta, f, st) : launch_main<D, false>(l, n_cta, f, st);
     if (e != cudaSuccess) return e;
     const uint64_t rows = static_cast<uint64_t>(l.a.n_q) * l.a.n_head;
     cudaLaunchConfig_t cfg = {};

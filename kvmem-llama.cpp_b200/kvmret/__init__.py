@@ -1018,16 +1018,18 @@ def _used_on(stream, index, *tensors):
 
 def _head_rows(x, name):
     """A [n_tok][heads][d_head] view whose tokens may be strided: its strides
-    inside a token must be dense."""
+    inside a token must be dense. Returns its shape and token stride."""
     shape = x.shape
-    _want(x.is_cuda and len(shape) == 3, f"{name}: a [n_tok][heads][d_head] CUDA tensor")
+    if not (x.is_cuda and len(shape) == 3):
+        raise KvmretError(f"{name}: a [n_tok][heads][d_head] CUDA tensor")
     n, h, d = shape
     row = h * d
     s0, s1, s2 = x.stride()
     if not (s2 == 1 and s1 == d and (n < 2 or s0 >= row)) and n * row:
-        _want((s2 == 1 or d == 1) and (s1 == d or h == 1),
-              f"{name}: the heads of a token must be contiguous")
-        _want(n < 2 or s0 >= row, f"{name}: the tokens must not overlap")
+        if not ((s2 == 1 or d == 1) and (s1 == d or h == 1)):
+            raise KvmretError(f"{name}: the heads of a token must be contiguous")
+        if n > 1 and s0 < row:
+            raise KvmretError(f"{name}: the tokens must not overlap")
     return shape, s0 if n > 1 else row
 
 
@@ -1053,7 +1055,7 @@ def qk_norm_rope(q, k, pos, q_weight=None, k_weight=None, eps=1e-6, freq_base=1e
     k_rot, q_raw, k_raw): f16 tensors, None where not wanted; *_raw is the
     normed row without the rotation (query_add rows, append's k_cap)."""
     import torch
-    empty, f16, index = torch.empty, torch.float16, q.get_device()
+    empty, like, f16, index = torch.empty_strided, torch.empty_like, torch.float16, q.get_device()
     kind = q.dtype
     t = (TYPE_F16 if kind is f16 else TYPE_BF16 if kind is torch.bfloat16 else
          TYPE_F32 if kind is torch.float32 else None)
@@ -1067,10 +1069,11 @@ def qk_norm_rope(q, k, pos, q_weight=None, k_weight=None, eps=1e-6, freq_base=1e
                                   w.is_contiguous() and w.numel() == d):
             raise KvmretError(f"{name}: {d} contiguous f32 values on cuda:{index}")
     dev = q.device
-    o0 = empty((n, hq, d), dtype=f16, device=dev) if q_rot else None
-    o1 = empty((n, hkv, d), dtype=f16, device=dev) if k_rot else None
-    o2 = empty((n, hq, d), dtype=f16, device=dev) if q_raw else None
-    o3 = empty((n, hkv, d), dtype=f16, device=dev) if k_raw else None
+    sq, sk = ((n, hq, d), (hq * d, d, 1)), ((n, hkv, d), (hkv * d, d, 1))
+    o0 = empty(*sq, dtype=f16, device=dev) if q_rot else None
+    o1 = empty(*sk, dtype=f16, device=dev) if k_rot else None
+    o2 = (like(o0) if q_rot else empty(*sq, dtype=f16, device=dev)) if q_raw else None
+    o3 = (like(o1) if k_rot else empty(*sk, dtype=f16, device=dev)) if k_raw else None
     a = _QK.pack(q.data_ptr(), k.data_ptr(), qs, ks, 0 if q_weight is None else q_weight.data_ptr(),
                  0 if k_weight is None else k_weight.data_ptr(), _index(pos, n, index, "pos"),
                  o0.data_ptr() if q_rot else 0, o1.data_ptr() if k_rot else 0,
@@ -1129,11 +1132,11 @@ def _attn_args(q, index, d_head, tail, tail_table, tail_len, q_start, scale, lse
     prefix's, the result, the shape."""
     import torch
     f16 = torch.float16
-    _want(q.dtype is f16 and q.get_device() == index, f"q: f16 on cuda:{index}")
     (n, h, d), stride = _head_rows(q, "q")
-    _want(d == d_head, f"q: heads of {d_head}")
+    if not (q.dtype is f16 and q.get_device() == index and d == d_head):
+        raise KvmretError(f"q: f16 heads of {d_head} on cuda:{index}")
     if out is None:
-        out = torch.empty((n, h, d), dtype=f16, device=q.device)
+        out = torch.empty_strided((n, h, d), (h * d, d, 1), dtype=f16, device=q.device)
     else:
         _want(out.dtype is f16 and out.get_device() == index and out.shape == q.shape and
               out.is_contiguous(), "out: contiguous f16 like q")
@@ -1165,7 +1168,7 @@ def _attn_ws(shape, n_head_kv, n_seq, dev):
             _ws_bytes.clear()
         nb = _ws_bytes[key] = int(lib.kvmret_prefix_attn_ws_bytes(shape[0], shape[1], n_head_kv,
                                                                   shape[2], n_seq))
-    return torch.empty(nb, dtype=torch.uint8, device=dev), nb
+    return torch.empty_strided((nb,), (1,), dtype=torch.uint8, device=dev), nb
 
 
 def prefix_attn(q, prefix, prefix_len, tail=None, tail_table=None, tail_len=None, q_start=None,
@@ -1197,7 +1200,8 @@ def prefix_attn(q, prefix, prefix_len, tail=None, tail_table=None, tail_len=None
             held = min(held, prefix_ntok.numel())
         held *= prefix.page_tokens
         most = held if max_prefix is None else max_prefix
-        _want(0 <= most <= held, f"max_prefix: at most the {held} tokens of the pages")
+        if not 0 <= most <= held:
+            raise KvmretError(f"max_prefix: at most the {held} tokens of the pages")
         if prefix_len is not None:
             length = _index(prefix_len, 1, index, "prefix_len")
     ws, nb = _attn_ws(shape, pages.n_head_kv, tails[0], q.device)
