@@ -91,14 +91,19 @@ struct Octet<float> {
     }
 };
 
-// RoPE of a lane's pairs; cs: the token's {cos, sin} of pairs 8j ..
-__device__ __forceinline__ void rotate(float (&lo)[8], float (&hi)[8], const float2 *cs) {
+// RoPE of lane j's pairs 8j .. with the token's table (angles()).
+template <int D>
+__device__ __forceinline__ void rotate(float (&lo)[8], float (&hi)[8], const float2 *cs, uint32_t j) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const float2 t = cs[e];
-        const float a = lo[e], b = hi[e];
+    for (int e = 0; e < 8; e += 2) {
+        const float4 t = reinterpret_cast<const float4 *>(cs)[e / 2 * Row<D>::lanes + j];
+        float a = lo[e], b = hi[e];
         lo[e] = __fsub_rn(__fmul_rn(a, t.x), __fmul_rn(b, t.y));
         hi[e] = __fadd_rn(__fmul_rn(a, t.y), __fmul_rn(b, t.x));
+        a = lo[e + 1];
+        b = hi[e + 1];
+        lo[e + 1] = __fsub_rn(__fmul_rn(a, t.z), __fmul_rn(b, t.w));
+        hi[e + 1] = __fadd_rn(__fmul_rn(a, t.w), __fmul_rn(b, t.z));
     }
 }
 
@@ -144,74 +149,114 @@ __device__ __forceinline__ void hadamard(float (&lo)[8], float (&hi)[8], float s
     }
 }
 
-// The {cos, sin} table of a CTA's tokens in shared memory.
+// The {cos, sin} table of a CTA's tokens in shared memory: of each token first
+// pairs 8j, 8j + 1 of every lane j, then 8j + 2, 8j + 3 and so on, so that the
+// lanes of a row read 16 neighbouring bytes each. (In pair order four lanes
+// met in a bank, and the L1 bound a chunk of 2048 tokens at 27 us, now 22.)
 template <int D>
 __device__ __forceinline__ void angles(float2 *cs, const int32_t *pos, uint32_t n,
                                        const Theta &th) {
-    for (uint32_t i = threadIdx.x; i < n * (D / 2); i += kThreads)
-        cs[i] = rope_cs(pos[i / (D / 2)], th.v[i % (D / 2)]);
+    for (uint32_t i = threadIdx.x; i < n * (D / 2); i += kThreads) {
+        const uint32_t t = i / (D / 2), p = i % (D / 2);
+        const uint32_t at = (p % 8 / 2 * Row<D>::lanes + p / 8) * 2 + p % 2;
+        cs[t * (D / 2) + at] = rope_cs(pos[t], th.v[p]);
+    }
 }
 
 // y = x / sqrt(mean(x^2) + eps) * w per head row, f32 throughout (the sum of
 // squares per lane, then over the row's lanes by shuffles), rounded once into
-// each wanted output. CTA = tokens x a range of heads.
+// each wanted output. CTA = tokens x a range of heads; a thread has the octets
+// of kFly rows on their way at a time, the first ones while the CTA's cosines
+// and sines are computed (double precision, about 1 us).
+constexpr int kFly = 2;
 template <int D, typename T, bool FWHT>
 __global__ void __launch_bounds__(kThreads)
     qk_kernel(const __grid_constant__ QkNormRope a, uint32_t tokens, uint32_t heads,
               float fwht_scale) {
     constexpr uint32_t L = Row<D>::lanes, G = kThreads / L;
-    extern __shared__ float2 cs[];
+    __shared__ __align__(16) float2 cs[256];  // tokens * D / 2 <= 256
+    __shared__ __align__(16) float ws[2][D];  // weights of q, k: lane by lane like cs
     const uint32_t t0 = blockIdx.x * tokens, nt = min(tokens, a.n_tok - t0);
     const uint32_t h0 = blockIdx.y * heads, nh = min(heads, a.n_head + a.n_head_kv - h0);
-    const uint32_t j = threadIdx.x % L;
+    const uint32_t j = threadIdx.x % L, rows = nt * nh;
+    struct Place {
+        uint32_t dt, hh;
+        bool is_q;
+    };
+    auto place = [&](uint32_t r) {
+        const uint32_t dt = nt == 1 ? 0 : r / nh, h = h0 + r - dt * nh;
+        return Place{dt, h < a.n_head ? h : h - a.n_head, h < a.n_head};
+    };
+    Octet<T> u[kFly], v[kFly];
+    auto load = [&](uint32_t r0) {
+#pragma unroll
+        for (int f = 0; f < kFly; ++f) {
+            const uint32_t r = r0 + f * G;
+            if (r >= rows) break;
+            const Place p = place(r);
+            const uint64_t t = t0 + p.dt;
+            const T *src = (p.is_q ? static_cast<const T *>(a.q) + t * a.q_stride
+                                   : static_cast<const T *>(a.k) + t * a.k_stride) +
+                           static_cast<uint64_t>(p.hh) * D + 8 * j;
+            u[f].load(src);
+            v[f].load(src + D / 2);
+        }
+    };
+    const uint32_t first = threadIdx.x / L;
+    load(first);
+    for (uint32_t i = threadIdx.x; i < 2 * D; i += kThreads) {
+        const uint32_t c = i % D, o = c % (D / 2);  // octet o / 8 of its half
+        const float *w = i < D ? a.q_weight : a.k_weight;
+        ws[i / D][((c / (D / 2) * 2 + o % 8 / 4) * L + o / 8) * 4 + o % 4] = w ? __ldg(w + c) : 1.0f;
+    }
     angles<D>(cs, a.pos + t0, nt, a.theta);
     __syncthreads();
-    const uint32_t rows = nt * nh;
-    for (uint32_t r0 = 0; r0 < rows; r0 += G) {
-        const uint32_t r = r0 + threadIdx.x / L;
-        const bool act = r < rows;
-        const uint32_t dt = act ? r / nh : 0, h = h0 + (act ? r - dt * nh : 0);
-        const uint64_t t = t0 + dt;
-        const bool is_q = h < a.n_head;
-        const uint32_t hh = is_q ? h : h - a.n_head;
-        const T *src = is_q ? static_cast<const T *>(a.q) + t * a.q_stride
-                            : static_cast<const T *>(a.k) + t * a.k_stride;
-        src += static_cast<uint64_t>(hh) * D + 8 * j;
-        float lo[8] = {}, hi[8] = {};
-        if (act) {
-            Octet<T> u, v;
-            u.load(src);
-            v.load(src + D / 2);
-            u.get(lo);
-            v.get(hi);
-        }
-        float ss = 0.0f;
+    // (whole warps take part in the shuffles: the bound is the CTA's)
+    for (uint32_t rb = 0; rb < rows; rb += kFly * G) {
+        if (rb) load(rb + first);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss += lo[e] * lo[e] + hi[e] * hi[e];
-#pragma unroll
-        for (uint32_t o = L / 2; o >= 1; o /= 2) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        const float inv = __frsqrt_rn(ss * (1.0f / D) + a.eps);
-        const float *w = is_q ? a.q_weight : a.k_weight;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            lo[e] *= inv;
-            hi[e] *= inv;
-            if (w) {
-                lo[e] *= __ldg(w + 8 * j + e);
-                hi[e] *= __ldg(w + D / 2 + 8 * j + e);
+        for (int f = 0; f < kFly; ++f) {
+            if (rb + f * G >= rows) break;
+            const uint32_t r = rb + f * G + first;
+            const bool act = r < rows;
+            const Place p = place(act ? r : 0);
+            float lo[8] = {}, hi[8] = {};
+            if (act) {
+                u[f].get(lo);
+                v[f].get(hi);
             }
-        }
-        const uint64_t o = (t * (is_q ? a.n_head : a.n_head_kv) + hh) * D + 8 * j;
-        uint16_t *raw = is_q ? a.q_raw : a.k_raw, *rot = is_q ? a.q_rot : a.k_rot;
-        if (act && raw) {
-            *reinterpret_cast<uint4 *>(raw + o) = pack_f16(lo);
-            *reinterpret_cast<uint4 *>(raw + o + D / 2) = pack_f16(hi);
-        }
-        rotate(lo, hi, cs + dt * (D / 2) + 8 * j);
-        if constexpr (FWHT) hadamard<D>(lo, hi, fwht_scale);
-        if (act && rot) {
-            *reinterpret_cast<uint4 *>(rot + o) = pack_f16(lo);
-            *reinterpret_cast<uint4 *>(rot + o + D / 2) = pack_f16(hi);
+            float ss = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ss += lo[e] * lo[e] + hi[e] * hi[e];
+#pragma unroll
+            for (uint32_t o = L / 2; o >= 1; o /= 2) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            const float inv = __frsqrt_rn(ss * (1.0f / D) + a.eps);
+            const float4 *w = reinterpret_cast<const float4 *>(ws[p.is_q ? 0 : 1]) + j;
+#pragma unroll
+            for (int e = 0; e < 8; e += 4) {
+                const float4 wl = w[e / 4 * L], wh = w[(2 + e / 4) * L];
+                lo[e] *= inv * wl.x;
+                lo[e + 1] *= inv * wl.y;
+                lo[e + 2] *= inv * wl.z;
+                lo[e + 3] *= inv * wl.w;
+                hi[e] *= inv * wh.x;
+                hi[e + 1] *= inv * wh.y;
+                hi[e + 2] *= inv * wh.z;
+                hi[e + 3] *= inv * wh.w;
+            }
+            const uint64_t o =
+                ((t0 + p.dt) * static_cast<uint64_t>(p.is_q ? a.n_head : a.n_head_kv) + p.hh) * D + 8 * j;
+            uint16_t *raw = p.is_q ? a.q_raw : a.k_raw, *rot = p.is_q ? a.q_rot : a.k_rot;
+            if (act && raw) {
+                *reinterpret_cast<uint4 *>(raw + o) = pack_f16(lo);
+                *reinterpret_cast<uint4 *>(raw + o + D / 2) = pack_f16(hi);
+            }
+            rotate<D>(lo, hi, cs + p.dt * (D / 2), j);
+            if constexpr (FWHT) hadamard<D>(lo, hi, fwht_scale);
+            if (act && rot) {
+                *reinterpret_cast<uint4 *>(rot + o) = pack_f16(lo);
+                *reinterpret_cast<uint4 *>(rot + o + D / 2) = pack_f16(hi);
+            }
         }
     }
 }
@@ -313,21 +358,33 @@ template <int D, int KT, int VT>
 __global__ void __launch_bounds__(kThreads)
     append_kernel(const __grid_constant__ PagedAppend a, uint32_t tokens, float fwht_scale) {
     constexpr uint32_t L = Row<D>::lanes, SPAN = 512;
-    __shared__ float2 cs[256];  // tokens * D / 2 <= 256
+    __shared__ __align__(16) float2 cs[256];  // tokens * D / 2 <= 256
     __shared__ __align__(16) uint8_t stage[kThreads / 32][SPAN / 32 * 34];
     const uint32_t t0 = blockIdx.x * tokens, nt = min(tokens, a.n_tok - t0);
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const uint32_t E = a.pages.n_head_kv * D, spans = (E + SPAN - 1) / SPAN;
+    const uint32_t E = a.pages.n_head_kv * D, spans = (E + SPAN - 1) / SPAN, n_items = 2 * nt * spans;
+    const uint32_t g = lane / L, j = lane % L;
+    uint4 u = make_uint4(0, 0, 0, 0), v = u;
+    int32_t cell = -1;
+    auto load = [&](uint32_t i) {
+        const uint32_t s = i >> 1, dt = spans == 1 ? s : s / spans, e0 = (s - dt * spans) * SPAN;
+        const uint64_t t = t0 + dt;
+        cell = __ldg(a.cells + t);
+        if (e0 + (g + 1) * D <= E) {
+            const uint16_t *p = (i & 1 ? a.v + t * a.v_stride : a.k + t * a.k_stride) + e0 + g * D + 8 * j;
+            u = __ldg(reinterpret_cast<const uint4 *>(p));
+            v = __ldg(reinterpret_cast<const uint4 *>(p + D / 2));
+        }
+    };
+    if (warp < n_items) load(warp);  // on its way while the angles are computed
     if (a.pos) {
         angles<D>(cs, a.pos + t0, nt, a.theta);
         __syncthreads();
     }
-    const uint32_t g = lane / L, j = lane % L;
-    for (uint32_t i = warp; i < 2 * nt * spans; i += kThreads / 32) {
+    for (uint32_t i = warp; i < n_items; i += kThreads / 32) {
+        if (i != warp) load(i);
         const bool is_v = i & 1;
-        const uint32_t dt = (i >> 1) / spans, e0 = ((i >> 1) - dt * spans) * SPAN;
-        const uint64_t t = t0 + dt;
-        const int32_t cell = __ldg(a.cells + t);
+        const uint32_t s = i >> 1, dt = spans == 1 ? s : s / spans, e0 = (s - dt * spans) * SPAN;
         if (cell < 0 || static_cast<uint32_t>(cell) >= a.pages.n_pages * a.pages.page_tokens)
             continue;  // no such cell: nothing is written
         const uint32_t page = static_cast<uint32_t>(cell) / a.pages.page_tokens;
@@ -336,16 +393,15 @@ __global__ void __launch_bounds__(kThreads)
         const uint32_t n = min(SPAN, E - e0);
         float lo[8] = {}, hi[8] = {};
         if (act) {
-            const uint16_t *s = (is_v ? a.v + t * a.v_stride : a.k + t * a.k_stride) + e0 + g * D + 8 * j;
-            unpack_f16(__ldg(reinterpret_cast<const uint4 *>(s)), lo);
-            unpack_f16(__ldg(reinterpret_cast<const uint4 *>(s + D / 2)), hi);
+            unpack_f16(u, lo);
+            unpack_f16(v, hi);
         }
         if (is_v) {
             uint8_t *dst = a.pages.v + page * a.pages.v_page + off * a.pages.v_row +
                            e0 / 32 * Fmt<VT>::block;
             store_span<D, VT>(dst, stage[warp], n, act, lo, hi);
         } else {
-            if (a.pos) rotate(lo, hi, cs + dt * (D / 2) + 8 * j);
+            if (a.pos) rotate<D>(lo, hi, cs + dt * (D / 2), j);
             if (a.fwht_n) hadamard<D>(lo, hi, fwht_scale);
             uint8_t *dst = a.pages.k + page * a.pages.k_page + off * a.pages.k_row +
                            e0 / 32 * Fmt<KT>::block;
@@ -358,17 +414,25 @@ float fwht_scale(uint32_t n) {
     return n ? 1.0f / std::sqrt(static_cast<float>(n)) : 0.0f;
 }
 
+// Many tokens: a CTA takes all heads of a few (enough rows to fill its threads
+// kFly times), so that a token's angles are computed once. Few: a CTA takes one
+// pass of rows of one token, so that there are CTAs for the SMs. (64 + 8 heads
+// of 128, bf16 in, four outputs: 256 tokens 5.1 us split, 7.2 us not; 512 tokens
+// 10.0 and 7.3 us; 2048 tokens 31 and 22 us = 5.1 TB/s.)
 template <int D, typename T>
 cudaError_t launch_qk_t(const QkNormRope &a, cudaStream_t st) {
+    constexpr uint32_t G = kThreads / Row<D>::lanes;
     const uint32_t heads_all = a.n_head + a.n_head_kv;
-    const uint32_t tokens = kThreads / (D / 2), heads = heads_all;
+    const bool many = a.n_tok >= 512;
+    const uint32_t fill = std::max<uint32_t>(256 / D, (kFly * G + heads_all - 1) / heads_all);
+    const uint32_t tokens = many ? std::min<uint32_t>(kThreads / (D / 2), fill) : 1;
+    const uint32_t heads = many ? heads_all : G;
     const dim3 grid((a.n_tok + tokens - 1) / tokens, (heads_all + heads - 1) / heads);
-    const size_t smem = tokens * (D / 2) * sizeof(float2);
     const float s = fwht_scale(a.fwht_n);
     if (a.fwht_n)
-        qk_kernel<D, T, true><<<grid, kThreads, smem, st>>>(a, tokens, heads, s);
+        qk_kernel<D, T, true><<<grid, kThreads, 0, st>>>(a, tokens, heads, s);
     else
-        qk_kernel<D, T, false><<<grid, kThreads, smem, st>>>(a, tokens, heads, s);
+        qk_kernel<D, T, false><<<grid, kThreads, 0, st>>>(a, tokens, heads, s);
     return cudaGetLastError();
 }
 
