@@ -28,7 +28,7 @@
 namespace kvmret {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kAppendThreads = 128;
 
 template <int D>
 struct Row {
@@ -156,7 +156,7 @@ __device__ __forceinline__ void hadamard(float (&lo)[8], float (&hi)[8], float s
 template <int D>
 __device__ __forceinline__ void angles(float2 *cs, const int32_t *pos, uint32_t n,
                                        const Theta &th) {
-    for (uint32_t i = threadIdx.x; i < n * (D / 2); i += kThreads) {
+    for (uint32_t i = threadIdx.x; i < n * (D / 2); i += blockDim.x) {
         const uint32_t t = i / (D / 2), p = i % (D / 2);
         const uint32_t at = (p % 8 / 2 * Row<D>::lanes + p / 8) * 2 + p % 2;
         cs[t * (D / 2) + at] = rope_cs(pos[t], th.v[p]);
@@ -355,11 +355,11 @@ __device__ __forceinline__ void store_span(uint8_t *dst, uint8_t *stage, uint32_
 // CTA = `tokens` tokens; each warp takes spans of 512 elements of their K and
 // V rows. K: rotate, transform, format; V: format.
 template <int D, int KT, int VT>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kAppendThreads)
     append_kernel(const __grid_constant__ PagedAppend a, uint32_t tokens, float fwht_scale) {
     constexpr uint32_t L = Row<D>::lanes, SPAN = 512;
     __shared__ __align__(16) float2 cs[256];  // tokens * D / 2 <= 256
-    __shared__ __align__(16) uint8_t stage[kThreads / 32][SPAN / 32 * 34];
+    __shared__ __align__(16) uint8_t stage[kAppendThreads / 32][SPAN / 32 * 34];
     const uint32_t t0 = blockIdx.x * tokens, nt = min(tokens, a.n_tok - t0);
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint32_t E = a.pages.n_head_kv * D, spans = (E + SPAN - 1) / SPAN, n_items = 2 * nt * spans;
@@ -381,7 +381,7 @@ __global__ void __launch_bounds__(kThreads)
         angles<D>(cs, a.pos + t0, nt, a.theta);
         __syncthreads();
     }
-    for (uint32_t i = warp; i < n_items; i += kThreads / 32) {
+    for (uint32_t i = warp; i < n_items; i += kAppendThreads / 32) {
         if (i != warp) load(i);
         const bool is_v = i & 1;
         const uint32_t s = i >> 1, dt = spans == 1 ? s : s / spans, e0 = (s - dt * spans) * SPAN;
@@ -443,10 +443,14 @@ cudaError_t launch_qk_d(const QkNormRope &a, cudaStream_t st) {
     return launch_qk_t<D, uint16_t>(a, st);
 }
 
+// Four warps with a token's spans: 8 tokens of 1024 + 1024 elements take 2.0 us
+// (q8_0 + q4_0: 2.9), 2048 tokens 4.9 us (8.0); with four tokens to eight warps
+// 3.2 (4.9) and 5.2 us (8.6).
 template <int D, int KT, int VT>
 cudaError_t launch_append_t(const PagedAppend &a, cudaStream_t st) {
-    const uint32_t tokens = 256 / (D / 2);
-    append_kernel<D, KT, VT><<<(a.n_tok + tokens - 1) / tokens, kThreads, 0, st>>>(
+    const uint32_t spans = (a.pages.n_head_kv * D + 511) / 512;
+    const uint32_t tokens = std::min<uint32_t>(256 / (D / 2), std::max<uint32_t>(1, kAppendThreads / 64 / spans));
+    append_kernel<D, KT, VT><<<(a.n_tok + tokens - 1) / tokens, kAppendThreads, 0, st>>>(
         a, tokens, fwht_scale(a.fwht_n));
     return cudaGetLastError();
 }
