@@ -50,25 +50,35 @@ namespace {
 // QUANT: some K or V rows are q8_0 or q4_0 blocks.
 template <int D, bool QUANT>
 struct Cfg {
-    static constexpr int NS = D == 256 ? 1 : 2;     // streams
+    static constexpr int NS = D == 256 || QUANT ? 1 : 2;  // streams
+    static constexpr int NB = 3 - NS;               // S tiles of a stream
     static constexpr int BN = D == 256 ? 64 : 128;  // keys of a tile
     static constexpr int PR = 128 * NS;             // rows of a unit
-    static constexpr int threads = 128 + 128 * NS + (QUANT ? 128 : 0);
+    static constexpr int threads = 128 + 128 * NS + (QUANT ? 256 : 0);
     static constexpr uint32_t stage = BN * D * 2;   // one K or V tile
-    static constexpr int stages = QUANT ? (D == 64 ? 6 : 3) : D == 64 ? 8 : 5;
+    static constexpr int stages = QUANT ? (D == 64 ? 8 : D == 128 ? 4 : 3) : D == 64 ? 8 : 5;
     static constexpr uint32_t q_bytes = 128 * D * 2;
-    // tiles of quant blocks as they lie in memory, on their way
-    static constexpr int raws = QUANT ? (D == 64 ? 6 : 3) : 0;
-    static constexpr uint32_t raw = BN * (D == 64 ? 80 : D == 128 ? 144 : 272);
+    // tiles of quant blocks as they lie in memory, on their way: two of K, one or
+    // two of V as their formats leave room (AttnLaunch)
+    static constexpr int raws = QUANT ? 2 : 0;
     static constexpr uint32_t raw0 = NS * q_bytes + stages * stage;
-    static constexpr uint32_t tiles = raw0 + raws * raw;
+    static constexpr uint32_t raw_bytes = QUANT ? 3 * BN * (D == 64 ? 80 : D == 128 ? 144 : 272) + 2048 : 0;
+    static constexpr uint32_t tiles = raw0 + raw_bytes;
     static __host__ __device__ constexpr uint32_t s_col(int s) { return s * 128; }
     static __host__ __device__ constexpr uint32_t o_col(int s) { return 256 + s * (D == 64 ? 64 : 128); }
-    // Ring positions of the K and V tiles of tile t. With conversions K goes a
-    // tile ahead (K0 K1 V0 K2 V1 ..), so that three stages are enough for scores
-    // not to wait for a stage that a V still holds.
-    static __device__ __forceinline__ uint32_t k_pos(uint32_t t) { return QUANT ? (t ? 2 * t - 1 : 0) : 2 * t; }
-    static __device__ __forceinline__ uint32_t v_pos(uint32_t t) { return QUANT ? 2 * t + 2 : 2 * t + 1; }
+    // The stage of the K or V tile of tile t, and how often it was used before.
+    // TMA fills one ring in the order K0 V0 K1 V1 ..; the converting warps have
+    // a ring each, so that a K does not wait for the P V of another tile.
+    static constexpr int k_stages = D == 64 ? 4 : 2, v_stages = D == 64 ? 4 : D == 128 ? 2 : 1;
+    static_assert(!QUANT || stages == k_stages + v_stages, "stages");
+    static __device__ __forceinline__ uint32_t k_stage(uint32_t t) { return QUANT ? t % k_stages : 2 * t % stages; }
+    static __device__ __forceinline__ uint32_t k_round(uint32_t t) { return QUANT ? t / k_stages : 2 * t / stages; }
+    static __device__ __forceinline__ uint32_t v_stage(uint32_t t) {
+        return QUANT ? k_stages + t % v_stages : (2 * t + 1) % stages;
+    }
+    static __device__ __forceinline__ uint32_t v_round(uint32_t t) {
+        return QUANT ? t / v_stages : (2 * t + 1) / stages;
+    }
 };
 // Bytes of the box that holds a head's row of quant blocks: it starts on a
 // 16-byte boundary at or up to 12 bytes before the row.
@@ -95,6 +105,7 @@ struct AttnLaunch {
     float2 *ml;      // [slot][row tile][128] maximum and sum
     float4 *o;       // [slot][row tile][D / 4][128]
     uint32_t max_slots;
+    uint32_t raw_k, raw_v, n_raw_v;  // bytes of a raw K, V tile; raw V tiles
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -200,34 +211,27 @@ __device__ __forceinline__ bool elect_one() {
     return p;
 }
 
-// One key's COLS columns of quant blocks at shared address `src` (4-byte
-// aligned; 8-byte with 128 columns), eight columns at a time to put(chunk, x).
-// A block's payload starts two bytes after its start: with even blocks (which
-// start on a word) its words straddle two, with odd ones they are whole.
-template <int COLS, int TYPE, typename Put>
-__device__ __forceinline__ void convert_row(uint32_t src, Put put) {
-    constexpr uint32_t BLOCK = TYPE == KVMRET_TYPE_Q8_0 ? 34 : 18, NB = COLS / 32, W = NB * BLOCK / 4;
-    uint32_t w[W];
-    if constexpr (COLS == 128) {
+// One key's NB quant blocks at shared address `src` (4-byte aligned), eight columns
+// at a time to put(chunk, x), beginning with block `first` (which spreads the
+// lanes over the banks). The loop stays one: the code of a tile would not fit
+// the instruction caches beside the softmax's. A block's payload starts two
+// bytes after its start, so its words straddle those of memory: in even blocks
+// (which start on a word) by their upper half, in odd ones (which start between)
+// by none.
+template <int NB, int TYPE, typename Put>
+__device__ __forceinline__ void convert_row(uint32_t src, uint32_t first, Put put) {
+    constexpr uint32_t BLOCK = TYPE == KVMRET_TYPE_Q8_0 ? 34 : 18, NW = (BLOCK - 2) / 4;
+#pragma unroll 1
+    for (uint32_t i = 0; i < NB; ++i) {
+        const uint32_t b = (i + first) % NB, at = src + b * BLOCK / 4 * 4;
+        const uint32_t sel = b & 1 ? 0x7654 : 0x5432;
+        uint32_t w[NW + 1];
 #pragma unroll
-        for (uint32_t i = 0; i < W; i += 2)
-            asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[i]), "=r"(w[i + 1]) : "r"(src + 4 * i));
-    } else {
-#pragma unroll
-        for (uint32_t i = 0; i < W; ++i)
-            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[i]) : "r"(src + 4 * i));
-    }
-#pragma unroll
-    for (uint32_t b = 0; b < NB; ++b) {
-        constexpr uint32_t NW = (BLOCK - 2) / 4;
-        const uint32_t at = b * BLOCK / 4;  // the word of the block's start
-        const bool odd = b & 1;
-        const uint32_t dd = odd ? __byte_perm(w[at], 0, 0x3232) : __byte_perm(w[at], 0, 0x1010);
+        for (uint32_t k = 0; k <= NW; ++k) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[k]) : "r"(at + 4 * k));
+        const uint32_t dd = __byte_perm(w[0], 0, b & 1 ? 0x3232 : 0x1010);
         const __half2 d = *reinterpret_cast<const __half2 *>(&dd);
-        uint32_t p[NW];
 #pragma unroll
-        for (uint32_t i = 0; i < NW; ++i)
-            p[i] = odd ? w[at + 1 + i] : __byte_perm(w[at + i], w[at + i + 1 < W ? at + i + 1 : at + i], 0x5432);
+        for (uint32_t k = 0; k < NW; ++k) w[k] = __byte_perm(w[k], w[k + 1], sel);
         // halves of bytes 2k, 2k + 1 of u, less `bias`, times d
         auto pair = [&](uint32_t u, uint32_t k, uint32_t bias) {
             const uint32_t h = __byte_perm(u, 0x64646464u, k ? 0x4342 : 0x4140);
@@ -235,23 +239,20 @@ __device__ __forceinline__ void convert_row(uint32_t src, Put put) {
                                               *reinterpret_cast<const __half2 *>(&bias)), d);
             return *reinterpret_cast<const uint32_t *>(&x);
         };
-        if constexpr (TYPE == KVMRET_TYPE_Q8_0) {
 #pragma unroll
-            for (uint32_t c = 0; c < 4; ++c) {
-                const uint32_t u0 = p[2 * c] ^ 0x80808080u, u1 = p[2 * c + 1] ^ 0x80808080u;
-                const uint32_t x[4] = {pair(u0, 0, 0x64806480u), pair(u0, 1, 0x64806480u),
-                                       pair(u1, 0, 0x64806480u), pair(u1, 1, 0x64806480u)};
-                put(4 * b + c, x);
+        for (uint32_t c = 0; c < 4; ++c) {
+            uint32_t u0, u1, bias;
+            if constexpr (TYPE == KVMRET_TYPE_Q8_0) {
+                u0 = w[2 * c] ^ 0x80808080u;
+                u1 = w[2 * c + 1] ^ 0x80808080u;
+                bias = 0x64806480u;
+            } else {  // lower halves: columns 0 .. 15, upper: 16 .. 31
+                u0 = (w[2 * (c % 2)] >> (c < 2 ? 0 : 4)) & 0x0f0f0f0fu;
+                u1 = (w[2 * (c % 2) + 1] >> (c < 2 ? 0 : 4)) & 0x0f0f0f0fu;
+                bias = 0x64086408u;
             }
-        } else {
-#pragma unroll
-            for (uint32_t c = 0; c < 4; ++c) {  // lower halves: columns 0 .. 15, upper: 16 .. 31
-                const uint32_t s = c < 2 ? 0 : 4;
-                const uint32_t u0 = (p[2 * (c % 2)] >> s) & 0x0f0f0f0fu, u1 = (p[2 * (c % 2) + 1] >> s) & 0x0f0f0f0fu;
-                const uint32_t x[4] = {pair(u0, 0, 0x64086408u), pair(u0, 1, 0x64086408u),
-                                       pair(u1, 0, 0x64086408u), pair(u1, 1, 0x64086408u)};
-                put(4 * b + c, x);
-            }
+            const uint32_t x[4] = {pair(u0, 0, bias), pair(u0, 1, bias), pair(u1, 0, bias), pair(u1, 1, bias)};
+            put(4 * b + c, x);
         }
     }
 }
@@ -273,9 +274,9 @@ __device__ __forceinline__ void scan(uint32_t &x, uint32_t &y) {
     }
 }
 
-template <int D>
+template <int D, bool QUANT>
 __device__ bool make_plan(const AttnLaunch &l, Plan &p, Start &start) {
-    constexpr int BN = Cfg<D, false>::BN, PR = Cfg<D, false>::PR;
+    constexpr int BN = Cfg<D, QUANT>::BN, PR = Cfg<D, QUANT>::PR;
     const PrefixAttn &a = l.a;
     const uint32_t lane = threadIdx.x & 31;
     const uint32_t G = a.n_head / a.n_head_kv, H = a.n_head_kv;
@@ -379,9 +380,9 @@ __device__ bool make_plan(const AttnLaunch &l, Plan &p, Start &start) {
 
 // Where the pieces of every row lie, for the join: by one warp of each CTA, a
 // lane a row, the CTAs taking blocks of 32 rows in turn.
-template <int D>
+template <int D, bool QUANT>
 __device__ void note_rows(const AttnLaunch &l, const Plan &p) {
-    constexpr int BN = Cfg<D, false>::BN, PR = Cfg<D, false>::PR, NS = Cfg<D, false>::NS;
+    constexpr int BN = Cfg<D, QUANT>::BN, PR = Cfg<D, QUANT>::PR, NS = Cfg<D, QUANT>::NS;
     const PrefixAttn &a = l.a;
     const uint32_t lane = threadIdx.x & 31, n_cta = gridDim.x;
     const uint32_t G = a.n_head / a.n_head_kv, H = a.n_head_kv;
@@ -461,7 +462,7 @@ struct Small {
     static constexpr int NS = C::NS;
     alignas(16) uint32_t mask[kMeta][4];  // valid keys of a tile
     float2 ml[NS][128];                   // statistics on their way to the other stream
-    uint64_t bars[2 * C::stages + kMeta + 2 * kSegs + 6 * NS + 2 + 2 * C::raws + (QUANT ? kMeta : 0)];
+    uint64_t bars[2 * C::stages + kMeta + 2 * kSegs + (4 + 2 * C::NB) * NS + 2 + 4 * C::raws + (QUANT ? kMeta : 0)];
     TileInfo tile[QUANT ? kMeta : 1];
     Plan plan;
     Seg seg[kSegs];
@@ -475,7 +476,7 @@ template <int D, bool QUANT>
 __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
     attn_tc_kernel(const __grid_constant__ AttnLaunch l) {
     using C = Cfg<D, QUANT>;
-    constexpr int BN = C::BN, PR = C::PR, NS = C::NS, ST = C::stages, RS = C::raws;
+    constexpr int BN = C::BN, PR = C::PR, NS = C::NS, NB = C::NB, ST = C::stages, RS = C::raws;
     constexpr uint32_t KB = BN * 128, QB = 128 * 128;  // bytes of a 64-column block of K / V, of Q
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     Small<D, QUANT> &sm = *reinterpret_cast<Small<D, QUANT> *>(smem_raw + C::tiles);
@@ -497,15 +498,22 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
     auto seg_empty = [&](uint32_t i) { return bar0 + 8u * (2 * ST + kMeta + kSegs + i); };
     constexpr uint32_t SB = 2 * ST + kMeta + 2 * kSegs;
     auto q_ready = [&](uint32_t s) { return bar0 + 8u * (SB + s); };
-    auto s_full = [&](uint32_t s) { return bar0 + 8u * (SB + NS + s); };
-    auto p_ready = [&](uint32_t s) { return bar0 + 8u * (SB + 2 * NS + s); };
-    auto pv_done = [&](uint32_t s) { return bar0 + 8u * (SB + 3 * NS + s); };
-    auto o_done = [&](uint32_t s) { return bar0 + 8u * (SB + 4 * NS + s); };
-    auto o_read = [&](uint32_t s) { return bar0 + 8u * (SB + 5 * NS + s); };
-    const uint32_t drain = bar0 + 8u * (SB + 6 * NS), planned = drain + 8;
-    auto raw_full = [&](uint32_t i) { return drain + 16 + 8u * i; };
-    auto raw_empty = [&](uint32_t i) { return drain + 16 + 8u * (RS + i); };
-    auto meta_empty = [&](uint32_t i) { return drain + 16 + 8u * (2 * RS + i); };
+    // one for each S tile of a stream
+    auto s_full = [&](uint32_t s, uint32_t b) { return bar0 + 8u * (SB + NS + NB * s + b); };
+    auto p_ready = [&](uint32_t s, uint32_t b) { return bar0 + 8u * (SB + (1 + NB) * NS + NB * s + b); };
+    constexpr uint32_t SP = SB + (1 + 2 * NB) * NS;
+    auto pv_done = [&](uint32_t s) { return bar0 + 8u * (SP + s); };
+    auto o_done = [&](uint32_t s) { return bar0 + 8u * (SP + NS + s); };
+    auto o_read = [&](uint32_t s) { return bar0 + 8u * (SP + 2 * NS + s); };
+    const uint32_t drain = bar0 + 8u * (SP + 3 * NS), planned = drain + 8;
+    // raw tiles i of K (v = 0), V
+    auto raw_full = [&](uint32_t v, uint32_t i) { return drain + 16 + 8u * (v * RS + i); };
+    auto raw_empty = [&](uint32_t v, uint32_t i) { return drain + 16 + 8u * (2 * RS + v * RS + i); };
+    auto meta_empty = [&](uint32_t i) { return drain + 16 + 8u * (4 * RS + i); };
+    auto raw_tile = [&](uint32_t v, uint32_t i) {
+        return base + C::raw0 + (v ? 2 * l.raw_k + i * l.raw_v : i * l.raw_k);
+    };
+    auto raw_count = [&](uint32_t v) { return v ? l.n_raw_v : 2u; };
 
     if (threadIdx.x == 0) {
         sm.fail = 0;
@@ -520,18 +528,21 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
         }
         for (int s = 0; s < NS; ++s) {
             mbar_init(q_ready(s), 4);
-            mbar_init(s_full(s), 1);
-            mbar_init(p_ready(s), 4);
+            for (int b = 0; b < NB; ++b) {
+                mbar_init(s_full(s, b), 1);
+                mbar_init(p_ready(s, b), 4);
+            }
             mbar_init(pv_done(s), 1);
             mbar_init(o_done(s), 4);
             mbar_init(o_read(s), 4);
         }
         mbar_init(drain, 1);
         mbar_init(planned, 1);
-        for (int i = 0; i < RS; ++i) {
-            mbar_init(raw_full(i), 1);
-            mbar_init(raw_empty(i), 4);
-        }
+        for (int i = 0; i < RS; ++i)
+            for (int v = 0; v < 2; ++v) {
+                mbar_init(raw_full(v, i), 1);
+                mbar_init(raw_empty(v, i), 4);
+            }
         if constexpr (QUANT)
             for (int i = 0; i < kMeta; ++i) mbar_init(meta_empty(i), 4);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -558,7 +569,7 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
     if (warp == 2) {  // ---- the pieces ----
         Start start;
         Plan p;
-        if (!make_plan<D>(l, p, start)) stop = true;
+        if (!make_plan<D, QUANT>(l, p, start)) stop = true;
         if (lane == 0) {
             plan = p;
             mbar_arrive(planned);
@@ -581,29 +592,30 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
             if (g.n == 0) break;
         }
     } else if (warp == 3) {  // ---- the join's notes ----
-        if (wait(planned, 0) && plan.ok) note_rows<D>(l, plan);
+        if (wait(planned, 0) && plan.ok) note_rows<D, QUANT>(l, plan);
     } else if (warp == 0) {  // ---- producer ----
         if (lane < 4 && (lane < 2 ? a.prefix.max_len != 0 : a.n_seq != 0))
             asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&l.map[lane]))
                          : "memory");
-        uint32_t q = 0, j = 0;  // stages (quant: raw tiles) and tiles so far
+        uint32_t q = 0, j = 0;  // stages and tiles so far
+        uint32_t nr[2] = {0, 0};  // raw tiles of K, V
         // The raw tile of a K (v = 0) or V operand that is in quant blocks.
         auto load_raw = [&](uint32_t kind, uint32_t v, uint32_t h, uint32_t off, int32_t id, bool use) {
             const PageView &pv = (kind ? a.tail : a.prefix).pages;
             const int32_t type = v ? pv.v_type : pv.k_type;
             if (type == KVMRET_TYPE_F16) return;  // the converting warps fetch it
-            const uint32_t slot = q % (RS ? RS : 1), round = q / (RS ? RS : 1);
-            if (round && !wait(raw_empty(slot), (round - 1) & 1u)) return;
-            ++q;
+            const uint32_t n = raw_count(v), slot = nr[v] % n, round = nr[v] / n;
+            if (round && !wait(raw_empty(v, slot), (round - 1) & 1u)) return;
+            ++nr[v];
             const uint32_t T = pv.page_tokens, bx = raw_box<D>(type);
             const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, use)) * min(T, static_cast<uint32_t>(BN)) * bx;
-            if (lane == 0) mbar_expect_tx(raw_full(slot), bytes);
+            if (lane == 0) mbar_expect_tx(raw_full(v, slot), bytes);
             __syncwarp();
             const uint32_t row = D / 32 * (type == KVMRET_TYPE_Q8_0 ? 34 : 18);
             if (use)
-                tma_load_3d(base + C::raw0 + slot * C::raw + lane * T * bx, &l.map[2 * kind + v],
+                tma_load_3d(raw_tile(v, slot) + lane * T * bx, &l.map[2 * kind + v],
                             static_cast<int32_t>(h * row / 16 * 8), static_cast<int32_t>(off), id,
-                            raw_full(slot));
+                            raw_full(v, slot));
         };
         uint32_t k_kind = 2, k_h = 0, k_off = 0;  // the tile before
         int32_t k_id = -1;
@@ -699,9 +711,10 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
         }
         if (stop) {  // gave up: drain the loads already issued (bounded)
             if (lane == 0) atomicExch(&sm.fail, 1u);
-            constexpr uint32_t N = QUANT ? (RS ? RS : 1) : ST;
-            for (uint32_t i = q > N ? q - N : 0; i < q; ++i)
-                mbar_wait_clk(QUANT ? raw_full(i % N) : full(i % N), (i / N) & 1u);
+            for (uint32_t i = q > ST ? q - ST : 0; i < q; ++i) mbar_wait_clk(full(i % ST), (i / ST) & 1u);
+            for (uint32_t v = 0; QUANT && v < 2; ++v)
+                for (uint32_t n = raw_count(v), i = nr[v] > n ? nr[v] - n : 0; i < nr[v]; ++i)
+                    mbar_wait_clk(raw_full(v, i % n), (i / n) & 1u);
         }
     } else if (warp == 1) {  // ---- products ----
         // Tiles are taken in the CTA's order: the stream whose current tile is
@@ -734,30 +747,31 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
             }
             fresh[s] = true;
         };
-        uint32_t nq[2] = {0, 0};
+        uint32_t nq[2] = {0, 0}, cur[2] = {0, 0};
         // a stage is free once each stream has passed it: a tile of one stream
         // alone counts for both
         auto release = [&](uint32_t s, uint32_t st) {
             mma_commit(empty(st));
             if (NS == 2 && !sh[s].both) mma_commit(empty(st));
         };
-        // scores of the stream's current tile; `after`: once the product before,
-        // which reads the P that S will overwrite, has completed (the last wait, so
-        // that the issue follows it at once)
-        auto scores = [&](uint32_t s, bool after) {
+        // Scores of the stream's current tile, its n-th, into S tile n % NB. With one
+        // S tile, `after`: once the product before, which reads the P that S will
+        // overwrite, has completed (the last wait, so that the issue follows it).
+        auto scores = [&](uint32_t s, uint32_t n, bool after) {
             if (fresh[s] && !wait(q_ready(s), nq[s]++ & 1u)) return;
-            const uint32_t k = C::k_pos(sh[s].tile), st = __shfl_sync(0xffffffffu, k % ST, 0);
-            if (!wait(full(st), (k / ST) & 1u)) return;
-            if (after && !wait(pv_done(s), tiles[s] & 1u)) return;
+            const uint32_t st = __shfl_sync(0xffffffffu, C::k_stage(sh[s].tile), 0);
+            if (!wait(full(st), C::k_round(sh[s].tile) & 1u)) return;
+            if (after && !wait(pv_done(s), (n - 1) & 1u)) return;
             tc_fence_after();
             if (elect_one()) {
                 const uint32_t la = ((ubase + s * C::q_bytes) >> 4) | (1u << 16);
                 const uint32_t lb = ((ubase + NS * C::q_bytes + st * C::stage) >> 4) | (1u << 16);
+                const uint32_t to = tmem + C::s_col(s) + n % NB * BN;
 #pragma unroll
                 for (uint32_t c = 0; c < D / 16; ++c)  // 16 columns: 32 bytes of a block
-                    mma_ss(tmem + C::s_col(s), desc(la + (c / 4) * (QB / 16) + 2 * (c % 4)),
+                    mma_ss(to, desc(la + (c / 4) * (QB / 16) + 2 * (c % 4)),
                            desc(lb + (c / 4) * (KB / 16) + 2 * (c % 4)), id_s, c != 0);
-                mma_commit(s_full(s));
+                mma_commit(s_full(s, n % NB));
                 release(s, st);
             }
             __syncwarp();
@@ -765,34 +779,49 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
 #pragma unroll
         for (uint32_t s = 0; s < NS; ++s) {
             if (!stop) open(s);
-            if (!stop && live[s]) scores(s, false);
+            if (!stop && live[s]) scores(s, 0, false);
+            cur[s] = sh[s].tile;
         }
         auto turn = [&](uint32_t s) {
-            const uint32_t v = C::v_pos(sh[s].tile), st = __shfl_sync(0xffffffffu, v % ST, 0);
-            if (!wait(full(st), (v / ST) & 1u) || !wait(p_ready(s), tiles[s] & 1u)) return;
+            const uint32_t n = tiles[s]++, st = __shfl_sync(0xffffffffu, C::v_stage(cur[s]), 0);
+            const uint32_t add = !fresh[s];
+            const bool both = sh[s].both;
+            fresh[s] = false;
+            sh[s].tile += sh[s].step;
+            const bool same = sh[s].any();
+            // with two S tiles the next scores come first, if their K is there (a new
+            // piece's Q comes only after this tile's P)
+            bool ahead = false;
+            if (NB == 2) {
+                if (n && !wait(pv_done(s), (n - 1) & 1u)) return;
+                if (same) {
+                    const uint32_t t = sh[s].tile;
+                    ahead = __all_sync(0xffffffffu, mbar_try(full(C::k_stage(t)), C::k_round(t) & 1u));
+                    if (ahead) scores(s, n + 1, false);
+                }
+            }
+            if (stop || !wait(full(st), C::v_round(cur[s]) & 1u) || !wait(p_ready(s, n % NB), (n / NB) & 1u))
+                return;
             tc_fence_after();
             if (elect_one()) {
                 const uint32_t lb = ((ubase + NS * C::q_bytes + st * C::stage) >> 4) | (KB / 16) << 16;
-                const uint32_t add = !fresh[s];
+                const uint32_t p = tmem + C::s_col(s) + n % NB * BN;
 #pragma unroll
                 for (uint32_t c = 0; c < BN / 16; ++c)  // 16 keys: 8 columns of P, 2 KiB of V
-                    mma_ts(tmem + C::o_col(s), tmem + C::s_col(s) + 8 * c, desc(lb + 128 * c), id_o,
-                           c ? 1u : add);
-                release(s, st);
+                    mma_ts(tmem + C::o_col(s), p + 8 * c, desc(lb + 128 * c), id_o, c ? 1u : add);
+                mma_commit(empty(st));
+                if (NS == 2 && !both) mma_commit(empty(st));
                 mma_commit(pv_done(s));
             }
             __syncwarp();
-            fresh[s] = false;
-            sh[s].tile += sh[s].step;
-            if (!sh[s].any()) open(s);
-            if (!stop && live[s]) scores(s, true);
-            ++tiles[s];
+            if (!same) open(s);
+            if (!stop && live[s] && !ahead) scores(s, n + 1, NB == 1);
+            cur[s] = sh[s].tile;
         };
         uint32_t last = 1;
         while (!stop && (live[0] || (NS == 2 && live[1]))) {
             const bool one = NS == 2 && live[1] &&
-                             (!live[0] || sh[1].tile < sh[0].tile ||
-                              (sh[1].tile == sh[0].tile && last == 0));
+                             (!live[0] || cur[1] < cur[0] || (cur[1] == cur[0] && last == 0));
             last = one;
             if (NS == 2 && one)
                 turn(1);
@@ -810,21 +839,22 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
             mbar_wait(drain, 0);
         }
     } else if (QUANT && warp >= 4 + 4 * NS) {  // ---- conversion of quant blocks ----
-        // A thread a key's row (head size 256: half of it): blocks from the raw
-        // tile to f16(d * q) in the stage's swizzled layout. Whole numbers become
-        // halves by their bits (0x6400 + u is 1024 + u), one subtraction and one
-        // product by d, rounded once. Operands in f16 go to their stage by TMA,
-        // issued by the first of these warps with all four arrivals.
-        const uint32_t tid = threadIdx.x & 127, wq = warp - 4 - 4 * NS;
+        // The first four of these warps have K, the others V. A thread a key's row
+        // (head size 256: half of it): blocks from the raw tile to f16(d * q) in the
+        // stage's swizzled layout. Whole numbers become halves by their bits
+        // (0x6400 + u is 1024 + u), one subtraction and one product by d, rounded
+        // once. Operands in f16 go to their stage by TMA, issued by the first warp
+        // with all four arrivals.
+        const uint32_t tid = threadIdx.x & 127, wq = (warp - 4 - 4 * NS) & 3, v = (warp - 4 - 4 * NS) >> 2;
         const uint32_t key = tid % BN, half = tid / BN;  // half: 0 unless the head size is 256
         uint32_t nr = 0;                                 // raw tiles so far
-        uint32_t flight = 0;                             // stages with an f16 load under way
-        auto unit = [&](uint32_t j, uint32_t v) {
+        uint32_t flight = 0;                             // the tile after the last f16 load
+        auto unit = [&](uint32_t j) {
             const TileInfo &ti = sm.tile[j % kMeta];
             const PageView &pv = (ti.kind ? a.tail : a.prefix).pages;
             const int32_t type = v ? pv.v_type : pv.k_type;
-            const uint32_t pos = v ? C::v_pos(j) : C::k_pos(j), st = pos % ST;
-            if (pos >= ST && !wait(empty(st), (pos / ST - 1) & 1u)) return;
+            const uint32_t st = v ? C::v_stage(j) : C::k_stage(j), round = v ? C::v_round(j) : C::k_round(j);
+            if (round && !wait(empty(st), (round - 1) & 1u)) return;
             const uint32_t stage = ring + st * C::stage;
             if (type == KVMRET_TYPE_F16) {
                 if (wq != 0) return;
@@ -842,17 +872,17 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
                         tma_load_4d(stage + b * KB + lane * T * 128, &l.map[2 * ti.kind + v],
                                     static_cast<int32_t>(64 * b), static_cast<int32_t>(ti.h),
                                     static_cast<int32_t>(ti.off), id, full(st));
-                flight = pos + 1;
+                flight = j + 1;
                 return;
             }
-            const uint32_t slot = nr % (RS ? RS : 1);
-            if (!wait(raw_full(slot), (nr / (RS ? RS : 1)) & 1u)) return;
+            const uint32_t n_raw = raw_count(v), slot = nr % n_raw;
+            if (!wait(raw_full(v, slot), (nr / n_raw) & 1u)) return;
             ++nr;
             const bool q8 = type == KVMRET_TYPE_Q8_0;
             const uint32_t block = q8 ? 34 : 18, row = D / 32 * block;
-            const uint32_t src = base + C::raw0 + slot * C::raw + key * raw_box<D>(type) +
+            const uint32_t src = raw_tile(v, slot) + key * raw_box<D>(type) +
                                  (ti.h * row) % 16 + half * 4 * block;
-            constexpr uint32_t COLS = D < 128 ? D : 128;
+            constexpr uint32_t blocks = D < 128 ? D / 32 : 4;
             const uint32_t dst = stage + key * 128;
             auto put = [&](uint32_t chunk, const uint32_t(&x)[4]) {  // 8 columns
                 const uint32_t ch = half * 16 + chunk;
@@ -862,31 +892,30 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
                              : "memory");
             };
             if (q8)
-                convert_row<COLS, KVMRET_TYPE_Q8_0>(src, put);
+                convert_row<blocks, KVMRET_TYPE_Q8_0>(src, key / 8, put);
             else
-                convert_row<COLS, KVMRET_TYPE_Q4_0>(src, put);
+                convert_row<blocks, KVMRET_TYPE_Q4_0>(src, key / 8, put);
             fence_async_smem();
             __syncwarp();
             if (lane == 0) {
                 mbar_arrive(full(st));
-                mbar_arrive(raw_empty(slot));
+                mbar_arrive(raw_empty(v, slot));
             }
         };
         for (uint32_t j = 0;; ++j) {
-            if (!wait(meta(j % kMeta), (j / kMeta) & 1u)) break;
-            const bool end = sm.tile[j % kMeta].kind == 2;
-            if (!end) unit(j, 0);
-            if (!stop && j) unit(j - 1, 1);
-            if (stop || end) break;
+            if (!wait(meta(j % kMeta), (j / kMeta) & 1u) || sm.tile[j % kMeta].kind == 2) break;
+            unit(j);
+            if (stop) break;
             // K of tile j in its stage: P V of tile j - 8 is past, its mask read
-            if (j >= 8 && lane == 0) mbar_arrive(meta_empty((j - 8) % kMeta));
+            if (v == 0 && j >= 8 && lane == 0) mbar_arrive(meta_empty((j - 8) % kMeta));
             __syncwarp();
         }
         if (stop) {
             if (lane == 0) atomicExch(&sm.fail, 1u);
-            if (wq == 0 && flight)  // the f16 loads under way
-                for (uint32_t i = flight > ST ? flight - ST : 0; i < flight; ++i)
-                    mbar_wait_clk(full(i % ST), (i / ST) & 1u);
+            if (wq == 0)  // the f16 loads under way
+                for (uint32_t t = flight > 4 ? flight - 4 : 0; t < flight; ++t)
+                    mbar_wait_clk(full(v ? C::v_stage(t) : C::k_stage(t)),
+                                  (v ? C::v_round(t) : C::k_round(t)) & 1u);
         }
     } else if (warp >= 4) {  // ---- softmax, a thread a row ----
         const uint32_t s = (warp - 4) >> 2, qd = warp & 3, r = 32 * qd + lane;
@@ -895,7 +924,7 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
         // (above zero, so that -inf stays -inf; a scale of zero gives equal scores all the same)
         const float c = fmaxf(fabsf(a.scale) * 1.44269504f, 1e-37f);
         const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;  // a negative scale turns Q
-        const uint32_t ts = tmem + ((32 * qd) << 16) + C::s_col(s);
+        const uint32_t ts0 = tmem + ((32 * qd) << 16) + C::s_col(s);
         const uint32_t to = tmem + ((32 * qd) << 16) + C::o_col(s);
         constexpr uint32_t kRows = 128 / (D / 8);  // rows that one pass of the Q load covers
         const uint32_t step_t = kRows / G, step_h = kRows - step_t * G;
@@ -979,24 +1008,29 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
             const uint32_t tile0 = g.tile0 - g.j0;
             float m = -INFINITY, sum = 0.0f;  // of c q . k
             for (bool begin = true; sh.any(); sh.tile += sh.step, begin = false) {
-                const uint32_t jj = sh.tile;
-                if (!wait(s_full(s), ns++ & 1u) || !wait(meta(jj % kMeta), (jj / kMeta) & 1u)) break;
+                const uint32_t jj = sh.tile, n = ns++, ts = ts0 + n % NB * BN;  // its n-th tile
+                if (!wait(s_full(s, n % NB), (n / NB) & 1u) || !wait(meta(jj % kMeta), (jj / kMeta) & 1u))
+                    break;
                 tc_fence_after();
                 const uint4 mw = *reinterpret_cast<const uint4 *>(sm.mask[jj % kMeta]);
                 const bool whole = (mw.x & mw.y & (BN == 128 ? mw.z & mw.w : 0xffffffffu)) == 0xffffffffu;
                 // a tile's first token is at most tile * BN: all of it seen?
                 const bool clear = whole && __all_sync(0xffffffffu, (tile0 + jj + 1) * BN <= seen);
+                // With two S tiles these scores did not wait for the product before: its
+                // end, without which O may still change and the phases of pv_done and of
+                // the V stage may be one further back than their parities tell.
+                auto past = [&] { return NB == 1 || n == 0 || wait(pv_done(s), (n - 1) & 1u); };
                 uint32_t x[32];
                 if (!clear) {
                     // the S columns of keys that do not count become -inf, the V rows of
                     // cells without a token zeros
                     if (!whole) {
-                        const uint32_t k = C::v_pos(jj);
-                        if (!wait(full(k % ST), (k / ST) & 1u)) break;
+                        const uint32_t st = C::v_stage(jj);
+                        if (!past() || !wait(full(st), C::v_round(jj) & 1u)) break;
                         for (uint32_t i = tid; i < BN * 8; i += 128) {  // a lane 16 bytes
                             const uint32_t key = i / 8;
                             if (sm.mask[jj % kMeta][key / 32] >> (key % 32) & 1u) continue;
-                            const uint32_t at = ring + (k % ST) * C::stage + i * 16;
+                            const uint32_t at = ring + st * C::stage + i * 16;
 #pragma unroll
                             for (uint32_t z = 0; z < D / 64; ++z)
                                 asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at + z * KB),
@@ -1073,7 +1107,8 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
                         m = mn;
                         sum *= f;
                         if (begin) continue;
-                        // O stands still: its last product came before these scores
+                        if (!past()) break;
+                        tc_fence_after();
 #pragma unroll 1
                         for (uint32_t col = 0; col < D; col += 16) {
                             uint32_t o[16];
@@ -1083,6 +1118,7 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
                             tmem_st16(to + col, o);
                         }
                     }
+                    if (stop) break;
                     sum += s0 + s1;
                     // P over the first columns of S
 #pragma unroll
@@ -1096,9 +1132,11 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
                     if (!wait(o_read(1 - s), (joins - 1) & 1u)) break;
                     owed = false;
                 }
+                // (at the piece's last tile, whose product is waited for below)
+                if (sh.tile + sh.step >= sh.end && !past()) break;
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(p_ready(s));
+                if (lane == 0) mbar_arrive(p_ready(s, n % NB));
             }
             if (stop) break;
             // the last scores are in: Q may be replaced while the last product runs
@@ -1319,19 +1357,25 @@ uint64_t up256(uint64_t v) { return (v + 255) / 256 * 256; }
 
 // The workspace: one word per CTA, the rows' notes, the pieces.
 struct WsLayout {
-    uint64_t at, ml, o, bytes, slots;
+    uint64_t at, ml, o, bytes, slots[2];  // [1]: of 256 rows
     WsLayout(uint32_t n_q, uint32_t n_head, uint32_t n_head_kv, uint32_t d, uint32_t n_seq) {
-        const uint64_t pr = d == 256 ? 128 : 256, ns = pr / 128;
-        const uint64_t rows = static_cast<uint64_t>(n_q) * (n_head / n_head_kv);
-        const uint64_t pairs = (rows + pr - 1) / pr, pg = (pairs + 7) / 8;
-        // prefix: n_pg * gs <= pairs + n_pg units a KV head, and a range each;
-        // tails: a pair per sequence more than whole pairs of the rows
-        slots = (pairs + pg) * n_head_kv + 2 * kMaxCtas +
-                (n_seq ? (n_seq + rows / pr) * n_head_kv : 0);
+        // units of 128 rows or (f16 pages, heads of 64 and 128) 256, whichever takes
+        // more; a slot has a part for each 128
+        uint64_t parts = 0;
+        for (uint64_t pr = 128; pr <= (d == 256 ? 128u : 256u); pr *= 2) {
+            const uint64_t rows = static_cast<uint64_t>(n_q) * (n_head / n_head_kv);
+            const uint64_t pairs = (rows + pr - 1) / pr, pg = (pairs + 7) / 8;
+            // prefix: n_pg * gs <= pairs + n_pg units a KV head, and a range each;
+            // tails: a pair per sequence more than whole pairs of the rows
+            const uint64_t n = (pairs + pg) * n_head_kv + 2 * kMaxCtas +
+                               (n_seq ? (n_seq + rows / pr) * n_head_kv : 0);
+            slots[pr / 256] = n;
+            parts = std::max(parts, n * pr / 128);
+        }
         at = up256(kMaxCtas * 4);
         ml = at + up256(2ull * n_q * n_head * sizeof(RowPieces));
-        o = ml + up256(slots * ns * 128 * 8);
-        bytes = o + slots * ns * 128 * d * 4;
+        o = ml + up256(parts * 128 * 8);
+        bytes = o + parts * 128 * d * 4;
     }
 };
 
@@ -1351,7 +1395,7 @@ cudaError_t launch_main(const AttnLaunch &l, uint32_t n_cta, DeviceFacts *f, cud
 }
 
 template <int D>
-cudaError_t launch_t(AttnLaunch &l, cudaStream_t st) {
+cudaError_t launch_t(AttnLaunch &l, const WsLayout &w, cudaStream_t st) {
     DeviceFacts *f = device_facts();
     const uint32_t n_cta = attn_ctas(f);
     const KeyList *lists[2] = {&l.a.prefix, &l.a.tail};
@@ -1365,6 +1409,17 @@ cudaError_t launch_t(AttnLaunch &l, cudaStream_t st) {
         if (e == cudaSuccess)
             e = encode_pages<D>(&l.map[2 * i + 1], v.v, v.v_row, v.v_page, v.v_type, v);
         if (e != cudaSuccess) return e;
+    }
+    l.max_slots = static_cast<uint32_t>(w.slots[quant || D == 256 ? 0 : 1]);
+    if (quant) {
+        int32_t worst[2] = {KVMRET_TYPE_Q4_0, KVMRET_TYPE_Q4_0};
+        for (const KeyList *kl : lists)
+            for (int v = 0; v < 2; ++v)
+                if (kl->max_len && (v ? kl->pages.v_type : kl->pages.k_type) == KVMRET_TYPE_Q8_0)
+                    worst[v] = KVMRET_TYPE_Q8_0;
+        l.raw_k = Cfg<D, true>::BN * raw_box<D>(worst[0]);
+        l.raw_v = Cfg<D, true>::BN * raw_box<D>(worst[1]);
+        l.n_raw_v = std::min<uint32_t>(2, (Cfg<D, true>::raw_bytes - 2 * l.raw_k) / l.raw_v);
     }
     e = quant ? launch_main<D, true>(l, n_cta, f, st) : launch_main<D, false>(l, n_cta, f, st);
     if (e != cudaSuccess) return e;
@@ -1397,10 +1452,9 @@ cudaError_t launch_prefix_attn(const PrefixAttn &a, void *ws, cudaStream_t st) {
     l.at = reinterpret_cast<RowPieces *>(b + w.at);
     l.ml = reinterpret_cast<float2 *>(b + w.ml);
     l.o = reinterpret_cast<float4 *>(b + w.o);
-    l.max_slots = static_cast<uint32_t>(w.slots);
-    if (a.d_head == 64) return launch_t<64>(l, st);
-    if (a.d_head == 128) return launch_t<128>(l, st);
-    return launch_t<256>(l, st);
+    if (a.d_head == 64) return launch_t<64>(l, w, st);
+    if (a.d_head == 128) return launch_t<128>(l, w, st);
+    return launch_t<256>(l, w, st);
 }
 
 }  // namespace kvmret

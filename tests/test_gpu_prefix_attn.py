@@ -459,3 +459,52 @@ def test_on_a_stream_given_by_its_handle():
     torch.cuda.synchronize()
     b = kvmret.qk_norm_rope(args[0], args[0][:, :2], pos)
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("d,hkv,g,page,kt,vt,rows", [
+    (128, 8, 8, 128, F16, F16, 1), (128, 8, 8, 128, F16, F16, 40), (64, 8, 8, 64, F16, F16, 3),
+    (256, 4, 8, 128, F16, F16, 9), (128, 8, 8, 128, Q8, Q4, 1), (128, 4, 8, 32, Q8, Q8, 33),
+    (64, 8, 8, 128, Q4, Q8, 2), (256, 8, 4, 64, Q8, Q4, 2), (256, 8, 1, 128, Q8, Q8, 5),
+    (128, 8, 4, 128, Q8, F16, 3), (64, 8, 8, 64, F16, Q4, 3), (256, 8, 4, 128, F16, Q8, 40),
+])
+def test_long_prefixes(d, hkv, g, page, kt, vt, rows):
+    """Many tiles to a CTA, so that every ring goes round often: 20,000 shared
+    tokens, `rows` new tokens of each of three sequences with tails of 1700,
+    `rows` and 300 + rows."""
+    n_pre, tl = 20000, [1700, rows, 300 + rows]
+    rng = np.random.default_rng(d + rows)
+    pool = Pool(rng, -(-n_pre // page), page, hkv, d, kt, vt)
+    width = -(-max(tl) // page)
+    tpool = Pool(rng, 3 * width, page, hkv, d, kt, vt)
+    table = rng.permutation(-(-n_pre // page)).astype(np.int32)
+    own = rng.permutation(3 * width).reshape(3, width).astype(np.int32)
+    pre = pool.fill(table, n_pre)
+    tails = [tpool.fill(own[s], t) for s, t in enumerate(tl)]
+    q = (rng.standard_normal((3 * rows, hkv * g, d)) * 1.5).astype(np.float16)
+    start = np.arange(4, dtype=np.int32) * rows
+    got, lse = kvmret.prefix_attn(dev(q), pool.device(), dev(np.array([n_pre], np.int32)), tpool.device(),
+                                  dev(own), dev(np.array(tl, np.int32)), dev(start),
+                                  prefix_table=dev(table), lse=True)
+    qd, scale = dev(q).double(), d ** -0.5
+    for s in range(3):
+        k, v = (torch.cat([dev(pre[i]), dev(tails[s][i])]) for i in (0, 1))  # [keys][hkv][d]
+        total = k.shape[0]
+        seen = total - rows + 1 + torch.arange(rows, device="cuda")
+        hide = torch.arange(total, device="cuda") >= seen[:, None]
+        for h in range(hkv):
+            x = qd[s * rows:(s + 1) * rows, h * g:(h + 1) * g]  # [rows][g][d]
+            w = (x @ k[:, h].T * scale).masked_fill(hide[:, None], -math.inf)
+            mag = (x.abs() @ k[:, h].abs().T * scale).masked_fill(hide[:, None], 0)
+            ds = ((2e-6 + (2.0 ** -11 if kt != F16 else 0)) * mag + 2.0 ** -22 *
+                  w.masked_fill(hide[:, None], 0).abs()).amax(-1)
+            wl = torch.logsumexp(w, -1)
+            p = torch.exp(w - wl[..., None])
+            want, mass = p @ v[:, h], p @ v[:, h].abs()
+            # a probability below f16's normal range, of a largest one of at least 1
+            small = 2.0 ** -25 * v[:, h].abs().sum(0) * torch.exp(w.amax(-1) - wl)[..., None]
+            tol = (2 * ds[..., None] + 2.0 ** -11 + 1e-5 + (2.0 ** -11 if vt != F16 else 0)) * mass + \
+                small + 2.0 ** -11 * want.abs() + 2.0 ** -25
+            err = (got[s * rows:(s + 1) * rows, h * g:(h + 1) * g].double() - want).abs()
+            assert bool((err <= tol).all()), (s, h, float((err - tol).max()))
+            el = (lse[s * rows:(s + 1) * rows, h * g:(h + 1) * g].double() - wl).abs()
+            assert bool((el <= ds + 2e-6 * (1 + wl.abs())).all()), (s, h)
