@@ -66,6 +66,10 @@ struct Cfg {
     static constexpr uint32_t tiles = raw0 + raw_bytes;
     static __host__ __device__ constexpr uint32_t s_col(int s) { return s * 128; }
     static __host__ __device__ constexpr uint32_t o_col(int s) { return 256 + s * (D == 64 ? 64 : 128); }
+    // P of S tile b: one stream leaves columns for it, two put it over its S
+    static __host__ __device__ constexpr uint32_t p_col(int s, uint32_t b) {
+        return NS == 2 ? s_col(s) : (D == 256 ? 128 : 384) + b * (BN / 2);
+    }
     // The stage of the K or V tile of tile t, and how often it was used before.
     // TMA fills one ring in the order K0 V0 K1 V1 ..; the converting warps have
     // a ring each, so that a K does not wait for the P V of another tile.
@@ -793,7 +797,6 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
             // piece's Q comes only after this tile's P)
             bool ahead = false;
             if (NB == 2) {
-                if (n && !wait(pv_done(s), (n - 1) & 1u)) return;
                 if (same) {
                     const uint32_t t = sh[s].tile;
                     ahead = __all_sync(0xffffffffu, mbar_try(full(C::k_stage(t)), C::k_round(t) & 1u));
@@ -805,7 +808,7 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
             tc_fence_after();
             if (elect_one()) {
                 const uint32_t lb = ((ubase + NS * C::q_bytes + st * C::stage) >> 4) | (KB / 16) << 16;
-                const uint32_t p = tmem + C::s_col(s) + n % NB * BN;
+                const uint32_t p = tmem + C::p_col(s, n % NB);
 #pragma unroll
                 for (uint32_t c = 0; c < BN / 16; ++c)  // 16 keys: 8 columns of P, 2 KiB of V
                     mma_ts(tmem + C::o_col(s), p + 8 * c, desc(lb + 128 * c), id_o, c ? 1u : add);
@@ -1064,7 +1067,9 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
                     // way (a piece's first tile starts with that of its first columns).
                     // Only when a row's maximum has moved by more than 8 the pass is
                     // repeated with the new one; S still stands, P is in registers.
-                    uint32_t y[32], pk[BN / 2];
+                    constexpr int STEP = NS == 1 ? 64 : BN;
+                    uint32_t y[32], pk[STEP / 2];
+                    const uint32_t tp = tmem + ((32 * qd) << 16) + C::p_col(s, n % NB);
                     float top = -INFINITY, s0, s1;
                     auto column_max = [&](const uint32_t *v) {
 #pragma unroll
@@ -1076,24 +1081,29 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
                         s0 = s1 = 0.0f;
                         top = -INFINITY;
                         tmem_ld32_nowait(ts, x);
+#pragma unroll 1
+                        for (int w0 = 0; w0 < BN / 32; w0 += STEP / 32) {
 #pragma unroll
-                        for (int w = 0; w < BN / 32; ++w) {
-                            uint32_t *const v = w & 1 ? y : x;
-                            tmem_ld_wait(v);
-                            if (w + 1 < BN / 32) tmem_ld32_nowait(ts + 32 * (w + 1), w & 1 ? x : y);
-                            column_max(v);
-                            if (w == 0 && first) {
-                                m = top * c;
-                                neg = m == -INFINITY ? 0.0f : -m;
-                            }
+                            for (int w = 0; w < STEP / 32; ++w) {
+                                uint32_t *const v = w & 1 ? y : x;
+                                tmem_ld_wait(v);
+                                if (w + 1 < STEP / 32 || w0 + w + 1 < BN / 32)
+                                    tmem_ld32_nowait(ts + 32 * (w0 + w + 1), w & 1 ? x : y);
+                                column_max(v);
+                                if (w == 0 && w0 == 0 && first) {
+                                    m = top * c;
+                                    neg = m == -INFINITY ? 0.0f : -m;
+                                }
 #pragma unroll
-                            for (int k = 0; k < 16; ++k) {
-                                uint32_t e0 = v[2 * k], e1 = v[2 * k + 1];
-                                fma_pair(e0, e1, c, neg);
-                                const float p0 = ex2(__uint_as_float(e0)), p1 = ex2(__uint_as_float(e1));
-                                add_pair(s0, s1, p0, p1);
-                                pk[16 * w + k] = pack_h2(p0, p1);
+                                for (int k = 0; k < 16; ++k) {
+                                    uint32_t e0 = v[2 * k], e1 = v[2 * k + 1];
+                                    fma_pair(e0, e1, c, neg);
+                                    const float p0 = ex2(__uint_as_float(e0)), p1 = ex2(__uint_as_float(e1));
+                                    add_pair(s0, s1, p0, p1);
+                                    pk[16 * w + k] = pack_h2(p0, p1);
+                                }
                             }
+                            if (NS == 1) tmem_st32(tp + 16 * w0, *reinterpret_cast<const uint32_t(*)[32]>(pk));
                         }
                     };
                     bool first = begin;
@@ -1120,10 +1130,10 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
                     }
                     if (stop) break;
                     sum += s0 + s1;
-                    // P over the first columns of S
+                    if (NS == 2)
 #pragma unroll
-                    for (int w = 0; w < BN / 64; ++w)
-                        tmem_st32(ts + 32 * w, *reinterpret_cast<const uint32_t(*)[32]>(pk + 32 * w));
+                        for (int w = 0; w < BN / 64; ++w)
+                            tmem_st32(tp + 32 * w, *reinterpret_cast<const uint32_t(*)[32]>(pk + 32 * w));
                     tmem_st_wait();
                 }
                 // a new piece's output begins with this tile's product: the other
