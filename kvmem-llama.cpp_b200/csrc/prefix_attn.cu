@@ -12,24 +12,46 @@
 // A CTA (one per SM) walks its pieces (prefix_attn_plan.cuh). Warps:
 //   0      producer: page list, the tile's mask of valid keys, TMA loads of K
 //          and V tiles into a ring of shared-memory stages (128-byte swizzle,
-//          no multicast);
-//   2      walks the pieces and leaves each in a short ring for the others;
+//          no multicast), or of quant blocks into raw tiles;
+//   2      plans, walks the pieces and leaves each in a short ring for the others;
 //   3      notes for the join where each row's pieces lie;
-//   1      one lane issues the products: S = Q K^T (both in shared memory)
-//          and O += P V (P in tensor memory over its S, V as it lies: keys
-//          along K, MN-major);
+//   1      an elected lane issues the products: S = Q K^T (both in shared memory)
+//          and O += P V (P in tensor memory, V as it lies: keys along K, MN-major);
 //   4-7    softmax of stream 0, a thread a row; also loads Q, rescales and
 //          hands on O;
-//   8-11   the same for stream 1 (head size 256 has one stream: its output
-//          takes half of the tensor memory).
-// With more than 128 rows the two streams are two tiles of rows over the same
-// key tiles; otherwise they are the same rows over every other key tile, each
-// with its own output. While one stream is in its softmax the other one's
-// products run. P and S of a stream share columns, so its next S waits until
-// the product that reads P has completed.
+//   8-11   f16, head sizes 64 and 128: the same for stream 1;
+//   8-15   quantised K or V: four warps turn K blocks into f16 tiles, four V.
+// Tiles of 128 keys (head size 256: 64), 128 rows a stream.
+//   Two streams (f16): with more than 128 rows they are two tiles of rows over
+//     the same key tiles, otherwise the same rows over every other key tile,
+//     each with its own output. While one stream is in its softmax the other
+//     one's products run. P lies over its S, so a stream's next S waits until
+//     the product that reads P has completed.
+//   One stream (quantised, whose converting warps take the other one's registers;
+//     head size 256, whose output takes its tensor memory): S has two tiles and
+//     P columns of its own, so the next scores are issued before this softmax
+//     ends, and the softmax can be a loop of 64 keys.
 // Cells without a token may hold anything, NaN too: their scores are replaced
 // after the product, their V rows zeroed in shared memory before it.
 // Every wait is bounded; on a timeout the outputs become NaN (the join).
+//
+// What bounds it. Memory asks 24 us of 16 rows by 8 heads over 32,768 f16 tokens
+// and their tails, the call takes 48: 6 us until the first scores (plan, pages,
+// queries, first tiles, each a dependent read), 4 us for the join, between them
+// a chain of softmax and product per tile that reads at 4.3 TB/s. With 256 rows a
+// unit the chain is 4400 clocks for 2 * 128 x 128 scores: 2048 exponentials a
+// scheduler, and the products of one stream run during the softmax of the other
+// (tensor pipe active 48 %): 2048 rows by 64 heads over 32,768 tokens take 2.2 ms,
+// 1.03 PFLOP/s. Quantised: 55 us for the first shape (10 by its bytes), bound by
+// the same chain, of one stream: 3000 clocks a tile.
+// The instruction caches count: conversions as straight code of a tile were 12 %
+// slower than a loop over blocks (68 and 61 us), the softmax of one stream as
+// straight code of 128 keys 10 % (61 and 55).
+// Tried and worse: 64-key tiles with two S tiles for both streams (3.6 ms against
+// 2.2; a 64-key product takes 58 clocks, a 128-key one 64); exponentials of 1/8 to
+// 3/8 of the keys as polynomials (2.5 to 2.6 against 2.4 ms); products of both
+// streams in any order (3.9 against 3.2); one converting warpgroup and two
+// streams (75 us against 55).
 #include "prefix_attn.cuh"
 
 #include <cuda_fp16.h>
@@ -293,7 +315,7 @@ __device__ bool make_plan(const AttnLaunch &l, Plan &p, Start &start) {
         const SeqShape sh = seq_shape(a, s);
         pairs = (sh.q_len * G + PR - 1) / PR;
         const uint32_t n = sh.q_len ? tg.tiles(sh.len) : 0;
-        tiles = (n ? n + kUnit : 0) * pairs * H;
+        tiles = (n ? n + kUnit<BN> : 0) * pairs * H;
     };
     const bool pre = a.prefix.max_len != 0;
     const int32_t len0 = pre && a.prefix.len ? __ldg(a.prefix.len) : 0x7fffffff;
@@ -417,7 +439,7 @@ __device__ void note_rows(const AttnLaunch &l, const Plan &p) {
                 const uint32_t row = (t - q0) * G + gq, pair = row / PR, u = pair * H + h;
                 const uint32_t n = min(tiles, pair_tiles<BN, PR>(*sh, tg, pair, G));
                 if (n)
-                    put(r[1], p.own, (p.gs == 1 ? p.p_total : 0) + tile + u * (tiles + kUnit) + kUnit, n,
+                    put(r[1], p.own, (p.gs == 1 ? p.p_total : 0) + tile + u * (tiles + kUnit<BN>) + kUnit<BN>, n,
                         p.t_slot0 + pair0 * H + u, 1, row);
             }
             l.at[2 * x] = r[0];
@@ -434,7 +456,7 @@ __device__ void note_rows(const AttnLaunch &l, const Plan &p) {
         SeqShape sh = {};
         if (s0 + lane < a.n_seq) sh = seq_shape(a, s0 + lane);
         const uint32_t pairs = (sh.q_len * G + PR - 1) / PR, n = sh.q_len ? tg.tiles(sh.len) : 0;
-        const uint32_t tiles = (n ? n + kUnit : 0) * pairs * H;
+        const uint32_t tiles = (n ? n + kUnit<BN> : 0) * pairs * H;
         uint32_t ti = tiles, pi = pairs;
         scan(ti, pi);
         for (uint32_t w = 0; w < min(32u, a.n_seq - s0); ++w) {

@@ -24,9 +24,13 @@
 namespace kvmret {
 namespace {
 
-// Of 16 sequences over 32,768 shared tokens, with tails of 1 to 700: 33 us with
-// kUnit = @, @ us with 0.
-constexpr uint32_t kUnit = 2;
+// Tiles of BN keys for what a piece costs beside its tiles, about 128 keys' worth.
+// Sixteen sequences over 32,768 shared tokens, tails of 1 to 700: 47.5 us with
+// this, 55.6 with none, 48.3 with 256; heads of 256 over q8_0 (tiles of 64 keys):
+// 49 us with this, 61 with 64. 32 sequences of up to five rows: 135.6, 135.9 with
+// none, 133.9 with 256.
+template <int BN>
+constexpr uint32_t kUnit = 128 / BN;
 
 // Key tiles of a list with pages of T tokens: a page of at least BN tokens is
 // ceil(T / BN) tiles, else BN / T whole pages make one.
@@ -179,7 +183,7 @@ struct Walk {
             fresh = false;
             const uint32_t tiles = sh.q_len ? geom.tiles(sh.len) : 0;
             const uint32_t pairs = (sh.q_len * G + PR - 1) / PR;
-            const uint32_t mine = (tiles ? tiles + kUnit : 0) * pairs * a.n_head_kv;
+            const uint32_t mine = (tiles ? tiles + kUnit<BN> : 0) * pairs * a.n_head_kv;
             if (y >= seq_tile + mine) {
                 seq_tile += mine;
                 seq_pair += pairs;
@@ -187,12 +191,12 @@ struct Walk {
                 fresh = true;
                 continue;
             }
-            const uint32_t at = y - seq_tile, all = tiles + kUnit, u = at / all;
+            const uint32_t at = y - seq_tile, all = tiles + kUnit<BN>, u = at / all;
             uint32_t t = at - u * all, n = min(y1 - y, all - t);
             y += n;
-            if (t + n <= kUnit) continue;
-            n -= t < kUnit ? kUnit - t : 0;
-            t = t < kUnit ? 0 : t - kUnit;
+            if (t + n <= kUnit<BN>) continue;
+            n -= t < kUnit<BN> ? kUnit<BN> - t : 0;
+            t = t < kUnit<BN> ? 0 : t - kUnit<BN>;
             const uint32_t pair = u / a.n_head_kv;
             const uint32_t lim = pair_tiles<BN, PR>(sh, geom, pair, G);
             if (t >= lim) continue;
