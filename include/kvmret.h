@@ -658,10 +658,15 @@ typedef struct kvmret_attn {
  * left as they were. Tokens past a length may hold anything; those within it
  * must be finite. `prefix` (NULL with max_prefix = 0) and `tail` (NULL with
  * n_seq = 0) have one n_head_kv and d_head; page_tokens is a multiple of 16; the
- * types may differ. Scores, statistics and sums are f32; quantised values are
- * rounded to f16 (d * q) before the products. ws_dev: 256-byte aligned workspace
+ * types may differ. Scores, statistics and sums are f32, the weights p_j f16;
+ * quantised values are rounded to f16 (d * q) before the products and must lie in
+ * its range. A query that is not finite spoils its own row alone. q_start that
+ * descends, or a wait within the kernel that gives up (after about two seconds),
+ * leaves NaN in every row from q_start[0] to q_start[n_seq] - 1. ws_dev: 256-byte aligned workspace
  * of kvmret_prefix_attn_ws_bytes, written and read by this call alone (calls that
- * may overlap, graphs included, need one each). n_q <= 65535, n_head <= 65535. */
+ * may overlap, graphs included, need one each). n_q <= 65535, n_head <= 65535,
+ * n_q * n_head <= 2^31 - 1, and rows times key tiles, counted at 16 tokens a
+ * tile from the bounds, stay below 2^32 (refused otherwise). */
 size_t kvmret_prefix_attn_ws_bytes(uint32_t n_q, uint32_t n_head, uint32_t n_head_kv,
                                    uint32_t d_head, uint32_t n_seq);
 int kvmret_prefix_attn(const kvmret_pages *prefix, const kvmret_pages *tail, const kvmret_attn *a,

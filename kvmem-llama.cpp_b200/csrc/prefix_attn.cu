@@ -1134,7 +1134,8 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
                         pass(first);
                         first = false;
                         if (!__any_sync(0xffffffffu, top * c > m + 8.0f)) break;
-                        const float mn = fmaxf(m, top * c);
+                        // (a row's own maximum decides: what it gets depends on no other row)
+                        const float mn = top * c > m + 8.0f ? top * c : m;
                         const float f = m == -INFINITY ? 0.0f : ex2(m - mn);
                         m = mn;
                         sum *= f;
@@ -1267,10 +1268,11 @@ __global__ void __launch_bounds__(kJoinRows *D / 4)
     uint32_t bad = 0;
     for (uint32_t i = tid; i < n_cta; i += NT) bad |= l.fail[i];
     bad = __syncthreads_or(bad);
-    if (bad) {  // every row NaN
+    if (bad) {  // every row of the batch NaN
         for (uint32_t i = tid; i < kJoinRows * D; i += NT)
-            if (row0 + i / D < n_rows) a.out[static_cast<uint64_t>(row0) * D + i] = 0x7fff;
-        if (a.lse && tid < kJoinRows && row0 + tid < n_rows) a.lse[row0 + tid] = NAN;
+            if (row0 + i / D >= begin && row0 + i / D < end)
+                a.out[static_cast<uint64_t>(row0) * D + i] = 0x7fff;
+        if (a.lse && tid < kJoinRows && row0 + tid >= begin && row0 + tid < end) a.lse[row0 + tid] = NAN;
         return;
     }
     // a warp lists a row's pieces and weighs them
@@ -1285,7 +1287,10 @@ __global__ void __launch_bounds__(kJoinRows *D / 4)
             const uint32_t i = i0 + lane;
             const uint32_t id = i < e0.n ? e0.id + i * e0.step : e1.id + (i - e0.n) * e1.step;
             const float2 ml = i < n_all ? l.ml[id] : make_float2(-INFINITY, 0.0f);
-            const uint32_t have = __ballot_sync(0xffffffffu, ml.x != -INFINITY);
+            // a piece without keys has a sum of zero; one whose scores are all NaN has
+            // no maximum either, but a NaN sum
+            const bool held = ml.x != -INFINITY || ml.y != 0.0f;
+            const uint32_t have = __ballot_sync(0xffffffffu, held);
             float mt = ml.x;
             for (int o = 16; o; o >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, o));
             mt = fmaxf(mt, top);
@@ -1294,7 +1299,7 @@ __global__ void __launch_bounds__(kJoinRows *D / 4)
             for (uint32_t j = lane; j < n; j += 32) s_w[w][j] *= f;
             sum *= f;
             top = mt;
-            if (ml.x != -INFINITY) {
+            if (held) {
                 const uint32_t at = n + __popc(have & ((1u << lane) - 1));
                 const float e = ex2(ml.x - top);
                 s_id[w][at] = id;

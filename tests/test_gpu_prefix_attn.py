@@ -508,3 +508,79 @@ def test_long_prefixes(d, hkv, g, page, kt, vt, rows):
             assert bool((err <= tol).all()), (s, h, float((err - tol).max()))
             el = (lse[s * rows:(s + 1) * rows, h * g:(h + 1) * g].double() - wl).abs()
             assert bool((el <= ds + 2e-6 * (1 + wl.abs())).all()), (s, h)
+
+
+@pytest.mark.parametrize("d,kind", [(64, F16), (128, F16), (256, F16), (128, Q8)])
+def test_rows_that_are_not_finite_stay_alone(d, kind):
+    """An infinite or NaN query row changes no other row."""
+    case = ([1, 4, 30], [20, 9, 400], 900, 8, 2, d, 64, 32, kind, kind)
+    pool, tpool, table, own, _, _, start, q, tl = build(case)
+    bad = np.array([2, 7, 34])
+    args = [pool.device(), dev(np.array([900], np.int32)), tpool.device(), dev(own), dev(tl), dev(start)]
+    want, lse = kvmret.prefix_attn(dev(q), *args, prefix_table=dev(table), lse=True)
+    q[bad[0], :, 5] = np.nan
+    q[bad[1], :, 0] = np.inf
+    q[bad[2], :, d - 1] = -np.inf
+    got, lse2 = kvmret.prefix_attn(dev(q), *args, prefix_table=dev(table), lse=True)
+    good = np.setdiff1d(np.arange(q.shape[0]), bad)
+    assert torch.equal(got[good], want[good]) and torch.equal(lse2[good], lse[good])
+    assert not torch.isfinite(got[bad].float()).any()
+
+
+def test_descending_starts_leave_nan():
+    """Row starts that descend cannot be walked: the rows from the first start to
+    the last are NaN, the others as they were, and the next call is right."""
+    case = ([2, 2, 2], [9, 40, 77], 600, 8, 2, 128, 64, 32, F16, F16)
+    pool, tpool, table, own, pre, tails, start, q, tl = build(case)
+    rows = torch.zeros((8, 8, 128), dtype=torch.float16, device="cuda")
+    rows[1:7] = dev(q)
+    out = torch.full_like(rows, 7.0)
+    args = [pool.device(), dev(np.array([600], np.int32)), tpool.device(), dev(own), dev(tl)]
+    kw = dict(prefix_table=dev(table), lse=True)
+    _, lse = kvmret.prefix_attn(rows, *args, dev(np.array([1, 5, 3, 7], np.int32)), out=out, **kw)
+    assert torch.isnan(out[1:7]).all() and torch.isnan(lse[1:7]).all()
+    assert torch.all(out[0] == 7) and torch.all(out[7] == 7)
+    _, lse = kvmret.prefix_attn(rows, *args, dev(start + 1), out=out, **kw)
+    check(out[1:7], lse[1:7], reference(q.astype(np.float64), 2, 128 ** -0.5, pre, tails, start, (F16, F16)))
+
+
+@pytest.mark.parametrize("kind", [F16, Q8])
+def test_pages_named_more_than_once(kind):
+    """The same page twice in the prefix and in the tails of several sequences."""
+    rng = np.random.default_rng(3)
+    pool = Pool(rng, 3, 32, 2, 128, kind, kind)
+    pool.fill(np.arange(3), 96)
+    k, v = (values(b, kind).reshape(3, 32, 2, 128) for b in pool.bufs)
+    table, own = np.array([1, 1, 0, 1], np.int32), np.array([[2, 2], [2, 0]], np.int32)
+    tl, start = np.array([40, 50], np.int32), np.array([0, 3, 5], np.int32)
+    q = rng.standard_normal((5, 8, 128)).astype(np.float16)
+    pages = pool.device()
+    got, lse = kvmret.prefix_attn(dev(q), pages, dev(np.array([120], np.int32)), pages, dev(own), dev(tl),
+                                  dev(start), prefix_table=dev(table), lse=True)
+    pre = [x[table].reshape(-1, 2, 128)[:120] for x in (k, v)]
+    tails = [[x[own[s]].reshape(-1, 2, 128)[:tl[s]] for x in (k, v)] for s in range(2)]
+    check(got, lse, reference(q.astype(np.float64), 2, 128 ** -0.5, pre, tails, start, (kind, kind)))
+
+
+def test_two_graphs_at_once():
+    """Two captured calls over one cache, replayed at the same time again and
+    again, each on a stream of its own."""
+    case = ([1] * 6, [50] * 6, 5000, 16, 4, 128, 128, 32, Q8, F16)
+    pool, tpool, table, own, _, _, start, q, tl = build(case)
+    args = (pool.device(), dev(np.array([5000], np.int32)), tpool.device(), dev(own), dev(tl), dev(start))
+    t = dev(table)
+    qs = [dev(q), dev(q[::-1].copy())]
+    want = [kvmret.prefix_attn(x, *args, prefix_table=t) for x in qs]
+    graphs, outs = [], []
+    for x in qs:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(kvmret.prefix_attn(x, *args, prefix_table=t))
+    side = [torch.cuda.Stream() for _ in qs]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for g, s in zip(graphs, side):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs, want))
