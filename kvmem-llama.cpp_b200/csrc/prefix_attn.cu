@@ -132,6 +132,7 @@ struct AttnLaunch {
     float4 *o;       // [slot][row tile][D / 4][128]
     uint32_t max_slots;
     uint32_t raw_k, raw_v, n_raw_v;  // bytes of a raw K, V tile; raw V tiles
+    Divs by;
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -305,8 +306,8 @@ __device__ bool make_plan(const AttnLaunch &l, Plan &p, Start &start) {
     constexpr int BN = Cfg<D, QUANT>::BN, PR = Cfg<D, QUANT>::PR;
     const PrefixAttn &a = l.a;
     const uint32_t lane = threadIdx.x & 31;
-    const uint32_t G = a.n_head / a.n_head_kv, H = a.n_head_kv;
-    const TileGeom<BN> tg(a.n_seq ? a.tail.pages.page_tokens : BN);
+    const uint32_t G = l.by.G.d, H = a.n_head_kv;
+    const TileGeom<BN> tg(l.by.list[1]);
     bool ok = true;
     auto shape = [&](uint32_t s, uint32_t &tiles, uint32_t &pairs) {
         tiles = pairs = 0;
@@ -351,7 +352,7 @@ __device__ bool make_plan(const AttnLaunch &l, Plan &p, Start &start) {
         const uint64_t most = static_cast<uint64_t>(held) * a.prefix.pages.page_tokens;
         const uint32_t len = min(a.prefix.max_len, static_cast<uint32_t>(max(len0, 0)));
         p.p_len = most < len ? static_cast<uint32_t>(most) : len;
-        p.np = TileGeom<BN>(a.prefix.pages.page_tokens).tiles(p.p_len);
+        p.np = TileGeom<BN>(l.by.list[0]).tiles(p.p_len);
     }
     const int32_t nq = static_cast<int32_t>(a.n_q);
     p.q0 = static_cast<uint32_t>(min(max(q_first, 0), nq));
@@ -359,7 +360,7 @@ __device__ bool make_plan(const AttnLaunch &l, Plan &p, Start &start) {
     p.n_pair = (p.rows + PR - 1) / PR;
     // 8 CTAs side by side leave at most 5 % of the 148 SMs without a group
     p.n_pg = (p.n_pair + 7) / 8;
-    p.gs = p.n_pg ? (p.n_pair + p.n_pg - 1) / p.n_pg : 1;
+    p.gs = p.n_pg > 1 ? (p.n_pair + p.n_pg - 1) / p.n_pg : max(p.n_pair, 1u);
     if (p.gs > gridDim.x) {
         p.gs = gridDim.x;
         p.n_pg = (p.n_pair + p.gs - 1) / p.gs;
@@ -372,11 +373,11 @@ __device__ bool make_plan(const AttnLaunch &l, Plan &p, Start &start) {
     p.ok = ok;
     if (!ok) p.p_total = p.t_total = 0;
     if (p.gs == 1) {
-        p.pre.set(p.p_total + p.t_total, gridDim.x);
+        p.pre.set(p.p_total + p.t_total, l.by.ctas);
         p.own = p.pre;
     } else {
         p.pre.set(p.p_total, p.groups);
-        p.own.set(p.t_total, gridDim.x);
+        p.own.set(p.t_total, l.by.ctas);
     }
     start = {0, 0, 0};
     uint32_t x, x1, y, y1;
@@ -411,10 +412,10 @@ __device__ void note_rows(const AttnLaunch &l, const Plan &p) {
     constexpr int BN = Cfg<D, QUANT>::BN, PR = Cfg<D, QUANT>::PR, NS = Cfg<D, QUANT>::NS;
     const PrefixAttn &a = l.a;
     const uint32_t lane = threadIdx.x & 31, n_cta = gridDim.x;
-    const uint32_t G = a.n_head / a.n_head_kv, H = a.n_head_kv;
+    const uint32_t G = l.by.G.d, H = a.n_head_kv;
     // rows of the tokens [q0, q0 + q_len); tails from tile `tile` and pair `pair` on
     auto note = [&](uint32_t q0, uint32_t q_len, const SeqShape *sh, uint32_t tile, uint32_t pair0) {
-        const TileGeom<BN> tg(sh ? a.tail.pages.page_tokens : BN);
+        const TileGeom<BN> tg(l.by.list[1]);
         const uint32_t tiles = sh ? tg.tiles(sh->len) : 0;
         const uint32_t begin = q0 * a.n_head, end = begin + q_len * a.n_head;
         uint32_t b = begin / 32;
@@ -422,7 +423,7 @@ __device__ void note_rows(const AttnLaunch &l, const Plan &p) {
         for (; b * 32 < end; b += n_cta) {
             const uint32_t x = 32 * b + lane;
             if (x < begin || x >= end) continue;
-            const uint32_t t = x / a.n_head, head = x - t * a.n_head, h = head / G, gq = head - h * G;
+            const uint32_t t = x / a.n_head, head = x - t * a.n_head, h = l.by.G(head), gq = head - h * G;
             RowPieces r[2] = {};
             auto put = [&](RowPieces &e, const Cuts &cuts, uint32_t x0, uint32_t n, uint32_t slot0,
                            uint32_t step, uint32_t row) {
@@ -437,7 +438,7 @@ __device__ void note_rows(const AttnLaunch &l, const Plan &p) {
             }
             if (tiles) {
                 const uint32_t row = (t - q0) * G + gq, pair = row / PR, u = pair * H + h;
-                const uint32_t n = min(tiles, pair_tiles<BN, PR>(*sh, tg, pair, G));
+                const uint32_t n = min(tiles, pair_tiles<BN, PR>(*sh, tg, pair, l.by.G));
                 if (n)
                     put(r[1], p.own, (p.gs == 1 ? p.p_total : 0) + tile + u * (tiles + kUnit<BN>) + kUnit<BN>, n,
                         p.t_slot0 + pair0 * H + u, 1, row);
@@ -450,7 +451,7 @@ __device__ void note_rows(const AttnLaunch &l, const Plan &p) {
         note(0, a.n_q, nullptr, 0, 0);
         return;
     }
-    const TileGeom<BN> tg(a.tail.pages.page_tokens);
+    const TileGeom<BN> tg(l.by.list[1]);
     uint32_t base_t = 0, base_p = 0;
     for (uint32_t s0 = 0; s0 < a.n_seq; s0 += 32) {
         SeqShape sh = {};
@@ -601,7 +602,7 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
             mbar_arrive(planned);
         }
         __syncwarp();
-        Walk<BN, PR> walk(a, plan, start.seq, start.tile, start.pair);
+        Walk<BN, PR> walk(a, plan, l.by, start.seq, start.tile, start.pair);
         uint32_t j = 0;
         for (uint32_t i = 0;; ++i) {
             Seg g = {};
@@ -654,8 +655,8 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
             if (lane == 0) mbar_arrive(seg_empty(sg % kSegs));
             const KeyList &kl = g.tail ? a.tail : a.prefix;
             const CUtensorMap *mk = &l.map[g.tail ? 2 : 0], *mv = mk + 1;
-            const TileGeom<BN> geom(kl.pages.page_tokens);
-            const uint32_t T = geom.T, box = min(T, static_cast<uint32_t>(BN));
+            const TileGeom<BN> geom(l.by.list[g.tail]);
+            const uint32_t T = geom.c.T, box = min(T, static_cast<uint32_t>(BN));
             const uint64_t list = g.tail ? static_cast<uint64_t>(g.seq) * kl.n_list : 0;
             for (uint32_t i = 0; i < g.n && !stop; ++i, ++j) {
                 // lane p < ppt: page p of the tile, and how many of its tokens count
@@ -663,7 +664,7 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
                 geom.locate(g.tile0 + i, page, off);
                 int32_t id = -1;
                 uint32_t held = 0;
-                if (lane < geom.ppt && page + lane < kl.n_list) {
+                if (lane < geom.c.ppt && page + lane < kl.n_list) {
                     const uint32_t at = page + lane;
                     id = kl.table ? __ldg(kl.table + list + at) : static_cast<int32_t>(at);
                     if (id >= 0 && static_cast<uint32_t>(id) < kl.pages.n_pages) {
@@ -678,7 +679,7 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
                     const uint32_t key = 32 * w + lane, pk = T < BN ? key / T : 0;
                     const uint32_t h = __shfl_sync(0xffffffffu, held, pk);
                     const uint32_t o = T < BN ? key - pk * T : off + key;
-                    const uint32_t b = __ballot_sync(0xffffffffu, pk < geom.ppt && o < h);
+                    const uint32_t b = __ballot_sync(0xffffffffu, pk < geom.c.ppt && o < h);
                     if (lane == w) mask = b;
                 }
                 if constexpr (QUANT) {
@@ -945,14 +946,14 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
     } else if (warp >= 4) {  // ---- softmax, a thread a row ----
         const uint32_t s = (warp - 4) >> 2, qd = warp & 3, r = 32 * qd + lane;
         const uint32_t tid = threadIdx.x & 127;
-        const uint32_t G = a.n_head / a.n_head_kv;
+        const uint32_t G = l.by.G.d;
         // (above zero, so that -inf stays -inf; a scale of zero gives equal scores all the same)
         const float c = fmaxf(fabsf(a.scale) * 1.44269504f, 1e-37f);
         const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;  // a negative scale turns Q
         const uint32_t ts0 = tmem + ((32 * qd) << 16) + C::s_col(s);
         const uint32_t to = tmem + ((32 * qd) << 16) + C::o_col(s);
         constexpr uint32_t kRows = 128 / (D / 8);  // rows that one pass of the Q load covers
-        const uint32_t step_t = kRows / G, step_h = kRows - step_t * G;
+        const uint32_t step_t = l.by.G(kRows), step_h = kRows - step_t * G;
         uint32_t ns = 0, sg = 0;  // tiles and pieces so far
         uint32_t joins = 0;       // outputs joined with the other stream's
         bool owed = false;        // it may still be reading this one's
@@ -977,7 +978,7 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
             const uint32_t ch = tid % CH, q1 = tid / CH;
             const uint16_t *const q = a.q + static_cast<uint64_t>(g.q0) * a.q_stride +
                                       static_cast<uint64_t>(g.h) * G * D + 8 * ch;
-            uint32_t t = (at0 + q1) / G, hg = at0 + q1 - t * G;
+            uint32_t t = l.by.G(at0 + q1), hg = at0 + q1 - t * G;
             // n passes: all loads first. Only warps that hold a row look at their
             // scores, so rows past the last one of 32 stay as they are.
             auto load = [&](uint32_t i0, auto n) {
@@ -1029,7 +1030,7 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
             const bool idle = 32 * qd >= rows;  // no row of this warp: P may be anything
             // how far the row sees into the list
             uint32_t seen = 0xffffffffu;
-            if (g.tail) seen = tail_seen(g.len, g.q_len, (g.row0 + row_first() + min(r, rows - 1)) / G);
+            if (g.tail) seen = tail_seen(g.len, g.q_len, l.by.G(g.row0 + row_first() + min(r, rows - 1)));
             const uint32_t tile0 = g.tile0 - g.j0;
             float m = -INFINITY, sum = 0.0f;  // of c q . k
             for (bool begin = true; sh.any(); sh.tile += sh.step, begin = false) {
@@ -1064,10 +1065,10 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
                         }
                         fence_async_smem();
                     }
-                    const TileGeom<BN> geom((g.tail ? a.tail : a.prefix).pages.page_tokens);
+                    const TileGeom<BN> geom(l.by.list[g.tail]);
                     uint32_t page, off;
                     geom.locate(tile0 + jj, page, off);
-                    const uint32_t pos0 = page * geom.T + off;
+                    const uint32_t pos0 = page * geom.c.T + off;
                     const uint32_t lim = seen > pos0 ? min(seen - pos0, static_cast<uint32_t>(BN)) : 0;
 #pragma unroll 1
                     for (uint32_t w = 0; w < BN / 32 && !idle; ++w) {
@@ -1447,6 +1448,11 @@ cudaError_t launch_t(AttnLaunch &l, const WsLayout &w, cudaStream_t st) {
             e = encode_pages<D>(&l.map[2 * i + 1], v.v, v.v_row, v.v_page, v.v_type, v);
         if (e != cudaSuccess) return e;
     }
+    l.by.G.set(l.a.n_head / l.a.n_head_kv);
+    l.by.H.set(l.a.n_head_kv);
+    l.by.ctas.set(n_cta);
+    for (int i = 0; i < 2; ++i)
+        l.by.list[i].set(lists[i]->max_len ? lists[i]->pages.page_tokens : Cfg<D, false>::BN, Cfg<D, false>::BN);
     l.max_slots = static_cast<uint32_t>(w.slots[quant || D == 256 ? 0 : 1]);
     if (quant) {
         int32_t worst[2] = {KVMRET_TYPE_Q4_0, KVMRET_TYPE_Q4_0};

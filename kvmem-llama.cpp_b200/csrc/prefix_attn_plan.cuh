@@ -32,25 +32,55 @@ namespace {
 template <int BN>
 constexpr uint32_t kUnit = 128 / BN;
 
+// Division by a number that the host knows: n / d = (mulhi(n, m) + n) >> s with
+// s = ceil(log2 d), m = floor(2^32 (2^s - d) / d) + 1, exact for every n below 2^32
+// (Granlund and Montgomery 1994). The plan is a chain of some twenty divisions,
+// before which no CTA has work.
+struct Div {
+    uint32_t d, m, s;
+    void set(uint32_t by) {
+        d = by;
+        for (s = 0; (1ull << s) < by; ++s) {}
+        m = static_cast<uint32_t>((((1ull << s) - by) << 32) / by) + 1;
+    }
+    __device__ __forceinline__ uint32_t operator()(uint32_t n) const {
+        return static_cast<uint32_t>((static_cast<uint64_t>(__umulhi(n, m)) + n) >> s);
+    }
+};
+
 // Key tiles of a list with pages of T tokens: a page of at least BN tokens is
 // ceil(T / BN) tiles, else BN / T whole pages make one.
+struct PageTiles {
+    uint32_t T, tpp, ppt;  // page tokens, tiles per page (T >= BN), pages per tile (T < BN)
+    Div whole, pages;      // by the tokens of whole pages (T >= BN: one) of a tile, by tpp
+    void set(uint32_t t, uint32_t bn) {
+        T = t;
+        tpp = t >= bn ? (t - 1) / bn + 1 : 1;
+        ppt = t >= bn ? 1 : bn / t;
+        whole.set(ppt * t);
+        pages.set(tpp);
+    }
+};
+// What the host knows of a call's divisions.
+struct Divs {
+    Div G, H, ctas;  // query heads a KV head, KV heads, CTAs
+    PageTiles list[2];  // of the prefix, the tails
+};
 template <int BN>
 struct TileGeom {
-    uint32_t T, tpp, ppt;  // page tokens, tiles per page (T >= BN), pages per tile (T < BN)
-    __device__ __forceinline__ explicit TileGeom(uint32_t t)
-        : T(t), tpp(t >= BN ? (t + BN - 1) / BN : 1), ppt(t >= BN ? 1 : BN / t) {}
+    const PageTiles &c;
+    __device__ __forceinline__ explicit TileGeom(const PageTiles &of) : c(of) {}
     __device__ __forceinline__ uint32_t tiles(uint32_t len) const {
-        if (T < BN) return (len + ppt * T - 1) / (ppt * T);
-        const uint32_t full = len / T, rem = len - full * T;
-        return full * tpp + (rem + BN - 1) / BN;
+        const uint32_t full = c.whole(len), rem = len - full * c.whole.d;
+        return c.T < BN ? full + (rem != 0) : full * c.tpp + (rem + BN - 1) / BN;
     }
     __device__ __forceinline__ void locate(uint32_t tile, uint32_t &page, uint32_t &off) const {
-        if (T < BN) {
-            page = tile * ppt;
+        if (c.T < BN) {
+            page = tile * c.ppt;
             off = 0;
         } else {
-            page = tile / tpp;
-            off = (tile - page * tpp) * BN;
+            page = c.pages(tile);
+            off = (tile - page * c.tpp) * BN;
         }
     }
 };
@@ -61,6 +91,10 @@ struct Cuts {
     __device__ __forceinline__ void set(uint32_t total, uint32_t parts) {
         q = total / parts;
         r = total - q * parts;
+    }
+    __device__ __forceinline__ void set(uint32_t total, const Div &parts) {
+        q = parts(total);
+        r = total - q * parts.d;
     }
     __device__ __forceinline__ uint32_t at(uint32_t i) const { return q * i + min(i, r); }
     // the range that holds tile x of the line
@@ -105,8 +139,8 @@ __device__ __forceinline__ uint32_t tail_seen(uint32_t len, uint32_t q_len, uint
 // tiles of a tail that the rows of a pair reach
 template <int BN, int PR>
 __device__ __forceinline__ uint32_t pair_tiles(const SeqShape &s, const TileGeom<BN> &g,
-                                               uint32_t pair, uint32_t G) {
-    const uint32_t last = min(s.q_len - 1, (pair * PR + PR - 1) / G);
+                                               uint32_t pair, const Div &G) {
+    const uint32_t last = min(s.q_len - 1, G(pair * PR + PR - 1));
     return g.tiles(tail_seen(s.len, s.q_len, last));
 }
 
@@ -124,7 +158,8 @@ template <int BN, int PR>
 struct Walk {
     const PrefixAttn &a;
     const Plan &p;  // in shared memory
-    uint32_t G, cta;
+    const Divs &by;
+    uint32_t cta;
     uint32_t x, x1;       // prefix line: next tile, end
     uint32_t part, lane;  // the range and the CTA's place in its group
     uint32_t y, y1;       // tails' line
@@ -133,12 +168,11 @@ struct Walk {
     SeqShape sh;
     bool fresh;
 
-    __device__ __forceinline__ Walk(const PrefixAttn &a_, const Plan &p_, uint32_t s, uint32_t tile,
-                                    uint32_t pair)
-        : a(a_), p(p_), G(a_.n_head / a_.n_head_kv), cta(blockIdx.x), seq(s),
-          seq_tile(tile), seq_pair(pair), fresh(true) {
+    __device__ __forceinline__ Walk(const PrefixAttn &a_, const Plan &p_, const Divs &by_, uint32_t s,
+                                    uint32_t tile, uint32_t pair)
+        : a(a_), p(p_), by(by_), cta(blockIdx.x), seq(s), seq_tile(tile), seq_pair(pair), fresh(true) {
         ranges(p, cta, x, x1, y, y1);
-        part = cta / p.gs;
+        part = p.gs == 1 ? cta : cta / p.gs;
         lane = cta - part * p.gs;
     }
     static __device__ __forceinline__ void ranges(const Plan &p, uint32_t cta, uint32_t &x,
@@ -162,7 +196,7 @@ struct Walk {
         while (x < x1) {
             const uint32_t u = x / p.np, t = x - u * p.np, n = min(x1 - x, p.np - t);
             x += n;
-            const uint32_t pg = u / a.n_head_kv, pair = pg * p.gs + lane;
+            const uint32_t pg = by.H(u), pair = pg * p.gs + lane;
             if (pair >= p.n_pair) continue;
             g.tail = 0;
             g.seq = 0;
@@ -177,12 +211,12 @@ struct Walk {
             g.slot = (u + part) * p.gs + lane;
             return true;
         }
-        const TileGeom<BN> geom(a.tail.pages.page_tokens);
+        const TileGeom<BN> geom(by.list[1]);
         while (y < y1 && seq < a.n_seq) {
             if (fresh) sh = seq_shape(a, seq);
             fresh = false;
             const uint32_t tiles = sh.q_len ? geom.tiles(sh.len) : 0;
-            const uint32_t pairs = (sh.q_len * G + PR - 1) / PR;
+            const uint32_t pairs = (sh.q_len * by.G.d + PR - 1) / PR;
             const uint32_t mine = (tiles ? tiles + kUnit<BN> : 0) * pairs * a.n_head_kv;
             if (y >= seq_tile + mine) {
                 seq_tile += mine;
@@ -197,8 +231,8 @@ struct Walk {
             if (t + n <= kUnit<BN>) continue;
             n -= t < kUnit<BN> ? kUnit<BN> - t : 0;
             t = t < kUnit<BN> ? 0 : t - kUnit<BN>;
-            const uint32_t pair = u / a.n_head_kv;
-            const uint32_t lim = pair_tiles<BN, PR>(sh, geom, pair, G);
+            const uint32_t pair = by.H(u);
+            const uint32_t lim = pair_tiles<BN, PR>(sh, geom, pair, by.G);
             if (t >= lim) continue;
             n = min(n, lim - t);
             g.tail = 1;
@@ -208,7 +242,7 @@ struct Walk {
             g.h = u - pair * a.n_head_kv;
             g.q0 = sh.q0;
             g.row0 = pair * PR;
-            g.rows = min(static_cast<uint32_t>(PR), sh.q_len * G - g.row0);
+            g.rows = min(static_cast<uint32_t>(PR), sh.q_len * by.G.d - g.row0);
             g.tile0 = t;
             g.n = n;
             g.slot = p.t_slot0 + seq_pair * a.n_head_kv + u + cta;
