@@ -76,6 +76,7 @@ struct Cfg {
     static constexpr int NB = 3 - NS;               // S tiles of a stream
     static constexpr int BN = D == 256 ? 64 : 128;  // keys of a tile
     static constexpr int PR = 128 * NS;             // rows of a unit
+    static constexpr int parts = NS;                // parts of a tile that P is handed on in
     static constexpr int threads = 128 + 128 * NS + (QUANT ? 256 : 0);
     static constexpr uint32_t stage = BN * D * 2;   // one K or V tile
     static constexpr int stages = QUANT ? (D == 64 ? 8 : D == 128 ? 4 : 3) : D == 64 ? 8 : 5;
@@ -489,7 +490,7 @@ struct Small {
     static constexpr int NS = C::NS;
     alignas(16) uint32_t mask[kMeta][4];  // valid keys of a tile
     float2 ml[NS][128];                   // statistics on their way to the other stream
-    uint64_t bars[2 * C::stages + kMeta + 2 * kSegs + (4 + 2 * C::NB) * NS + 2 + 4 * C::raws + (QUANT ? kMeta : 0)];
+    uint64_t bars[2 * C::stages + kMeta + 2 * kSegs + (7 + C::NB) * NS + 2 + 4 * C::raws + (QUANT ? kMeta : 0)];
     TileInfo tile[QUANT ? kMeta : 1];
     Plan plan;
     Seg seg[kSegs];
@@ -525,14 +526,15 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
     auto seg_empty = [&](uint32_t i) { return bar0 + 8u * (2 * ST + kMeta + kSegs + i); };
     constexpr uint32_t SB = 2 * ST + kMeta + 2 * kSegs;
     auto q_ready = [&](uint32_t s) { return bar0 + 8u * (SB + s); };
-    // one for each S tile of a stream
+    // one for each S tile of a stream; P has one for each S tile, or each part of it
     auto s_full = [&](uint32_t s, uint32_t b) { return bar0 + 8u * (SB + NS + NB * s + b); };
-    auto p_ready = [&](uint32_t s, uint32_t b) { return bar0 + 8u * (SB + (1 + NB) * NS + NB * s + b); };
-    constexpr uint32_t SP = SB + (1 + 2 * NB) * NS;
+    auto p_ready = [&](uint32_t s, uint32_t i) { return bar0 + 8u * (SB + (1 + NB) * NS + 2 * s + i); };
+    constexpr uint32_t SP = SB + (3 + NB) * NS;
+    auto pv_half = [&](uint32_t s) { return bar0 + 8u * (SP + 3 * NS + s); };
     auto pv_done = [&](uint32_t s) { return bar0 + 8u * (SP + s); };
     auto o_done = [&](uint32_t s) { return bar0 + 8u * (SP + NS + s); };
     auto o_read = [&](uint32_t s) { return bar0 + 8u * (SP + 2 * NS + s); };
-    const uint32_t drain = bar0 + 8u * (SP + 3 * NS), planned = drain + 8;
+    const uint32_t drain = bar0 + 8u * (SP + 4 * NS), planned = drain + 8;
     // raw tiles i of K (v = 0), V
     auto raw_full = [&](uint32_t v, uint32_t i) { return drain + 16 + 8u * (v * RS + i); };
     auto raw_empty = [&](uint32_t v, uint32_t i) { return drain + 16 + 8u * (2 * RS + v * RS + i); };
@@ -555,10 +557,9 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
         }
         for (int s = 0; s < NS; ++s) {
             mbar_init(q_ready(s), 4);
-            for (int b = 0; b < NB; ++b) {
-                mbar_init(s_full(s, b), 1);
-                mbar_init(p_ready(s, b), 4);
-            }
+            for (int b = 0; b < NB; ++b) mbar_init(s_full(s, b), 1);
+            for (int i = 0; i < 2; ++i) mbar_init(p_ready(s, i), 4);
+            mbar_init(pv_half(s), 1);
             mbar_init(pv_done(s), 1);
             mbar_init(o_done(s), 4);
             mbar_init(o_read(s), 4);
@@ -826,20 +827,30 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
                     if (ahead) scores(s, n + 1, false);
                 }
             }
-            if (stop || !wait(full(st), C::v_round(cur[s]) & 1u) || !wait(p_ready(s, n % NB), (n / NB) & 1u))
-                return;
-            tc_fence_after();
-            if (elect_one()) {
-                const uint32_t lb = ((ubase + NS * C::q_bytes + st * C::stage) >> 4) | (KB / 16) << 16;
-                const uint32_t p = tmem + C::p_col(s, n % NB);
+            if (stop || !wait(full(st), C::v_round(cur[s]) & 1u)) return;
 #pragma unroll
-                for (uint32_t c = 0; c < BN / 16; ++c)  // 16 keys: 8 columns of P, 2 KiB of V
-                    mma_ts(tmem + C::o_col(s), p + 8 * c, desc(lb + 128 * c), id_o, c ? 1u : add);
-                mma_commit(empty(st));
-                if (NS == 2 && !both) mma_commit(empty(st));
-                mma_commit(pv_done(s));
+            for (uint32_t h = 0; h < C::parts; ++h) {
+                const bool got = NS == 2 ? wait(p_ready(s, h), n & 1u) : wait(p_ready(s, n & 1u), (n >> 1) & 1u);
+                if (!got) return;
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint32_t lb = ((ubase + NS * C::q_bytes + st * C::stage) >> 4) | (KB / 16) << 16;
+                    const uint32_t p = tmem + C::p_col(s, n % NB);
+#pragma unroll
+                    for (uint32_t i = 0; i < BN / 16 / C::parts; ++i) {  // 16 keys: 8 columns of P, 2 KiB of V
+                        const uint32_t c = h * (BN / 16 / C::parts) + i;
+                        mma_ts(tmem + C::o_col(s), p + 8 * c, desc(lb + 128 * c), id_o, c ? 1u : add);
+                    }
+                    if (h + 1 < C::parts) {
+                        mma_commit(pv_half(s));
+                    } else {
+                        mma_commit(empty(st));
+                        if (NS == 2 && !both) mma_commit(empty(st));
+                        mma_commit(pv_done(s));
+                    }
+                }
+                __syncwarp();
             }
-            __syncwarp();
             if (!same) open(s);
             if (!stop && live[s] && !ahead) scores(s, n + 1, NB == 1);
             cur[s] = sh[s].tile;
@@ -1084,15 +1095,26 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
                     }
                     tmem_st_wait();
                 }
-                if (!idle) {
-                    // One pass with the maximum as it stands: p and the tile's own
-                    // maximum together, 32 columns at a time with the next ones on their
-                    // way (a piece's first tile starts with that of its first columns).
-                    // Only when a row's maximum has moved by more than 8 the pass is
-                    // repeated with the new one; S still stands, P is in registers.
-                    constexpr int STEP = NS == 1 ? 64 : BN;
+                // a new piece's output begins with this tile's product: the other
+                // stream must have read the last one
+                if (begin && owed) {
+                    if (!wait(o_read(1 - s), (joins - 1) & 1u)) break;
+                    owed = false;
+                }
+                // One pass with the maximum as it stands: p and the keys' own maximum
+                // together, 32 columns at a time with the next ones on their way (a
+                // piece's first tile starts with that of its first columns). Only when a
+                // row's maximum has moved by more than 8 the pass is repeated with the
+                // new one; S still stands. Two streams hand the halves of P on one by
+                // one, so that the first half's product runs during the second half's
+                // softmax (2048 rows over 32,768 tokens: 2.35 ms, 2.44 in one piece; 16 rows: 44
+                // and 47 us).
+                constexpr int KEYS = BN / C::parts, STEP = KEYS < 64 ? KEYS : 64;
+#pragma unroll 1
+                for (uint32_t h = 0; h < C::parts && !idle; ++h) {
                     uint32_t y[32], pk[STEP / 2];
-                    const uint32_t tp = tmem + ((32 * qd) << 16) + C::p_col(s, n % NB);
+                    const uint32_t tp = tmem + ((32 * qd) << 16) + C::p_col(s, n % NB) + h * (KEYS / 2);
+                    const uint32_t tk = ts + h * KEYS;
                     float top = -INFINITY, s0, s1;
                     auto column_max = [&](const uint32_t *v) {
 #pragma unroll
@@ -1103,15 +1125,15 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
                         float neg = m == -INFINITY ? 0.0f : -m;
                         s0 = s1 = 0.0f;
                         top = -INFINITY;
-                        tmem_ld32_nowait(ts, x);
+                        tmem_ld32_nowait(tk, x);
 #pragma unroll 1
-                        for (int w0 = 0; w0 < BN / 32; w0 += STEP / 32) {
+                        for (int w0 = 0; w0 < KEYS / 32; w0 += STEP / 32) {
 #pragma unroll
                             for (int w = 0; w < STEP / 32; ++w) {
                                 uint32_t *const v = w & 1 ? y : x;
                                 tmem_ld_wait(v);
-                                if (w + 1 < STEP / 32 || w0 + w + 1 < BN / 32)
-                                    tmem_ld32_nowait(ts + 32 * (w0 + w + 1), w & 1 ? x : y);
+                                if (w + 1 < STEP / 32 || w0 + w + 1 < KEYS / 32)
+                                    tmem_ld32_nowait(tk + 32 * (w0 + w + 1), w & 1 ? x : y);
                                 column_max(v);
                                 if (w == 0 && w0 == 0 && first) {
                                     m = top * c;
@@ -1129,7 +1151,7 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
                             if (NS == 1) tmem_st32(tp + 16 * w0, *reinterpret_cast<const uint32_t(*)[32]>(pk));
                         }
                     };
-                    bool first = begin;
+                    bool first = begin && h == 0;
 #pragma unroll 1
                     for (;;) {
                         pass(first);
@@ -1140,8 +1162,11 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
                         const float f = m == -INFINITY ? 0.0f : ex2(m - mn);
                         m = mn;
                         sum *= f;
-                        if (begin) continue;
-                        if (!past()) break;
+                        if (h == 0 ? begin : !wait(pv_half(s), n & 1u)) {
+                            if (stop) break;
+                            continue;
+                        }
+                        if (h == 0 && !past()) break;
                         tc_fence_after();
 #pragma unroll 1
                         for (uint32_t col = 0; col < D; col += 16) {
@@ -1154,23 +1179,21 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
                     }
                     if (stop) break;
                     sum += s0 + s1;
-                    if (NS == 2)
-#pragma unroll
-                        for (int w = 0; w < BN / 64; ++w)
-                            tmem_st32(tp + 32 * w, *reinterpret_cast<const uint32_t(*)[32]>(pk + 32 * w));
+                    if (NS == 2) tmem_st32(tp, *reinterpret_cast<const uint32_t(*)[32]>(pk));
                     tmem_st_wait();
+                    if (h + 1 < C::parts) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(p_ready(s, h));
+                    }
                 }
-                // a new piece's output begins with this tile's product: the other
-                // stream must have read the last one
-                if (begin && owed) {
-                    if (!wait(o_read(1 - s), (joins - 1) & 1u)) break;
-                    owed = false;
-                }
+                if (stop) break;
+                if (idle && C::parts == 2 && lane == 0) mbar_arrive(p_ready(s, 0));
                 // (at the piece's last tile, whose product is waited for below)
                 if (sh.tile + sh.step >= sh.end && !past()) break;
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(p_ready(s, n % NB));
+                if (lane == 0) mbar_arrive(p_ready(s, NS == 2 ? 1 : n & 1u));
             }
             if (stop) break;
             // the last scores are in: Q may be replaced while the last product runs
