@@ -1046,13 +1046,21 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
             float m = -INFINITY, sum = 0.0f;  // of c q . k
             for (bool begin = true; sh.any(); sh.tile += sh.step, begin = false) {
                 const uint32_t jj = sh.tile, n = ns++, ts = ts0 + n % NB * BN;  // its n-th tile
-                if (!wait(s_full(s, n % NB), (n / NB) & 1u) || !wait(meta(jj % kMeta), (jj / kMeta) & 1u))
-                    break;
-                tc_fence_after();
+                // what the tile's mask says, while the scores are on their way (behind
+                // their wait this takes 4 to 8 % of a long call)
+                if (!wait(meta(jj % kMeta), (jj / kMeta) & 1u)) break;
                 const uint4 mw = *reinterpret_cast<const uint4 *>(sm.mask[jj % kMeta]);
                 const bool whole = (mw.x & mw.y & (BN == 128 ? mw.z & mw.w : 0xffffffffu)) == 0xffffffffu;
                 // a tile's first token is at most tile * BN: all of it seen?
                 const bool clear = whole && __all_sync(0xffffffffu, (tile0 + jj + 1) * BN <= seen);
+                // a new piece's output begins with this tile's product: the other
+                // stream must have read the last one
+                if (begin && owed) {
+                    if (!wait(o_read(1 - s), (joins - 1) & 1u)) break;
+                    owed = false;
+                }
+                if (!wait(s_full(s, n % NB), (n / NB) & 1u)) break;
+                tc_fence_after();
                 // With two S tiles these scores did not wait for the product before: its
                 // end, without which O may still change and the phases of pv_done and of
                 // the V stage may be one further back than their parities tell.
@@ -1094,12 +1102,6 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
                         tmem_st32(ts + 32 * w, x);
                     }
                     tmem_st_wait();
-                }
-                // a new piece's output begins with this tile's product: the other
-                // stream must have read the last one
-                if (begin && owed) {
-                    if (!wait(o_read(1 - s), (joins - 1) & 1u)) break;
-                    owed = false;
                 }
                 // One pass with the maximum as it stands: p and the keys' own maximum
                 // together, 32 columns at a time with the next ones on their way (a
