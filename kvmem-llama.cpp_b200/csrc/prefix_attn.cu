@@ -36,22 +36,23 @@
 // Every wait is bounded; on a timeout the outputs become NaN (the join).
 //
 // What bounds it. Memory asks 24 us of 16 rows by 8 heads over 32,768 f16 tokens
-// and their tails, the call takes 48: 6 us until the first scores (plan, pages,
+// and their tails, the call takes 43: 5 us until the first scores (plan, pages,
 // queries, first tiles, each a dependent read), 4 us for the join, between them
-// a chain of softmax and product per tile that reads at 4.3 TB/s. With 256 rows a
-// unit the chain is 4400 clocks for 2 * 128 x 128 scores: 2048 exponentials a
-// scheduler, and the products of one stream run during the softmax of the other
-// (tensor pipe active 48 %): 2048 rows by 64 heads over 32,768 tokens take 2.2 ms,
-// 1.03 PFLOP/s. Quantised: 55 us for the first shape (10 by its bytes), bound by
-// the same chain, of one stream: 3000 clocks a tile.
+// a chain of softmax and product per tile that reads at 4.5 TB/s. With 256 rows a
+// unit the chain is about 4000 clocks for 2 * 128 x 128 scores: 2048 exponentials
+// a scheduler, the products of one stream during the softmax of the other (tensor
+// pipe active 45 %): 2048 rows by 64 heads over 32,768 tokens take 2.15 to 2.4 ms
+// as the clock stands, about 1 PFLOP/s. Quantised: 53 us for the first shape (10 by
+// its bytes), bound by the same chain of one stream, 3000 clocks a tile.
 // The instruction caches count: conversions as straight code of a tile were 12 %
 // slower than a loop over blocks (68 and 61 us), the softmax of one stream as
 // straight code of 128 keys 10 % (61 and 55).
-// Tried and worse: 64-key tiles with two S tiles for both streams (3.6 ms against
-// 2.2; a 64-key product takes 58 clocks, a 128-key one 64); exponentials of 1/8 to
-// 3/8 of the keys as polynomials (2.5 to 2.6 against 2.4 ms); products of both
-// streams in any order (3.9 against 3.2); one converting warpgroup and two
-// streams (75 us against 55).
+// Tried and no better: 64-key tiles with two S tiles for both streams (3.6 ms
+// against 2.2; a 64-key product takes 58 clocks, a 128-key one 64); exponentials of
+// 1/8 to 3/8 of the keys as polynomials (2.5 to 2.6 against 2.4 ms); a warp for S
+// and one for P V (2.28 to 2.38 against 2.15 to 2.25 ms); the products' warp asking
+// for all it needs at once (the same); one converting warpgroup and two streams
+// (75 us against 55).
 #include "prefix_attn.cuh"
 
 #include <cuda_fp16.h>
