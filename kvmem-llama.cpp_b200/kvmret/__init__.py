@@ -1100,6 +1100,8 @@ class Pages:
             _want(x.shape[0] > 0 and x[0].is_contiguous() and x[0].numel() * x.element_size() ==
                   page_tokens * row_bytes(t, n_head_kv * d_head),
                   "pages: a page must be page_tokens contiguous rows of its type")
+            # (a stride of zero, of a repeated page, would read as dense pages)
+            _want(x.shape[0] == 1 or x.stride(0) > 0, "pages: the page axis must not be expanded")
             strides.append(x.stride(0) * x.element_size() if x.shape[0] > 1 else 0)
         self.k, self.v, self.index = k, v, k.get_device()
         self.n_pages, self.page_tokens = k.shape[0], page_tokens

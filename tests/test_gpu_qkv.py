@@ -285,3 +285,14 @@ def test_wrapper_refusals():
     for call in bad:
         with pytest.raises(kvmret.KvmretError):
             call()
+
+
+def test_pages_of_an_expanded_axis_are_refused():
+    """One page repeated by a stride of zero is no paged cache: the stride would
+    be taken for dense pages."""
+    one = torch.zeros(1, 16, 2, 128, dtype=torch.float16, device="cuda")
+    full = torch.zeros(3, 16, 2, 128, dtype=torch.float16, device="cuda")
+    for k, v in ((one.expand(3, 16, 2, 128), full), (full, one.expand(3, 16, 2, 128))):
+        with pytest.raises(kvmret.KvmretError):
+            kvmret.Pages(k, v, 16, 2, 128)
+    assert kvmret.Pages(one, one.clone(), 16, 2, 128).n_pages == 1
