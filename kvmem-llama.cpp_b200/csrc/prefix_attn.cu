@@ -612,7 +612,17 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
                 g.j0 = j;
                 j += g.n;
             }
-            if (i >= kSegs && !wait(seg_empty(i % kSegs), (i / kSegs - 1) & 1u)) break;
+            // This wait lasts as long as a whole piece, which a very long list makes
+            // longer than the limit: it goes on as long as no other warp gave up.
+            bool room = i < kSegs;
+            for (uint32_t t = 0; !room && t < 64; ++t) {
+                room = __all_sync(0xffffffffu, mbar_wait_clk(seg_empty(i % kSegs), (i / kSegs - 1) & 1u));
+                if (__any_sync(0xffffffffu, *static_cast<volatile uint32_t *>(&sm.fail))) break;
+            }
+            if (!room) {
+                stop = true;
+                break;
+            }
             if (lane == 0) {
                 sm.seg[i % kSegs] = g;
                 mbar_arrive(seg_full(i % kSegs));
