@@ -584,3 +584,45 @@ def test_two_graphs_at_once():
                 g.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+@pytest.mark.parametrize("d,pre_kinds,tail_kinds", [
+    (128, (Q8, Q4), (F16, F16)), (128, (F16, F16), (Q4, Q8)), (64, (Q4, F16), (F16, Q8)),
+    (256, (F16, Q8), (Q8, F16)), (256, (Q8, Q8), (F16, F16)),
+])
+def test_prefix_and_tails_of_different_types(d, pre_kinds, tail_kinds):
+    """A quantised window with tails in f16 and other mixtures: tiles that are
+    converted and tiles that are copied alternate in one CTA's order."""
+    rng = np.random.default_rng(d)
+    new, tl, n_pre, hq, hkv = [1, 4, 20], [300, 150, 40], 1300, 16, 4
+    pool, tpool = Pool(rng, 12, 128, hkv, d, *pre_kinds), Pool(rng, 30, 32, hkv, d, *tail_kinds)
+    table = rng.permutation(12)[:11].astype(np.int32)
+    own = rng.permutation(30).reshape(3, 10).astype(np.int32)
+    pre = pool.fill(table, n_pre)
+    tails = [tpool.fill(own[s], t) for s, t in enumerate(tl)]
+    start = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+    q = (rng.standard_normal((25, hq, d)) * 1.5).astype(np.float16)
+    got, lse = kvmret.prefix_attn(dev(q), pool.device(), dev(np.array([n_pre], np.int32)), tpool.device(),
+                                  dev(own), dev(np.array(tl, np.int32)), dev(start),
+                                  prefix_table=dev(table), lse=True)
+    check(got, lse, reference(q.astype(np.float64), hkv, d ** -0.5, pre, tails, start, (Q8, Q8)))
+
+
+def test_many_sequences():
+    """A thousand sequences, some without rows or without tokens, over no prefix
+    and over a short one: more than the split looks at in one go."""
+    rng = np.random.default_rng(8)
+    n, hq, hkv, d = 1000, 4, 2, 64
+    new, tl = rng.integers(0, 3, n), rng.integers(0, 40, n)
+    tpool = Pool(rng, 3 * n, 16, hkv, d, F16, F16)
+    own = rng.permutation(3 * n).reshape(n, 3).astype(np.int32)
+    tails = [tpool.fill(own[s], int(t)) for s, t in enumerate(tl)]
+    start = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+    q = rng.standard_normal((int(start[-1]), hq, d)).astype(np.float16)
+    pool = Pool(rng, 5, 16, hkv, d, F16, F16)
+    for n_pre in (0, 70):
+        pre = pool.fill(np.arange(5), n_pre)
+        got, lse = kvmret.prefix_attn(dev(q), pool.device() if n_pre else None,
+                                      dev(np.array([n_pre], np.int32)) if n_pre else None, tpool.device(),
+                                      dev(own), dev(tl.astype(np.int32)), dev(start), lse=True)
+        check(got, lse, reference(q.astype(np.float64), hkv, d ** -0.5, pre, tails, start, (F16, F16)))
