@@ -41,7 +41,7 @@
 // a chain of softmax and product per tile that reads at 4.5 TB/s. With 256 rows a
 // unit the chain is about 4000 clocks for 2 * 128 x 128 scores: 2048 exponentials
 // a scheduler, the products of one stream during the softmax of the other (tensor
-// pipe active 45 %): 2048 rows by 64 heads over 32,768 tokens take 2.15 to 2.4 ms
+// pipe active 45 %): 2048 rows by 64 heads over 32,768 tokens take 2.15 to 2.5 ms
 // as the clock stands, about 1 PFLOP/s. Quantised: 53 us for the first shape (10 by
 // its bytes), bound by the same chain of one stream, 3000 clocks a tile.
 // The instruction caches count: conversions as straight code of a tile were 12 %
