@@ -894,8 +894,11 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
         // once to the tensor cores' type: outputs are 2.9e-4 to 5.2e-4 off in the mean
         // instead of the 2.9e-4 of f16 pages (most of which P's and the output's own
         // rounding make). d * q whole would take two f16 tiles each for K and V, twice
-        // the products, and leave them one stage each. Operands in f16 go to their stage by TMA, issued by the first warp
-        // with all four arrivals.
+        // the products, and leave them one stage each. Operands in f16 go to their
+        // stage by TMA, issued by the first warp. Each of the four warps waits for the
+        // stage and arrives on it, whatever the tile's type: so none can fall a phase
+        // of `empty` behind or get one ahead (its parity would then name another
+        // phase), and none still reads a tile's entry when that is written anew.
         const uint32_t tid = threadIdx.x & 127, wq = (warp - 4 - 4 * NS) & 3, v = (warp - 4 - 4 * NS) >> 2;
         const uint32_t key = tid % BN, half = tid / BN;  // half: 0 unless the head size is 256
         uint32_t nr = 0;                                 // raw tiles so far
@@ -908,21 +911,23 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
             if (round && !wait(empty(st), (round - 1) & 1u)) return;
             const uint32_t stage = ring + st * C::stage;
             if (type == KVMRET_TYPE_F16) {
-                if (wq != 0) return;
+                if (wq != 0) {
+                    __syncwarp();  // every lane has read the tile's entry
+                    if (lane == 0) mbar_arrive(full(st));
+                    return;
+                }
                 const uint32_t T = pv.page_tokens, box = min(T, static_cast<uint32_t>(BN));
                 const int32_t id = lane < 8 ? ti.page[lane] : -1;
+                const int32_t h = static_cast<int32_t>(ti.h), off = static_cast<int32_t>(ti.off);
+                const CUtensorMap *const map = &l.map[2 * ti.kind + v];
                 const uint32_t n = __popc(__ballot_sync(0xffffffffu, id >= 0));
-                if (lane == 0) {
-                    for (int i = 0; i < 3; ++i) mbar_arrive(full(st));
-                    mbar_expect_tx(full(st), n * box * D * 2);
-                }
+                if (lane == 0) mbar_expect_tx(full(st), n * box * D * 2);
                 __syncwarp();
                 if (id >= 0)
 #pragma unroll
                     for (uint32_t b = 0; b < D / 64; ++b)
-                        tma_load_4d(stage + b * KB + lane * T * 128, &l.map[2 * ti.kind + v],
-                                    static_cast<int32_t>(64 * b), static_cast<int32_t>(ti.h),
-                                    static_cast<int32_t>(ti.off), id, full(st));
+                        tma_load_4d(stage + b * KB + lane * T * 128, map, static_cast<int32_t>(64 * b), h, off,
+                                    id, full(st));
                 flight = j + 1;
                 return;
             }

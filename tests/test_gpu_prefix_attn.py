@@ -626,3 +626,59 @@ def test_many_sequences():
                                       dev(np.array([n_pre], np.int32)) if n_pre else None, tpool.device(),
                                       dev(own), dev(tl.astype(np.int32)), dev(start), lse=True)
         check(got, lse, reference(q.astype(np.float64), hkv, d ** -0.5, pre, tails, start, (F16, F16)))
+
+
+def check_rows(got, lse, q, spans, hkv, quant_k, quant_v):
+    """Rows against a float64 softmax on the GPU: spans of (first row, end, k, v), the
+    keys [tokens][hkv][d] that the span's last row sees, one fewer the row before."""
+    scale, g = q.shape[-1] ** -0.5, q.shape[1] // hkv
+    qd = q.double()
+    for a, b, k, v in spans:
+        hide = torch.arange(k.shape[0], device="cuda") >= \
+            (k.shape[0] - (b - a) + 1 + torch.arange(b - a, device="cuda"))[:, None]
+        for h in range(hkv):
+            x, kh, vh = qd[a:b, h * g:(h + 1) * g].transpose(0, 1), k[:, h], v[:, h]  # [g][rows][d]
+            w = (x @ kh.T * scale).masked_fill(hide, -math.inf)
+            mag = (x.abs() @ kh.abs().T * scale).masked_fill(hide, 0)
+            ds = ((2e-6 + (2.0 ** -11 if quant_k else 0)) * mag + 2.0 ** -22 *
+                  w.masked_fill(hide, 0).abs()).amax(-1)
+            wl = torch.logsumexp(w, -1)
+            p = torch.exp(w - wl[..., None])
+            want, mass = p @ vh, p @ vh.abs()
+            small = 2.0 ** -25 * vh.abs().sum(0) * torch.exp(w.amax(-1) - wl)[..., None]
+            tol = (2 * ds[..., None] + 2.0 ** -11 + 1e-5 + (2.0 ** -11 if quant_v else 0)) * mass + \
+                small + 2.0 ** -11 * want.abs() + 2.0 ** -25
+            err = (got[a:b, h * g:(h + 1) * g].transpose(0, 1).double() - want).abs()
+            assert bool((err <= tol).all()), (a, h, float((err - tol).max()))
+            el = (lse[a:b, h * g:(h + 1) * g].T.double() - wl).abs()
+            assert bool((el <= ds + 2e-6 * (1 + wl.abs())).all()), (a, h)
+
+
+@pytest.mark.parametrize("d,pre_kinds,tail_kinds", [
+    (256, (Q8, F16), (Q8, F16)), (256, (F16, Q8), (Q4, F16)), (128, (Q8, F16), (F16, Q4)),
+    (128, (F16, Q4), (F16, F16)), (64, (F16, Q8), (Q8, F16)), (64, (Q4, F16), (Q4, F16)),
+])
+def test_long_lists_with_one_operand_in_f16(d, pre_kinds, tail_kinds):
+    """Tiles whose K or V is copied, by the dozen to a CTA, the copied operand changing
+    on the way: every ring of the conversion goes round often. Again and again, with
+    the same bits."""
+    rng = np.random.default_rng(d + 1)
+    n, hkv, g, n_pre = 40, 4, 8, 12000
+    tl = rng.integers(500, 900, n)
+    pool = Pool(rng, -(-n_pre // 128), 128, hkv, d, *pre_kinds)
+    width = -(-int(tl.max()) // 64)
+    tpool = Pool(rng, n * width, 64, hkv, d, *tail_kinds)
+    table = rng.permutation(-(-n_pre // 128)).astype(np.int32)
+    own = rng.permutation(n * width).reshape(n, width).astype(np.int32)
+    pre = [dev(x) for x in pool.fill(table, n_pre)]
+    tails = [[dev(x) for x in tpool.fill(own[s], int(t))] for s, t in enumerate(tl)]
+    q = dev((rng.standard_normal((n, hkv * g, d)) * 1.5).astype(np.float16))
+    args = (q, pool.device(), dev(np.array([n_pre], np.int32)), tpool.device(), dev(own),
+            dev(tl.astype(np.int32)), dev(np.arange(n + 1, dtype=np.int32)))
+    t = dev(table)
+    got, lse = kvmret.prefix_attn(*args, prefix_table=t, lse=True)
+    spans = [(s, s + 1, torch.cat([pre[0], tails[s][0]]), torch.cat([pre[1], tails[s][1]]))
+             for s in range(n)]
+    check_rows(got, lse, q, spans, hkv, True, True)
+    for _ in range(20):
+        assert torch.equal(kvmret.prefix_attn(*args, prefix_table=t), got)
