@@ -1006,14 +1006,19 @@ def _launch(index, stream, fn, *args):
         _check(rc)
 
 
-def _used_on(stream, index, *tensors):
-    """Tensors made here are used on the caller's stream: torch must not hand
-    their memory on before that stream has passed."""
+def _on_stream(stream, index, call):
+    """call() with the caller's stream current, so that what it allocates comes from
+    that stream's memory: memory freed on torch's current stream may still be in use
+    there. The results may be used on either stream."""
     import torch
-    ext = torch.cuda.ExternalStream(stream, device=index)
-    for x in tensors:
+    ours, theirs = torch.cuda.current_stream(index), torch.cuda.ExternalStream(stream, device=index)
+    with torch.cuda.stream(theirs):
+        got = call()
+    for x in got if isinstance(got, tuple) else (got,):
         if x is not None:
-            x.record_stream(ext)
+            x.record_stream(ours)
+            x.record_stream(theirs)  # (an `out` of the caller's)
+    return got
 
 
 def _head_rows(x, name):
@@ -1056,6 +1061,10 @@ def qk_norm_rope(q, k, pos, q_weight=None, k_weight=None, eps=1e-6, freq_base=1e
     normed row without the rotation (query_add rows, append's k_cap)."""
     import torch
     empty, like, f16, index = torch.empty_strided, torch.empty_like, torch.float16, q.get_device()
+    if stream and index >= 0:
+        return _on_stream(stream, index, lambda: qk_norm_rope(
+            q, k, pos, q_weight, k_weight, eps, freq_base, freq_scale, fwht_n, q_rot, k_rot, q_raw,
+            k_raw))
     kind = q.dtype
     t = (TYPE_F16 if kind is f16 else TYPE_BF16 if kind is torch.bfloat16 else
          TYPE_F32 if kind is torch.float32 else None)
@@ -1079,9 +1088,7 @@ def qk_norm_rope(q, k, pos, q_weight=None, k_weight=None, eps=1e-6, freq_base=1e
                  o0.data_ptr() if q_rot else 0, o1.data_ptr() if k_rot else 0,
                  o2.data_ptr() if q_raw else 0, o3.data_ptr() if k_raw else 0,
                  n, hq, hkv, d, d, fwht_n, t, eps, freq_base, freq_scale)
-    _launch(index, stream, _qk_call, a)
-    if stream:
-        _used_on(stream, index, o0, o1, o2, o3)
+    _launch(index, 0, _qk_call, a)
     return o0, o1, o2, o3
 
 
@@ -1189,6 +1196,10 @@ def prefix_attn(q, prefix, prefix_len, tail=None, tail_table=None, tail_len=None
     pages = prefix if prefix is not None else tail
     _want(pages is not None, "a prefix or tails")
     index = pages.index
+    if stream:
+        return _on_stream(stream, index, lambda: prefix_attn(
+            q, prefix, prefix_len, tail, tail_table, tail_len, q_start, prefix_table, prefix_ntok,
+            max_prefix, scale, lse, out))
     front, tails, got, shape = _attn_args(q, index, pages.d_head, tail, tail_table, tail_len, q_start,
                                           scale, lse, out)
     most = length = table = ntok = 0
@@ -1207,9 +1218,7 @@ def prefix_attn(q, prefix, prefix_len, tail=None, tail_table=None, tail_len=None
         if prefix_len is not None:
             length = _index(prefix_len, 1, index, "prefix_len")
     ws, nb = _attn_ws(shape, pages.n_head_kv, tails[0], q.device)
-    _launch(index, stream, _attn_call, None if prefix is None else prefix.ref,
+    _launch(index, 0, _attn_call, None if prefix is None else prefix.ref,
             None if tail is None else tail.ref,
             _ATTN.pack(*front, most, length, table, ntok, *tails), ws.data_ptr(), nb)
-    if stream:
-        _used_on(stream, index, ws, *(got if lse else (got,)))
     return got

@@ -682,3 +682,31 @@ def test_long_lists_with_one_operand_in_f16(d, pre_kinds, tail_kinds):
     check_rows(got, lse, q, spans, hkv, True, True)
     for _ in range(20):
         assert torch.equal(kvmret.prefix_attn(*args, prefix_table=t), got)
+
+
+def test_a_given_stream_takes_no_memory_still_in_use():
+    """With a stream given by its handle, outputs and workspace come from that stream's
+    memory: what was freed on the current stream may have work before it there."""
+    case = ([1] * 6, [30] * 6, 900, 8, 2, 128, 64, 32, F16, F16)
+    pool, tpool, table, own, _, _, start, q, tl = build(case)
+    args = (dev(q), pool.device(), dev(np.array([900], np.int32)), tpool.device(), dev(own), dev(tl),
+            dev(start))
+    t, pos = dev(table), torch.arange(6, device="cuda", dtype=torch.int32)
+    want = kvmret.prefix_attn(*args, prefix_table=t)
+    want_qk = kvmret.qk_norm_rope(args[0], args[0][:, :2], pos)
+    side = torch.cuda.Stream()
+    sizes = (want.numel() * 2, int(kvmret.lib.kvmret_prefix_attn_ws_bytes(6, 8, 2, 128, 6)),
+             want_qk[1].numel() * 2)
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    torch.cuda._sleep(200_000_000)  # the current stream is busy for a tenth of a second
+    freed = [torch.full((n,), 255, dtype=torch.uint8, device="cuda") for n in sizes for _ in range(4)]
+    spans = [(x.data_ptr(), x.numel()) for x in freed]
+    del freed
+    got = kvmret.prefix_attn(*args, prefix_table=t, stream=side.cuda_stream)
+    got_qk = kvmret.qk_norm_rope(args[0], args[0][:, :2], pos, stream=side.cuda_stream)
+    for x in (got, got_qk[0], got_qk[1]):
+        assert all(x.data_ptr() + x.numel() * 2 <= a or x.data_ptr() >= a + n for a, n in spans)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+    assert torch.equal(got_qk[0], want_qk[0]) and torch.equal(got_qk[1], want_qk[1])
