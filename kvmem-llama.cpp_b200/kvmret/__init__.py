@@ -923,6 +923,8 @@ def gemm_f16_nt(a, b, alpha=1.0, stream=0):
     """C = alpha * a @ b.T on the tensor cores; a [m][k], b [n][k] f16 CUDA tensors
     (m % 128 == 0, n % 16 == 0, k % 64 == 0). Returns (C f32 CUDA tensor, error flag)."""
     import torch
+    if stream:
+        return _on_stream(stream, a.get_device(), lambda: gemm_f16_nt(a, b, alpha))
     m, k = a.shape
     n = b.shape[0]
     c = torch.empty((m, n), dtype=torch.float32, device=a.device)
@@ -936,6 +938,8 @@ def gemm_f16_nt_split(a, b, alpha=1.0, stream=0):
     """gemm_f16_nt through the workspace form (one CTA per SM when the tiles
     would leave SMs idle: lockstep main CTAs plus helpers on the k tails)."""
     import torch
+    if stream:
+        return _on_stream(stream, a.get_device(), lambda: gemm_f16_nt_split(a, b, alpha))
     m, k = a.shape
     n = b.shape[0]
     c = torch.empty((m, n), dtype=torch.float32, device=a.device)

@@ -137,3 +137,25 @@ def test_prefill_top_k_above_block_count_selects_all():
     sel, n_sel, _ = r.prefill_score(torch.from_numpy(q).cuda(), 64)
     assert n_sel == w.n_blocks and sel.all()
     r.close()
+
+
+@pytest.mark.parametrize("fn", [kvmret.gemm_f16_nt, kvmret.gemm_f16_nt_split])
+def test_gemm_on_a_given_stream_takes_no_memory_still_in_use(fn):
+    """C, the error words and the workspace come from the given stream's memory."""
+    g = torch.Generator(device="cuda").manual_seed(2)
+    a = torch.randn(256, 1024, device="cuda", generator=g).half()
+    b = torch.randn(512, 1024, device="cuda", generator=g).half()
+    want, _ = fn(a, b)
+    side = torch.cuda.Stream()
+    sizes = (want.numel() * 4, 16, max(1, int(kvmret.lib.kvmret_gemm_ws_bytes(256, 512, 1024))))
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    torch.cuda._sleep(200_000_000)
+    freed = [torch.full((n,), 255, dtype=torch.uint8, device="cuda") for n in sizes]
+    spans = [(x.data_ptr(), x.numel()) for x in freed]
+    del freed
+    c, err = fn(a, b, stream=side.cuda_stream)
+    for x in (c, err):
+        assert all(x.data_ptr() + x.numel() * 4 <= p or x.data_ptr() >= p + n for p, n in spans)
+    torch.cuda.synchronize()
+    assert torch.equal(c, want) and int(err[0]) == 0
