@@ -641,11 +641,14 @@ typedef struct kvmret_attn {
     float *lse_dev;                  /* [n_q][n_head] log of the sum (natural), NULL: not wanted */
     uint32_t n_q, n_head;
     float scale;                     /* of the scores, e.g. 1 / sqrt(d_head) */
-    uint32_t max_prefix;             /* bound on the prefix's tokens; 0: no prefix */
+    uint32_t max_prefix;             /* bound on the prefix's tokens; its first
+                                        ceil(max_prefix / page_tokens) pages are listed; 0: no prefix */
     const int32_t *prefix_len_dev;   /* its tokens (one word), NULL: max_prefix */
     const int32_t *prefix_table_dev; /* its pages in order, NULL: pages 0, 1, 2, ... */
     const uint32_t *prefix_ntok_dev; /* tokens held by each listed page (a window's slots may
-                                        be partly filled), NULL: full pages */
+                                        be partly filled), NULL: full pages. The prefix is then
+                                        these tokens one after another, and its length counts
+                                        them; max_prefix still says how many pages are listed */
     uint32_t n_seq, tail_pages;      /* tail_pages: row length of tail_table */
     const int32_t *q_start_dev;      /* [n_seq + 1], ascending */
     const int32_t *tail_table_dev;   /* [n_seq][tail_pages] */

@@ -324,7 +324,7 @@ __device__ bool make_plan(const AttnLaunch &l, Plan &p, Start &start) {
     const int32_t len0 = pre && a.prefix.len ? __ldg(a.prefix.len) : 0x7fffffff;
     const int32_t q_first = a.n_seq ? __ldg(a.q_start) : 0;
     const int32_t q_last = a.n_seq ? __ldg(a.q_start + a.n_seq) : static_cast<int32_t>(a.n_q);
-    // totals of the tails; the last listed page that holds tokens
+    // totals of the tails
     uint32_t t0, n0;
     shape(lane, t0, n0);
     uint32_t tiles = t0, pairs = n0;
@@ -336,24 +336,55 @@ __device__ bool make_plan(const AttnLaunch &l, Plan &p, Start &start) {
         pairs += n;
     }
     ok = __all_sync(0xffffffffu, ok);
-    uint32_t held = pre ? a.prefix.n_list : 0;
-    if (held && a.prefix.ntok) {
+    // the last listed page with tokens, and how many the pages hold
+    uint32_t held = pre ? a.prefix.n_list : 0, all = 0;
+    const uint32_t T = a.prefix.pages.page_tokens;
+    const bool partial = held && a.prefix.ntok;
+    auto page_holds = [&](uint32_t i) {
+        const uint32_t n = min(__ldg(a.prefix.ntok + i), T);
+        return !a.prefix.table || static_cast<uint32_t>(__ldg(a.prefix.table + i)) < a.prefix.pages.n_pages ? n : 0;
+    };
+    if (partial) {
         held = 0;
 #pragma unroll 8
-        for (uint32_t i = lane; i < a.prefix.n_list; i += 32)
-            if (__ldg(a.prefix.ntok + i)) held = i + 1;
+        for (uint32_t i = lane; i < a.prefix.n_list; i += 32) {
+            const uint32_t n = page_holds(i);
+            if (n) held = i + 1;
+            all += n;
+        }
     }
     for (int o = 16; o; o >>= 1) {
         tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
         pairs += __shfl_xor_sync(0xffffffffu, pairs, o);
         held = max(held, __shfl_xor_sync(0xffffffffu, held, o));
+        all += __shfl_xor_sync(0xffffffffu, all, o);
     }
     p.p_len = 0;
     p.np = 0;
     if (pre) {
-        const uint64_t most = static_cast<uint64_t>(held) * a.prefix.pages.page_tokens;
+        // p_len is a place of the list (page * T + offset): that behind the last token
+        const uint64_t most = static_cast<uint64_t>(held) * T;
         const uint32_t len = min(a.prefix.max_len, static_cast<uint32_t>(max(len0, 0)));
-        p.p_len = most < len ? static_cast<uint32_t>(most) : len;
+        if (!partial) {
+            p.p_len = most < len ? static_cast<uint32_t>(most) : len;
+        } else if (len >= all) {
+            p.p_len = static_cast<uint32_t>(most);
+        } else if (len) {  // the page that holds token len - 1
+            uint32_t before = 0;
+            for (uint32_t i0 = 0; i0 < a.prefix.n_list; i0 += 32) {
+                const uint32_t n = i0 + lane < a.prefix.n_list ? page_holds(i0 + lane) : 0;
+                uint32_t upto = n, unused = 0;
+                scan(upto, unused);
+                const uint32_t sum = __shfl_sync(0xffffffffu, upto, 31);
+                const uint32_t hit = __ballot_sync(0xffffffffu, before + upto >= len);
+                if (hit) {
+                    const int w = __ffs(hit) - 1;
+                    p.p_len = (i0 + w) * T + len - (before + __shfl_sync(0xffffffffu, upto - n, w));
+                    break;
+                }
+                before += sum;
+            }
+        }
         p.np = TileGeom<BN>(l.by.list[0]).tiles(p.p_len);
     }
     const int32_t nq = static_cast<int32_t>(a.n_q);

@@ -14,7 +14,7 @@ struct KeyList {
     PageView pages;
     const int32_t *table;    // page ids; null: 0, 1, 2, ...
     const uint32_t *ntok;    // tokens held by each listed page; null: full
-    const int32_t *len;      // tokens (device); null: max_len
+    const int32_t *len;      // tokens (device; with ntok: of those that the pages hold); null: max_len
     uint32_t max_len;        // bound on the tokens (0: no such keys)
     uint32_t n_list;         // pages of one list
 };

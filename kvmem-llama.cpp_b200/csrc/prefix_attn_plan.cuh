@@ -110,7 +110,7 @@ struct Plan {
     uint32_t p_total, t_total;  // tiles of the prefix line and of the tails
     Cuts pre, own;              // their ranges (gs == 1: of the joint line)
     uint32_t np;                // tiles of the prefix
-    uint32_t p_len;             // its tokens
+    uint32_t p_len;             // its tokens (with partly filled pages: the place behind the last)
     uint32_t q0, rows;          // first row token; rows of a KV head (all sequences)
     uint32_t n_pair, n_pg, gs, groups;
     uint32_t t_slot0;           // first workspace slot of the tails

@@ -1193,10 +1193,12 @@ def prefix_attn(q, prefix, prefix_len, tail=None, tail_table=None, tail_len=None
     sequence's own tail (Pages with tail_table [n_seq][pages] and tail_len
     [n_seq] int32; sequence s has rows q_start[s] .. q_start[s + 1] - 1, the
     last tokens of its tail). prefix_table: the prefix's pages in order;
-    prefix_ntok: the tokens that each of them holds; max_prefix: a bound on
-    the prefix (default: what its pages hold). Either part may be None.
+    prefix_ntok: the tokens that each of them holds (the prefix is these one
+    after another, and prefix_len and max_prefix count them); max_prefix: a
+    bound on the prefix (default: what its pages hold). Either part may be None.
     scale defaults to d_head ** -0.5. Returns out (rows of no sequence: as
     they were), with lse=True also the f32 [n_q][n_head] log-sum-exp."""
+    import torch
     pages = prefix if prefix is not None else tail
     _want(pages is not None, "a prefix or tails")
     index = pages.index
@@ -1221,6 +1223,10 @@ def prefix_attn(q, prefix, prefix_len, tail=None, tail_table=None, tail_len=None
             raise KvmretError(f"max_prefix: at most the {held} tokens of the pages")
         if prefix_len is not None:
             length = _index(prefix_len, 1, index, "prefix_len")
+        if ntok and most < held:  # tokens, which may lie in any of the pages
+            cut = (torch.full((1,), most, dtype=torch.int32, device=q.device) if prefix_len is None
+                   else prefix_len.clamp(max=most))
+            most, length = held, cut.data_ptr()
     ws, nb = _attn_ws(shape, pages.n_head_kv, tails[0], q.device)
     _launch(index, 0, _attn_call, None if prefix is None else prefix.ref,
             None if tail is None else tail.ref,

@@ -710,3 +710,39 @@ def test_a_given_stream_takes_no_memory_still_in_use():
     torch.cuda.synchronize()
     assert torch.equal(got, want)
     assert torch.equal(got_qk[0], want_qk[0]) and torch.equal(got_qk[1], want_qk[1])
+
+
+@pytest.mark.parametrize("absent", [False, True])
+def test_length_counts_the_tokens_of_partly_filled_pages(absent):
+    """prefix_len and max_prefix with prefix_ntok: the first tokens that the pages
+    hold, wherever a page ends; pages without tokens, and page ids outside the pool,
+    hold none. More pages than the split looks at in one go."""
+    rng = np.random.default_rng(21)
+    hq, hkv, d, page, n = 4, 2, 128, 32, 45
+    pool = Pool(rng, n, page, hkv, d, F16, F16)
+    table = rng.permutation(n).astype(np.int32)
+    ntok = rng.integers(0, page + 1, n).astype(np.uint32)
+    ntok[:2], ntok[7], ntok[40] = (5, page), 0, page + 9  # (what is past a page does not count)
+    there = np.minimum(ntok, page).astype(np.int32)
+    pre = pool.fill(table, n * page, there)
+    if absent:  # the filled values of these pages are no longer listed
+        keep = np.ones(n, bool)
+        keep[[3, 33]] = False
+        lost = np.repeat(~keep, there)
+        pre = [x[~lost] for x in pre]
+        table[3], table[33], there = -1, n, there * keep
+    total = int(there.sum())
+    q = rng.standard_normal((3, hq, d)).astype(np.float16)
+    pages, qd, t, nt = pool.device(), dev(q), dev(table), dev(ntok.view(np.int32))
+    length = torch.zeros(1, dtype=torch.int32, device="cuda")
+    edges = np.cumsum(there)
+    for m in sorted({0, 1, 4, 5, 6, 36, 37, 38, int(edges[2]), int(edges[2]) + 1, int(edges[31]),
+                     int(edges[31]) + 1, int(edges[40]) - 1, total - 1, total, total + 1, n * page}):
+        want = reference(q.astype(np.float64), hkv, d ** -0.5, [x[:m] for x in pre], None, None,
+                         (F16, F16))
+        length.fill_(m)
+        check(*kvmret.prefix_attn(qd, pages, length, prefix_table=t, prefix_ntok=nt, lse=True), want)
+        if m:
+            for longest in (None, torch.full_like(length, m + 3)):
+                check(*kvmret.prefix_attn(qd, pages, longest, prefix_table=t, prefix_ntok=nt,
+                                          max_prefix=m, lse=True), want)
