@@ -1099,15 +1099,18 @@ def qk_norm_rope(q, k, pos, q_weight=None, k_weight=None, eps=1e-6, freq_base=1e
 class Pages:
     """A paged cache of one layer: k and v are CUDA tensors whose first axis is
     the page and whose other axes hold page_tokens rows of n_head_kv * d_head
-    elements of k_type / v_type (f16 values, or the bytes of q8_0 / q4_0
-    blocks); the page axis may be strided. Cell c is token c % page_tokens of
+    elements of k_type / v_type (float16 values, or uint8 or int8 bytes of any
+    type's rows); the page axis may be strided. Cell c is token c % page_tokens of
     page c // page_tokens."""
 
     def __init__(self, k, v, page_tokens, n_head_kv, d_head, k_type=TYPE_F16, v_type=TYPE_F16):
         _want(k.is_cuda and v.device == k.device and k.shape[0] == v.shape[0],
               "pages: k and v CUDA tensors of one device, with one first axis")
+        import torch
         strides = []
         for x, t in ((k, k_type), (v, v_type)):
+            _want(x.dtype in (torch.uint8, torch.int8) or (t == TYPE_F16 and x.dtype is torch.float16),
+                  "pages: float16 values of TYPE_F16, or bytes of any type")
             _want(x.shape[0] > 0 and x[0].is_contiguous() and x[0].numel() * x.element_size() ==
                   page_tokens * row_bytes(t, n_head_kv * d_head),
                   "pages: a page must be page_tokens contiguous rows of its type")

@@ -128,3 +128,36 @@ def test_window_attn_refuses_no_context():
 def test_ws_bytes_of_bad_shapes():
     for shape in ((1, 3, 2, 128, 1), (1, 4, 0, 128, 1), (1, 4, 2, 96, 1), (70000, 4, 2, 128, 1)):
         assert lib.kvmret_prefix_attn_ws_bytes(*shape) == 0
+
+
+class _Rows:
+    """What Pages asks of a tensor, on the CPU: a CUDA tensor of zeros would do."""
+
+    def __init__(self, x):
+        self.x, self.is_cuda, self.device, self.dtype = x, True, "cuda:0", x.dtype
+        self.shape, self.stride, self.element_size = x.shape, x.stride, x.element_size
+        self.data_ptr, self.get_device = x.data_ptr, lambda: 0
+
+    def __getitem__(self, i):
+        return self.x[i]
+
+
+@pytest.mark.parametrize("dtype,kind,good", [
+    ("float16", kvmret.TYPE_F16, True), ("uint8", kvmret.TYPE_F16, True), ("int8", kvmret.TYPE_Q8_0, True),
+    ("uint8", kvmret.TYPE_Q4_0, True), ("bfloat16", kvmret.TYPE_F16, False),
+    ("int16", kvmret.TYPE_F16, False), ("float32", kvmret.TYPE_F16, False),
+    ("float16", kvmret.TYPE_Q8_0, False), ("int16", kvmret.TYPE_Q4_0, False),
+])
+def test_pages_refuse_other_element_types(dtype, kind, good):
+    """A cache of another type with as many bytes would be read as this one's."""
+    import torch
+    dt = getattr(torch, dtype)
+    bytes_ = 16 * kvmret.row_bytes(kind, 256)
+    x = _Rows(torch.zeros(2, bytes_ // dt.itemsize, dtype=dt))
+    f = _Rows(torch.zeros(2, 16, 2, 128, dtype=torch.float16))
+    for k, v, types in ((x, f, (kind, kvmret.TYPE_F16)), (f, x, (kvmret.TYPE_F16, kind))):
+        if good:
+            assert kvmret.Pages(k, v, 16, 2, 128, *types).n_pages == 2
+        else:
+            with pytest.raises(kvmret.KvmretError, match="float16"):
+                kvmret.Pages(k, v, 16, 2, 128, *types)
