@@ -667,9 +667,12 @@ typedef struct kvmret_attn {
  * descends, or a wait within the kernel that gives up (after about two seconds),
  * leaves NaN in every row from q_start[0] to q_start[n_seq] - 1. ws_dev: 256-byte aligned workspace
  * of kvmret_prefix_attn_ws_bytes, written and read by this call alone (calls that
- * may overlap, graphs included, need one each). n_q <= 65535, n_head <= 65535,
- * n_q * n_head <= 2^31 - 1, and rows times key tiles, counted at 16 tokens a
- * tile from the bounds, stay below 2^32 (refused otherwise). */
+ * may overlap, graphs included, need one each). It grows with the rows: f32 partial
+ * outputs of about 2.2 n_q * n_head * d_head, and of up to 640 * 128 * d_head more
+ * for lists that several SMs share (64 heads of 128: 1.5 MB for one row, 23 MB for
+ * 16, 0.11 GB for 1024). n_q <= 65535, n_head <= 65535, n_q * n_head <= 2^31 - 1, and
+ * rows times key tiles, counted at 16 tokens a tile from the bounds, as well as the
+ * workspace's rows stay below 2^32 (refused otherwise). */
 size_t kvmret_prefix_attn_ws_bytes(uint32_t n_q, uint32_t n_head, uint32_t n_head_kv,
                                    uint32_t d_head, uint32_t n_seq);
 int kvmret_prefix_attn(const kvmret_pages *prefix, const kvmret_pages *tail, const kvmret_attn *a,

@@ -152,6 +152,8 @@ int prefix_attn_call(const KeyList &prefix, const kvmret_pages *tail, const kvmr
     r.n_seq = a->n_seq;
     r.q_start = a->q_start_dev;
     const size_t need = prefix_attn_ws_bytes(a->n_q, a->n_head, pv.n_head_kv, pv.d_head, a->n_seq);
+    if (need / (4ull * pv.d_head) > 0xffffffffull)  // its rows are counted in 32 bits
+        return fail(KVMRET_ERR_ARG, "%u rows of %u heads are too many for one workspace", a->n_q, a->n_head);
     if (need && (!ws || ws_bytes < need || (reinterpret_cast<uintptr_t>(ws) & 255)))
         return fail(KVMRET_ERR_ARG, "workspace of %zu bytes at 256-byte alignment, %zu needed",
                     ws_bytes, need);

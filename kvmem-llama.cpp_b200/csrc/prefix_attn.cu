@@ -119,20 +119,27 @@ constexpr uint32_t kAttnTmem = 512;
 constexpr int kSegs = 4;  // pieces ahead
 constexpr int kMeta = 16;  // tiles whose masks are held (more than the ring reaches back)
 
-// Where one row's pieces lie: entry i of n has its statistics at ml[id + i *
-// step], its output in the same slot and row.
+// Where one row's pieces lie among the workspace's rows: the first at row id, the
+// i-th of n at rest + i * step.
 struct RowPieces {
-    uint32_t id, step, n, pad;
+    uint32_t id, rest, step, n;
+    __device__ __forceinline__ uint32_t at(uint32_t i) const { return i ? rest + i * step : id; }
 };
+// A row's output in the workspace: rows by eights, so that both a warp with a row
+// a lane and the join with eight rows of one column move whole 128-byte lines.
+template <int D>
+__device__ __forceinline__ uint64_t out_at(uint32_t id, uint32_t col) {
+    return static_cast<uint64_t>(id >> 3) * (D / 4 * 8) + col * 8 + (id & 7);
+}
 
 struct AttnLaunch {
     PrefixAttn a;
     CUtensorMap map[4];  // prefix K, V, tail K, V
     uint32_t *fail;  // [CTA] 1: a wait gave up, or q_start was not ascending
     RowPieces *at;   // [n_q * n_head][2] pieces of the prefix, of the tail
-    float2 *ml;      // [slot][row tile][128] maximum and sum
-    float4 *o;       // [slot][row tile][D / 4][128]
-    uint32_t max_slots;
+    float2 *ml;      // [row] maximum and sum
+    float4 *o;       // [row / 8][D / 4][8]
+    Rooms rooms;
     uint32_t raw_k, raw_v, n_raw_v;  // bytes of a raw K, V tile; raw V tiles
     Divs by;
 };
@@ -289,18 +296,16 @@ __device__ __forceinline__ void convert_row(uint32_t src, uint32_t first, Put pu
 // The plan of the split, by one warp, in every CTA alike. `start` receives the
 // sequence that holds the CTA's first tail tile. False when q_start descends.
 struct Start {
-    uint32_t seq, pair, tile;
+    uint32_t seq, tile;
 };
 // inclusive sums over the warp's lanes
-__device__ __forceinline__ void scan(uint32_t &x, uint32_t &y) {
+__device__ __forceinline__ uint32_t scan(uint32_t x) {
     const uint32_t lane = threadIdx.x & 31;
     for (uint32_t o = 1; o < 32; o <<= 1) {
-        const uint32_t u = __shfl_up_sync(0xffffffffu, x, o), v = __shfl_up_sync(0xffffffffu, y, o);
-        if (lane >= o) {
-            x += u;
-            y += v;
-        }
+        const uint32_t u = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += u;
     }
+    return x;
 }
 
 template <int D, bool QUANT>
@@ -311,30 +316,21 @@ __device__ bool make_plan(const AttnLaunch &l, Plan &p, Start &start) {
     const uint32_t G = l.by.G.d, H = a.n_head_kv;
     const TileGeom<BN> tg(l.by.list[1]);
     bool ok = true;
-    auto shape = [&](uint32_t s, uint32_t &tiles, uint32_t &pairs) {
-        tiles = pairs = 0;
-        if (s >= a.n_seq) return;
+    auto shape = [&](uint32_t s) -> uint32_t {  // tiles of sequence s
+        if (s >= a.n_seq) return 0;
         ok = ok && __ldg(a.q_start + s) <= __ldg(a.q_start + s + 1);
         const SeqShape sh = seq_shape(a, s);
-        pairs = (sh.q_len * G + PR - 1) / PR;
         const uint32_t n = sh.q_len ? tg.tiles(sh.len) : 0;
-        tiles = (n ? n + kUnit<BN> : 0) * pairs * H;
+        return (n ? n + kUnit<BN> : 0) * ((sh.q_len * G + PR - 1) / PR) * H;
     };
     const bool pre = a.prefix.max_len != 0;
     const int32_t len0 = pre && a.prefix.len ? __ldg(a.prefix.len) : 0x7fffffff;
     const int32_t q_first = a.n_seq ? __ldg(a.q_start) : 0;
     const int32_t q_last = a.n_seq ? __ldg(a.q_start + a.n_seq) : static_cast<int32_t>(a.n_q);
     // totals of the tails
-    uint32_t t0, n0;
-    shape(lane, t0, n0);
-    uint32_t tiles = t0, pairs = n0;
+    uint32_t t0 = shape(lane), tiles = t0;
 #pragma unroll 4
-    for (uint32_t s = 32 + lane; s < a.n_seq; s += 32) {
-        uint32_t t, n;
-        shape(s, t, n);
-        tiles += t;
-        pairs += n;
-    }
+    for (uint32_t s = 32 + lane; s < a.n_seq; s += 32) tiles += shape(s);
     ok = __all_sync(0xffffffffu, ok);
     // the last listed page with tokens, and how many the pages hold
     uint32_t held = pre ? a.prefix.n_list : 0, all = 0;
@@ -355,7 +351,6 @@ __device__ bool make_plan(const AttnLaunch &l, Plan &p, Start &start) {
     }
     for (int o = 16; o; o >>= 1) {
         tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
-        pairs += __shfl_xor_sync(0xffffffffu, pairs, o);
         held = max(held, __shfl_xor_sync(0xffffffffu, held, o));
         all += __shfl_xor_sync(0xffffffffu, all, o);
     }
@@ -373,8 +368,7 @@ __device__ bool make_plan(const AttnLaunch &l, Plan &p, Start &start) {
             uint32_t before = 0;
             for (uint32_t i0 = 0; i0 < a.prefix.n_list; i0 += 32) {
                 const uint32_t n = i0 + lane < a.prefix.n_list ? page_holds(i0 + lane) : 0;
-                uint32_t upto = n, unused = 0;
-                scan(upto, unused);
+                const uint32_t upto = scan(n);
                 const uint32_t sum = __shfl_sync(0xffffffffu, upto, 31);
                 const uint32_t hit = __ballot_sync(0xffffffffu, before + upto >= len);
                 if (hit) {
@@ -401,8 +395,7 @@ __device__ bool make_plan(const AttnLaunch &l, Plan &p, Start &start) {
     p.groups = p.gs == 1 ? gridDim.x : gridDim.x / p.gs;
     p.p_total = p.np * p.n_pg * H;
     p.t_total = tiles;
-    p.t_slot0 = (p.n_pg * H + p.groups) * p.gs;
-    ok = ok && p.t_slot0 + pairs * H + gridDim.x <= l.max_slots;  // (so it is when it ascends)
+    ok = ok && (p.n_pg * H + p.groups) * p.gs <= l.rooms.n_pre;  // (so it always is)
     p.ok = ok;
     if (!ok) p.p_total = p.t_total = 0;
     if (p.gs == 1) {
@@ -412,28 +405,24 @@ __device__ bool make_plan(const AttnLaunch &l, Plan &p, Start &start) {
         p.pre.set(p.p_total, p.groups);
         p.own.set(p.t_total, l.by.ctas);
     }
-    start = {0, 0, 0};
+    start = {0, 0};
     uint32_t x, x1, y, y1;
     Walk<BN, PR>::ranges(p, blockIdx.x, x, x1, y, y1);
     if (y >= y1) return ok;  // no tails here
-    uint32_t base_t = 0, base_p = 0;
+    uint32_t base_t = 0;
     for (uint32_t s0 = 0; s0 < a.n_seq; s0 += 32) {
-        if (s0) shape(s0 + lane, t0, n0);
-        uint32_t ti = t0, pi = n0;
-        scan(ti, pi);
-        const uint32_t all_t = __shfl_sync(0xffffffffu, ti, 31), all_p = __shfl_sync(0xffffffffu, pi, 31);
+        if (s0) t0 = shape(s0 + lane);
+        uint32_t ti = scan(t0);
+        const uint32_t all_t = __shfl_sync(0xffffffffu, ti, 31);
         ti += base_t - t0;
-        pi += base_p - n0;
         const uint32_t hit = __ballot_sync(0xffffffffu, y >= ti && y < ti + t0);
         if (hit) {
             const int w = __ffs(hit) - 1;
             start.seq = s0 + w;
-            start.pair = __shfl_sync(0xffffffffu, pi, w);
             start.tile = __shfl_sync(0xffffffffu, ti, w);
             break;
         }
         base_t += all_t;
-        base_p += all_p;
     }
     return ok;
 }
@@ -442,12 +431,13 @@ __device__ bool make_plan(const AttnLaunch &l, Plan &p, Start &start) {
 // lane a row, the CTAs taking blocks of 32 rows in turn.
 template <int D, bool QUANT>
 __device__ void note_rows(const AttnLaunch &l, const Plan &p) {
-    constexpr int BN = Cfg<D, QUANT>::BN, PR = Cfg<D, QUANT>::PR, NS = Cfg<D, QUANT>::NS;
+    constexpr int BN = Cfg<D, QUANT>::BN, PR = Cfg<D, QUANT>::PR;
     const PrefixAttn &a = l.a;
+    const Rooms &rooms = l.rooms;
     const uint32_t lane = threadIdx.x & 31, n_cta = gridDim.x;
     const uint32_t G = l.by.G.d, H = a.n_head_kv;
-    // rows of the tokens [q0, q0 + q_len); tails from tile `tile` and pair `pair` on
-    auto note = [&](uint32_t q0, uint32_t q_len, const SeqShape *sh, uint32_t tile, uint32_t pair0) {
+    // rows of the tokens [q0, q0 + q_len); tails from tile `tile` on
+    auto note = [&](uint32_t q0, uint32_t q_len, const SeqShape *sh, uint32_t tile) {
         const TileGeom<BN> tg(l.by.list[1]);
         const uint32_t tiles = sh ? tg.tiles(sh->len) : 0;
         const uint32_t begin = q0 * a.n_head, end = begin + q_len * a.n_head;
@@ -458,52 +448,54 @@ __device__ void note_rows(const AttnLaunch &l, const Plan &p) {
             if (x < begin || x >= end) continue;
             const uint32_t t = x / a.n_head, head = x - t * a.n_head, h = l.by.G(head), gq = head - h * G;
             RowPieces r[2] = {};
-            auto put = [&](RowPieces &e, const Cuts &cuts, uint32_t x0, uint32_t n, uint32_t slot0,
-                           uint32_t step, uint32_t row) {
+            // the first piece's range; the number of pieces
+            auto cut = [&](RowPieces &e, const Cuts &cuts, uint32_t x0, uint32_t n) {
                 const uint32_t first = cuts.owner(x0);
                 e.n = cuts.owner(x0 + n - 1) + 1 - first;
-                e.id = ((slot0 + first * step) * NS + row % PR / 128) * 128 + row % 128;
-                e.step = step * NS * 128;
+                return first;
             };
             if (p.np) {
                 const uint32_t row = (t - p.q0) * G + gq, pair = row / PR, pg = pair / p.gs, u = pg * H + h;
-                put(r[0], p.pre, u * p.np, p.np, u * p.gs + pair - pg * p.gs, p.gs, row);
+                const uint32_t first = cut(r[0], p.pre, u * p.np, p.np);
+                r[0].step = p.gs * rooms.cap;
+                r[0].id = r[0].rest = ((u + first) * p.gs + pair - pg * p.gs) * rooms.cap + row % PR;
             }
             if (tiles) {
                 const uint32_t row = (t - q0) * G + gq, pair = row / PR, u = pair * H + h;
                 const uint32_t n = min(tiles, pair_tiles<BN, PR>(*sh, tg, pair, l.by.G));
-                if (n)
-                    put(r[1], p.own, (p.gs == 1 ? p.p_total : 0) + tile + u * (tiles + kUnit<BN>) + kUnit<BN>, n,
-                        p.t_slot0 + pair0 * H + u, 1, row);
+                if (n) {
+                    const uint32_t first = cut(r[1], p.own, (p.gs == 1 ? p.p_total : 0) + tile +
+                                               u * (tiles + kUnit<BN>) + kUnit<BN>, n);
+                    r[1].id = rooms.tail + ((q0 - p.q0) * H + h * q_len) * G + row;
+                    r[1].step = rooms.cap;
+                    r[1].rest = rooms.over + first * rooms.cap + row % PR;
+                }
             }
             l.at[2 * x] = r[0];
             l.at[2 * x + 1] = r[1];
         }
     };
     if (!a.n_seq) {
-        note(0, a.n_q, nullptr, 0, 0);
+        note(0, a.n_q, nullptr, 0);
         return;
     }
     const TileGeom<BN> tg(l.by.list[1]);
-    uint32_t base_t = 0, base_p = 0;
+    uint32_t base_t = 0;
     for (uint32_t s0 = 0; s0 < a.n_seq; s0 += 32) {
         SeqShape sh = {};
         if (s0 + lane < a.n_seq) sh = seq_shape(a, s0 + lane);
         const uint32_t pairs = (sh.q_len * G + PR - 1) / PR, n = sh.q_len ? tg.tiles(sh.len) : 0;
         const uint32_t tiles = (n ? n + kUnit<BN> : 0) * pairs * H;
-        uint32_t ti = tiles, pi = pairs;
-        scan(ti, pi);
+        const uint32_t ti = scan(tiles);
         for (uint32_t w = 0; w < min(32u, a.n_seq - s0); ++w) {
             SeqShape one;
             one.q0 = __shfl_sync(0xffffffffu, sh.q0, w);
             one.q_len = __shfl_sync(0xffffffffu, sh.q_len, w);
             one.len = __shfl_sync(0xffffffffu, sh.len, w);
-            note(one.q0, one.q_len, &one, base_t + __shfl_sync(0xffffffffu, ti - tiles, w),
-                 base_p + __shfl_sync(0xffffffffu, pi - pairs, w));
+            note(one.q0, one.q_len, &one, base_t + __shfl_sync(0xffffffffu, ti - tiles, w));
             __syncwarp();
         }
         base_t += __shfl_sync(0xffffffffu, ti, 31);
-        base_p += __shfl_sync(0xffffffffu, pi, 31);
     }
 }
 
@@ -635,7 +627,7 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
             mbar_arrive(planned);
         }
         __syncwarp();
-        Walk<BN, PR> walk(a, plan, l.by, start.seq, start.tile, start.pair);
+        Walk<BN, PR> walk(a, plan, l.by, l.rooms, start.seq, start.tile);
         uint32_t j = 0;
         for (uint32_t i = 0;; ++i) {
             Seg g = {};
@@ -1087,7 +1079,7 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
             // two streams over the same rows: their outputs are joined here, half of
             // the columns by each
             const bool two = NS == 2 && !sh.both && g.n > 1;
-            const uint64_t slot = static_cast<uint64_t>(g.slot) * NS + (sh.both ? s : 0);
+            const uint32_t id = g.room + row_first() + r;  // the row in the workspace
             const bool idle = 32 * qd >= rows;  // no row of this warp: P may be anything
             // how far the row sees into the list
             uint32_t seen = 0xffffffffu;
@@ -1268,7 +1260,7 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
                 sum = f0 * sum + f1 * other.y;
             }
             if (!idle) {
-                if (r < rows && (s == 0 || !two)) l.ml[slot * 128 + r] = make_float2(m, sum);
+                if (r < rows && (s == 0 || !two)) l.ml[id] = make_float2(m, sum);
                 const uint32_t tx = tmem + ((32 * qd) << 16) + C::o_col(NS - 1 - s);
                 const uint32_t c0 = two ? s * (D / 2) : 0, c1 = two ? c0 + D / 2 : D;
 #pragma unroll 1
@@ -1287,7 +1279,7 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
                     if (r < rows) {
 #pragma unroll
                         for (uint32_t k = 0; k < 8; ++k)
-                            l.o[(slot * (D / 4) + col / 4 + k) * 128 + r] =
+                            l.o[out_at<D>(id, col / 4 + k)] =
                                 make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]),
                                             __uint_as_float(o[4 * k + 2]), __uint_as_float(o[4 * k + 3]));
                     }
@@ -1361,7 +1353,7 @@ __global__ void __launch_bounds__(kJoinRows *D / 4)
         float top = -INFINITY, sum = 0.0f;
         for (uint32_t i0 = 0; i0 < n_all; i0 += 32) {
             const uint32_t i = i0 + lane;
-            const uint32_t id = i < e0.n ? e0.id + i * e0.step : e1.id + (i - e0.n) * e1.step;
+            const uint32_t id = i < e0.n ? e0.at(i) : e1.at(i - e0.n);
             const float2 ml = i < n_all ? l.ml[id] : make_float2(-INFINITY, 0.0f);
             // a piece without keys has a sum of zero; one whose scores are all NaN has
             // no maximum either, but a NaN sum
@@ -1403,8 +1395,7 @@ __global__ void __launch_bounds__(kJoinRows *D / 4)
         for (uint32_t i = 0; i < 16; ++i) {
             o[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             if (i0 + i < n) {
-                const uint32_t id = s_id[r][i0 + i];
-                o[i] = l.o[(static_cast<uint64_t>(id / 128) * (D / 4) + col) * 128 + id % 128];
+                o[i] = l.o[out_at<D>(s_id[r][i0 + i], col)];
             }
         }
 #pragma unroll
@@ -1468,27 +1459,30 @@ uint32_t attn_ctas(DeviceFacts *f) {
 
 uint64_t up256(uint64_t v) { return (v + 255) / 256 * 256; }
 
-// The workspace: one word per CTA, the rows' notes, the pieces.
+// The workspace: one word per CTA, the rows' notes, the pieces' rows (Rooms).
 struct WsLayout {
-    uint64_t at, ml, o, bytes, slots[2];  // [1]: of 256 rows
+    uint64_t at, ml, o, bytes, rows;
+    Rooms rooms[2];  // units of 128 rows; of 256 (f16 pages, heads of 64 and 128)
     WsLayout(uint32_t n_q, uint32_t n_head, uint32_t n_head_kv, uint32_t d, uint32_t n_seq) {
-        // units of 128 rows or (f16 pages, heads of 64 and 128) 256, whichever takes
-        // more; a slot has a part for each 128
-        uint64_t parts = 0;
+        const uint64_t mine = static_cast<uint64_t>(n_q) * (n_head / n_head_kv);
+        const uint64_t own = n_seq ? (mine * n_head_kv + 7) / 8 * 8 : 0;
+        rows = 0;  // of whichever units take more
         for (uint64_t pr = 128; pr <= (d == 256 ? 128u : 256u); pr *= 2) {
-            const uint64_t rows = static_cast<uint64_t>(n_q) * (n_head / n_head_kv);
-            const uint64_t pairs = (rows + pr - 1) / pr, pg = (pairs + 7) / 8;
-            // prefix: n_pg * gs <= pairs + n_pg units a KV head, and a range each;
-            // tails: a pair per sequence more than whole pairs of the rows
-            const uint64_t n = (pairs + pg) * n_head_kv + 2 * kMaxCtas +
-                               (n_seq ? (n_seq + rows / pr) * n_head_kv : 0);
-            slots[pr / 256] = n;
-            parts = std::max(parts, n * pr / 128);
+            // the prefix has n_pg * gs <= pairs + n_pg units a KV head, and each CTA a
+            // range that may begin in a unit's middle
+            const uint64_t pairs = (mine + pr - 1) / pr, cap = std::min<uint64_t>(pr, (mine + 7) / 8 * 8);
+            const uint64_t n_pre = (pairs + (pairs + 7) / 8) * n_head_kv + kMaxCtas;
+            Rooms &r = rooms[pr / 256];
+            r.cap = static_cast<uint32_t>(cap);
+            r.n_pre = static_cast<uint32_t>(n_pre);
+            r.tail = static_cast<uint32_t>(n_pre * cap);
+            r.over = static_cast<uint32_t>(n_pre * cap + own);
+            rows = std::max(rows, n_pre * cap + own + (n_seq ? kMaxCtas * cap : 0));
         }
         at = up256(kMaxCtas * 4);
         ml = at + up256(2ull * n_q * n_head * sizeof(RowPieces));
-        o = ml + up256(parts * 128 * 8);
-        bytes = o + parts * 128 * d * 4;
+        o = ml + up256(rows * 8);
+        bytes = o + rows * d * 4;
     }
 };
 
@@ -1528,7 +1522,7 @@ cudaError_t launch_t(AttnLaunch &l, const WsLayout &w, cudaStream_t st) {
     l.by.ctas.set(n_cta);
     for (int i = 0; i < 2; ++i)
         l.by.list[i].set(lists[i]->max_len ? lists[i]->pages.page_tokens : Cfg<D, false>::BN, Cfg<D, false>::BN);
-    l.max_slots = static_cast<uint32_t>(w.slots[quant || D == 256 ? 0 : 1]);
+    l.rooms = w.rooms[quant || D == 256 ? 0 : 1];
     if (quant) {
         int32_t worst[2] = {KVMRET_TYPE_Q4_0, KVMRET_TYPE_Q4_0};
         for (const KeyList *kl : lists)

@@ -7,9 +7,9 @@
 // tiles of BN. The units' tiles, laid end to end, are cut into equal
 // contiguous ranges, one per CTA, so a long list is shared by many CTAs and a
 // short one by none; each (unit, CTA) piece leaves its unnormalised output,
-// maximum and sum in a workspace slot (one part for each row tile), and the join
-// adds a row's pieces in a fixed order, so results repeat run to run. Where a
-// row's pieces lie is written down by a spare warp of the attention kernel.
+// maximum and sum in rows of the workspace (Rooms), and the join adds a row's pieces
+// in a fixed order, so results repeat run to run. Where a row's pieces lie is written
+// down by a spare warp of the attention kernel.
 //   Prefix: when a KV head has more than PR rows (n_pair > 1), `gs` CTAs walk
 //     the same keys side by side, one row pair each, so that all but one of
 //     them find the tile in L2; the ranges are then per group of gs CTAs.
@@ -104,6 +104,19 @@ struct Cuts {
     }
 };
 
+// The workspace's rows, as the host knows them. A piece of the prefix has a room of
+// `cap` rows by its unit and range; of a tail's unit the first piece has the unit's
+// own rows (each row of the batch has one) and every further one a room by its CTA,
+// which begins at most one unit in its middle. So the rows follow those of the
+// batch, however few of them a unit has: 1024 sequences of one row, 64 query and 8 KV
+// heads of 128 take 0.11 GB (a tile of 256 rows for each piece would be 1.1 GB).
+struct Rooms {
+    uint32_t cap;    // rows of a room: a unit's, or all of a KV head's if they are fewer
+    uint32_t n_pre;  // rooms of the prefix, from row 0 on
+    uint32_t tail;   // first row of the tails' units
+    uint32_t over;   // first room of the tails' further pieces
+};
+
 // The split, alike in every CTA. (Tile counts fit 32 bits: the host checks their
 // bound.)
 struct Plan {
@@ -113,7 +126,6 @@ struct Plan {
     uint32_t p_len;             // its tokens (with partly filled pages: the place behind the last)
     uint32_t q0, rows;          // first row token; rows of a KV head (all sequences)
     uint32_t n_pair, n_pg, gs, groups;
-    uint32_t t_slot0;           // first workspace slot of the tails
     uint32_t ok;                // 0: q_start descends somewhere, nothing is done
 };
 
@@ -151,7 +163,7 @@ struct Seg {
     uint32_t len, q_len;      // the list's tokens; a tail's new ones
     uint32_t tile0, n;        // key tiles (n == 0: no more pieces)
     uint32_t j0;              // tiles of the CTA's pieces before this one
-    uint32_t slot;
+    uint32_t room;  // first of its rows in the workspace
 };
 
 template <int BN, int PR>
@@ -159,18 +171,19 @@ struct Walk {
     const PrefixAttn &a;
     const Plan &p;  // in shared memory
     const Divs &by;
+    const Rooms &rooms;
     uint32_t cta;
     uint32_t x, x1;       // prefix line: next tile, end
     uint32_t part, lane;  // the range and the CTA's place in its group
     uint32_t y, y1;       // tails' line
-    uint32_t seq;         // the sequence that holds y, its first tile and pair
-    uint32_t seq_tile, seq_pair;
+    uint32_t seq;         // the sequence that holds y, its first tile
+    uint32_t seq_tile;
     SeqShape sh;
     bool fresh;
 
-    __device__ __forceinline__ Walk(const PrefixAttn &a_, const Plan &p_, const Divs &by_, uint32_t s,
-                                    uint32_t tile, uint32_t pair)
-        : a(a_), p(p_), by(by_), cta(blockIdx.x), seq(s), seq_tile(tile), seq_pair(pair), fresh(true) {
+    __device__ __forceinline__ Walk(const PrefixAttn &a_, const Plan &p_, const Divs &by_,
+                                    const Rooms &r, uint32_t s, uint32_t tile)
+        : a(a_), p(p_), by(by_), rooms(r), cta(blockIdx.x), seq(s), seq_tile(tile), fresh(true) {
         ranges(p, cta, x, x1, y, y1);
         part = p.gs == 1 ? cta : cta / p.gs;
         lane = cta - part * p.gs;
@@ -208,7 +221,7 @@ struct Walk {
             g.rows = min(static_cast<uint32_t>(PR), p.rows - g.row0);
             g.tile0 = t;
             g.n = n;
-            g.slot = (u + part) * p.gs + lane;
+            g.room = ((u + part) * p.gs + lane) * rooms.cap;
             return true;
         }
         const TileGeom<BN> geom(by.list[1]);
@@ -220,7 +233,6 @@ struct Walk {
             const uint32_t mine = (tiles ? tiles + kUnit<BN> : 0) * pairs * a.n_head_kv;
             if (y >= seq_tile + mine) {
                 seq_tile += mine;
-                seq_pair += pairs;
                 ++seq;
                 fresh = true;
                 continue;
@@ -245,7 +257,8 @@ struct Walk {
             g.rows = min(static_cast<uint32_t>(PR), sh.q_len * by.G.d - g.row0);
             g.tile0 = t;
             g.n = n;
-            g.slot = p.t_slot0 + seq_pair * a.n_head_kv + u + cta;
+            g.room = t ? rooms.over + cta * rooms.cap
+                       : rooms.tail + ((sh.q0 - p.q0) * a.n_head_kv + g.h * sh.q_len) * by.G.d + g.row0;
             return true;
         }
         return false;

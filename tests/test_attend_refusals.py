@@ -161,3 +161,21 @@ def test_pages_refuse_other_element_types(dtype, kind, good):
         else:
             with pytest.raises(kvmret.KvmretError, match="float16"):
                 kvmret.Pages(k, v, 16, 2, 128, *types)
+
+
+def test_workspace_follows_the_rows():
+    """Partial outputs are kept for rows, not for whole tiles of each sequence: about
+    2.2 rows for each of the batch's, and what lists that several SMs share take."""
+    size = lib.kvmret_prefix_attn_ws_bytes
+    for n, h, hkv, d in ((1, 64, 8, 128), (16, 64, 8, 128), (1024, 64, 8, 128), (65535, 8, 8, 64),
+                         (65535, 64, 8, 128), (300, 5, 1, 256)):
+        for seqs in (0, 1, n):
+            mine = -(-n * h // hkv // 8) * 8  # of a KV head, by eights
+            rows = 2.2 * n * h + (2 * 160 + 2 * hkv) * min(256, mine) + 8
+            assert 0 < size(n, h, hkv, d, seqs) <= rows * (4 * d + 8) + 32 * n * h + 4096
+    assert size(1, 64, 8, 128, 1) < 4 << 20 and size(1024, 64, 8, 128, 1024) < 128 << 20
+
+
+def test_prefix_attn_refuses_rows_that_no_workspace_counts():
+    assert attn(pages_desc(), pages_desc(), n_q=65535, n_head=32764) == -1
+    assert b"workspace" in lib.kvmret_last_error() and b"too many" in lib.kvmret_last_error()

@@ -746,3 +746,34 @@ def test_length_counts_the_tokens_of_partly_filled_pages(absent):
             for longest in (None, torch.full_like(length, m + 3)):
                 check(*kvmret.prefix_attn(qd, pages, longest, prefix_table=t, prefix_ntok=nt,
                                           max_prefix=m, lse=True), want)
+
+
+@pytest.mark.parametrize("case", [
+    ([1], [40], 20000, 64, 8, 128, 128, 32, F16, F16),
+    ([1] * 300, [17] * 300, 0, 8, 2, 128, 128, 16, F16, F16),
+    ([1, 3] * 40, [90, 5] * 40, 700, 12, 4, 64, 64, 16, F16, F16),
+    ([5, 2, 60], [500, 2, 60], 900, 7, 1, 256, 64, 64, F16, F16),
+    ([1] * 70, [70] * 70, 300, 16, 2, 128, 32, 32, Q8, Q4),
+    ([400, 3], [600, 3], 200, 16, 2, 128, 128, 64, F16, F16),
+    ([400, 3], [600, 3], 0, 16, 4, 64, 64, 64, Q8, Q8),
+])
+def test_workspace_is_kept_to_and_need_not_be_clean(case, monkeypatch):
+    """Nothing outside the workspace is written, and what it held before does not matter."""
+    pool, tpool, table, own, _, _, start, q, tl = build(case)
+    prefix = case[2]
+    args = (dev(q), pool.device() if prefix else None, dev(np.array([prefix], np.int32)), tpool.device(),
+            dev(own), dev(tl), dev(start))
+    kw = dict(prefix_table=dev(table) if prefix else None, lse=True)
+    want, lse = kvmret.prefix_attn(*args, **kw)
+    room, held = 16 << 20, []
+
+    def workspace(shape, n_head_kv, n_seq, device):
+        nb = int(kvmret.lib.kvmret_prefix_attn_ws_bytes(shape[0], shape[1], n_head_kv, shape[2], n_seq))
+        held.append(torch.full((nb + 2 * room,), 0xa5, dtype=torch.uint8, device=device))
+        held[-1][room:room + nb] = 0xff
+        return held[-1][room:room + nb], nb
+
+    monkeypatch.setattr(kvmret, "_attn_ws", workspace)
+    got, lse2 = kvmret.prefix_attn(*args, **kw)
+    assert torch.equal(got, want) and torch.equal(lse2, lse)
+    assert bool((held[0][:room] == 0xa5).all()) and bool((held[0][-room:] == 0xa5).all())
