@@ -1431,7 +1431,9 @@ int kvmret_window_attn(kvmret_ctx *c, uint32_t layer, const kvmret_pages *tail,
     p.ntok = c->d_win_ntok;  // 0 for an empty slot
     p.n_list = c->win_slots;
     p.max_len = c->win_slots * c->cfg.block_tokens;
-    return kvmret::prefix_attn_call(p, tail, a, ws, ws_bytes, c->st);
+    TRY(kvmret::prefix_attn_call(p, tail, a, ws, ws_bytes, c->st));
+    c->prof.launches += a->n_q ? 2 : 0;  // the attention and its join
+    return KVMRET_OK;
 }
 
 int kvmret_window_layout(kvmret_ctx *c, uint32_t *ids, int32_t *bases, uint32_t *n_out) {

@@ -777,3 +777,20 @@ def test_workspace_is_kept_to_and_need_not_be_clean(case, monkeypatch):
     got, lse2 = kvmret.prefix_attn(*args, **kw)
     assert torch.equal(got, want) and torch.equal(lse2, lse)
     assert bool((held[0][:room] == 0xa5).all()) and bool((held[0][-room:] == 0xa5).all())
+
+
+def test_window_attention_is_counted_among_the_launches():
+    w = synth.Workload("count", n_layer=1, n_head=4, n_head_kv=2, d_head=128, block_tokens=64,
+                       n_blocks=8, budget_blocks=4, sink_blocks=1, reserve_blocks=1, n_planted=1, seed=5)
+    r = kvmret.Retriever(config_for(w))
+    append_history(r, synth.NumpyHistory(w), cuts=[])
+    r.prof_enable()
+    q = torch.zeros(3, 4, 128, dtype=torch.float16, device="cuda")
+    tails = kvmret.Pages(*(torch.zeros(1, 16, 2, 128, dtype=torch.float16, device="cuda") for _ in "kv"),
+                         16, 2, 128)
+    ones = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    args = (tails, ones, torch.ones(1, dtype=torch.int32, device="cuda"))
+    r.window_attn(0, q, *args, torch.tensor([0, 3], dtype=torch.int32, device="cuda"))
+    r.window_attn(0, q[:0], *args, torch.zeros(2, dtype=torch.int32, device="cuda"))
+    assert r.prof_read()["launches"] == 2
+    r.close()
