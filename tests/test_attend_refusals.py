@@ -179,3 +179,14 @@ def test_workspace_follows_the_rows():
 def test_prefix_attn_refuses_rows_that_no_workspace_counts():
     assert attn(pages_desc(), pages_desc(), n_q=65535, n_head=32764) == -1
     assert b"workspace" in lib.kvmret_last_error() and b"too many" in lib.kvmret_last_error()
+
+
+def test_numbers_that_no_field_holds_are_refused():
+    """Packed arguments: a negative count or a number past float32 is the library's error."""
+    qk = [0] * 11 + [1, 8, 2, 128, 128, 0, kvmret.TYPE_F16, 1e-6, 1e6, 1.0]
+    assert len(kvmret._pack(kvmret._QK, *qk)) == ctypes.sizeof(kvmret.QkArgs)
+    for at, bad in ((16, -1), (18, 1e300), (19, 1e39), (20, -1e39)):
+        with pytest.raises(kvmret.KvmretError, match="range"):
+            kvmret._pack(kvmret._QK, *qk[:at], bad, *qk[at + 1:])
+    with pytest.raises(kvmret.KvmretError, match="range"):
+        kvmret._pack(kvmret._ATTN, 0, 0, 0, 0, 1, 4, 1e300, 0, 0, 0, 0, 0, 0, 0, 0, 0)

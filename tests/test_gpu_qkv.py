@@ -296,3 +296,15 @@ def test_pages_of_an_expanded_axis_are_refused():
         with pytest.raises(kvmret.KvmretError):
             kvmret.Pages(k, v, 16, 2, 128)
     assert kvmret.Pages(one, one.clone(), 16, 2, 128).n_pages == 1
+
+
+def test_numbers_out_of_range_are_refused():
+    q = torch.zeros(4, 8, 128, dtype=torch.float16, device="cuda")
+    k, pos = q[:, :2], torch.zeros(4, dtype=torch.int32, device="cuda")
+    for kw in (dict(fwht_n=-1), dict(eps=1e300), dict(freq_base=1e39), dict(freq_scale=-1e39)):
+        with pytest.raises(kvmret.KvmretError):
+            kvmret.qk_norm_rope(q, k, pos, **kw)
+    p = kvmret.Pages(*(torch.zeros(1, 16, 2, 128, dtype=torch.float16, device="cuda") for _ in "kv"),
+                     16, 2, 128)
+    with pytest.raises(kvmret.KvmretError):
+        kvmret.prefix_attn(q, p, None, scale=1e300)
