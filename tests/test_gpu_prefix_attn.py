@@ -794,3 +794,78 @@ def test_window_attention_is_counted_among_the_launches():
     r.window_attn(0, q[:0], *args, torch.zeros(2, dtype=torch.int32, device="cuda"))
     assert r.prof_read()["launches"] == 2
     r.close()
+
+
+@pytest.mark.parametrize("d,g,new,n_pre,kt,vt", [
+    (128, 8, [345], 0, F16, F16), (128, 8, [345], 3000, F16, F16),      # 11 units of 256 rows: groups of 6
+    (64, 8, [300, 45], 1100, F16, F16), (128, 8, [345], 0, Q8, Q4),      # 22 units of 128: groups of 8
+    (128, 8, [40, 305], 2100, Q8, Q4), (256, 5, [403], 1500, F16, F16),  # 16: groups of 8
+    (256, 5, [403], 0, Q4, Q8), (64, 4, [1100], 700, Q8, F16),           # 35: groups of 7
+])
+def test_chunks_of_many_units(d, g, new, n_pre, kt, vt):
+    """More than eight units of rows a KV head: groups of SMs walk the prefix side by
+    side, the last group not always full, and causality cuts each unit's tail elsewhere."""
+    rng = np.random.default_rng(d + g + n_pre)
+    hkv, page = 4, 64
+    tl = [n + 150 * s for s, n in enumerate(new)]
+    pool = Pool(rng, -(-n_pre // page) + 1, page, hkv, d, kt, vt)
+    width = -(-max(tl) // page)
+    tpool = Pool(rng, len(new) * width, page, hkv, d, kt, vt)
+    table = rng.permutation(-(-n_pre // page) + 1)[:-(-n_pre // page)].astype(np.int32)
+    own = rng.permutation(len(new) * width).reshape(len(new), width).astype(np.int32)
+    pre = [dev(x) for x in pool.fill(table, n_pre)]
+    tails = [[dev(x) for x in tpool.fill(own[s], t)] for s, t in enumerate(tl)]
+    start = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+    q = dev((rng.standard_normal((int(start[-1]), hkv * g, d)) * 1.5).astype(np.float16))
+    got, lse = kvmret.prefix_attn(q, pool.device() if n_pre else None,
+                                  dev(np.array([n_pre], np.int32)) if n_pre else None, tpool.device(),
+                                  dev(own), dev(np.array(tl, np.int32)), dev(start),
+                                  prefix_table=dev(table) if n_pre else None, lse=True)
+    spans = [(int(start[s]), int(start[s + 1]), torch.cat([pre[0], tails[s][0]]),
+              torch.cat([pre[1], tails[s][1]])) for s in range(len(new))]
+    check_rows(got, lse, q, spans, hkv, kt != F16, vt != F16)
+
+
+def test_a_thousand_heads_to_a_kv_head():
+    rng = np.random.default_rng(12)
+    pool, tpool = Pool(rng, 3, 64, 1, 64, F16, F16), Pool(rng, 2, 64, 1, 64, F16, F16)
+    pre, tail = [dev(x) for x in pool.fill(np.arange(3), 150)], [dev(x) for x in tpool.fill([0, 1], 70)]
+    q = dev((rng.standard_normal((3, 1000, 64)) * 1.5).astype(np.float16))
+    got, lse = kvmret.prefix_attn(q, pool.device(), None, tpool.device(), dev(np.array([[0, 1]], np.int32)),
+                                  dev(np.array([70], np.int32)), dev(np.array([0, 3], np.int32)),
+                                  max_prefix=150, lse=True)
+    check_rows(got, lse, q, [(0, 3, torch.cat([pre[0], tail[0]]), torch.cat([pre[1], tail[1]]))], 1,
+               False, False)
+
+
+def test_the_most_sequences():
+    """65,535 sequences of one row: tails of 0 to 16 tokens, pages shared by many."""
+    rng = np.random.default_rng(13)
+    n, hq, hkv, d, n_pages = 65535, 4, 2, 64, 500
+    pool = Pool(rng, n_pages, 16, hkv, d, F16, F16)
+    k, v = (dev(x).view(n_pages, 16, hkv, d) for x in pool.fill(np.arange(n_pages), 16 * n_pages))
+    own, tl = dev(rng.integers(0, n_pages, (n, 1)).astype(np.int32)), dev(rng.integers(0, 17, n).astype(np.int32))
+    q = torch.randn(n, hq, d, device="cuda").half()
+    got, lse = kvmret.prefix_attn(q, None, None, pool.device(), own, tl,
+                                  torch.arange(n + 1, dtype=torch.int32, device="cuda"), lse=True)
+    hide = (torch.arange(16, device="cuda") >= tl[:, None])[:, None]  # [n][1][16]
+    for h in range(hq):
+        kh, vh = (x[own[:, 0].long(), :, h // 2] for x in (k, v))  # [n][16][d]
+        x = q[:, h].double()
+        w = torch.einsum("nd,nkd->nk", x, kh) * d ** -0.5
+        mag = torch.einsum("nd,nkd->nk", x.abs(), kh.abs()) * d ** -0.5
+        w = w.masked_fill(hide[:, 0], -math.inf)
+        top = w.amax(-1, keepdim=True).clamp(min=-1e300)
+        p = torch.exp(w - top)
+        total = p.sum(-1, keepdim=True)
+        ds = ((2e-6 + 2.0 ** -22) * mag).amax(-1, keepdim=True)
+        seen = torch.where(total > 0, total, 1.0)
+        want = torch.einsum("nk,nkd->nd", p, vh) / seen
+        mass = torch.einsum("nk,nkd->nd", p, vh.abs()) / seen
+        tol = (2 * ds + 2.0 ** -11 + 1e-5) * mass + 2.0 ** -25 * vh.abs().sum(1) / seen + \
+            2.0 ** -11 * want.abs() + 2.0 ** -25
+        assert bool(((got[:, h].double() - want).abs() <= tol).all())
+        empty = tl == 0
+        assert torch.equal(torch.isneginf(lse[:, h]), empty) and bool((got[empty] == 0).all())
+        wl = (top + torch.log(seen))[~empty, 0]
+        assert bool(((lse[~empty, h].double() - wl).abs() <= ds[~empty, 0] + 2e-6 * (1 + wl.abs())).all())

@@ -308,3 +308,13 @@ def test_numbers_out_of_range_are_refused():
                      16, 2, 128)
     with pytest.raises(kvmret.KvmretError):
         kvmret.prefix_attn(q, p, None, scale=1e300)
+
+
+@pytest.mark.parametrize("n,hq,hkv,d,dt,fwht", [
+    (512, 32, 8, 64, "f16", False), (777, 7, 1, 64, "f32", True), (513, 32, 4, 256, "bf16", True),
+    (1030, 3, 1, 256, "f16", False), (2049, 1, 1, 128, "f32", True),
+])
+def test_qk_norm_rope_of_chunks(n, hq, hkv, d, dt, fwht):
+    """Many tokens (a CTA takes all heads of a few): every head size, row counts that
+    leave a CTA's last pass part empty."""
+    test_qk_norm_rope(n, hq, hkv, d, dt, fwht, True)
