@@ -1435,25 +1435,16 @@ cudaError_t encode_pages(CUtensorMap *map, const uint8_t *at, uint64_t row, uint
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
-// What a launch asks of the device, kept per device: its SM count, and which
-// kernels have been allowed their shared memory (bit 2 * log2(D / 64) + QUANT).
-struct DeviceFacts {
-    std::atomic<uint32_t> ctas{0}, allowed{0};
-};
-DeviceFacts *device_facts() {
-    static DeviceFacts facts[64];
-    int dev = 0;
-    return cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64 ? &facts[dev] : nullptr;
-}
-uint32_t attn_ctas(DeviceFacts *f) {
-    uint32_t n = f ? f->ctas.load(std::memory_order_relaxed) : 0;
-    if (n) return n;
+// CTAs of a launch: the current device's SMs, asked for once a device.
+uint32_t attn_ctas() {
+    static std::atomic<uint32_t> known[64];
     int dev = 0, sm = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess ||
-        cudaDeviceGetAttribute(&sm, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sm <= 0)
-        sm = 148;
+    const bool one = cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64;
+    uint32_t n = one ? known[dev].load(std::memory_order_relaxed) : 0;
+    if (n) return n;
+    if (cudaDeviceGetAttribute(&sm, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sm <= 0) sm = 148;
     n = std::min<uint32_t>(static_cast<uint32_t>(sm), kMaxCtas);
-    if (f) f->ctas.store(n, std::memory_order_relaxed);
+    if (one) known[dev].store(n, std::memory_order_relaxed);
     return n;
 }
 
@@ -1487,24 +1478,19 @@ struct WsLayout {
 };
 
 template <int D, bool QUANT>
-cudaError_t launch_main(const AttnLaunch &l, uint32_t n_cta, DeviceFacts *f, cudaStream_t st) {
+cudaError_t launch_main(const AttnLaunch &l, uint32_t n_cta, cudaStream_t st) {
     const size_t smem = Cfg<D, QUANT>::tiles + sizeof(Small<D, QUANT>);
-    constexpr uint32_t bit = 1u << ((D == 64 ? 0 : D == 128 ? 2 : 4) + QUANT);
-    if (!f || !(f->allowed.load(std::memory_order_relaxed) & bit)) {
-        const cudaError_t e =
-            cudaFuncSetAttribute(attn_tc_kernel<D, QUANT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 static_cast<int>(smem));
-        if (e != cudaSuccess) return e;
-        if (f) f->allowed.fetch_or(bit, std::memory_order_relaxed);
-    }
+    // (at every launch: a context made after a device reset does not know it)
+    const cudaError_t e = cudaFuncSetAttribute(
+        attn_tc_kernel<D, QUANT>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (e != cudaSuccess) return e;
     attn_tc_kernel<D, QUANT><<<n_cta, Cfg<D, QUANT>::threads, smem, st>>>(l);
     return cudaGetLastError();
 }
 
 template <int D>
 cudaError_t launch_t(AttnLaunch &l, const WsLayout &w, cudaStream_t st) {
-    DeviceFacts *f = device_facts();
-    const uint32_t n_cta = attn_ctas(f);
+    const uint32_t n_cta = attn_ctas();
     const KeyList *lists[2] = {&l.a.prefix, &l.a.tail};
     bool quant = false;
     cudaError_t e = cudaSuccess;
@@ -1533,7 +1519,7 @@ cudaError_t launch_t(AttnLaunch &l, const WsLayout &w, cudaStream_t st) {
         l.raw_v = Cfg<D, true>::BN * raw_box<D>(worst[1]);
         l.n_raw_v = std::min<uint32_t>(2, (Cfg<D, true>::raw_bytes - 2 * l.raw_k) / l.raw_v);
     }
-    e = quant ? launch_main<D, true>(l, n_cta, f, st) : launch_main<D, false>(l, n_cta, f, st);
+    e = quant ? launch_main<D, true>(l, n_cta, st) : launch_main<D, false>(l, n_cta, st);
     if (e != cudaSuccess) return e;
     const uint64_t rows = static_cast<uint64_t>(l.a.n_q) * l.a.n_head;
     cudaLaunchConfig_t cfg = {};
