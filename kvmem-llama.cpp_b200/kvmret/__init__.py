@@ -655,9 +655,13 @@ class Retriever:
                                               q_start, scale, lse, out)
         with torch.cuda.device(c.device):
             ws, nb = _attn_ws(shape, c.n_head_kv, tails[0], q.device)
+            try:
+                a = _ATTN.pack(*front, 0, 0, 0, 0, *tails)
+            except _RANGE as e:
+                raise KvmretError(f"argument out of range: {e}") from None
             with _Ordered(self.stream_ptr):
-                _check(_window_attn_call(self.h, layer, None if tail is None else tail.ref,
-                                         _pack(_ATTN, *front, 0, 0, 0, 0, *tails), ws.data_ptr(), nb))
+                _check(_window_attn_call(self.h, layer, None if tail is None else tail.ref, a,
+                                         ws.data_ptr(), nb))
         return got
 
     def window_layout(self):
@@ -987,15 +991,7 @@ def _want(ok, msg):
 _QK = struct.Struct("=11Q6Iifff")
 _ATTN = struct.Struct("=QQQQIIfIQQQIIQQQ")
 assert _QK.size == ctypes.sizeof(QkArgs) and _ATTN.size == ctypes.sizeof(AttnArgs)
-
-
-def _pack(layout, *fields):
-    try:
-        return layout.pack(*fields)
-    except (struct.error, OverflowError) as e:  # a number that its field cannot hold
-        raise KvmretError(f"argument out of range: {e}") from None
-
-
+_RANGE = (struct.error, OverflowError)  # a number that its field cannot hold
 _packed = ctypes.c_char_p
 _qk_call = ctypes.CFUNCTYPE(ctypes.c_int, _packed, _P)(("kvmret_qk_norm_rope", lib))
 _attn_call = ctypes.CFUNCTYPE(ctypes.c_int, _P, _P, _packed, _P, ctypes.c_size_t,
@@ -1096,11 +1092,14 @@ def qk_norm_rope(q, k, pos, q_weight=None, k_weight=None, eps=1e-6, freq_base=1e
     o1 = empty(*sk, dtype=f16, device=dev) if k_rot else None
     o2 = (like(o0) if q_rot else empty(*sq, dtype=f16, device=dev)) if q_raw else None
     o3 = (like(o1) if k_rot else empty(*sk, dtype=f16, device=dev)) if k_raw else None
-    a = _pack(_QK, q.data_ptr(), k.data_ptr(), qs, ks, 0 if q_weight is None else q_weight.data_ptr(),
-                 0 if k_weight is None else k_weight.data_ptr(), _index(pos, n, index, "pos"),
-                 o0.data_ptr() if q_rot else 0, o1.data_ptr() if k_rot else 0,
-                 o2.data_ptr() if q_raw else 0, o3.data_ptr() if k_raw else 0,
-                 n, hq, hkv, d, d, fwht_n, t, eps, freq_base, freq_scale)
+    try:
+        a = _QK.pack(q.data_ptr(), k.data_ptr(), qs, ks, 0 if q_weight is None else q_weight.data_ptr(),
+                     0 if k_weight is None else k_weight.data_ptr(), _index(pos, n, index, "pos"),
+                     o0.data_ptr() if q_rot else 0, o1.data_ptr() if k_rot else 0,
+                     o2.data_ptr() if q_raw else 0, o3.data_ptr() if k_raw else 0,
+                     n, hq, hkv, d, d, fwht_n, t, eps, freq_base, freq_scale)
+    except _RANGE as e:
+        raise KvmretError(f"argument out of range: {e}") from None
     _launch(index, 0, _qk_call, a)
     return o0, o1, o2, o3
 
@@ -1210,7 +1209,6 @@ def prefix_attn(q, prefix, prefix_len, tail=None, tail_table=None, tail_len=None
     bound on the prefix (default: what its pages hold). Either part may be None.
     scale defaults to d_head ** -0.5. Returns out (rows of no sequence: as
     they were), with lse=True also the f32 [n_q][n_head] log-sum-exp."""
-    import torch
     pages = prefix if prefix is not None else tail
     _want(pages is not None, "a prefix or tails")
     index = pages.index
@@ -1236,11 +1234,15 @@ def prefix_attn(q, prefix, prefix_len, tail=None, tail_table=None, tail_len=None
         if prefix_len is not None:
             length = _index(prefix_len, 1, index, "prefix_len")
         if ntok and most < held:  # tokens, which may lie in any of the pages
+            import torch
             cut = (torch.full((1,), most, dtype=torch.int32, device=q.device) if prefix_len is None
                    else prefix_len.clamp(max=most))
             most, length = held, cut.data_ptr()
+    try:
+        a = _ATTN.pack(*front, most, length, table, ntok, *tails)
+    except _RANGE as e:
+        raise KvmretError(f"argument out of range: {e}") from None
     ws, nb = _attn_ws(shape, pages.n_head_kv, tails[0], q.device)
     _launch(index, 0, _attn_call, None if prefix is None else prefix.ref,
-            None if tail is None else tail.ref,
-            _pack(_ATTN, *front, most, length, table, ntok, *tails), ws.data_ptr(), nb)
+            None if tail is None else tail.ref, a, ws.data_ptr(), nb)
     return got

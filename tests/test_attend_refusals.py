@@ -181,12 +181,28 @@ def test_prefix_attn_refuses_rows_that_no_workspace_counts():
     assert b"workspace" in lib.kvmret_last_error() and b"too many" in lib.kvmret_last_error()
 
 
+class _OnCpu:
+    """A CPU tensor that passes for one of the wrappers' device."""
+    is_cuda = True
+
+    def __init__(self, x):
+        self.x = x
+
+    def __getattr__(self, name):
+        return getattr(self.x, name)
+
+    def __getitem__(self, i):
+        return self.x[i]
+
+
 def test_numbers_that_no_field_holds_are_refused():
-    """Packed arguments: a negative count or a number past float32 is the library's error."""
-    qk = [0] * 11 + [1, 8, 2, 128, 128, 0, kvmret.TYPE_F16, 1e-6, 1e6, 1.0]
-    assert len(kvmret._pack(kvmret._QK, *qk)) == ctypes.sizeof(kvmret.QkArgs)
-    for at, bad in ((16, -1), (18, 1e300), (19, 1e39), (20, -1e39)):
+    """A negative count or a number past float32 is the library's error, before any launch."""
+    import torch
+    q, k = (_OnCpu(torch.zeros(4, h, 128, dtype=torch.float16)) for h in (8, 2))
+    pos = torch.zeros(4, dtype=torch.int32)
+    for kw in (dict(fwht_n=-1), dict(eps=1e300), dict(freq_base=1e39), dict(freq_scale=-1e39)):
         with pytest.raises(kvmret.KvmretError, match="range"):
-            kvmret._pack(kvmret._QK, *qk[:at], bad, *qk[at + 1:])
+            kvmret.qk_norm_rope(q, k, pos, **kw)
+    p = kvmret.Pages(*(_OnCpu(torch.zeros(1, 16, 2, 128, dtype=torch.float16)) for _ in "kv"), 16, 2, 128)
     with pytest.raises(kvmret.KvmretError, match="range"):
-        kvmret._pack(kvmret._ATTN, 0, 0, 0, 0, 1, 4, 1e300, 0, 0, 0, 0, 0, 0, 0, 0, 0)
+        kvmret.prefix_attn(q, p, None, scale=1e300)
