@@ -786,7 +786,10 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
         // as they could be, in any order, lets the streams fall into step: 3.9 ms
         // instead of 3.2 ms for 2048 rows over 32,768 tokens.)
         constexpr uint32_t id_s = idesc(BN, false), id_o = idesc(D, true);
-        constexpr uint32_t kHi = 64u | (1u << 14) | (2u << 29);  // upper halves of the descriptors
+        // Upper halves of the descriptors (tc.cuh): 8-row atoms every 1024 bytes, 128-byte
+        // swizzle. V is MN-major: rows of 64 dimensions, one a key, and in the leading
+        // offset the bytes to the next 64 dimensions.
+        constexpr uint32_t kHi = 64u | (1u << 14) | (2u << 29);
         const uint32_t ubase = __shfl_sync(0xffffffffu, base, 0);
         auto desc = [](uint32_t lo) { return static_cast<uint64_t>(kHi) << 32 | lo; };
         Share<NS> sh[2];

@@ -50,22 +50,9 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
     }
 }
 
-// Whether the phase with the given parity has completed.
-__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    return done;
-}
-
-// The same for warps whose code must stay short (instruction fetch is what a
-// warp between two busy ones waits for): the limit is counted in SM clocks,
-// about 2 s.
+// The same wait for warps whose code must stay short (instruction fetch is what a
+// warp between two busy ones waits for): mbar_try asks once, mbar_wait_clk again
+// and again with a limit counted in SM clocks, about 2 s.
 __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
     uint32_t done;
     asm volatile(
@@ -120,14 +107,6 @@ __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
 __device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr) {
     return static_cast<uint64_t>((saddr >> 4) & 0x3FFFu) | (1ull << 16) | (64ull << 32) |
            (1ull << 46) | (2ull << 61);
-}
-
-// The same for an MN-major tile: rows of 64 MN elements (128 bytes), one per K
-// index; 8-row atoms every 1024 bytes along K (stride byte offset), the next
-// 64 MN elements `block` bytes on (leading byte offset).
-__device__ __forceinline__ uint64_t sw128_desc_mn(uint32_t saddr, uint32_t block) {
-    return static_cast<uint64_t>((saddr >> 4) & 0x3FFFu) |
-           (static_cast<uint64_t>(block >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
 }
 
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
