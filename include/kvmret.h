@@ -664,13 +664,13 @@ typedef struct kvmret_attn {
  * types may differ. Scores, statistics and sums are f32, the weights p_j f16;
  * quantised values are rounded to f16 (d * q) before the products and must lie in
  * its range. A query that is not finite spoils its own row alone. q_start that
- * descends, or a wait within the kernel that gives up (after about two seconds),
+ * descends, or a wait within the kernel that gives up (after two seconds without a change),
  * leaves NaN in every row from q_start[0] to q_start[n_seq] - 1. ws_dev: 256-byte aligned workspace
  * of kvmret_prefix_attn_ws_bytes, written and read by this call alone (calls that
  * may overlap, graphs included, need one each). It grows with the rows: f32 partial
  * outputs of about 2.2 n_q * n_head * d_head, and of up to 640 * 128 * d_head more
- * for lists that several SMs share (64 heads of 128: 1.5 MB for one row, 23 MB for
- * 16, 0.11 GB for 1024). n_q <= 65535, n_head <= 65535, n_q * n_head <= 2^31 - 1, and
+ * for lists that several SMs share (64 heads of 128: 1.4 MB for one row, 23 MB for
+ * 16, 0.12 GB for 1024). n_q <= 65535, n_head <= 65535, n_q * n_head <= 2^31 - 1, and
  * rows times key tiles, counted at 16 tokens a tile from the bounds, as well as the
  * workspace's rows stay below 2^32 (refused otherwise). */
 size_t kvmret_prefix_attn_ws_bytes(uint32_t n_q, uint32_t n_head, uint32_t n_head_kv,
@@ -682,7 +682,10 @@ int kvmret_prefix_attn(const kvmret_pages *prefix, const kvmret_pages *tail, con
  * the steps and appends enqueued so far; a->max_prefix, prefix_len_dev,
  * prefix_table_dev and prefix_ntok_dev are not read. block_tokens must be a
  * multiple of 16. K of the window is rotated at window positions 0 .., so the
- * next token's position is the window's token count. */
+ * next token's position is the window's token count. The context's stream is ordered
+ * with no other: q, the tail's pages, table and lengths must have been written by
+ * work on it or on a stream that it waits for (cudaStreamWaitEvent), and what reads
+ * out or lse, or reuses ws, must run on it or wait for it. */
 int kvmret_window_attn(kvmret_ctx *ctx, uint32_t layer, const kvmret_pages *tail,
                        const kvmret_attn *a, void *ws_dev, size_t ws_bytes);
 

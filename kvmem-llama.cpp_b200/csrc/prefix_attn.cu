@@ -41,8 +41,8 @@
 // a chain of softmax and product per tile that reads at 4.5 TB/s. With 256 rows a
 // unit the chain is about 4000 clocks for 2 * 128 x 128 scores: 2048 exponentials
 // a scheduler, the products of one stream during the softmax of the other (tensor
-// pipe active 45 %): 2048 rows by 64 heads over 32,768 tokens take 2.15 to 2.5 ms
-// as the clock stands, about 1 PFLOP/s. Quantised: 53 us for the first shape (10 by
+// pipe active 47 %): 2048 rows by 64 heads over 32,768 tokens take 2.18 to 2.5 ms
+// as the clock stands, 0.9 to 1.04 PFLOP/s. Quantised: 54 us for the first shape (10 by
 // its bytes), bound by the same chain of one stream, 3000 clocks a tile.
 // The instruction caches count: conversions as straight code of a tile were 12 %
 // slower than a loop over blocks (68 and 61 us), the softmax of one stream as
@@ -783,8 +783,8 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
         // first gets its P V product and, once that has read P, its next scores.
         // While it waits for its softmax the other stream's turn comes, so the two
         // stay half a period apart. (Both products of a turn being issued as soon
-        // as they could be, in any order, lets the streams fall into step: 3.9 ms
-        // instead of 3.2 ms for 2048 rows over 32,768 tokens.)
+        // as they could be, in any order, lets the streams fall into step: 2048 rows over
+        // 32,768 tokens took a fifth longer.)
         constexpr uint32_t id_s = idesc(BN, false), id_o = idesc(D, true);
         // Upper halves of the descriptors (tc.cuh): 8-row atoms every 1024 bytes, 128-byte
         // swizzle. V is MN-major: rows of 64 dimensions, one a key, and in the leading
@@ -917,7 +917,7 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
         // (head size 256: half of it): blocks from the raw tile to f16(d * q) in the
         // stage's swizzled layout. Whole numbers become halves by their bits
         // (0x6400 + u is 1024 + u), one subtraction and one product by d, rounded
-        // once to the tensor cores' type: outputs are 2.9e-4 to 5.2e-4 off in the mean
+        // once to the tensor cores' type: outputs are 2.9e-4 to 6e-4 off in the mean
         // instead of the 2.9e-4 of f16 pages (most of which P's and the output's own
         // rounding make). d * q whole would take two f16 tiles each for K and V, twice
         // the products, and leave them one stage each. Operands in f16 go to their
@@ -1154,8 +1154,7 @@ __global__ void __launch_bounds__(Cfg<D, QUANT>::threads, 1)
                 // row's maximum has moved by more than 8 the pass is repeated with the
                 // new one; S still stands. Two streams hand the halves of P on one by
                 // one, so that the first half's product runs during the second half's
-                // softmax (2048 rows over 32,768 tokens: 2.35 ms, 2.44 in one piece; 16 rows: 44
-                // and 47 us).
+                // softmax (2048 rows over 32,768 tokens took 4 % longer in one piece, 16 rows 7 %).
                 constexpr int KEYS = BN / C::parts, STEP = KEYS < 64 ? KEYS : 64;
 #pragma unroll 1
                 for (uint32_t h = 0; h < C::parts && !idle; ++h) {

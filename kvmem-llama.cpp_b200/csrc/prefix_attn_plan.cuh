@@ -25,10 +25,11 @@ namespace kvmret {
 namespace {
 
 // Tiles of BN keys for what a piece costs beside its tiles, about 128 keys' worth.
-// Sixteen sequences over 32,768 shared tokens, tails of 1 to 700: 47.5 us with
-// this, 55.6 with none, 48.3 with 256; heads of 256 over q8_0 (tiles of 64 keys):
-// 49 us with this, 61 with 64. 32 sequences of up to five rows: 135.6, 135.9 with
-// none, 133.9 with 256.
+// Sixteen sequences over 32,768 shared tokens, tails of 1 to 700: 44.1 us with
+// this, 52.2 with none, 44.7 with 256 (q8_0 / q4_0: 54.5, 69.0, 55.6); heads of 256
+// (tiles of 64 keys) over q8_0 / q4_0: 54.3 us with this, 63.5 with none, 55.3 with 64,
+// 57.0 with 256. 32 sequences of up to five rows: 138.0, 139.0 with none, 136.4 with
+// 256 (medians, the builds in turn on one box).
 template <int BN>
 constexpr uint32_t kUnit = 128 / BN;
 
@@ -109,7 +110,7 @@ struct Cuts {
 // own rows (each row of the batch has one) and every further one a room by its CTA,
 // which begins at most one unit in its middle. So the rows follow those of the
 // batch, however few of them a unit has: 1024 sequences of one row, 64 query and 8 KV
-// heads of 128 take 0.11 GB (a tile of 256 rows for each piece would be 1.1 GB).
+// heads of 128 take 0.12 GB (a tile of 256 rows for each piece would be 1.2 GB).
 struct Rooms {
     uint32_t cap;    // rows of a room: a unit's, or all of a KV head's if they are fewer
     uint32_t n_pre;  // rooms of the prefix, from row 0 on
