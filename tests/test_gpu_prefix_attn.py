@@ -869,3 +869,110 @@ def test_the_most_sequences():
         assert torch.equal(torch.isneginf(lse[:, h]), empty) and bool((got[empty] == 0).all())
         wl = (top + torch.log(seen))[~empty, 0]
         assert bool(((lse[~empty, h].double() - wl).abs() <= ds[~empty, 0] + 2e-6 * (1 + wl.abs())).all())
+
+
+@pytest.mark.parametrize("kt,vt", [(F16, F16), (Q8, Q4), (Q8, F16)])
+def test_pages_between_others(kt, vt):
+    """K and V of several layers in one buffer, a page of each after another: the strides
+    of the pages, for the prefix and the tails, give what dense pages give."""
+    case = ([1, 3, 2], [40, 77, 9], 700, 8, 2, 128, 48, 32, kt, vt)
+    pool, tpool, table, own, _, _, start, q, tl = build(case)
+    args = (dev(np.array([700], np.int32)), dev(own), dev(tl), dev(start))
+    dense, tdense = pool.device(), tpool.device()
+
+    def spread(p):
+        k, v = (x.flatten(1).view(torch.uint8) for x in (p.k, p.v))
+        both = torch.full((p.n_pages, k.shape[1] + v.shape[1] + 96), 0xff, dtype=torch.uint8, device="cuda")
+        a, b = both[:, 32:32 + k.shape[1]], both[:, -v.shape[1] - 16:-16]
+        a.copy_(k)
+        b.copy_(v)
+        return kvmret.Pages(a, b, p.page_tokens, 2, 128, kt, vt)
+
+    want = kvmret.prefix_attn(dev(q), dense, args[0], tdense, *args[1:], prefix_table=dev(table), lse=True)
+    got = kvmret.prefix_attn(dev(q), spread(dense), args[0], spread(tdense), *args[1:],
+                             prefix_table=dev(table), lse=True)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("d,kt,vt", [(64, F16, F16), (128, Q8, Q4), (256, F16, Q8)])
+def test_contiguous_caches_as_one_page(d, kt, vt):
+    """A cache that is not paged: one page for the prefix, one for each tail."""
+    case = ([3, 1, 40], [900, 17, 1040], 4000, 12, 4, d, 4112, 1040, kt, vt)
+    pool, tpool, table, own, pre, tails, start, q, tl = build(case)
+    got, lse = kvmret.prefix_attn(dev(q), pool.device(), dev(np.array([4000], np.int32)), tpool.device(),
+                                  dev(own), dev(tl), dev(start), prefix_table=dev(table), lse=True)
+    spans = [(int(start[s]), int(start[s + 1]), *(torch.cat([dev(pre[i]), dev(tails[s][i])]) for i in (0, 1)))
+             for s in range(3)]
+    check_rows(got, lse, dev(q), spans, 4, kt != F16, vt != F16)
+
+
+def test_calls_from_threads():
+    """Several host threads at once, each on a stream of its own."""
+    import threading
+    cases = [([1] * 5, [50] * 5, 900, 8, 2, d, 64, 32, *kinds)
+             for d, kinds in ((64, (F16, F16)), (128, (Q8, Q4)), (256, (F16, F16)), (128, (F16, F16)))]
+    work, got = [], {}
+    for case in cases:
+        pool, tpool, table, own, _, _, start, q, tl = build(case)
+        work.append(((dev(q), pool.device(), dev(np.array([900], np.int32)), tpool.device(), dev(own),
+                      dev(tl), dev(start)), dev(table)))
+    torch.cuda.synchronize()
+
+    def run(i):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            got[i] = [kvmret.prefix_attn(*work[i][0], prefix_table=work[i][1]) for _ in range(30)]
+        s.synchronize()
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(len(cases))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for i, (args, table) in enumerate(work):
+        want = kvmret.prefix_attn(*args, prefix_table=table)
+        assert len(got[i]) == 30 and all(torch.equal(x, want) for x in got[i])
+
+
+def test_captured_window_attention():
+    """A call over a context's window in a graph: replays follow the window that later
+    steps build, and the tails' lengths."""
+    w = synth.Workload("graph", n_layer=2, n_head=8, n_head_kv=2, d_head=128, block_tokens=64,
+                       n_blocks=24, budget_blocks=6, sink_blocks=1, reserve_blocks=2, n_planted=3, seed=9)
+    r = kvmret.Retriever(config_for(w))
+    append_history(r, synth.NumpyHistory(w), cuts=[])
+    g = torch.Generator(device="cuda").manual_seed(4)
+    q = torch.randn(3, 8, 128, device="cuda", generator=g).half()
+    tails = kvmret.Pages(*(torch.randn(4, 16, 2, 128, device="cuda", generator=g).half() for _ in "kv"),
+                         16, 2, 128)
+    own = torch.tensor([[0], [2], [3]], dtype=torch.int32, device="cuda")
+    lens = torch.tensor([1, 9, 16], dtype=torch.int32, device="cuda")
+    start = torch.arange(4, dtype=torch.int32, device="cuda")
+
+    def step(seed):
+        rows = torch.randn(2, 1, 8 * 128, device="cuda", generator=torch.Generator(device="cuda").manual_seed(seed))
+        r.query_reset()
+        r.query_add(rows.half())
+        r.score()
+        r.select_apply_async()
+        r.step_collect()
+
+    step(1)
+    r.window_attn(1, q, tails, own, lens, start)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held, lse = r.window_attn(1, q, tails, own, lens, start, lse=True)
+    seen = []
+    for seed in (1, 2, 3):
+        step(seed)
+        lens += 0 if seed == 1 else -1
+        lens.clamp_(min=0)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        want, wl = r.window_attn(1, q, tails, own, lens, start, lse=True)
+        assert torch.equal(held, want) and torch.equal(lse, wl)
+        seen.append(held.clone())
+    assert not torch.equal(seen[0], seen[1])
+    r.close()
